@@ -423,6 +423,118 @@ int b4_swiglu_f16(const float* gate, const float* up, void* out, long long n, b4
 int b4_cast_f16(const float* in, void* out, long long n, b4_stream_t stream);
 const char* b4_nccl_error_string(int status);
 
+/* ---- Key/value cache in 4 bits --------------------------------------------------
+ * What a decode layer needs between its q/k/v projections and o: where a step's
+ * tokens go in a paged cache (b4_kv_tables), the write of their keys and values
+ * in this library's two 4-bit formats (b4_kv_append, read back by b4_kv_read),
+ * and attention over the pages (b4_kv_attention).  No counterpart in the
+ * reference, which stops at the projections.
+ *
+ * A page holds page_size tokens of every kv head; one kv head's part of a page
+ * is a block of contiguous bytes, so that a bulk copy brings it into shared
+ * memory whole:
+ *   codes of the keys     [page_size][head_dim / 2]   (packed as the weights are:
+ *   codes of the values   [page_size][head_dim / 2]    lower column, low nibble)
+ *   scales of the keys    [page_size]
+ *   scales of the values  [page_size]
+ * One scale per token and kv head: INT4 fp16 absmax / 7, value (code - 8) * scale
+ * (b4_quantise_int4_g128's codes where head_dim is 128); NF4 fp32 absmax, value
+ * NF4[code] * absmax (b4_quantise_nf4_b64's codes where head_dim is 64).
+ * blocks: uint8 [n_pages][kv_heads][b4_kv_block_bytes], 16-byte aligned.
+ * page_size 16, 32 or 64; head_dim 64 or 128; n_pages * page_size < 2^31.
+ *
+ * Every call here is launched as a programmatic dependent: it touches memory
+ * only after the preceding kernel on the stream has completed, and lets the next
+ * launch begin early. */
+#define B4_KV_INT4 0
+#define B4_KV_NF4 1
+#define B4_DTYPE_F16 0
+#define B4_DTYPE_BF16 1
+#define B4_DTYPE_F32 2
+typedef struct b4_kv_cache {
+    void* blocks;
+    int fmt;        /* B4_KV_* */
+    int n_pages;
+    int page_size;
+    int kv_heads;
+    int head_dim;
+} b4_kv_cache;
+int b4_kv_block_bytes(int fmt, int page_size, int head_dim, size_t* bytes);
+
+/* One scheduling step, on the device, in one launch: request r has cached[r]
+ * tokens in the cache and adds added[r] (lengths below 0 count as 0).
+ *   ctx_len[r]     = cached[r] + added[r]
+ *   q_starts       [n_req + 1] exclusive sums of added
+ *   tables[r][p]   for p from ceil(cached / page_size) to ceil(ctx / page_size):
+ *                  the next page of the ring, in request order; the other
+ *                  entries are left as they are
+ *   slots[i], positions[i]  for packed token i: its place in the cache (page *
+ *                  page_size + offset) and in its request; slots -1 and
+ *                  positions 0 from the last token up to max_tokens
+ * The ring free_pages[ring_size] is read from free_state[0] on, at most
+ * free_state[1] pages; free_state_out[0..2] = the next place, the pages left,
+ * and the pages that were missing.  A missing page's entry and slots are -1, and
+ * so are the slots past table_width pages; b4_kv_append skips those and
+ * b4_kv_attention counts such tokens as masked.  Lengths sum to less than 2^31.
+ * table_stride in entries; free_state_out must not overlap free_state, nor the
+ * other outputs an input.  n_req <= B4_KV_MAX_REQUESTS. */
+#define B4_KV_MAX_REQUESTS 16384
+typedef struct b4_kv_step {
+    int n_req, page_size, table_width, ring_size, max_tokens;
+    long long table_stride;
+    int32_t* tables;              /* [n_req][table_stride], in and out */
+    const int32_t* cached;        /* [n_req] */
+    const int32_t* added;         /* [n_req] */
+    const int32_t* free_pages;    /* [ring_size] */
+    const int32_t* free_state;    /* [2 or more] */
+    int32_t* ctx_len;             /* [n_req] */
+    int32_t* q_starts;            /* [n_req + 1] */
+    int32_t* slots;               /* [max_tokens] */
+    int32_t* positions;           /* [max_tokens] */
+    int32_t* free_state_out;      /* [3] */
+} b4_kv_step;
+int b4_kv_tables(const b4_kv_step* step, b4_stream_t stream);
+
+/* Quantises k and v [n_tokens][kv_heads][head_dim] (dtype fp16, bf16 or fp32;
+ * strides in elements, columns contiguous) into the cache at slots[n_tokens];
+ * slots outside the cache are skipped, and a slot may appear once.  Codes are
+ * those of the quantisers above, computed as they compute them in fp32 (a NaN
+ * becomes code 8 in INT4 and code 0 in NF4, and takes no part in absmax). */
+int b4_kv_append(const b4_kv_cache* cache, const void* k, const void* v, int dtype, long long k_stride_token,
+                 long long k_stride_head, long long v_stride_token, long long v_stride_head, const int32_t* slots,
+                 int n_tokens, b4_stream_t stream);
+/* The values that the cache holds at slots, fp32 [n_tokens][kv_heads][head_dim],
+ * contiguous; 0 for slots outside the cache. */
+int b4_kv_read(const b4_kv_cache* cache, const int32_t* slots, int n_tokens, float* k, float* v, b4_stream_t stream);
+
+/* out[t][h] = softmax(scale * q[t][h] . K + mask) V over the pages of t's request,
+ * kv head h / (heads / kv_heads).  Request r's queries are rows q_starts[r] ..
+ * q_starts[r + 1] of q, the last of its ctx_len[r] tokens: query i of n sees the
+ * keys below ctx - n + i + 1 (all ctx with B4_KV_FULL), and with window > 0 only
+ * the last `window` of those.  A query that sees no key gets zeros (lse -inf).
+ * q, out: dtype fp16 or bf16 [total_q][heads][head_dim], strides in elements,
+ * columns contiguous, rows 16-byte aligned.  lse (optional): fp32
+ * [total_q][heads], the natural logarithm of the sum of exp(scores).
+ * max_q: the most queries of one request (chooses the kernels; requests with
+ * more are computed all the same).  heads / kv_heads <= 64.
+ * ws: b4_kv_attention_workspace bytes of device memory, 16-byte aligned,
+ * ZERO-FILLED before its first use; calls leave ready for the next what must be
+ * zero.  Not shared with b4_gemv_ws, nor by calls that may run at the same time. */
+#define B4_KV_FULL 1
+typedef struct b4_kv_attn {
+    const void* q;
+    void* out;
+    float* lse;
+    const int32_t* tables;        /* [n_req][table_stride] */
+    const int32_t* ctx_len;       /* [n_req] */
+    const int32_t* q_starts;      /* [n_req + 1] */
+    long long table_stride, q_stride_token, q_stride_head, out_stride_token, out_stride_head;
+    int table_width, n_req, total_q, max_q, heads, dtype, window, flags;
+    float scale;
+} b4_kv_attn;
+int b4_kv_attention_workspace(const b4_kv_cache* cache, const b4_kv_attn* attn, size_t* bytes);
+int b4_kv_attention(const b4_kv_cache* cache, const b4_kv_attn* attn, void* ws, size_t ws_bytes, b4_stream_t stream);
+
 /* Reads (and with clear != 0 resets) the current device's error flags: non-zero
  * after a bounded wait ran out -- 1: a streaming kernel's wait on its copy
  * ring (the kernel then ended early), 2: the x-pair table kernel's count-in

@@ -25,6 +25,8 @@ __all__ = [
     "multi_default_config", "MAX_SEGMENTS", "GemvSegment", "repack_bnb_nf4", "FLAG_SPLIT", "FLAG_KSLICE",
     "gemv_ws", "workspace_size", "workspace", "default_config_ws", "multi_default_config_ws",
     "ENGINE_NF4_XTAB", "XTAB_WORKSPACE_BYTES",
+    "KV_INT4", "KV_NF4", "KVCache", "KVStep", "kv_block_bytes", "kv_tables", "kv_append", "kv_read", "kv_attention",
+    "kv_attention_workspace",
 ]
 
 
@@ -362,3 +364,9 @@ def unpack_codes(qw, out=None, stream=None):
         out = torch.empty((out_f, in_f), dtype=torch.uint8, device=qw.device)
     check("b4_unpack_codes", load().b4_unpack_codes(_ptr(qw), _ptr(out), in_f, out_f, _stream(stream)))
     return out
+
+
+# ---- 4-bit key/value cache ---------------------------------------------------------
+
+from .kv import (KV_INT4, KV_NF4, KVCache, KVStep, kv_append, kv_attention, kv_attention_workspace,  # noqa: E402
+                 kv_block_bytes, kv_read, kv_tables)

@@ -75,6 +75,41 @@ class GemvSegment(ctypes.Structure):
 
 MAX_SEGMENTS = 4
 
+KV_INT4 = 0
+KV_NF4 = 1
+KV_FULL = 1             # b4_kv_attn.flags: every query sees every key of its request
+DTYPE_F16 = 0
+DTYPE_BF16 = 1
+DTYPE_F32 = 2
+
+
+class KvCache(ctypes.Structure):
+    """b4_kv_cache (include/b4gemv.h)."""
+
+    _fields_ = [("blocks", ctypes.c_void_p)] + [(n, ctypes.c_int) for n in (
+        "fmt", "n_pages", "page_size", "kv_heads", "head_dim")]
+
+
+class KvStep(ctypes.Structure):
+    """b4_kv_step (include/b4gemv.h)."""
+
+    _fields_ = ([(n, ctypes.c_int) for n in ("n_req", "page_size", "table_width", "ring_size", "max_tokens")]
+                + [("table_stride", ctypes.c_longlong)]
+                + [(n, ctypes.c_void_p) for n in ("tables", "cached", "added", "free_pages", "free_state", "ctx_len",
+                                                  "q_starts", "slots", "positions", "free_state_out")])
+
+
+class KvAttn(ctypes.Structure):
+    """b4_kv_attn (include/b4gemv.h)."""
+
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("q", "out", "lse", "tables", "ctx_len", "q_starts")]
+                + [(n, ctypes.c_longlong) for n in ("table_stride", "q_stride_token", "q_stride_head",
+                                                    "out_stride_token", "out_stride_head")]
+                + [(n, ctypes.c_int) for n in ("table_width", "n_req", "total_q", "max_q", "heads", "dtype", "window",
+                                               "flags")]
+                + [("scale", ctypes.c_float)])
+
+
 _P = ctypes.c_void_p
 _I = ctypes.c_int
 
@@ -121,6 +156,14 @@ SIGNATURES = {
     "b4_tp_gemv_p2p_ex": (_I, [_I, _P, _P, _P, _P, _P, _I, _I, _P, _I, _P]),
     "b4_swiglu_f16": (_I, [_P, _P, _P, ctypes.c_longlong, _P]),
     "b4_cast_f16": (_I, [_P, _P, ctypes.c_longlong, _P]),
+    "b4_kv_block_bytes": (_I, [_I, _I, _I, ctypes.POINTER(ctypes.c_size_t)]),
+    "b4_kv_tables": (_I, [ctypes.POINTER(KvStep), _P]),
+    "b4_kv_append": (_I, [ctypes.POINTER(KvCache), _P, _P, _I, ctypes.c_longlong, ctypes.c_longlong, ctypes.c_longlong,
+                          ctypes.c_longlong, _P, _I, _P]),
+    "b4_kv_read": (_I, [ctypes.POINTER(KvCache), _P, _I, _P, _P, _P]),
+    "b4_kv_attention_workspace": (_I, [ctypes.POINTER(KvCache), ctypes.POINTER(KvAttn),
+                                       ctypes.POINTER(ctypes.c_size_t)]),
+    "b4_kv_attention": (_I, [ctypes.POINTER(KvCache), ctypes.POINTER(KvAttn), _P, ctypes.c_size_t, _P]),
     "b4_nccl_error_string": (ctypes.c_char_p, [_I]),
     "b4_device_error": (_I, [_I]),
     "b4_status_string": (ctypes.c_char_p, [_I]),
