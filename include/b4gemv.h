@@ -537,8 +537,8 @@ int b4_kv_attention(const b4_kv_cache* cache, const b4_kv_attn* attn, void* ws, 
 
 /* Reads (and with clear != 0 resets) the current device's error flags: non-zero
  * after a bounded wait ran out -- 1: a streaming kernel's wait on its copy
- * ring (the kernel then ended early), 2: the x-pair table kernel's count-in
- * (it then carried on without it) -- and that launch's y is not valid.
+ * ring (the kernel then ended early; the cache attention's: carried on), 2: the x-pair table kernel's count-in
+ * (it then carried on without it) -- and that launch's output is not valid.
  * Returns the flags, or -1 if they could not be read. */
 int b4_device_error(int clear);
 

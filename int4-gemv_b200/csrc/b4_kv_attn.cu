@@ -1,75 +1,61 @@
 // b4_kv_attn.cu -- attention over the 4-bit key/value cache.
 #include <cmath>
 
-#include "b4_kv.cuh"
+#include "b4_kv_attn_warp.cuh"
 
 namespace b4 {
 namespace {
 
-struct AttnParams {
-    KvLayout l;
-    const uint8_t* blocks;
-    b4_kv_attn a;
-};
-
-// The simple form: a warp per (query, head), one key at a time, the softmax's
-// maximum and sum running (one pass); lane i holds columns i * D / 32 onward.
-template <typename T, int FMT, int D>
-__global__ void __launch_bounds__(256) kv_attn_kernel(const AttnParams p)
+// The least columns (queries x heads that share a kv head) of a tile that hold
+// a request's queries, or 32 a tile.
+int tile_cols(const AttnParams& p)
 {
-    constexpr int C = D / 32;
-    kv_begin();
-    const int lane = threadIdx.x & 31;
-    const b4_kv_attn& a = p.a;
-    const long long rows = (long long)a.total_q * a.heads;
-    for (long long i = (long long)blockIdx.x * 8 + (threadIdx.x >> 5); i < rows; i += (long long)gridDim.x * 8) {
-        const int t = (int)(i / a.heads), h = (int)(i - (long long)t * a.heads), kvh = h / (a.heads / p.l.kv_heads);
-        int r = 0;
-        while (r < a.n_req - 1 && a.q_starts[r + 1] <= t) ++r;
-        if (t < a.q_starts[r] || t >= a.q_starts[r + 1]) continue;
-        const int ctx = max(0, min(a.ctx_len[r], a.table_width * p.l.page_size)), n = a.q_starts[r + 1] - a.q_starts[r];
-        const int end = a.flags & B4_KV_FULL ? ctx : min(ctx, ctx - n + (t - a.q_starts[r]) + 1);
-        const int begin = a.window > 0 ? max(0, end - a.window) : 0;
-        const T* q = static_cast<const T*>(a.q) + t * a.q_stride_token + h * a.q_stride_head + lane * C;
-        float qf[C], acc[C] = {}, m = -INFINITY, sum = 0.0f;
-        for (int j = 0; j < C; ++j) qf[j] = kv_float(q[j]) * a.scale;
-        for (int key = begin; key < end; ++key) {
-            const int page = a.tables[r * a.table_stride + (key >> p.l.page_shift)], row = key & (p.l.page_size - 1);
-            if (page < 0 || page >= p.l.n_pages) continue;
-            const uint8_t* block = p.blocks + ((long long)page * p.l.kv_heads + kvh) * p.l.block;
-            float s[2], kv[2][C];
-            for (int o = 0; o < 2; ++o) {
-                const int at = o * p.l.page_size + row;
-                const uint8_t* sp = block + p.l.page_size * D;
-                s[o] = FMT == B4_KV_INT4 ? __half2float(reinterpret_cast<const __half*>(sp)[at]) : reinterpret_cast<const float*>(sp)[at];
-                for (int j = 0; j < C; ++j) {
-                    const uint32_t c = block[at * (D / 2) + (lane * C + j) / 2] >> (4 * (j & 1)) & 15;
-                    kv[o][j] = FMT == B4_KV_INT4 ? (float)c - 8.0f : c_nf4_table[c];
-                }
-            }
-            float dot = 0.0f;
-            for (int j = 0; j < C; ++j) dot = fmaf(qf[j], kv[0][j], dot);
-            for (int o = 16; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
-            dot *= s[0];
-            const float next = fmaxf(m, dot);
-            const float keep = next == -INFINITY ? 0.0f : __expf(m - next), w = next == -INFINITY ? 0.0f : __expf(dot - next);
-            sum = sum * keep + w;
-            for (int j = 0; j < C; ++j) acc[j] = acc[j] * keep + w * s[1] * kv[1][j];
-            m = next;
-        }
-        const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
-        T* out = static_cast<T*>(a.out) + t * a.out_stride_token + h * a.out_stride_head + lane * C;
-        for (int j = 0; j < C; ++j) out[j] = kv_round<T>(acc[j] * inv);
-        if (a.lse && lane == 0) a.lse[i] = sum > 0.0f ? m + logf(sum) : -INFINITY;
-    }
+    const long long cols = (long long)std::max(1, p.a.max_q) * p.group;
+    return cols <= 8 ? 8 : cols <= 16 ? 16 : 32;
 }
 
-template <typename T, int FMT>
-cudaError_t attention(const AttnParams& p, cudaStream_t st)
+int sm_count()
 {
-    const dim3 grid((unsigned)std::min<long long>(((long long)p.a.total_q * p.a.heads + 7) / 8, 1 << 20));
-    return p.l.head_dim == 64 ? kv_launch(kv_attn_kernel<T, FMT, 64>, grid, 256, 0, st, p)
-                              : kv_launch(kv_attn_kernel<T, FMT, 128>, grid, 256, 0, st, p);
+    int dev = 0, n = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n < 1) return 148;
+    return n;
+}
+
+// [counters][first pieces][crossing pieces], one CTA an SM
+constexpr int kMaxWarps = 8;
+size_t warp_ws_bytes(const AttnParams& p, int sms)
+{
+    const size_t piece = (size_t)tile_cols(p) * (p.l.head_dim + 2) * 4;
+    return 4096 + (size_t)sms * (kMaxWarps + 2) * piece;
+}
+
+template <typename T, int FMT, int D, int NT>
+cudaError_t launch_warp(const AttnParams& p, void* ws, cudaStream_t st)
+{
+    using C = WarpCfg<FMT, D, NT>;
+    auto fn = kv_attn_warp_kernel<T, FMT, D, NT>;
+    const cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
+    if (e != cudaSuccess) return e;
+    const int sms = sm_count();
+    WarpWs w;
+    w.count = static_cast<int*>(ws);
+    w.first = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + 4096);
+    w.cross = w.first + (size_t)sms * C::kWarps * C::kPiece;
+    return kv_launch(fn, dim3((unsigned)sms), C::kWarps * 32, C::kSmem, st, p, w);
+}
+
+template <typename T, int FMT, int D>
+cudaError_t launch_cols(const AttnParams& p, void* ws, cudaStream_t st)
+{
+    const int cols = tile_cols(p);
+    return cols == 8 ? launch_warp<T, FMT, D, 1>(p, ws, st) : cols == 16 ? launch_warp<T, FMT, D, 2>(p, ws, st) : launch_warp<T, FMT, D, 4>(p, ws, st);
+}
+
+template <typename T>
+cudaError_t attention(const AttnParams& p, void* ws, cudaStream_t st)
+{
+    if (p.l.fmt == B4_KV_INT4) return p.l.head_dim == 64 ? launch_cols<T, B4_KV_INT4, 64>(p, ws, st) : launch_cols<T, B4_KV_INT4, 128>(p, ws, st);
+    return p.l.head_dim == 64 ? launch_cols<T, B4_KV_NF4, 64>(p, ws, st) : launch_cols<T, B4_KV_NF4, 128>(p, ws, st);
 }
 
 int attn_params(const b4_kv_cache* cache, const b4_kv_attn* a, AttnParams* p)
@@ -83,6 +69,7 @@ int attn_params(const b4_kv_cache* cache, const b4_kv_attn* a, AttnParams* p)
     if (a->table_stride < a->table_width || (long long)a->table_width * p->l.page_size > 0x7fffffffLL) return cudaErrorInvalidValue;
     p->blocks = static_cast<const uint8_t*>(cache->blocks);
     p->a = *a;
+    p->group = a->heads / p->l.kv_heads;
     return cudaSuccess;
 }
 
@@ -90,6 +77,17 @@ int attn_params(const b4_kv_cache* cache, const b4_kv_attn* a, AttnParams* p)
 }  // namespace b4
 
 using namespace b4;
+
+int b4::kv_attn_device_error(int clear)
+{
+    int v = 0;
+    if (cudaMemcpyFromSymbol(&v, g_device_error, sizeof(v)) != cudaSuccess) return -1;
+    if (clear && v) {
+        const int z = 0;
+        if (cudaMemcpyToSymbol(g_device_error, &z, sizeof(z)) != cudaSuccess) return -1;
+    }
+    return v;
+}
 
 extern "C" {
 
@@ -99,7 +97,7 @@ int b4_kv_attention_workspace(const b4_kv_cache* cache, const b4_kv_attn* a, siz
     const int e = attn_params(cache, a, &p);
     if (e != cudaSuccess) return e;
     if (!bytes) return cudaErrorInvalidValue;
-    *bytes = 0;
+    *bytes = a->total_q && a->n_req ? warp_ws_bytes(p, sm_count()) : 0;
     return cudaSuccess;
 }
 
@@ -113,9 +111,8 @@ int b4_kv_attention(const b4_kv_cache* cache, const b4_kv_attn* a, void* ws, siz
     const long long strides = a->q_stride_token | a->q_stride_head | a->out_stride_token | a->out_stride_head;
     if (!kv_aligned(a->q, 16) || !kv_aligned(a->out, 16) || strides % 8 != 0) return cudaErrorInvalidValue;
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-    const bool i4 = p.l.fmt == B4_KV_INT4;
-    if (a->dtype == B4_DTYPE_F16) return i4 ? attention<__half, B4_KV_INT4>(p, st) : attention<__half, B4_KV_NF4>(p, st);
-    return i4 ? attention<__nv_bfloat16, B4_KV_INT4>(p, st) : attention<__nv_bfloat16, B4_KV_NF4>(p, st);
+    if (!ws || !kv_aligned(ws, 16) || ws_bytes < warp_ws_bytes(p, sm_count())) return cudaErrorInvalidValue;
+    return a->dtype == B4_DTYPE_F16 ? attention<__half>(p, ws, st) : attention<__nv_bfloat16>(p, ws, st);
 }
 
 }  // extern "C"

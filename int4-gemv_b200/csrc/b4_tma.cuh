@@ -11,8 +11,8 @@ namespace b4 {
 
 // Set (atomicOr) by a kernel whose bounded wait ran out; read and cleared by
 // b4_device_error() through the reader of the translation unit that holds the
-// streaming kernels (gemv_tma.cu).  No relocatable device code, so the flag is
-// per translation unit; only that one includes this header.
+// streaming kernels.  No relocatable device code, so the flag is per translation
+// unit; gemv_tma.cu and b4_kv_attn.cu include this header and have a reader each.
 static __device__ int g_device_error;
 
 constexpr int kErrMbarrierTimeout = 1;
