@@ -437,9 +437,10 @@ const char* b4_nccl_error_string(int status);
  *   codes of the values   [page_size][head_dim / 2]    lower column, low nibble)
  *   scales of the keys    [page_size]
  *   scales of the values  [page_size]
- * One scale per token and kv head: INT4 fp16 absmax / 7, value (code - 8) * scale
- * (b4_quantise_int4_g128's codes where head_dim is 128); NF4 fp32 absmax, value
- * NF4[code] * absmax (b4_quantise_nf4_b64's codes where head_dim is 64).
+ * One scale per token and kv head.  INT4: fp16(absmax * (1 / 7)), the product and
+ * the reciprocal in fp32 (b4_quantise_int4_g128 divides: its scale may be the next
+ * fp16 number), value (code - 8) * scale; NF4: fp32 absmax, value NF4[code] *
+ * absmax (where head_dim is 64, b4_quantise_nf4_b64's codes and absmax).
  * blocks: uint8 [n_pages][kv_heads][b4_kv_block_bytes], 16-byte aligned.
  * page_size 16, 32 or 64; head_dim 64 or 128; n_pages * page_size < 2^31.
  *
@@ -497,9 +498,10 @@ int b4_kv_tables(const b4_kv_step* step, b4_stream_t stream);
 
 /* Quantises k and v [n_tokens][kv_heads][head_dim] (dtype fp16, bf16 or fp32;
  * strides in elements, columns contiguous) into the cache at slots[n_tokens];
- * slots outside the cache are skipped, and a slot may appear once.  Codes are
- * those of the quantisers above, computed as they compute them in fp32 (a NaN
- * becomes code 8 in INT4 and code 0 in NF4, and takes no part in absmax). */
+ * slots outside the cache are skipped, and a slot may appear once.  A
+ * code is the nearest by the fp32 quotient x / scale as in the quantisers above:
+ * lround(quotient) + 8, clamped (INT4), the first nearest level (NF4); a NaN
+ * becomes code 8 in INT4 and code 0 in NF4, and takes no part in absmax. */
 int b4_kv_append(const b4_kv_cache* cache, const void* k, const void* v, int dtype, long long k_stride_token,
                  long long k_stride_head, long long v_stride_token, long long v_stride_head, const int32_t* slots,
                  int n_tokens, b4_stream_t stream);

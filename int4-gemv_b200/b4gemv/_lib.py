@@ -156,14 +156,14 @@ SIGNATURES = {
     "b4_tp_gemv_p2p_ex": (_I, [_I, _P, _P, _P, _P, _P, _I, _I, _P, _I, _P]),
     "b4_swiglu_f16": (_I, [_P, _P, _P, ctypes.c_longlong, _P]),
     "b4_cast_f16": (_I, [_P, _P, ctypes.c_longlong, _P]),
+    # b4_kv_step and b4_kv_attn by address: a structure or its packed bytes
     "b4_kv_block_bytes": (_I, [_I, _I, _I, ctypes.POINTER(ctypes.c_size_t)]),
-    "b4_kv_tables": (_I, [ctypes.POINTER(KvStep), _P]),
+    "b4_kv_tables": (_I, [_P, _P]),
     "b4_kv_append": (_I, [ctypes.POINTER(KvCache), _P, _P, _I, ctypes.c_longlong, ctypes.c_longlong, ctypes.c_longlong,
                           ctypes.c_longlong, _P, _I, _P]),
     "b4_kv_read": (_I, [ctypes.POINTER(KvCache), _P, _I, _P, _P, _P]),
-    "b4_kv_attention_workspace": (_I, [ctypes.POINTER(KvCache), ctypes.POINTER(KvAttn),
-                                       ctypes.POINTER(ctypes.c_size_t)]),
-    "b4_kv_attention": (_I, [ctypes.POINTER(KvCache), ctypes.POINTER(KvAttn), _P, ctypes.c_size_t, _P]),
+    "b4_kv_attention_workspace": (_I, [ctypes.POINTER(KvCache), _P, ctypes.POINTER(ctypes.c_size_t)]),
+    "b4_kv_attention": (_I, [ctypes.POINTER(KvCache), _P, _P, ctypes.c_size_t, _P]),
     "b4_nccl_error_string": (ctypes.c_char_p, [_I]),
     "b4_device_error": (_I, [_I]),
     "b4_status_string": (ctypes.c_char_p, [_I]),

@@ -6,13 +6,18 @@
     kv_append(cache, k, v, step.slots)
     out = kv_attention(cache, q, tables, step.ctx_len, step.q_starts, max_q)
 
-Every call goes to the current stream of the tensors' device and returns without
-waiting.  Refused arguments raise ValueError before anything is launched; what
-only the library can refuse raises B4Error.
+Every call goes to the current stream of the tensors' device (or `stream`) and
+returns without waiting.  Refused arguments raise ValueError before anything is
+launched; what only the library can refuse raises B4Error.
+
+A decode step calls these for every layer, with kernels of a few microseconds:
+the checks make no objects, and a call's structure is packed as bytes in one
+go.
 """
 from __future__ import annotations
 
 import ctypes
+import struct
 from typing import NamedTuple
 
 from ._lib import (DTYPE_BF16, DTYPE_F16, DTYPE_F32, KV_FULL, KV_INT4, KV_NF4, KvAttn, KvCache, KvStep, check, load)
@@ -20,33 +25,51 @@ from ._lib import (DTYPE_BF16, DTYPE_F16, DTYPE_F32, KV_FULL, KV_INT4, KV_NF4, K
 __all__ = ["KV_INT4", "KV_NF4", "KVCache", "KVStep", "kv_block_bytes", "kv_tables", "kv_append", "kv_read",
            "kv_attention", "kv_attention_workspace"]
 
-_byref = ctypes.byref
+# b4_kv_step and b4_kv_attn as the C compiler lays them out (KvStep, KvAttn in _lib)
+_STEP = struct.Struct("@5i4xq10P")
+_ATTN = struct.Struct("@6P5q8if4x")
+assert _STEP.size == ctypes.sizeof(KvStep) and _ATTN.size == ctypes.sizeof(KvAttn)
+
+_torch = _int32 = _float32 = _raw_stream = _codes = None
 
 
-def _torch():
+def _load():
+    """torch's names and the library, once."""
+    global _torch, _int32, _float32, _raw_stream, _codes
     import torch
-    return torch
+    _torch, _int32, _float32 = torch, torch.int32, torch.float32
+    _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+        lambda index: torch.cuda.current_stream(index).cuda_stream)
+    _codes = {torch.float16: DTYPE_F16, torch.bfloat16: DTYPE_BF16, torch.float32: DTYPE_F32}
+    return load()
 
 
-def _raw_stream(device):
-    return _torch().cuda.current_stream(device).cuda_stream
+def _lib():
+    return load() if _torch is not None else _load()
 
 
-def _need(ok, what):
-    if not ok:
-        raise ValueError(what)
+def _ints(name, t, index, least):
+    if t.dtype is not _int32 or t.get_device() != index or not t.is_contiguous():
+        raise ValueError(f"{name}: a contiguous int32 tensor on cuda:{index}")
+    if t.numel() < least:
+        raise ValueError(f"{name}: {least} values at least, got {t.numel()}")
 
 
-def _ints(name, t, device, least):
-    torch = _torch()
-    _need(t.dtype == torch.int32 and t.device == device and t.is_contiguous(), f"{name}: a contiguous int32 tensor on {device}")
-    _need(t.numel() >= least, f"{name}: {least} values at least, got {t.numel()}")
+def _table(tables, index, n):
+    """(width, stride) of int32 [requests][width] with contiguous columns."""
+    if tables.dtype is not _int32 or tables.get_device() != index or index < 0 or tables.dim() != 2:
+        raise ValueError("tables: an int32 CUDA tensor [requests][width], on the device of the others")
+    rows, width = tables.shape
+    stride, one = tables.stride()
+    if rows < n or (width > 1 and one != 1):
+        raise ValueError(f"tables: {n} rows at least, columns contiguous")
+    return width, max(stride, width)
 
 
 def kv_block_bytes(fmt: int, page_size: int, head_dim: int) -> int:
     """Bytes of one kv head's part of a page."""
     n = ctypes.c_size_t(0)
-    check("b4_kv_block_bytes", load().b4_kv_block_bytes(fmt, page_size, head_dim, _byref(n)))
+    check("b4_kv_block_bytes", load().b4_kv_block_bytes(fmt, page_size, head_dim, ctypes.byref(n)))
     return n.value
 
 
@@ -56,18 +79,21 @@ class KVCache:
 
     def __init__(self, blocks, fmt: int, page_size: int, head_dim: int):
         size = kv_block_bytes(fmt, page_size, head_dim)
-        _need(blocks.is_cuda and blocks.dtype == _torch().uint8 and blocks.is_contiguous(), "blocks: a contiguous uint8 CUDA tensor")
-        _need(blocks.dim() == 3 and blocks.shape[2] == size, f"blocks: [pages][kv_heads][{size}], got {tuple(blocks.shape)}")
+        _load()
+        if not blocks.is_cuda or blocks.dtype != _torch.uint8 or not blocks.is_contiguous():
+            raise ValueError("blocks: a contiguous uint8 CUDA tensor")
+        if blocks.dim() != 3 or blocks.shape[2] != size:
+            raise ValueError(f"blocks: [pages][kv_heads][{size}], got {tuple(blocks.shape)}")
         self.blocks, self.fmt, self.page_size, self.head_dim = blocks, fmt, page_size, head_dim
         self.n_pages, self.kv_heads = blocks.shape[0], blocks.shape[1]
-        self.device = blocks.device
+        self.device, self.index = blocks.device, blocks.get_device()
         self._c = KvCache(blocks.data_ptr(), fmt, self.n_pages, page_size, self.kv_heads, head_dim)
-        self._ref = _byref(self._c)
+        self._ref = ctypes.byref(self._c)
 
     @classmethod
     def alloc(cls, fmt: int, n_pages: int, kv_heads: int, page_size: int = 64, head_dim: int = 128, device="cuda"):
         """A cache of n_pages pages (zero-filled)."""
-        torch = _torch()
+        import torch
         return cls(torch.zeros((n_pages, kv_heads, kv_block_bytes(fmt, page_size, head_dim)), dtype=torch.uint8,
                                device=device), fmt, page_size, head_dim)
 
@@ -87,115 +113,110 @@ def kv_tables(page_size: int, tables, cached, added, free_pages, free_state, max
     slots, positions, starts and lengths of one step.  free_pages is the ring
     of free pages, free_state its (place, pages left); the returned free_state is
     the next step's.  out: buffers to reuse (free_state must be another one)."""
-    torch = _torch()
-    dev = tables.device
-    n = cached.numel()
-    _need(tables.is_cuda and tables.dtype == torch.int32 and tables.dim() == 2 and tables.shape[0] >= n
-          and (tables.shape[1] <= 1 or tables.stride(1) == 1), "tables: int32 CUDA [requests][width], columns contiguous")
-    _ints("cached", cached, dev, 0)
-    _ints("added", added, dev, n)
-    _ints("free_pages", free_pages, dev, 0)
-    _ints("free_state", free_state, dev, 2)
+    lib = _lib()
+    index, n = tables.get_device(), cached.numel()
+    width, stride = _table(tables, index, n)
+    _ints("cached", cached, index, 0)
+    _ints("added", added, index, n)
+    _ints("free_pages", free_pages, index, 0)
+    _ints("free_state", free_state, index, 2)
     if out is None:
-        # one buffer for the five outputs, each on a 16-byte boundary
-        sizes = [n, n + 1, max_tokens, max_tokens, 3]
-        flat = torch.empty(sum((s + 3) // 4 * 4 for s in sizes), dtype=torch.int32, device=dev)
-        parts, at = [], 0
-        for s in sizes:
-            parts.append(flat[at:at + s])
-            at += (s + 3) // 4 * 4
-        out = KVStep(*parts)
+        if max_tokens < 0:
+            raise ValueError("max_tokens: 0 or more")
+        out = KVStep(*_torch.empty(2 * n + 2 * max_tokens + 4, dtype=_int32, device=tables.device).split(
+            (n, n + 1, max_tokens, max_tokens, 3)))
     else:
         for name, least in (("ctx_len", n), ("q_starts", n + 1), ("slots", max_tokens), ("positions", max_tokens), ("free_state", 3)):
-            _ints(name, getattr(out, name), dev, least)
-    c = KvStep(n, page_size, tables.shape[1], free_pages.numel(), max_tokens, max(tables.stride(0), tables.shape[1]),
-               tables.data_ptr(), cached.data_ptr(), added.data_ptr(), free_pages.data_ptr(), free_state.data_ptr(),
-               out.ctx_len.data_ptr(), out.q_starts.data_ptr(), out.slots.data_ptr(), out.positions.data_ptr(),
-               out.free_state.data_ptr())
-    check("b4_kv_tables", load().b4_kv_tables(_byref(c), stream.cuda_stream if stream is not None else _raw_stream(dev)))
+            _ints(name, getattr(out, name), index, least)
+    args = _STEP.pack(n, page_size, width, free_pages.numel(), max_tokens, stride, tables.data_ptr(), cached.data_ptr(),
+                      added.data_ptr(), free_pages.data_ptr(), free_state.data_ptr(), out[0].data_ptr(), out[1].data_ptr(),
+                      out[2].data_ptr(), out[3].data_ptr(), out[4].data_ptr())
+    status = lib.b4_kv_tables(args, stream.cuda_stream if stream is not None else _raw_stream(index))
+    if status:
+        check("b4_kv_tables", status)
     return out
-
-
-def _dtype(t):
-    torch = _torch()
-    return {torch.float16: DTYPE_F16, torch.bfloat16: DTYPE_BF16, torch.float32: DTYPE_F32}.get(t.dtype)
 
 
 def kv_append(cache: KVCache, k, v, slots, stream=None) -> None:
     """b4_kv_append: k and v [tokens][kv_heads][head_dim] (fp16, bf16 or fp32, any
     token and head strides, columns contiguous) into the cache at slots."""
-    shape = (slots.numel(), cache.kv_heads, cache.head_dim)
-    _ints("slots", slots, cache.device, 0)
-    code = _dtype(k)
-    _need(code is not None and v.dtype == k.dtype, "k and v: fp16, bf16 or fp32, both alike")
-    for t in (k, v):
-        _need(tuple(t.shape) == shape and t.device == cache.device and t.stride(2) == 1,
-              f"k and v: {shape} on {cache.device}, columns contiguous")
-    check("b4_kv_append", load().b4_kv_append(
-        cache._ref, k.data_ptr(), v.data_ptr(), code, k.stride(0), k.stride(1), v.stride(0), v.stride(1),
-        slots.data_ptr(), shape[0], stream.cuda_stream if stream is not None else _raw_stream(cache.device)))
+    index, n = cache.index, slots.numel()
+    _ints("slots", slots, index, 0)
+    code = _codes.get(k.dtype)
+    shape, ks, vs = (n, cache.kv_heads, cache.head_dim), k.stride(), v.stride()
+    if (code is None or v.dtype is not k.dtype or k.shape != shape or v.shape != shape or k.get_device() != index
+            or v.get_device() != index or ks[2] != 1 or vs[2] != 1):
+        raise ValueError(f"k and v: {shape}, both fp16, bf16 or fp32, on cuda:{index}, columns contiguous")
+    status = load().b4_kv_append(cache._ref, k.data_ptr(), v.data_ptr(), code, ks[0], ks[1], vs[0], vs[1], slots.data_ptr(), n,
+                                 stream.cuda_stream if stream is not None else _raw_stream(index))
+    if status:
+        check("b4_kv_append", status)
 
 
 def kv_read(cache: KVCache, slots, k=None, v=None, stream=None):
     """b4_kv_read: the fp32 values held at slots, as (k, v) [tokens][kv_heads][head_dim]."""
-    torch = _torch()
-    shape = (slots.numel(), cache.kv_heads, cache.head_dim)
-    _ints("slots", slots, cache.device, 0)
-    k = torch.empty(shape, device=cache.device) if k is None else k
-    v = torch.empty(shape, device=cache.device) if v is None else v
-    for t in (k, v):
-        _need(tuple(t.shape) == shape and t.dtype == torch.float32 and t.device == cache.device and t.is_contiguous(),
-              f"k and v: contiguous fp32 {shape} on {cache.device}")
-    check("b4_kv_read", load().b4_kv_read(cache._ref, slots.data_ptr(), shape[0], k.data_ptr(), v.data_ptr(),
-                                          stream.cuda_stream if stream is not None else _raw_stream(cache.device)))
+    index, n = cache.index, slots.numel()
+    _ints("slots", slots, index, 0)
+    shape = (n, cache.kv_heads, cache.head_dim)
+    k = _torch.empty(shape, device=cache.device) if k is None else k
+    v = _torch.empty(shape, device=cache.device) if v is None else v
+    for x in (k, v):
+        if x.shape != shape or x.dtype is not _float32 or x.get_device() != index or not x.is_contiguous():
+            raise ValueError(f"k and v: contiguous fp32 {shape} on cuda:{index}")
+    status = load().b4_kv_read(cache._ref, slots.data_ptr(), n, k.data_ptr(), v.data_ptr(),
+                               stream.cuda_stream if stream is not None else _raw_stream(index))
+    if status:
+        check("b4_kv_read", status)
     return k, v
 
 
-_WS = {}
+_WS, _WS_BYTES = {}, {}
 
 
-def _workspace(device, nbytes: int):
-    """The package's workspace for attention on `device`: zero-filled, grown on demand."""
-    ws = _WS.get(device.index)
+def _workspace(index, nbytes: int):
+    """The package's workspace for attention on a device: zero-filled, grown on demand."""
+    ws = _WS.get(index)
     if ws is None or ws.numel() < nbytes:
-        torch = _torch()
-        ws = torch.zeros(max(int(nbytes), 1 << 20), dtype=torch.uint8, device=device)
-        _WS[device.index] = ws
+        ws = _torch.zeros(max(int(nbytes), 1 << 20), dtype=_torch.uint8, device=f"cuda:{index}")
+        _WS[index] = ws
     return ws
 
 
 def _attn(cache, q, tables, ctx_len, q_starts, max_q, scale, window, causal, out, lse):
-    torch = _torch()
-    dev = cache.device
-    code = _dtype(q)
-    _need(code in (DTYPE_F16, DTYPE_BF16) and q.dim() == 3 and q.device == dev and q.shape[2] == cache.head_dim
-          and q.stride(2) == 1, f"q: fp16 or bf16 [tokens][heads][{cache.head_dim}] on {dev}, columns contiguous")
+    """A call's b4_kv_attn, packed, and its output."""
+    index, dim, n = cache.index, cache.head_dim, ctx_len.numel()
+    code = _codes.get(q.dtype)
+    if (code is None or code == DTYPE_F32 or q.dim() != 3 or q.get_device() != index or q.shape[2] != dim
+            or q.stride(2) != 1):
+        raise ValueError(f"q: fp16 or bf16 [tokens][heads][{dim}] on cuda:{index}, columns contiguous")
     total, heads, _ = q.shape
-    _need(heads % cache.kv_heads == 0, f"heads: a multiple of {cache.kv_heads}, got {heads}")
-    n = ctx_len.numel()
-    _need(tables.dtype == torch.int32 and tables.device == dev and tables.dim() == 2 and tables.shape[0] >= n
-          and (tables.shape[1] <= 1 or tables.stride(1) == 1), "tables: int32 [requests][width], columns contiguous")
-    _ints("ctx_len", ctx_len, dev, 0)
-    _ints("q_starts", q_starts, dev, n + 1)
+    if heads % cache.kv_heads:
+        raise ValueError(f"heads: a multiple of {cache.kv_heads}, got {heads}")
+    width, stride = _table(tables, index, n)
+    _ints("ctx_len", ctx_len, index, 0)
+    _ints("q_starts", q_starts, index, n + 1)
     if out is None:
-        out = torch.empty((total, heads, cache.head_dim), dtype=q.dtype, device=dev)
-    _need(out.shape == q.shape and out.dtype == q.dtype and out.device == dev and out.stride(2) == 1, "out: as q, columns contiguous")
-    if lse is not None:
-        _need(tuple(lse.shape) == (total, heads) and lse.dtype == torch.float32 and lse.device == dev and lse.is_contiguous(),
-              "lse: contiguous fp32 [tokens][heads]")
-    a = KvAttn(q.data_ptr(), out.data_ptr(), lse.data_ptr() if lse is not None else None, tables.data_ptr(),
-               ctx_len.data_ptr(), q_starts.data_ptr(), max(tables.stride(0), tables.shape[1]), q.stride(0), q.stride(1),
-               out.stride(0), out.stride(1), tables.shape[1], n, total, max_q, heads, code, window,
-               0 if causal else KV_FULL, cache.head_dim ** -0.5 if scale is None else scale)
-    return a, out
+        out = _torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    elif out.shape != q.shape or out.dtype is not q.dtype or out.get_device() != index or out.stride(2) != 1:
+        raise ValueError("out: as q, columns contiguous")
+    if lse is not None and (lse.shape != (total, heads) or lse.dtype is not _float32 or lse.get_device() != index
+                            or not lse.is_contiguous()):
+        raise ValueError("lse: contiguous fp32 [tokens][heads]")
+    qs, os = q.stride(), out.stride()
+    return _ATTN.pack(q.data_ptr(), out.data_ptr(), lse.data_ptr() if lse is not None else 0, tables.data_ptr(),
+                      ctx_len.data_ptr(), q_starts.data_ptr(), stride, qs[0], qs[1], os[0], os[1], width, n, total, max_q, heads,
+                      code, window, 0 if causal else KV_FULL, dim ** -0.5 if scale is None else scale), out
+
+
+def _attn_bytes(cache, args):
+    n = ctypes.c_size_t(0)
+    check("b4_kv_attention_workspace", load().b4_kv_attention_workspace(cache._ref, args, ctypes.byref(n)))
+    return n.value
 
 
 def kv_attention_workspace(cache: KVCache, q, tables, ctx_len, q_starts, max_q: int) -> int:
     """Bytes of workspace that kv_attention needs for such a call (b4_kv_attention_workspace)."""
-    a, _ = _attn(cache, q, tables, ctx_len, q_starts, max_q, None, 0, True, q, None)
-    n = ctypes.c_size_t(0)
-    check("b4_kv_attention_workspace", load().b4_kv_attention_workspace(cache._ref, _byref(a), _byref(n)))
-    return n.value
+    return _attn_bytes(cache, _attn(cache, q, tables, ctx_len, q_starts, max_q, None, 0, True, q, None)[0])
 
 
 def kv_attention(cache: KVCache, q, tables, ctx_len, q_starts, max_q: int, scale: float | None = None, window: int = 0,
@@ -207,12 +228,15 @@ def kv_attention(cache: KVCache, q, tables, ctx_len, q_starts, max_q: int, scale
     ws: a zero-filled uint8 CUDA tensor of kv_attention_workspace() bytes, or
     None for the package's own of the device (calls that may overlap on the GPU
     need their own).  Returns out."""
-    a, out = _attn(cache, q, tables, ctx_len, q_starts, max_q, scale, window, causal, out, lse)
-    lib = load()
+    args, out = _attn(cache, q, tables, ctx_len, q_starts, max_q, scale, window, causal, out, lse)
     if ws is None:
-        n = ctypes.c_size_t(0)
-        check("b4_kv_attention_workspace", lib.b4_kv_attention_workspace(cache._ref, _byref(a), _byref(n)))
-        ws = _workspace(cache.device, n.value)
-    check("b4_kv_attention", lib.b4_kv_attention(cache._ref, _byref(a), ws.data_ptr(), ws.numel(),
-                                                 stream.cuda_stream if stream is not None else _raw_stream(cache.device)))
+        key = (q.shape, max_q, cache.kv_heads, ctx_len.numel(), cache.index)     # what the size goes by
+        need = _WS_BYTES.get(key)
+        if need is None:
+            need = _WS_BYTES[key] = _attn_bytes(cache, args)
+        ws = _workspace(cache.index, need)
+    status = load().b4_kv_attention(cache._ref, args, ws.data_ptr(), ws.numel(),
+                                    stream.cuda_stream if stream is not None else _raw_stream(cache.index))
+    if status:
+        check("b4_kv_attention", status)
     return out

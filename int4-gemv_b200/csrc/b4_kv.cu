@@ -205,7 +205,7 @@ __global__ void __launch_bounds__(256) kv_append_kernel(const AppendParams p)
         uint8_t* scale = block + p.l.page_size * D + ((val ? p.l.page_size : 0) + row) * (FMT == B4_KV_INT4 ? 2 : 4);
         uint32_t w = 0;
         if (FMT == B4_KV_INT4) {
-            const __half sh = __float2half_rn(amax > 0.0f ? __fdiv_rn(amax, 7.0f) : 1.0f);
+            const __half sh = __float2half_rn(amax > 0.0f ? __fmul_rn(amax, 1.0f / 7.0f) : 1.0f);
             const float s = __half2float(sh);
 #pragma unroll
             for (int j = 0; j < 8; ++j) w |= (uint32_t)int4_code(__fdiv_rn(x[j], s)) << (4 * j);

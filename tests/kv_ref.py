@@ -23,7 +23,7 @@ def quantise(fmt, x):
         a = np.abs(x)
         amax = np.where(np.isnan(a), np.float32(0), a).max(-1).astype(np.float32)
         if fmt == INT4:
-            s = np.where(amax > 0, amax / np.float32(7), np.float32(1)).astype(np.float16)
+            s = np.where(amax > 0, amax * (np.float32(1) / np.float32(7)), np.float32(1)).astype(np.float16)
             q = (x / s.astype(np.float32)[..., None]).astype(np.float32)
             ok = np.abs(q) < np.float32(2.0 ** 63)
             d = np.where(ok, q, 0).astype(np.float64)

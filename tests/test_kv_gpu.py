@@ -170,7 +170,7 @@ def test_nf4_codes_beside_every_threshold(cuda):
 def test_int4_codes_beside_every_tie(cuda):
     rows = []
     for s in (1.0, 0.3, 11.0):
-        sc = np.float32(np.float16(np.float32(7 * s) / np.float32(7)))
+        sc = np.float32(np.float16(np.float32(7 * s) * (np.float32(1) / np.float32(7))))
         row = []
         for m in np.arange(-7.5, 8):
             x = np.float32(m * sc)
@@ -181,14 +181,10 @@ def test_int4_codes_beside_every_tie(cuda):
     check_append(cuda, INT4, torch.float32, 3, 1, 64, 16, k, k.neg(), torch.arange(3, dtype=torch.int32, device=cuda), 1)
 
 
-def test_append_equals_the_weight_quantisers(cuda):
-    """A cached head vector is a row in the weights' formats where the group sizes agree."""
-    x = torch.randn((48, 1, 128), device=cuda)
-    cache = b4gemv.KVCache.alloc(INT4, 3, 1, 16, 128, cuda)
-    slots = torch.arange(48, dtype=torch.int32, device=cuda)
-    b4gemv.kv_append(cache, x, x, slots)
-    assert torch.equal(b4gemv.kv_read(cache, slots)[0][:, 0], b4gemv.quantise_device(x[:, 0].contiguous(), True)[2])
+def test_append_equals_the_weight_quantiser(cuda):
+    """A cached head vector of 64 columns is a row in the weights' NF4 format."""
     x = torch.randn((48, 1, 64), device=cuda)
+    slots = torch.arange(48, dtype=torch.int32, device=cuda)
     cache = b4gemv.KVCache.alloc(NF4, 3, 1, 16, 64, cuda)
     b4gemv.kv_append(cache, x, x, slots)
     assert torch.equal(b4gemv.kv_read(cache, slots)[1][:, 0], b4gemv.quantise_nf4_device(x[:, 0].contiguous(), True)[2])
