@@ -7,11 +7,11 @@ namespace b4 {
 namespace {
 
 // The least columns (queries x heads that share a kv head) of a tile that hold
-// a request's queries, or 32 a tile.
+// a request's queries, or 16 a tile.
 int tile_cols(const AttnParams& p)
 {
     const long long cols = (long long)std::max(1, p.a.max_q) * p.group;
-    return cols <= 8 ? 8 : cols <= 16 ? 16 : 32;
+    return cols <= 8 ? 8 : 16;
 }
 
 int sm_count()
@@ -22,18 +22,18 @@ int sm_count()
 }
 
 // [counters][first pieces][crossing pieces], one CTA an SM
-constexpr int kMaxWarps = 8;
+constexpr int kMaxWarps = 16;
 size_t warp_ws_bytes(const AttnParams& p, int sms)
 {
     const size_t piece = (size_t)tile_cols(p) * (p.l.head_dim + 2) * 4;
     return 4096 + (size_t)sms * (kMaxWarps + 2) * piece;
 }
 
-template <typename T, int FMT, int D, int NT>
+template <typename T, int FMT, int D, int NT, int PT>
 cudaError_t launch_warp(const AttnParams& p, void* ws, cudaStream_t st)
 {
-    using C = WarpCfg<FMT, D, NT>;
-    auto fn = kv_attn_warp_kernel<T, FMT, D, NT>;
+    using C = WarpCfg<FMT, D, NT, PT>;
+    auto fn = kv_attn_warp_kernel<T, FMT, D, NT, PT>;
     const cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
     if (e != cudaSuccess) return e;
     const int sms = sm_count();
@@ -41,14 +41,15 @@ cudaError_t launch_warp(const AttnParams& p, void* ws, cudaStream_t st)
     w.count = static_cast<int*>(ws);
     w.first = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + 4096);
     w.cross = w.first + (size_t)sms * C::kWarps * C::kPiece;
-    return kv_launch(fn, dim3((unsigned)sms), C::kWarps * 32, C::kSmem, st, p, w);
+    return kv_launch(fn, dim3((unsigned)sms), C::kThreads, C::kSmem, st, p, w);
 }
 
 template <typename T, int FMT, int D>
 cudaError_t launch_cols(const AttnParams& p, void* ws, cudaStream_t st)
 {
-    const int cols = tile_cols(p);
-    return cols == 8 ? launch_warp<T, FMT, D, 1>(p, ws, st) : cols == 16 ? launch_warp<T, FMT, D, 2>(p, ws, st) : launch_warp<T, FMT, D, 4>(p, ws, st);
+    const bool one = tile_cols(p) == 8;
+    if (p.l.page_size == 16) return one ? launch_warp<T, FMT, D, 1, 16>(p, ws, st) : launch_warp<T, FMT, D, 2, 16>(p, ws, st);
+    return one ? launch_warp<T, FMT, D, 1, 32>(p, ws, st) : launch_warp<T, FMT, D, 2, 32>(p, ws, st);
 }
 
 template <typename T>
@@ -77,17 +78,6 @@ int attn_params(const b4_kv_cache* cache, const b4_kv_attn* a, AttnParams* p)
 }  // namespace b4
 
 using namespace b4;
-
-int b4::kv_attn_device_error(int clear)
-{
-    int v = 0;
-    if (cudaMemcpyFromSymbol(&v, g_device_error, sizeof(v)) != cudaSuccess) return -1;
-    if (clear && v) {
-        const int z = 0;
-        if (cudaMemcpyToSymbol(g_device_error, &z, sizeof(z)) != cudaSuccess) return -1;
-    }
-    return v;
-}
 
 extern "C" {
 

@@ -2,6 +2,8 @@
 // parameters, a request's extent, and the fp16 operands made from 4-bit codes.
 #pragma once
 
+#include <type_traits>
+
 #include "b4_kv.cuh"
 
 namespace b4 {
@@ -13,7 +15,7 @@ struct AttnParams {
     int group;              // query heads that share a kv head
 };
 
-constexpr int kChunk = 64;  // tokens that a warp takes at a time; a multiple of every page size
+constexpr int kChunk = 32;  // tokens that a warp takes at a time: one page of 32, two of 16, half of one of 64
 
 // What a launch needs of request r: its queries' first row and number, its tokens
 // (those that the table can hold), and the chunks that any of its queries sees.
@@ -21,17 +23,24 @@ struct AttnReq {
     int q0, n, ctx, chunk0, chunks;
 };
 
+__device__ __forceinline__ int attn_first_chunk(const b4_kv_attn& a, int ctx, int n)
+{
+    return a.window > 0 ? max(0, ctx - n + 1 - a.window) / kChunk : 0;
+}
+
+__device__ __forceinline__ AttnReq attn_extent(const b4_kv_attn& a, int q0, int n, int ctx)
+{
+    AttnReq q = {q0, n, ctx, attn_first_chunk(a, ctx, n), 1};
+    q.chunks = max(1, (ctx + kChunk - 1) / kChunk - q.chunk0);      // one even where nothing is seen: zeros are written
+    return q;
+}
+
 __device__ __forceinline__ AttnReq attn_request(const AttnParams& p, int r)
 {
     const b4_kv_attn& a = p.a;
-    AttnReq q;
-    q.q0 = max(0, min(__ldg(a.q_starts + r), a.total_q));
-    q.n = max(0, min(__ldg(a.q_starts + r + 1), a.total_q) - q.q0);
-    q.ctx = max(0, min(__ldg(a.ctx_len + r), a.table_width * p.l.page_size));
-    const int begin = a.window > 0 ? max(0, q.ctx - q.n + 1 - a.window) : 0;
-    q.chunk0 = begin / kChunk;
-    q.chunks = max(1, (q.ctx + kChunk - 1) / kChunk - q.chunk0);   // one even where nothing is seen: zeros are written
-    return q;
+    const int q0 = __ldg(a.q_starts + r), q1 = __ldg(a.q_starts + r + 1), ctx = __ldg(a.ctx_len + r);
+    const int from = max(0, min(q0, a.total_q));
+    return attn_extent(a, from, max(0, min(q1, a.total_q) - from), max(0, min(ctx, a.table_width * p.l.page_size)));
 }
 
 __device__ __forceinline__ float fast_exp2(float x)
@@ -48,6 +57,32 @@ __device__ __forceinline__ float fast_log2(float x)
     return y;
 }
 
+// a / b, a >= 0, b > 0; in 32 bits where both fit
+__device__ __forceinline__ long long div64(long long a, long long b)
+{
+    return ((a | b) >> 32) == 0 ? (long long)((uint32_t)a / (uint32_t)b) : a / b;
+}
+
+__device__ __forceinline__ uint32_t lds32(uint32_t at)
+{
+    uint32_t v;
+    asm("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(at));
+    return v;
+}
+
+__device__ __forceinline__ uint2 lds64(uint32_t at)
+{
+    uint2 v;
+    asm("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(at));
+    return v;
+}
+
+// 16 bytes from global memory to a shared address, past L1
+__device__ __forceinline__ void copy_async16(uint32_t dst, const void* src)
+{
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 // The NF4 levels as fp16 operands.  fp16 has 11 bits, the levels 24: rounded as
@@ -59,6 +94,14 @@ constexpr float kNf4Up = 1.67766535282135f;
 __device__ __forceinline__ uint32_t nf4_pair(uint32_t byte)
 {
     const __half lo = __float2half_rn(c_nf4_table[byte & 15] * kNf4Up), hi = __float2half_rn(c_nf4_table[byte >> 4] * kNf4Up);
+    return (uint32_t)__half_as_ushort(lo) | ((uint32_t)__half_as_ushort(hi) << 16);
+}
+
+// What the fp16 parts of nf4_pair leave of the levels: with it they are exact to 2^-22.
+__device__ __forceinline__ uint32_t nf4_pair_low(uint32_t byte)
+{
+    const float a = c_nf4_table[byte & 15] * kNf4Up, b = c_nf4_table[byte >> 4] * kNf4Up;
+    const __half lo = __float2half_rn(a - __half2float(__float2half_rn(a))), hi = __float2half_rn(b - __half2float(__float2half_rn(b)));
     return (uint32_t)__half_as_ushort(lo) | ((uint32_t)__half_as_ushort(hi) << 16);
 }
 
@@ -82,7 +125,41 @@ __device__ __forceinline__ uint32_t pack_half2(float lo, float hi)
     return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// 2^-e as a float, e an exponent field's offset: exact, for |e| <= 126
+// 2^e, |e| <= 126
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
+
+// W words of 8 query columns as fp16, negated where `negate`; the four lanes of a
+// row (lane & ~3) hold it together.  Returns what a product with them lacks: 1, or
+// for bf16 the power of two that was taken out of the row.
+template <typename T, int W>
+__device__ __forceinline__ float query_operand(uint4 (&v)[W], bool negate)
+{
+    float factor = 1.0f;
+    const uint32_t sign = negate ? 0x80008000u : 0u;
+    if (std::is_same<T, __nv_bfloat16>::value) {
+        uint32_t top = 0;
+#pragma unroll
+        for (int i = 0; i < W; ++i) {
+            const uint32_t x[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) top = max(top, max(x[j] << 16 & 0x7fffffffu, x[j] & 0x7fff0000u));
+        }
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const int e = min(max((int)(top >> 23) - 127, -110), 126);
+        const float up = pow2(10 - e);
+        factor = pow2(e - 10);
+#pragma unroll
+        for (int i = 0; i < W; ++i) {
+            uint32_t* x = reinterpret_cast<uint32_t*>(&v[i]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                x[j] = pack_half2(__uint_as_float(x[j] << 16) * up, __uint_as_float(x[j] & 0xffff0000u) * up);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < W; ++i) v[i] = make_uint4(v[i].x ^ sign, v[i].y ^ sign, v[i].z ^ sign, v[i].w ^ sign);
+    return factor;
+}
 
 }  // namespace b4

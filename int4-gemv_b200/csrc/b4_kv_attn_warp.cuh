@@ -9,12 +9,16 @@
 // 8-wide side is the queries and none of it is padding for groups of 8.  A token's
 // scale does not depend on the column, so the key's scale multiplies S and the
 // value's scale P, in fp32; the operands hold the bare levels (INT4: exact
-// integers; NF4: kNf4Up).  Softmax's maximum and sum run along the tokens, in
-// fp32, private to a warp; P goes to fp16 (its rounding is of the size of the
-// output's own), relative to the running maximum of the weights and a running
-// power of two that bounds the value scales, so small scales lose nothing.
+// integers; NF4: keys rounded to fp16 (kNf4Up), values as fp16 high and low parts
+// in two products, since an output over many tokens is far smaller than its
+// terms, and a level's rounding does not average out as the weights' does).
+// Softmax's maximum and sum run along the tokens, in fp32, private to a warp;
+// the maximum moves only when a score passes it by 2^8, which the weights'
+// range allows.  P goes to fp16 (its rounding is of the size of the output's own),
+// relative to that maximum and to a running power of two that bounds the value
+// scales, so small scales lose nothing.
 //
-// Split.  The (request, kv head, column tile, 64-token chunk) units of the whole
+// Split.  The (request, kv head, column tile, 32-token chunk) units of the whole
 // call form one sequence; every CTA gets an equal run of it, every warp of a CTA
 // an equal run of the CTA's, whatever the requests' lengths.  A segment (request,
 // head, tile) inside one warp's run is written by the warp; others leave a piece
@@ -23,40 +27,38 @@
 // order: the same bits every time, one launch, no wait between CTAs.
 //
 // Feed.  Each warp brings its own chunks into its own ring of shared memory with
-// bulk copies (a copy a page: a head's part of a page is one block), and reads page
-// ids one unit ahead of the copies, so a warp never waits for another.
+// 16-byte asynchronous copies, two or three chunks ahead, and reads page ids 32 at a
+// time, so a warp waits for nothing but its own data.  (Bulk copies measured slower
+// here: a warp that issues one spends some 35 instructions on it, and half a page
+// of 64 takes four.)
 #pragma once
 
 #include <type_traits>
 
 #include "b4_kv_attn.cuh"
-#include "b4_tma.cuh"
 
 namespace b4 {
 
-constexpr int kAttnStages = 2;
-
-template <int FMT, int D, int NT>
+// PT: tokens of a page in shared memory, 16 or 32 (half a page of 64 lies there as a page of 32)
+template <int FMT, int D, int NT, int PT>
 struct WarpCfg {
-    static constexpr int kWarps = FMT == B4_KV_NF4 && NT > 1 ? 6 : 8;  // what shared memory holds
+    static constexpr int kWarps = NT == 1 ? 16 : 12;                   // 128 and 168 registers a thread
+    static constexpr int kThreads = 32 * kWarps, kScan = 256;          // kScan threads add up the requests
     static constexpr int kRow = D / 2;                                 // bytes of a token's codes
     static constexpr int kScale = FMT == B4_KV_INT4 ? 2 : 4;
     static constexpr int kStage = 2 * kChunk * (kRow + kScale);
+    static constexpr int kStages = FMT == B4_KV_NF4 ? (D == 128 ? 2 : 3) : D == 128 && NT == 1 ? 3 : 4;
+    static constexpr int kPages = kChunk / PT, kBlock = 2 * PT * (kRow + kScale);
     static constexpr int kCols = 8 * NT;
     static constexpr int kPiece = kCols * (D + 2);                     // floats: output, maxima, sums
-    static constexpr int kTable = FMT == B4_KV_NF4 ? 65536 : 0;        // 256 rows of 32 copies, 256 bytes apart
-    static constexpr int kQ = NT == 1 ? 0 : kCols * D * 2;             // the queries' operands, of one warp
-    static constexpr int kRing = kWarps * kAttnStages * kStage;
-    static constexpr int kSmem = kTable + kRing + kWarps * kQ;
-    static_assert(kAttnStages * kStage >= kPiece * 4, "a warp's last piece goes into its ring");
+    static constexpr int kRing = kStages * kStage;                     // of one warp
+    // NF4: 256 rows of 32 copies of 8 bytes at shared address 65536, so that one byte permutation makes a lookup's
+    // address; the first warps' rings lie below it
+    static constexpr int kTable = 65536, kBelow = FMT == B4_KV_NF4 ? (NT == 1 ? 6 : 5) : kWarps;
+    static constexpr int kSmem = FMT == B4_KV_NF4 ? 2 * kTable + (kWarps - kBelow) * kRing : kWarps * kRing;
+    static_assert(kRing >= kPiece * 4, "a warp's last piece goes into its ring");
+    static_assert(FMT != B4_KV_NF4 || kBelow * kRing <= kTable - 8192 - 4096 * NT, "below the table: 1 KB of the system, the static part");
 };
-
-// a unit as the warp that reads it sees it
-struct __align__(16) AttnUnit {
-    int q0, n, ctx, head;      // the request's queries and tokens, the kv head
-    int tile, token, flags, pages;
-};
-constexpr int kUnitFirst = 1, kUnitLast = 2;   // of its segment
 
 struct WarpPiece {
     long long s0, s1;          // the segment's units
@@ -70,51 +72,51 @@ struct WarpWs {                // the workspace: counters, then pieces that othe
     float* cross;              // [grid][2] a CTA's part of a segment that began before it / goes on after it
 };
 
-// Walks the units of a run in order.
-struct UnitWalk {
-    AttnReq q;
-    int r, seg, chunk, tiles;
-};
+// A maximum that no score has set yet: finite, so that differences with it are.
+constexpr float kNoMax = -1e30f;
 
-template <typename T, int FMT, int D, int NT>
-__global__ void __launch_bounds__(WarpCfg<FMT, D, NT>::kWarps * 32, 1) kv_attn_warp_kernel(const AttnParams p, const WarpWs ws)
+template <typename T, int FMT, int D, int NT, int PT>
+__global__ void __launch_bounds__(WarpCfg<FMT, D, NT, PT>::kThreads, 1) kv_attn_warp_kernel(const AttnParams p, const WarpWs ws)
 {
-    using C = WarpCfg<FMT, D, NT>;
-    constexpr int kAttnWarps = C::kWarps, kThreads = 32 * kAttnWarps;
+    using C = WarpCfg<FMT, D, NT, PT>;
+    constexpr int kWarps = C::kWarps, kThreads = C::kThreads, kStages = C::kStages, kScan = C::kScan;
     extern __shared__ __align__(1024) uint8_t attn_smem[];
-    __shared__ uint64_t full[kAttnWarps][kAttnStages];
-    __shared__ AttnUnit units[kAttnWarps][kAttnStages];
-    __shared__ WarpPiece pieces[kAttnWarps][2];
-    __shared__ long long scan[kAttnWarps * 32 + 1], warp_sum[kAttnWarps];
+    __shared__ WarpPiece pieces[kWarps][2];
+    __shared__ long long scan[kScan + 1], warp_sum[kWarps];
+    __shared__ int4 cached[kScan];
+    __shared__ float2 joined[C::kCols][32];
+    __shared__ float factor[C::kCols][32];
     __shared__ int last_cta[2];
 
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int g = lane >> 2, t = lane & 3;
     const b4_kv_attn& a = p.a;
-    uint8_t* ring = attn_smem + C::kTable + warp * kAttnStages * C::kStage;
-    uint8_t* table = attn_smem;
-    if (lane < kAttnStages) mbar_init(&full[warp][lane], 1);
-    if (lane < 2) pieces[warp][lane].valid = 0;
+    const uint32_t smem_at = (uint32_t)__cvta_generic_to_shared(attn_smem);
+    auto ring_of = [&](int w) { return attn_smem + (w < C::kBelow ? w * C::kRing : 2 * C::kTable - smem_at + (w - C::kBelow) * C::kRing); };
+    if (tid < 2 * kWarps) pieces[tid >> 1][tid & 1].valid = 0;
     if (FMT == B4_KV_NF4) {
-        for (int b = tid; b < 256; b += kThreads) {
-            const uint32_t v = nf4_pair(b);
-            uint4* row = reinterpret_cast<uint4*>(table + b * 256);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) row[(i + b) & 7] = make_uint4(v, v, v, v);
+        // row b: 32 copies of (high, low) of byte b's two levels, the two swapped in the upper 16 copies: there the
+        // high parts alone (keys) lie in the odd banks, and the two products of the values add up to the same
+        for (int i = tid; i < 256 * 16; i += kThreads) {
+            const uint32_t b = i >> 4, hi = nf4_pair(b), lo = nf4_pair_low(b);
+            reinterpret_cast<uint4*>(attn_smem + C::kTable - smem_at)[i] = (i & 15) < 8 ? make_uint4(hi, lo, hi, lo) : make_uint4(lo, hi, lo, hi);
         }
     }
-    fence_mbar_init();
     kv_begin();
 
-    // ---- the call's units, and this warp's run of them ----
+    // ---- the call's units, and each warp's run of them ----
     auto tiles_of = [&](const AttnReq& q) { return (q.n * p.group + C::kCols - 1) / C::kCols; };
     auto units_of = [&](const AttnReq& q) { return (long long)p.l.kv_heads * tiles_of(q) * q.chunks; };
-    const int per = (a.n_req + kAttnWarps * 32 - 1) / (kAttnWarps * 32);
+    const int per = (a.n_req + kScan - 1) / kScan;
     {
         long long sum = 0;
-        for (int i = 0; i < per; ++i) {
-            const int r = tid * per + i;
-            if (r < a.n_req) sum += units_of(attn_request(p, r));
+        if (tid < kScan) {
+            for (int i = 0; i < per; ++i) {
+                const int r = tid * per + i;
+                if (r >= a.n_req) break;
+                const AttnReq q = attn_request(p, r);
+                if (per == 1) cached[r] = make_int4(q.q0, q.n, q.ctx, 0);
+                sum += units_of(q);
+            }
         }
         long long inc = sum;
 #pragma unroll
@@ -126,193 +128,121 @@ __global__ void __launch_bounds__(WarpCfg<FMT, D, NT>::kWarps * 32, 1) kv_attn_w
         __syncthreads();
         long long base = 0;
 #pragma unroll
-        for (int w = 0; w < kAttnWarps; ++w)
+        for (int w = 0; w < kScan / 32; ++w)
             if (w < warp) base += warp_sum[w];
-        scan[tid + 1] = base + inc;
+        if (tid < kScan) scan[tid + 1] = base + inc;
         if (tid == 0) scan[0] = 0;
         __syncthreads();
     }
-    const long long total = scan[kAttnWarps * 32];
+    auto request = [&](int r) {                // from shared memory where all fit there
+        if (per > 1) return attn_request(p, r);
+        const int4 x = cached[r];
+        return attn_extent(a, x.x, x.y, x.z);
+    };
+    const long long total = scan[kScan];
     if (total == 0) return;
-    // few units: four a CTA at least, so that fewer pieces cross CTAs
-    const long long ctas = min((long long)gridDim.x, (total + 3) / 4);
+    // Equal runs; few units: one a warp, so that fewer pieces cross CTAs.  Where a CTA's run is short, a segment's end
+    // nearby is worth more than equal runs (a join across CTAs costs some 2 us, a unit more a warp less): the run's ends
+    // move to it.
+    const int ctas = (int)min((long long)gridDim.x, (total + kWarps - 1) / kWarps);
     const int cta = blockIdx.x;
     if (cta >= ctas) return;
-    const long long c0 = cta * total / ctas, c1 = (cta + 1) * total / ctas;
-    const long long v0 = c0 + warp * (c1 - c0) / kAttnWarps, v1 = c0 + (warp + 1) * (c1 - c0) / kAttnWarps;
-
-    if (v0 < v1) {
-        // ---- walk: find the run's first unit, then step ----
-        UnitWalk w;
-        long long at;                          // the current request's first unit
-        {
-            int lo = 0, hi = kAttnWarps * 32;
-            while (hi - lo > 1) {
-                const int mid = (lo + hi) >> 1;
-                if (scan[mid] <= v0) lo = mid;
-                else hi = mid;
-            }
-            w.r = lo * per;
-            at = scan[lo];
-            for (;;) {
-                w.q = attn_request(p, w.r);
-                const long long u = units_of(w.q);
-                if (v0 < at + u) break;
-                at += u;
-                ++w.r;
-            }
-            w.tiles = tiles_of(w.q);
-            const long long in = v0 - at;
-            w.seg = (int)(in / w.q.chunks);
-            w.chunk = (int)(in - (long long)w.seg * w.q.chunks);
+    const long long share = div64(total, ctas), rest = total - share * ctas;
+    const int near = share <= 2 * kWarps ? kWarps : 0;
+    auto owner = [&](long long u) {            // the CTA that the unit is in before any end moves
+        return (int)(u < rest * (share + 1) ? div64(u, share + 1) : rest + div64(u - rest * (share + 1), share));
+    };
+    // the request that unit u is in, and that request's first unit
+    auto find = [&](long long u, long long& at) {
+        constexpr int kPer = kScan / 32;
+        unsigned m = __ballot_sync(0xffffffffu, scan[lane * kPer] <= u);
+        const int block = 31 - __clz(m);
+        m = __ballot_sync(0xffffffffu, lane < kPer && scan[block * kPer + lane] <= u);
+        const int i = block * kPer + 31 - __clz(m);
+        int r = i * per;
+        at = scan[i];
+        for (; r < a.n_req - 1; ++r) {
+            const long long n = units_of(request(r));
+            if (u < at + n) break;
+            at += n;
         }
-        const int pages_per = kChunk >> p.l.page_shift;
-        const uint64_t policy = evict_first_policy();
-        auto page_id = [&]() -> int {          // of this lane's page in the walk's unit, -1 where there is none
-            const int token = (w.q.chunk0 + w.chunk) * kChunk + (lane << p.l.page_shift);
-            if (lane >= pages_per || token >= w.q.ctx) return -1;
-            return __ldg(a.tables + (long long)w.r * a.table_stride + (token >> p.l.page_shift));
-        };
-        auto step = [&]() {
-            if (++w.chunk < w.q.chunks) return;
-            w.chunk = 0;
-            if (++w.seg < p.l.kv_heads * w.tiles) return;
-            w.seg = 0;
-            do {
-                w.q = attn_request(p, ++w.r);
-            } while (w.q.n == 0);
-            w.tiles = tiles_of(w.q);
-        };
-        auto issue = [&](int stage, int id) {  // the walk's unit into a stage
-            const bool there = (unsigned)id < (unsigned)p.l.n_pages;
-            const unsigned mask = __ballot_sync(0xffffffffu, there);
-            const int head = w.seg / w.tiles;
-            if (lane == 0) {
-                AttnUnit u;
-                u.q0 = w.q.q0;
-                u.n = w.q.n;
-                u.ctx = w.q.ctx;
-                u.head = head;
-                u.tile = w.seg - head * w.tiles;
-                u.token = (w.q.chunk0 + w.chunk) * kChunk;
-                u.flags = (w.chunk == 0 ? kUnitFirst : 0) | (w.chunk == w.q.chunks - 1 ? kUnitLast : 0);
-                u.pages = (int)mask;
-                units[warp][stage] = u;
-                fence_proxy_async();
-                mbar_arrive_expect_tx(&full[warp][stage], (uint32_t)(__popc(mask) * p.l.block));
-            }
-            __syncwarp();
-            if (there)
-                bulk_g2s(ring + stage * C::kStage + lane * (int)p.l.block, p.blocks + ((long long)id * p.l.kv_heads + head) * p.l.block,
-                         (uint32_t)p.l.block, &full[warp][stage], policy);
-        };
+        return r;
+    };
+    auto end_of = [&](int c) -> long long {    // where CTA c's run begins
+        const long long u = c * share + min((long long)c, rest);
+        if (near == 0 || u <= 0 || u >= total) return u;
+        long long at;
+        const int chunks = request(find(u, at)).chunks;
+        const long long s0 = at + div64(u - at, chunks) * chunks;
+        return u - s0 <= near ? s0 : s0 + chunks - u <= near ? s0 + chunks : u;
+    };
+    const long long c0 = end_of(cta), c1 = end_of(cta + 1);
+    auto run_start = [&](int w) {
+        const int n = (int)(c1 - c0);
+        return c0 + w * (n / kWarps) + min(w, n % kWarps);
+    };
 
-        const int count = (int)(v1 - v0);
-        long long seg_unit = v0 - w.chunk;     // the segment's first unit
-        int seg_chunks = w.q.chunks;
-        int ids[kAttnStages + 1], produced = 0;
-        // the first stages' page ids together, one round trip
-        UnitWalk start = w;
-#pragma unroll
-        for (int s = 0; s <= kAttnStages; ++s) {
-            ids[s] = -1;
-            if (s < count) {
-                if (s > 0) step();
-                ids[s] = page_id();
-            }
-        }
-        w = start;
-#pragma unroll
-        for (int s = 0; s < kAttnStages; ++s) {
-            if (s >= count) break;
-            issue(s, ids[s]);
-            ++produced;
-            if (s + 1 < count) step();
-        }
-        int next_id = ids[kAttnStages];
-
-        // ---- per segment: queries, running statistics, output ----
-        float o[NT][D / 8 / 2][4];             // m-tile mt: columns 2t, 2t + 1 of d = g * (D / 8) + 2 mt, and of d + 1
-        float mx[NT][2], sum[NT][2], qf[NT][2];
-        int lim[NT][2];                        // keys that a column sees: below lim, at or above lim - window
-        uint32_t qb[NT == 1 ? D / 8 : 1];
-        uint4* qs = reinterpret_cast<uint4*>(attn_smem + C::kTable + C::kRing + warp * C::kQ);
-        int vexp = -126;
+    if (const long long v0 = run_start(warp), v1 = run_start(warp + 1); v0 < v1) {
+        // ---- a warp's run ----
+        const int g = lane >> 2, t = lane & 3;
+        uint8_t* ring = ring_of(warp);
         constexpr int W = D / 32;              // packed words of a token's codes that a lane of the key operand holds
-        uint4 raw[NT == 1 ? W : 1];
+        constexpr int VW = D / 64;             // ... of the value operand
+        // this lane's places in a stage: its key and value rows of the chunk's two 16-token tiles, its token's scales.
+        // Row g of a tile's eight is token gr: the pairs 2, 3 and 6, 7 are swapped, so that the four lanes t of a value
+        // read (tokens gr(2t)) see rows of both parities and with them all banks
+        const int gr = g ^ (g >> 1 & 1);
+        const int k_at = gr * C::kRow + t * (W * 4), v_at = PT * C::kRow + (2 * t + (t & 1)) * C::kRow + g * (VW * 4);
+        constexpr int tile1 = PT == 16 ? C::kBlock : 16 * C::kRow;
+        const int v_other = t & 1 ? -C::kRow : C::kRow;
+        const int s_at = lane / PT * C::kBlock + PT * D + lane % PT * C::kScale;
+        const uint32_t t_key = C::kTable + lane * 8 + (lane >> 4) * 4, t_val = C::kTable + lane * 8;
 
-        auto col_row = [&](const AttnUnit& u, int col, int& token, int& head) -> bool {
+        float o[NT][D / 16][4];                // m-tile mt: columns 2t, 2t + 1 of d = g * (D / 8) + 2 mt, and of d + 1
+        float mx[NT][2], sum[NT][2], qf[NT][2];
+        uint32_t qb[NT][D / 8];
+        int lim[NT][2];                        // keys that a column sees: below lim, at or above lim - window
+        int vexp;
+        struct { int q0, n, ctx, head, tile, token; } u = {};   // the segment; a chunk's first token
+
+        auto col_row = [&](int col, int& token, int& head) -> bool {
             const int c = u.tile * C::kCols + col;
             token = c / p.group;
             head = u.head * p.group + (c - token * p.group);
             return c < u.n * p.group;
         };
-        auto q_words = [&](const AttnUnit& u, int nt, uint4 (&v)[W]) {
+        // a segment's queries as the right operand, in the order of the decoded codes.  A negative factor of the scores
+        // goes into the queries, so that a larger product is a larger score.
+        auto load_queries = [&](int nt, uint4 (&v)[W]) {
             int token, head;
-            const bool in = col_row(u, nt * 8 + g, token, head);
+            const bool in = col_row(nt * 8 + g, token, head);
             const uint4* src = reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + (u.q0 + token) * a.q_stride_token +
                                                               head * a.q_stride_head + t * (D / 4));
 #pragma unroll
             for (int i = 0; i < W; ++i) v[i] = in ? __ldg(src + i) : make_uint4(0, 0, 0, 0);
         };
-        // the operand's pairs in the order of the decoded codes, fp16; bf16 rows times a power of two that
-        // brings their largest to [2^10, 2^11), so that fp16's range holds them (its 11 bits hold bf16's 8)
-        auto q_operand = [&](uint4 (&v)[W], float& factor) {
-            factor = 1.0f;
-            if (std::is_same<T, __nv_bfloat16>::value) {
-                uint32_t top = 0;
-#pragma unroll
-                for (int i = 0; i < W; ++i) {
-                    const uint32_t x[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) top = max(top, max(x[j] << 16 & 0x7fffffffu, x[j] & 0x7fff0000u));
-                }
-                top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-                top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                const int e = min(max((int)(top >> 23) - 127, -110), 126);
-                const float up = pow2(10 - e);
-                factor = pow2(e - 10 < -126 ? -126 : e - 10);
-#pragma unroll
-                for (int i = 0; i < W; ++i) {
-                    uint32_t* x = reinterpret_cast<uint32_t*>(&v[i]);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        x[j] = pack_half2(__uint_as_float(x[j] << 16) * up, __uint_as_float(x[j] & 0xffff0000u) * up);
-                }
-            }
-            if (FMT == B4_KV_INT4) {
-#pragma unroll
-                for (int i = 0; i < W; ++i) v[i] = int4_pair_order(v[i]);
-            }
-        };
-        auto begin_segment = [&](const AttnUnit& u) {
+        auto begin_segment = [&](uint4 (&queries)[NT][W]) {
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
-                float factor;
-                if (NT == 1) {
-                    q_operand(*reinterpret_cast<uint4(*)[W]>(raw), factor);
+                int token, head;
+                uint4(&v)[W] = queries[nt];
+                const float factor = query_operand<T, W>(v, a.scale < 0.0f);
 #pragma unroll
-                    for (int i = 0; i < W; ++i) {
-                        qb[4 * i] = raw[i].x;
-                        qb[4 * i + 1] = raw[i].y;
-                        qb[4 * i + 2] = raw[i].z;
-                        qb[4 * i + 3] = raw[i].w;
-                    }
-                } else {
-                    uint4 v[W];
-                    q_words(u, nt, v);
-                    q_operand(v, factor);
-#pragma unroll
-                    for (int i = 0; i < W; ++i) qs[(nt * W + i) * 32 + lane] = v[i];
+                for (int i = 0; i < W; ++i) {
+                    const uint4 x = FMT == B4_KV_INT4 ? int4_pair_order(v[i]) : v[i];
+                    qb[nt][4 * i] = x.x;
+                    qb[nt][4 * i + 1] = x.y;
+                    qb[nt][4 * i + 2] = x.z;
+                    qb[nt][4 * i + 3] = x.w;
                 }
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
-                    qf[nt][j] = __shfl_sync(0xffffffffu, factor, (2 * t + j) * 4) * (a.scale * kLog2e) *
-                                (FMT == B4_KV_NF4 ? 1.0f / kNf4Up : 1.0f);
-                    int token, head;
-                    col_row(u, nt * 8 + 2 * t + j, token, head);
+                    // not 0, so that a masked score's -infinity stays one
+                    qf[nt][j] = fmaxf(__shfl_sync(0xffffffffu, factor, (2 * t + j) * 4) * (fabsf(a.scale) * kLog2e) *
+                                          (FMT == B4_KV_NF4 ? 1.0f / kNf4Up : 1.0f), 1e-30f);
+                    col_row(nt * 8 + 2 * t + j, token, head);
                     lim[nt][j] = a.flags & B4_KV_FULL ? u.ctx : min(u.ctx, u.ctx - u.n + token + 1);
-                    mx[nt][j] = -INFINITY;
+                    mx[nt][j] = kNoMax;
                     sum[nt][j] = 0.0f;
                 }
 #pragma unroll
@@ -320,414 +250,501 @@ __global__ void __launch_bounds__(WarpCfg<FMT, D, NT>::kWarps * 32, 1) kv_attn_w
 #pragma unroll
                     for (int j = 0; j < 4; ++j) o[nt][mt][j] = 0.0f;
             }
-            if (NT > 1) __syncwarp();
             vexp = -126;
         };
 
-        int stage = 0, phase = 0;
-        bool whole = false;                    // the current segment's first unit is in this run
-        AttnUnit u = units[warp][0];
-        if (NT == 1) q_words(u, 0, *reinterpret_cast<uint4(*)[W]>(raw));
-
-        for (int i = 0; i < count; ++i) {
-            const bool fresh = i == 0 || (u.flags & kUnitFirst);
-            if (fresh) {
-                begin_segment(u);
-                whole = u.flags & kUnitFirst;
-            }
-            AttnUnit nu;
-            if (i + 1 < count) {               // the next unit's queries are asked for before this one is computed
-                nu = units[warp][stage ^ 1];
-                if (NT == 1 && (nu.flags & kUnitFirst)) q_words(nu, 0, *reinterpret_cast<uint4(*)[W]>(raw));
-            }
-            mbar_wait_bounded(&full[warp][stage], phase);
-            const uint8_t* buf = ring + stage * C::kStage;
-            // every key seen by every column: no masks
-            const int seen = a.flags & B4_KV_FULL ? u.ctx : u.ctx - u.n + 1 + u.tile * C::kCols / p.group;
-            // the keys that some column of the tile sees
-            const int tile_end = a.flags & B4_KV_FULL ? u.ctx : min(u.ctx, u.ctx - u.n + 1 + (u.tile * C::kCols + C::kCols - 1) / p.group);
-            const int tile_begin = a.window > 0 ? u.ctx - u.n + 1 + u.tile * C::kCols / p.group - a.window : 0;
-            const bool masked = u.token + kChunk > min(seen, u.ctx) || u.pages != (1 << pages_per) - 1 ||
-                                (a.window > 0 && u.token < u.ctx - a.window);
-            constexpr int G = NT == 1 ? 4 : NT == 2 ? 2 : 1;       // 16-token tiles between two softmax steps
+        // 32 tokens; `masked` where some column does not see all of them
+        auto compute = [&](const uint8_t* buf, int there, bool masked) {
+            // the token of this lane: its scales
+            const uint8_t* sp = buf + s_at;
+            const float ks = FMT == B4_KV_INT4 ? __half2float(*reinterpret_cast<const __half*>(sp)) : *reinterpret_cast<const float*>(sp);
+            float vs = FMT == B4_KV_INT4 ? __half2float(*reinterpret_cast<const __half*>(sp + PT * C::kScale))
+                                         : *reinterpret_cast<const float*>(sp + PT * C::kScale);
+            float s[2][NT][4];
 #pragma unroll
-            for (int s0 = 0; s0 < 4; s0 += G) {
-                float s[G][NT][4], vs[G][2];
-                float top[NT][2], vtop = 0.0f;
+            for (int st = 0; st < 2; ++st) {
+                const uint8_t* kp = buf + k_at + st * tile1;
+                uint32_t k0[W], k1[W];
+                if (D == 128) {
+                    const uint4 x = *reinterpret_cast<const uint4*>(kp), y = *reinterpret_cast<const uint4*>(kp + 8 * C::kRow);
+                    k0[0] = x.x; k0[1] = x.y; k0[W - 2] = x.z; k0[W - 1] = x.w;
+                    k1[0] = y.x; k1[1] = y.y; k1[W - 2] = y.z; k1[W - 1] = y.w;
+                } else {
+                    const uint2 x = *reinterpret_cast<const uint2*>(kp), y = *reinterpret_cast<const uint2*>(kp + 8 * C::kRow);
+                    k0[0] = x.x; k0[1] = x.y;
+                    k1[0] = y.x; k1[1] = y.y;
+                }
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) top[nt][0] = top[nt][1] = -INFINITY;
+                for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                for (int st = 0; st < G; ++st) {
-                    const int tok = (s0 + st) * 16, blk = tok >> p.l.page_shift, row = tok & (p.l.page_size - 1);
-                    const uint8_t* bp = buf + blk * (int)p.l.block;
-                    const uint8_t* kp = bp + row * C::kRow;
-                    const uint8_t* sp = bp + p.l.page_size * D + (row + g) * C::kScale;
-                    uint32_t k0[W], k1[W];
-                    if (D == 128) {
-                        const uint4 x = *reinterpret_cast<const uint4*>(kp + g * C::kRow + t * 16);
-                        const uint4 y = *reinterpret_cast<const uint4*>(kp + (g + 8) * C::kRow + t * 16);
-                        k0[0] = x.x; k0[1] = x.y; k0[W - 2] = x.z; k0[W - 1] = x.w;
-                        k1[0] = y.x; k1[1] = y.y; k1[W - 2] = y.z; k1[W - 1] = y.w;
+                    for (int j = 0; j < 4; ++j) s[st][nt][j] = 0.0f;
+#pragma unroll
+                for (int i = 0; i < W; ++i) {
+                    uint32_t x[4], y[4];
+                    if (FMT == B4_KV_INT4) {
+                        int4_word_to_half2(k0[i], x);
+                        int4_word_to_half2(k1[i], y);
                     } else {
-                        const uint2 x = *reinterpret_cast<const uint2*>(kp + g * C::kRow + t * 8);
-                        const uint2 y = *reinterpret_cast<const uint2*>(kp + (g + 8) * C::kRow + t * 8);
-                        k0[0] = x.x; k0[1] = x.y;
-                        k1[0] = y.x; k1[1] = y.y;
-                    }
-                    float ks[2];
 #pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        const uint8_t* q = sp + 8 * j * C::kScale;
-                        ks[j] = FMT == B4_KV_INT4 ? __half2float(*reinterpret_cast<const __half*>(q)) : *reinterpret_cast<const float*>(q);
-                        q += p.l.page_size * C::kScale;
-                        vs[st][j] = FMT == B4_KV_INT4 ? __half2float(*reinterpret_cast<const __half*>(q)) : *reinterpret_cast<const float*>(q);
+                        for (int b = 0; b < 4; ++b) {
+                            x[b] = lds32(__byte_perm(k0[i], t_key, 0x7604 | b << 4));
+                            y[b] = lds32(__byte_perm(k1[i], t_key, 0x7604 | b << 4));
+                        }
                     }
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        mma_f16(s[st][nt], x[0], y[0], x[1], y[1], qb[nt][4 * i], qb[nt][4 * i + 1]);
+                        mma_f16(s[st][nt], x[2], y[2], x[3], y[3], qb[nt][4 * i + 2], qb[nt][4 * i + 3]);
+                    }
+                }
+            }
+#pragma unroll
+            for (int st = 0; st < 2; ++st)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const float k = __shfl_sync(0xffffffffu, ks, 16 * st + 8 * h + gr);
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) s[st][nt][j] = 0.0f;
+                        for (int j = 2 * h; j < 2 * h + 2; ++j) s[st][nt][j] *= k;
+                }
+            if (masked) {
+                const int key = u.token + lane;
+                const int end = a.flags & B4_KV_FULL ? u.ctx : min(u.ctx, u.ctx - u.n + 1 + (u.tile * C::kCols + C::kCols - 1) / p.group);
+                const int begin = a.window > 0 ? u.ctx - u.n + 1 + u.tile * C::kCols / p.group - a.window : 0;
+                const bool in = (there >> lane / PT & 1) && key < end && key >= begin;     // some column sees it
+                const unsigned some = __ballot_sync(0xffffffffu, in);
+                if (!in) vs = 0.0f;
 #pragma unroll
-                    for (int i2 = 0; i2 < W; ++i2) {
-                        uint32_t x[4], y[4];
-                        if (FMT == B4_KV_INT4) {
-                            int4_word_to_half2(k0[i2], x);
-                            int4_word_to_half2(k1[i2], y);
-                        } else {
-#pragma unroll
-                            for (int b = 0; b < 4; ++b) {
-                                x[b] = *reinterpret_cast<const uint32_t*>(table + __byte_perm(k0[i2], lane * 4, 0x7604 | b << 4));
-                                y[b] = *reinterpret_cast<const uint32_t*>(table + __byte_perm(k1[i2], lane * 4, 0x7604 | b << 4));
-                            }
-                        }
-#pragma unroll
-                        for (int nt = 0; nt < NT; ++nt) {
-                            uint4 b;
-                            if (NT == 1) b = make_uint4(qb[4 * i2], qb[4 * i2 + 1], qb[4 * i2 + 2], qb[4 * i2 + 3]);
-                            else b = qs[(nt * W + i2) * 32 + lane];
-                            mma_f16(s[st][nt], x[0], y[0], x[1], y[1], b.x, b.y);
-                            mma_f16(s[st][nt], x[2], y[2], x[3], y[3], b.z, b.w);
-                        }
-                    }
-                    bool in[2] = {true, true};
-                    if (masked) {
-#pragma unroll
-                        for (int j = 0; j < 2; ++j) {
-                            const int key = tok + g + 8 * j;
-                            in[j] = (u.pages >> (key >> p.l.page_shift) & 1) && u.token + key < tile_end && u.token + key >= tile_begin;
-                            if (!in[j]) vs[st][j] = 0.0f;
-                        }
-                    }
-#pragma unroll
-                    for (int j = 0; j < 2; ++j) vtop = fmaxf(vtop, vs[st][j] < INFINITY ? vs[st][j] : 0.0f);
+                for (int st = 0; st < 2; ++st)
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                         for (int j = 0; j < 4; ++j) {
-                            float& x = s[st][nt][j];
-                            x *= ks[j >> 1] * qf[nt][j & 1];
-                            if (masked) {
-                                const int key = u.token + tok + g + 8 * (j >> 1);
-                                const bool ok = in[j >> 1] && key < lim[nt][j & 1] &&
-                                                (a.window == 0 || key >= lim[nt][j & 1] - a.window);
-                                if (!ok) x = -INFINITY;
-                            }
-                            top[nt][j & 1] = fmaxf(top[nt][j & 1], x);
+                            const int x = 16 * st + gr + 8 * (j >> 1), at = u.token + x;
+                            if (!(some >> x & 1) || at >= lim[nt][j & 1] || (a.window > 0 && at < lim[nt][j & 1] - a.window))
+                                s[st][nt][j] = -INFINITY;
                         }
+            }
+            float top[NT][2];
+            bool moved = false;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    top[nt][j] = fmaxf(fmaxf(s[0][nt][j], s[0][nt][j + 2]), fmaxf(s[1][nt][j], s[1][nt][j + 2]));
+                    moved |= top[nt][j] * qf[nt][j] > mx[nt][j] + 8.0f;
                 }
-                // running maxima, of the scores and of the values' scales
-#pragma unroll
-                for (int off = 4; off < 32; off <<= 1) {
-                    vtop = fmaxf(vtop, __shfl_xor_sync(0xffffffffu, vtop, off));
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                        for (int j = 0; j < 2; ++j) top[nt][j] = fmaxf(top[nt][j], __shfl_xor_sync(0xffffffffu, top[nt][j], off));
-                }
-                const int ve = min(max((int)(__float_as_uint(vtop) >> 23) - 126, vexp), 126);
-                const float vkeep = pow2(max(vexp - ve, -126)), vdown = pow2(-ve);
-                bool moved = ve != vexp;
+            // finite, so that a weight of 0 makes 0 of it
+            vs = fminf(vs, 3.4028235e38f);
+            const unsigned vbits = __reduce_max_sync(0xffffffffu, vs < 3.4028235e38f ? __float_as_uint(fabsf(vs)) : 0u);
+            const int ve = max(vexp, min((int)(vbits >> 23) - 126, 126));
+            if (__any_sync(0xffffffffu, moved) || ve != vexp) {
+                const float vkeep = pow2(max(vexp - ve, -126));
                 vexp = ve;
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
+                for (int nt = 0; nt < NT; ++nt) {
+                    float keep[2];
 #pragma unroll
-                    for (int j = 0; j < 2; ++j) moved |= top[nt][j] > mx[nt][j];
-                if (__any_sync(0xffffffffu, moved)) {
+                    for (int j = 0; j < 2; ++j) {
+#pragma unroll
+                        for (int off = 4; off < 32; off <<= 1) top[nt][j] = fmaxf(top[nt][j], __shfl_xor_sync(0xffffffffu, top[nt][j], off));
+                        const float next = top[nt][j] == -INFINITY ? mx[nt][j] : fmaxf(mx[nt][j], top[nt][j] * qf[nt][j]);
+                        keep[j] = fast_exp2(mx[nt][j] - next);
+                        mx[nt][j] = next;
+                        sum[nt][j] *= keep[j];
+                        keep[j] *= vkeep;
+                    }
+#pragma unroll
+                    for (int mt = 0; mt < D / 16; ++mt)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) o[nt][mt][j] *= keep[j & 1];
+                }
+            }
+            vs *= pow2(-vexp);
+            // weights as the right operand: tokens along k, a query a lane's row
+            uint32_t pb[2][NT][2];
+#pragma unroll
+            for (int st = 0; st < 2; ++st)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const float v = __shfl_sync(0xffffffffu, vs, 16 * st + 8 * h + gr);
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) {
-                        float keep[2];
+                        float w[2];
 #pragma unroll
                         for (int j = 0; j < 2; ++j) {
-                            const float next = fmaxf(mx[nt][j], top[nt][j]);
-                            keep[j] = next == -INFINITY ? 1.0f : fast_exp2(mx[nt][j] - next);
-                            mx[nt][j] = next;
-                            sum[nt][j] *= keep[j];
-                            keep[j] *= vkeep;
+                            w[j] = fast_exp2(fmaf(s[st][nt][2 * h + j], qf[nt][j], -mx[nt][j]));
+                            sum[nt][j] += w[j];
                         }
-#pragma unroll
-                        for (int mt = 0; mt < D / 16; ++mt)
-#pragma unroll
-                            for (int j = 0; j < 4; ++j) o[nt][mt][j] *= keep[j & 1];
+                        pb[st][nt][h] = movmatrix(pack_half2(w[0] * v, w[1] * v));
                     }
                 }
-                // weights, as the right operand: tokens along k, a query a lane's row
-                uint32_t pb[G][NT][2];
-                const uint32_t swap = t & 1 ? 0x1032 : 0x3210;     // odd lanes read their pair's second token first
+            // values: lane (g, t) holds d = g * (D / 8) .. of the tokens 2t, 2t + 1, 2t + 8, 2t + 9
 #pragma unroll
-                for (int st = 0; st < G; ++st)
+            for (int st = 0; st < 2; ++st) {
+                const uint8_t* vp = buf + v_at + st * tile1;
+                uint32_t v[4][VW];
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt)
+                for (int j = 0; j < 4; ++j) {
+                    const uint8_t* x = vp + (j & 1 ? v_other : 0) + (j >> 1) * 8 * C::kRow;
+                    if (VW == 2) {
+                        const uint2 y = *reinterpret_cast<const uint2*>(x);
+                        v[j][0] = y.x;
+                        v[j][VW - 1] = y.y;
+                    } else {
+                        v[j][0] = *reinterpret_cast<const uint32_t*>(x);
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < VW; ++i) {
+                    if (FMT == B4_KV_INT4) {
+                        // halves: two bytes of the first token, the same two of the second: four columns' pairs
+#pragma unroll
+                        for (int b = 0; b < 2; ++b) {
+                            uint32_t e[4], f[4];
+                            int4_word_to_half2(__byte_perm(v[0][i], v[1][i], b ? 0x7632 : 0x5410), e);
+                            int4_word_to_half2(__byte_perm(v[2][i], v[3][i], b ? 0x7632 : 0x5410), f);
+#pragma unroll
+                            for (int c = 0; c < 2; ++c)
+#pragma unroll
+                                for (int nt = 0; nt < NT; ++nt)
+                                    mma_f16(o[nt][4 * i + 2 * b + c], e[2 * c], e[2 * c + 1], f[2 * c], f[2 * c + 1], pb[st][nt][0], pb[st][nt][1]);
+                        }
+                    } else {
+                        uint32_t e[2], f[2];                       // bytes of (first token, second token), even and odd columns
 #pragma unroll
                         for (int j = 0; j < 2; ++j) {
-                            float w0 = mx[nt][0] == -INFINITY ? 0.0f : fast_exp2(s[st][nt][2 * j] - mx[nt][0]);
-                            float w1 = mx[nt][1] == -INFINITY ? 0.0f : fast_exp2(s[st][nt][2 * j + 1] - mx[nt][1]);
-                            sum[nt][0] += w0;
-                            sum[nt][1] += w1;
-                            const float v = vs[st][j] * vdown;
-                            float x0 = w0 * v, x1 = w1 * v;
-                            if (masked) {                      // 0 whatever an unseen token's scale is
-                                x0 = w0 == 0.0f ? 0.0f : x0;
-                                x1 = w1 == 0.0f ? 0.0f : x1;
-                            }
-                            pb[st][nt][j] = __byte_perm(movmatrix(pack_half2(x0, x1)), 0, swap);
-                        }
-                // values: lane (g, t) holds d = g * (D / 8) .. of the tokens 2t, 2t + 1, 2t + 8, 2t + 9
-#pragma unroll
-                for (int st = 0; st < G; ++st) {
-                    const int tok = (s0 + st) * 16, blk = tok >> p.l.page_shift, row = tok & (p.l.page_size - 1);
-                    const uint8_t* vp = buf + blk * (int)p.l.block + (p.l.page_size + row) * C::kRow + g * (D / 16);
-                    const int ta = 2 * t + (t & 1), tb = 2 * t + 1 - (t & 1);
-                    constexpr int VW = D / 64;                     // packed words of a token that a lane holds
-                    uint32_t v[4][VW];
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const uint8_t* q = vp + ((j & 1 ? tb : ta) + 8 * (j >> 1)) * C::kRow;
-                        if (VW == 2) {
-                            const uint2 x = *reinterpret_cast<const uint2*>(q);
-                            v[j][0] = x.x;
-                            v[j][VW - 1] = x.y;
-                        } else {
-                            v[j][0] = *reinterpret_cast<const uint32_t*>(q);
-                        }
-                    }
-#pragma unroll
-                    for (int i2 = 0; i2 < VW; ++i2) {
-                        uint32_t e[2], f[2];                       // NF4: bytes of (first token, second token), even and odd columns
-                        if (FMT == B4_KV_NF4) {
-#pragma unroll
-                            for (int j = 0; j < 2; ++j) {
-                                const uint32_t x = v[2 * j][i2], y = v[2 * j + 1][i2];
-                                e[j] = (x & 0x0f0f0f0fu) | (y << 4 & 0xf0f0f0f0u);
-                                f[j] = (x >> 4 & 0x0f0f0f0fu) | (y & 0xf0f0f0f0u);
-                            }
+                            const uint32_t x = v[2 * j][i], y = v[2 * j + 1][i];
+                            e[j] = (x & 0x0f0f0f0fu) | (y << 4 & 0xf0f0f0f0u);
+                            f[j] = (x >> 4 & 0x0f0f0f0fu) | (y & 0xf0f0f0f0u);
                         }
 #pragma unroll
                         for (int b = 0; b < 4; ++b) {
-                            uint32_t lo[2], hi[2];
+                            uint2 lo[2], hi[2];
 #pragma unroll
                             for (int j = 0; j < 2; ++j) {
-                                if (FMT == B4_KV_INT4) {
-                                    const uint32_t x = __byte_perm(v[2 * j][i2], v[2 * j + 1][i2], b | b << 4 | (4 + b) << 8 | (4 + b) << 12);
-                                    lo[j] = hsub2_bits(lop3_and_or<0x000f000fu, 0x64006400u>(x), 0x6408);
-                                    hi[j] = hsub2_bits(lop3_and_or<0x00f000f0u, 0x54005400u>(x), 0x5480);
-                                } else {
-                                    lo[j] = *reinterpret_cast<const uint32_t*>(table + __byte_perm(e[j], lane * 4, 0x7604 | b << 4));
-                                    hi[j] = *reinterpret_cast<const uint32_t*>(table + __byte_perm(f[j], lane * 4, 0x7604 | b << 4));
-                                }
+                                lo[j] = lds64(__byte_perm(e[j], t_val, 0x7604 | b << 4));
+                                hi[j] = lds64(__byte_perm(f[j], t_val, 0x7604 | b << 4));
                             }
 #pragma unroll
-                            for (int nt = 0; nt < NT; ++nt)
-                                mma_f16(o[nt][4 * i2 + b], lo[0], hi[0], lo[1], hi[1], pb[st][nt][0], pb[st][nt][1]);
+                            for (int nt = 0; nt < NT; ++nt) {
+                                mma_f16(o[nt][4 * i + b], lo[0].x, hi[0].x, lo[1].x, hi[1].x, pb[st][nt][0], pb[st][nt][1]);
+                                mma_f16(o[nt][4 * i + b], lo[0].y, hi[0].y, lo[1].y, hi[1].y, pb[st][nt][0], pb[st][nt][1]);
+                            }
                         }
                     }
                 }
             }
-            __syncwarp();
+        };
 
-            // the stage is free: the unit after next goes into it
-            if (produced < count) {
-                issue(stage, next_id);
-                ++produced;
-                if (produced < count) {
-                    step();
-                    next_id = page_id();
+        // ---- the run's segments ----
+        int r, stage = 0, feed = 0;
+        const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring) + lane * 16;
+        const int n16 = PT * C::kScale / 16, scale_at = lane < n16 ? lane * 16 : (p.l.page_size - PT) * C::kScale + lane * 16;
+        long long v = v0, at;                  // the next unit; the request's first
+        r = find(v0, at);
+        while (v < v1 && r < a.n_req) {
+            const AttnReq q = request(r);
+            const long long units = units_of(q);
+            if (v >= at + units) {
+                at += units;
+                ++r;
+                continue;
+            }
+            const int tiles = tiles_of(q), seg = (int)div64(v - at, q.chunks), first = (int)(v - at - (long long)seg * q.chunks);
+            const int last = (int)min((long long)q.chunks, first + (v1 - v));
+            u.q0 = q.q0;
+            u.n = q.n;
+            u.ctx = q.ctx;
+            u.head = seg / tiles;
+            u.tile = seg - u.head * tiles;
+            const long long seg_unit = at + (long long)seg * q.chunks;
+            v += last - first;
+
+            // the feed: page ids by 32, `ids` from page `base` on and the 32 after those
+            const int32_t* row = a.tables + (long long)r * a.table_stride;
+            const uint8_t* blocks = p.blocks + u.head * p.l.block;
+            const long long page_bytes = p.l.kv_heads * p.l.block;
+            int base = (q.chunk0 + first) * kChunk >> p.l.page_shift, next = q.chunk0 + first, queue = 0;
+            auto load_ids = [&](int page) { return (long long)page << p.l.page_shift < q.ctx ? __ldg(row + page) : -1; };
+            int ids = load_ids(base + lane), more = load_ids(base + 32 + lane);
+            auto issue = [&]() {               // the next chunk, if any, into stage `feed`
+                int there = 0;
+                if (next < q.chunk0 + last) {
+                    const int page = next * kChunk >> p.l.page_shift;
+                    if (page - base >= 32) {
+                        ids = more;
+                        base += 32;
+                        more = load_ids(base + 32 + lane);
+                    }
+                    const int half = PT == 32 ? next * kChunk & (p.l.page_size - 1) : 0;       // of a page of 64
+                    const uint32_t dst = ring_at + feed * C::kStage;
+#pragma unroll
+                    for (int i = 0; i < C::kPages; ++i) {
+                        // a chunk of two pages begins at an even place of the 32: its second page is among them
+                        const int id = __shfl_sync(0xffffffffu, ids, page - base + i);
+                        if ((unsigned)id >= (unsigned)p.l.n_pages) continue;
+                        there |= 1 << i;
+                        const uint8_t* src = blocks + id * page_bytes;
+                        const uint8_t *k = src + half * C::kRow + lane * 16, *v = k + p.l.page_size * C::kRow;
+                        constexpr int kCodes = PT * C::kRow, n16 = PT * C::kScale / 16;
+#pragma unroll
+                        for (int x = 0; x < kCodes; x += 512) {
+                            copy_async16(dst + i * C::kBlock + x, k + x);
+                            copy_async16(dst + i * C::kBlock + kCodes + x, v + x);
+                        }
+                        if (lane < 2 * n16) copy_async16(dst + i * C::kBlock + 2 * kCodes, src + p.l.page_size * D + half * C::kScale + scale_at);
+                    }
+                    ++next;
+                    if (++feed == kStages) feed = 0;
                 }
+                asm volatile("cp.async.commit_group;" ::: "memory");
+                queue = queue << 2 | there;
+            };
+            uint4 queries[NT][W];              // asked for before the feed waits for its page ids
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) load_queries(nt, queries[nt]);
+#pragma unroll 1
+            for (int i = 0; i < kStages; ++i) issue();
+            begin_segment(queries);
+
+            // every key of a chunk is seen by every column where the chunk lies in [clear, seen)
+            const int seen = a.flags & B4_KV_FULL ? u.ctx : min(u.ctx, u.ctx - u.n + 1 + u.tile * C::kCols / p.group);
+            const int clear = a.window > 0 ? u.ctx - a.window : 0;
+#pragma unroll 1
+            for (int c = first; c < last; ++c) {
+                u.token = (q.chunk0 + c) * kChunk;
+                const int there = queue >> (2 * kStages - 2) & 3;
+                asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
+                __syncwarp();
+                compute(ring + stage * C::kStage, there, u.token < clear || u.token + kChunk > seen || there != (1 << C::kPages) - 1);
+                __syncwarp();
+                issue();
+                if (++stage == kStages) stage = 0;
             }
 
             // ---- the end of a segment, or of the run ----
-            if ((u.flags & kUnitLast) || i + 1 == count) {
-                const float vup = pow2(vexp) * (FMT == B4_KV_NF4 ? 1.0f / kNf4Up : 1.0f);
+            const float vup = pow2(vexp) * (FMT == B4_KV_NF4 ? 1.0f / kNf4Up : 1.0f);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+#pragma unroll
+                    for (int off = 4; off < 32; off <<= 1) sum[nt][j] += __shfl_xor_sync(0xffffffffu, sum[nt][j], off);
+            if (first == 0 && last == q.chunks) {
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                    for (int j = 0; j < 2; ++j)
+                    for (int j = 0; j < 2; ++j) {
+                        int token, head;
+                        if (!col_row(nt * 8 + 2 * t + j, token, head)) continue;
+                        const float inv = sum[nt][j] > 0.0f ? vup / sum[nt][j] : 0.0f;
+                        T* dst = static_cast<T*>(a.out) + (u.q0 + token) * a.out_stride_token + head * a.out_stride_head + g * (D / 8);
+                        uint32_t w[D / 16];
 #pragma unroll
-                        for (int off = 4; off < 32; off <<= 1) sum[nt][j] += __shfl_xor_sync(0xffffffffu, sum[nt][j], off);
-                if (whole && (u.flags & kUnitLast)) {
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                        for (int j = 0; j < 2; ++j) {
-                            int token, head;
-                            if (!col_row(u, nt * 8 + 2 * t + j, token, head)) continue;
-                            const float inv = sum[nt][j] > 0.0f ? vup / sum[nt][j] : 0.0f;
-                            T* dst = static_cast<T*>(a.out) + (u.q0 + token) * a.out_stride_token + head * a.out_stride_head + g * (D / 8);
-                            uint32_t w[D / 16];
-#pragma unroll
-                            for (int mt = 0; mt < D / 16; ++mt) {
-                                const T lo = kv_round<T>(o[nt][mt][j] * inv), hi = kv_round<T>(o[nt][mt][j + 2] * inv);
-                                w[mt] = (uint32_t)*reinterpret_cast<const uint16_t*>(&lo) | (uint32_t)*reinterpret_cast<const uint16_t*>(&hi) << 16;
-                            }
-#pragma unroll
-                            for (int k = 0; k < D / 64; ++k)
-                                reinterpret_cast<uint4*>(dst)[k] = make_uint4(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
-                            if (a.lse && g == 0)
-                                a.lse[(long long)(u.q0 + token) * a.heads + head] =
-                                    sum[nt][j] > 0.0f ? (mx[nt][j] + fast_log2(sum[nt][j])) * kLn2 : -INFINITY;
+                        for (int mt = 0; mt < D / 16; ++mt) {
+                            const T lo = kv_round<T>(o[nt][mt][j] * inv), hi = kv_round<T>(o[nt][mt][j + 2] * inv);
+                            w[mt] = (uint32_t)*reinterpret_cast<const uint16_t*>(&lo) | (uint32_t)*reinterpret_cast<const uint16_t*>(&hi) << 16;
                         }
-                } else {
-                    // a piece [column][D], maxima, sums: the run's first goes to the workspace, its last into the ring
-                    const bool is_last = i + 1 == count;
-                    float* dst = is_last ? reinterpret_cast<float*>(ring) : ws.first + ((long long)cta * kAttnWarps + warp) * C::kPiece;
-                    __syncwarp();
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                        for (int j = 0; j < 2; ++j) {
-                            const int col = nt * 8 + 2 * t + j;
-#pragma unroll
-                            for (int mt = 0; mt < D / 16; mt += 2) {
-                                float4 x = make_float4(o[nt][mt][j] * vup, o[nt][mt][j + 2] * vup, o[nt][mt + 1][j] * vup, o[nt][mt + 1][j + 2] * vup);
-                                *reinterpret_cast<float4*>(dst + col * D + g * (D / 8) + 2 * mt) = x;
-                            }
-                            if (g == 0) {
-                                dst[C::kCols * D + col] = mx[nt][j];
-                                dst[C::kCols * (D + 1) + col] = sum[nt][j];
-                            }
-                        }
-                    if (lane == 0) {
-                        WarpPiece pc;
-                        pc.s0 = seg_unit;
-                        pc.s1 = seg_unit + seg_chunks;
-                        pc.q0 = u.q0;
-                        pc.n = u.n;
-                        pc.head = u.head;
-                        pc.tile = u.tile;
-                        pc.valid = 1;
-                        pieces[warp][is_last] = pc;
+                        for (int k = 0; k < D / 64; ++k)
+                            reinterpret_cast<uint4*>(dst)[k] = make_uint4(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
+                        if (a.lse && g == 0)
+                            a.lse[(long long)(u.q0 + token) * a.heads + head] =
+                                sum[nt][j] > 0.0f ? (mx[nt][j] + fast_log2(sum[nt][j])) * kLn2 : -INFINITY;
                     }
+            } else {
+                // a piece [column][D], maxima, sums: the run's last goes into the ring, which is free, its first to the workspace
+                const bool is_last = v == v1;
+                float* dst = is_last ? reinterpret_cast<float*>(ring) : ws.first + ((long long)cta * kWarps + warp) * C::kPiece;
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        const int col = nt * 8 + 2 * t + j;
+#pragma unroll
+                        for (int mt = 0; mt < D / 16; mt += 2) {
+                            float4 x = make_float4(o[nt][mt][j] * vup, o[nt][mt][j + 2] * vup, o[nt][mt + 1][j] * vup, o[nt][mt + 1][j + 2] * vup);
+                            *reinterpret_cast<float4*>(dst + col * D + g * (D / 8) + 2 * mt) = x;
+                        }
+                        if (g == 0) {
+                            dst[C::kCols * D + col] = mx[nt][j];
+                            dst[C::kCols * (D + 1) + col] = sum[nt][j];
+                        }
+                    }
+                if (lane == 0) {
+                    WarpPiece pc;
+                    pc.s0 = seg_unit;
+                    pc.s1 = seg_unit + q.chunks;
+                    pc.q0 = u.q0;
+                    pc.n = u.n;
+                    pc.head = u.head;
+                    pc.tile = u.tile;
+                    pc.valid = 1;
+                    pieces[warp][is_last] = pc;
                 }
-            }
-            if (i + 1 < count) {
-                if (u.flags & kUnitLast) {
-                    seg_unit = v0 + i + 1;
-                    // a segment's chunks are counted when it ends in another run: from its request's extent
-                    const int begin = a.window > 0 ? max(0, nu.ctx - nu.n + 1 - a.window) : 0;
-                    seg_chunks = max(1, (nu.ctx + kChunk - 1) / kChunk - begin / kChunk);
-                }
-                u = nu;
-                stage ^= 1;
-                if (stage == 0) phase ^= 1;
             }
         }
     }
     __syncthreads();
 
-    // ---- join the pieces of this CTA, in unit order ----
-    auto emit = [&](const WarpPiece& pc, int e, const float4& x, float m, float l) {    // four columns' outputs of one query
+    // ---- join the pieces of this CTA, in unit order: lane i looks at piece i (a warp's first at 2 warp, its last after it) ----
+    auto piece_of = [&](int i) -> const float* {
+        return i & 1 ? reinterpret_cast<const float*>(ring_of(i >> 1)) : ws.first + ((long long)cta * kWarps + (i >> 1)) * C::kPiece;
+    };
+    const bool mine = lane < 2 * kWarps && pieces[lane >> 1][lane & 1].valid;
+    const long long my_s0 = mine ? pieces[lane >> 1][lane & 1].s0 : -1;
+    const uint32_t have = __ballot_sync(0xffffffffu, mine);
+    // the pieces of the segment of piece f
+    auto same = [&](int f) {
+        const long long s0 = __shfl_sync(0xffffffffu, my_s0, f);    // by every lane
+        return __ballot_sync(0xffffffffu, mine && s0 == my_s0);
+    };
+    // maxima and sums of every segment (at its first piece) and the pieces' factors, a column a warp
+    for (int col = warp; col < C::kCols; col += kWarps) {
+        float m = kNoMax, l = 0.0f, f = 0.0f;
+        if (mine) {
+            const float* b = piece_of(lane) + C::kCols * D + col;
+            m = b[0];
+            l = b[C::kCols];
+        }
+        for (uint32_t todo = have; todo;) {
+            const int at = __ffs(todo) - 1;
+            const uint32_t list = same(at);
+            const bool in = list >> lane & 1;
+            float top = in ? m : kNoMax;
+#pragma unroll
+            for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+            if (in) f = fast_exp2(m - top);
+            float all = in ? f * l : 0.0f;
+#pragma unroll
+            for (int off = 16; off > 0; off >>= 1) all += __shfl_xor_sync(0xffffffffu, all, off);
+            if (lane == at) {
+                joined[col][at].x = top;
+                joined[col][at].y = all;
+            }
+            todo &= ~list;
+        }
+        factor[col][lane] = f;
+    }
+    __syncthreads();
+    auto emit = [&](const WarpPiece& pc, int e, float2 x, float m, float l) {      // two columns' outputs of one query
         const int c = pc.tile * C::kCols + e / D, token = c / p.group, head = pc.head * p.group + (c - token * p.group);
         if (c >= pc.n * p.group) return;
         const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-        T w[4] = {kv_round<T>(x.x * inv), kv_round<T>(x.y * inv), kv_round<T>(x.z * inv), kv_round<T>(x.w * inv)};
-        *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + (pc.q0 + token) * a.out_stride_token + head * a.out_stride_head + e % D) =
-            *reinterpret_cast<const uint2*>(w);
+        const T w[2] = {kv_round<T>(x.x * inv), kv_round<T>(x.y * inv)};
+        *reinterpret_cast<uint32_t*>(static_cast<T*>(a.out) + (pc.q0 + token) * a.out_stride_token + head * a.out_stride_head + e % D) =
+            (uint32_t)*reinterpret_cast<const uint16_t*>(w) | (uint32_t)*reinterpret_cast<const uint16_t*>(w + 1) << 16;
         if (a.lse && e % D == 0)
             a.lse[(long long)(pc.q0 + token) * a.heads + head] = l > 0.0f ? (m + fast_log2(l)) * kLn2 : -INFINITY;
     };
-    // joins `n` pieces (piece i at base(i)) for the four values at e
-    auto join = [&](int n, int e, auto base, float4& x, float& m, float& l) {
-        const int col = e / D;
-        m = -INFINITY;
-        for (int i = 0; i < n; ++i) m = fmaxf(m, base(i)[C::kCols * D + col]);
-        x = make_float4(0, 0, 0, 0);
-        l = 0.0f;
-        for (int i = 0; i < n; ++i) {
-            const float* b = base(i);
-            const float mi = b[C::kCols * D + col], k = mi == -INFINITY ? 0.0f : fast_exp2(mi - m);
-            const float4 y = *reinterpret_cast<const float4*>(b + e);
-            l += k * b[C::kCols * (D + 1) + col];
-            x.x += k * y.x;
-            x.y += k * y.y;
-            x.z += k * y.z;
-            x.w += k * y.w;
+    int cross[2] = {-1, -1};                   // the first pieces of the segments that began before this CTA, that go on after it
+    for (uint32_t todo = have; todo;) {
+        const int at = __ffs(todo) - 1;
+        const uint32_t list = same(at), lasts = list & 0xaaaaaaaau, firsts = list & 0x55555555u;
+        todo &= ~list;
+        const WarpPiece& pc = pieces[at >> 1][at & 1];
+        const bool inside = pc.s0 >= c0 && pc.s1 <= c1, begins = pc.s0 >= c0;
+        if (!inside) {
+            if (begins) cross[1] = at;
+            else cross[0] = at;
         }
-    };
-    auto piece_at = [&](int i) -> const float* {
-        return i & 1 ? reinterpret_cast<const float*>(attn_smem + C::kTable + (i >> 1) * kAttnStages * C::kStage)
-                     : ws.first + ((long long)cta * kAttnWarps + (i >> 1)) * C::kPiece;
-    };
-    WarpPiece cross[2];
-    cross[0].valid = cross[1].valid = 0;
-    for (int i = 0; i < 2 * kAttnWarps;) {
-        const WarpPiece pc = pieces[i >> 1][i & 1];
-        if (!pc.valid) {
-            ++i;
-            continue;
-        }
-        uint64_t list = i;                     // four bits a piece
-        int n = 1, j = i + 1;
-        for (; j < 2 * kAttnWarps; ++j) {
-            const WarpPiece& x = pieces[j >> 1][j & 1];
-            if (!x.valid) continue;
-            if (x.s0 != pc.s0) break;
-            list |= (uint64_t)j << (4 * n);
-            ++n;
-        }
-        i = j;
-        const bool inside = pc.s0 >= c0 && pc.s1 <= c1;
-        const int which = pc.s0 >= c0;
-        if (!inside) cross[which] = pc;
-        for (int e = tid * 4; e < C::kCols * D; e += kThreads * 4) {
-            float4 x;
-            float m, l;
-            join(n, e, [&](int k) { return piece_at((int)(list >> (4 * k)) & 15); }, x, m, l);
+        const int w0 = (__ffs(lasts) - 1) >> 1, w1 = (31 - __clz(lasts)) >> 1;
+        for (int e = tid * 2; e < C::kCols * D; e += kThreads * 2) {
+            const int col = e / D;
+            float2 x = make_float2(0.0f, 0.0f);
+            if (lasts) {
+#pragma unroll 4
+                for (int w = w0; w <= w1; ++w) {
+                    const bool in = lasts >> (2 * w + 1) & 1;
+                    const float k = in ? factor[col][2 * w + 1] : 0.0f;
+                    const float2 y = *reinterpret_cast<const float2*>(ring_of(in ? w : w0) + e * 4);
+                    x.x += k * y.x;
+                    x.y += k * y.y;
+                }
+            }
+            if (firsts) {                      // one at most: a run's first piece ends its segment
+                const int i = __ffs(firsts) - 1;
+                const float k = factor[col][i];
+                const float2 y = *reinterpret_cast<const float2*>(piece_of(i) + e);
+                x.x += k * y.x;
+                x.y += k * y.y;
+            }
+            const float2 ml = joined[col][at];
             if (inside) {
-                emit(pc, e, x, m, l);
+                emit(pc, e, x, ml.x, ml.y);
             } else {
-                float* dst = ws.cross + ((long long)cta * 2 + which) * C::kPiece;
-                *reinterpret_cast<float4*>(dst + e) = x;
+                float* dst = ws.cross + ((long long)cta * 2 + begins) * C::kPiece;
+                *reinterpret_cast<float2*>(dst + e) = x;
                 if (e % D == 0) {
-                    dst[C::kCols * D + e / D] = m;
-                    dst[C::kCols * (D + 1) + e / D] = l;
+                    dst[C::kCols * D + col] = ml.x;
+                    dst[C::kCols * (D + 1) + col] = ml.y;
                 }
             }
         }
     }
-    if (!cross[0].valid && !cross[1].valid) return;
+    if (cross[0] < 0 && cross[1] < 0) return;
 
-    // ---- segments that cross CTAs: the last to arrive joins them ----
-    auto owner = [&](long long u) { return (int)(((u + 1) * ctas - 1) / total); };
-    __threadfence();
+    // ---- segments that cross CTAs: the last to arrive joins them, in CTA order ----
+    auto span = [&](const WarpPiece& pc, int& f) {         // the CTAs that hold pieces of the segment
+        f = owner(min(pc.s0 + near, total - 1));
+        return max(owner(max(pc.s1 - near - 1, 0LL)) - f, 0) + 1;
+    };
     __syncthreads();
     if (tid < 2) {
-        last_cta[tid] = 0;
-        if (cross[tid].valid) {
-            const int f = owner(cross[tid].s0), n = owner(cross[tid].s1 - 1) - f + 1;
-            last_cta[tid] = atomicAdd(ws.count + f, 1) == n - 1;
-            if (last_cta[tid]) ws.count[f] = 0;
+        const int at = tid ? cross[1] : cross[0];
+        int last = 0;
+        if (at >= 0) {
+            int f;
+            const int n = span(pieces[at >> 1][at & 1], f);
+            __threadfence();
+            last = atomicAdd(ws.count + f, 1) == n - 1;
+            if (last) ws.count[f] = 0;
+            __threadfence();
         }
+        last_cta[tid] = last;
     }
     __syncthreads();
-    __threadfence();
-#pragma unroll
+#pragma unroll 1
     for (int k = 0; k < 2; ++k) {
         if (!last_cta[k]) continue;
-        const WarpPiece pc = cross[k];
-        const int f = owner(pc.s0), n = owner(pc.s1 - 1) - f + 1;
-        for (int e = tid * 4; e < C::kCols * D; e += kThreads * 4) {
-            float4 x;
-            float m, l;
-            join(n, e, [&](int c) -> const float* { return ws.cross + ((long long)(f + c) * 2 + (c == 0)) * C::kPiece; }, x, m, l);
-            emit(pc, e, x, m, l);
+        const int at = k ? cross[1] : cross[0];
+        const WarpPiece& pc = pieces[at >> 1][at & 1];
+        int f;
+        const int n = span(pc, f);
+        auto part = [&](int c) -> const float* { return ws.cross + ((long long)(f + c) * 2 + (c == 0)) * C::kPiece; };
+        __syncthreads();
+        for (int col = warp; col < C::kCols; col += kWarps) {
+            float m = kNoMax, l = 0.0f;
+            for (int c = lane; c < n; c += 32) {           // a running pair a lane
+                const float* b = part(c) + C::kCols * D + col;
+                const float mc = __ldcg(b), lc = __ldcg(b + C::kCols), next = fmaxf(m, mc);
+                l = l * fast_exp2(m - next) + lc * fast_exp2(mc - next);
+                m = next;
+            }
+            float top = m;
+#pragma unroll
+            for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+            l *= fast_exp2(m - top);
+#pragma unroll
+            for (int off = 16; off > 0; off >>= 1) l += __shfl_xor_sync(0xffffffffu, l, off);
+            if (lane == 0) joined[col][0] = make_float2(top, l);
+        }
+        __syncthreads();
+        for (int e = tid * 2; e < C::kCols * D; e += kThreads * 2) {
+            const int col = e / D;
+            const float2 ml = joined[col][0];
+            float2 x = make_float2(0.0f, 0.0f);
+#pragma unroll 8
+            for (int c = 0; c < n; ++c) {
+                const float* b = part(c);
+                const float w = fast_exp2(__ldcg(b + C::kCols * D + col) - ml.x);
+                const float2 y = __ldcg(reinterpret_cast<const float2*>(b + e));
+                x.x += w * y.x;
+                x.y += w * y.y;
+            }
+            emit(pc, e, x, ml.x, ml.y);
         }
     }
 }
