@@ -10,51 +10,51 @@ namespace {
 // ---- block tables, slots, positions ----------------------------------------------
 // Every CTA scans the requests' lengths itself (new tokens and new pages, both
 // exclusive sums, in shared memory), so there is no second launch and no wait
-// between CTAs; then the CTAs share the packed tokens (request found by binary
-// search over the scanned starts) and the new table entries.  A slot in a new
-// page comes straight from the ring, not through the table, which another CTA
-// may still be writing.
-constexpr int kTabThreads = 256;
+// between CTAs; then the threads of the grid share the packed tokens and the new
+// table entries, one each where the grid allows, and find their request by binary
+// search in the sums: the time is a handful of dependent loads, whatever the
+// requests' lengths.  A slot in a new page comes straight from the ring, not through
+// the table, which another CTA may still be writing.
+constexpr int kTabThreads = 256, kTabGrid = 148 * 8;
 
 __device__ __forceinline__ int sat(long long v) { return (int)(v > INT_MAX ? INT_MAX : v); }
 
-__device__ __forceinline__ int pages_of(long long tokens, int page_size, int width)
+__device__ __forceinline__ int pages_of(long long tokens, int shift, int width)
 {
-    const long long p = (tokens + page_size - 1) / page_size;
+    const long long p = (tokens + (1 << shift) - 1) >> shift;
     return (int)(p < width ? p : width);
 }
 
-struct TabLengths {
-    long long cached, added;
-    int held, fresh;
-};
-
-__device__ __forceinline__ TabLengths tab_lengths(const b4_kv_step& s, int r)
+// the last of n ascending values that is at most x (values[0] <= x)
+__device__ __forceinline__ int last_at_most(const int* values, int n, long long x)
 {
-    TabLengths l;
-    l.cached = max(__ldg(s.cached + r), 0);
-    l.added = max(__ldg(s.added + r), 0);
-    l.held = pages_of(l.cached, s.page_size, s.table_width);
-    l.fresh = pages_of(l.cached + l.added, s.page_size, s.table_width) - l.held;
-    return l;
+    int lo = 0;
+    for (int step = 1 << (31 - __clz(n)); step > 0; step >>= 1)
+        if (lo + step < n && values[lo + step] <= x) lo += step;
+    return lo;
 }
 
-__global__ void __launch_bounds__(kTabThreads) kv_tables_kernel(const b4_kv_step s)
+__global__ void __launch_bounds__(kTabThreads) kv_tables_kernel(const b4_kv_step s, const int shift)
 {
     extern __shared__ int tab_smem[];
     int* start = tab_smem;                    // [n_req] first token of a request
-    int* first = tab_smem + s.n_req;          // [n_req] its first new page, counted from the ring's place
+    int* first = start + s.n_req;             // [n_req] its first new page, counted from the ring's place
+    int* cached = first + s.n_req;            // [n_req]
     __shared__ long long warp_tok[kTabThreads / 32], warp_pag[kTabThreads / 32];
     kv_begin();
 
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int ring_at = __ldg(s.free_state), ring_left = __ldg(s.free_state + 1);
     const int per = (s.n_req + kTabThreads - 1) / kTabThreads;
     const int r0 = min((int)threadIdx.x * per, s.n_req), r1 = min(r0 + per, s.n_req);
     long long tok = 0, pag = 0;
-    for (int r = r0; r < r1; ++r) {
-        const TabLengths l = tab_lengths(s, r);
-        tok += l.added;
-        pag += l.fresh;
+#pragma unroll 4
+    for (int r = r0; r < r1; ++r) {           // sums within the thread
+        const int c = max(__ldg(s.cached + r), 0), n = max(__ldg(s.added + r), 0);
+        cached[r] = c;
+        start[r] = n;
+        tok += n;
+        pag += pages_of((long long)c + n, shift, s.table_width) - pages_of(c, shift, s.table_width);
     }
     long long it = tok, ip = pag;
 #pragma unroll
@@ -81,21 +81,22 @@ __global__ void __launch_bounds__(kTabThreads) kv_tables_kernel(const b4_kv_step
         all_pag += warp_pag[w];
     }
     const bool writer = blockIdx.x == 0;
-    for (int r = r0; r < r1; ++r) {
-        const TabLengths l = tab_lengths(s, r);
+    for (int r = r0; r < r1; ++r) {           // the thread's own entries: exclusive sums over all
+        const long long c = cached[r], n = start[r];
+        const int fresh = pages_of(c + n, shift, s.table_width) - pages_of(c, shift, s.table_width);
         start[r] = sat(bt);
         first[r] = sat(bp);
         if (writer) {
-            s.ctx_len[r] = sat(l.cached + l.added);
+            s.ctx_len[r] = sat(c + n);
             s.q_starts[r] = sat(bt);
         }
-        bt += l.added;
-        bp += l.fresh;
+        bt += n;
+        bp += fresh;
     }
     __syncthreads();
 
-    const int head = s.ring_size > 0 ? (int)((unsigned)max(__ldg(s.free_state), 0) % (unsigned)s.ring_size) : 0;
-    const int left = min(max(__ldg(s.free_state + 1), 0), s.ring_size);
+    const int head = s.ring_size > 0 ? (int)((unsigned)max(ring_at, 0) % (unsigned)s.ring_size) : 0;
+    const int left = min(max(ring_left, 0), s.ring_size);
     if (writer && threadIdx.x == 0) {
         s.q_starts[s.n_req] = sat(all_tok);
         const int taken = (int)(all_pag < left ? all_pag : left);
@@ -110,33 +111,26 @@ __global__ void __launch_bounds__(kTabThreads) kv_tables_kernel(const b4_kv_step
         return __ldg(s.free_pages + at);
     };
 
-    const int n_tok = sat(all_tok);
-    for (long long i = (long long)blockIdx.x * kTabThreads + threadIdx.x; i < s.max_tokens;
-         i += (long long)gridDim.x * kTabThreads) {
+    const int n_tok = sat(all_tok), n_pag = sat(all_pag);
+    const long long id0 = (long long)blockIdx.x * kTabThreads + threadIdx.x, ids = (long long)gridDim.x * kTabThreads;
+    for (long long i = id0; i < s.max_tokens; i += ids) {
         int slot = -1, pos = 0;
         if (i < n_tok) {
-            int lo = 0, hi = s.n_req;         // the last request that starts at or before i
-            while (hi - lo > 1) {
-                const int mid = (lo + hi) >> 1;
-                if (start[mid] <= i) lo = mid;
-                else hi = mid;
-            }
-            const long long c = max(__ldg(s.cached + lo), 0), at = c + (i - start[lo]);
-            const long long p = at / s.page_size;
+            const int r = last_at_most(start, s.n_req, i);
+            const long long c = cached[r], at = c + (i - start[r]), p = at >> shift;
             pos = sat(at);
             if (p < s.table_width) {
-                const int held = pages_of(c, s.page_size, s.table_width);
-                const int id = p < held ? s.tables[lo * s.table_stride + p] : ring(first[lo] + (int)p - held);
-                if (id >= 0) slot = id * s.page_size + (int)(at - p * s.page_size);
+                const int held = pages_of(c, shift, s.table_width);
+                const int id = p < held ? s.tables[r * s.table_stride + p] : ring(first[r] + (int)p - held);
+                if (id >= 0) slot = (id << shift) + (int)(at & ((1 << shift) - 1));
             }
         }
         s.slots[i] = slot;
         s.positions[i] = pos;
     }
-    const int warps = gridDim.x * (kTabThreads / 32);
-    for (int r = blockIdx.x * (kTabThreads / 32) + warp; r < s.n_req; r += warps) {
-        const TabLengths l = tab_lengths(s, r);
-        for (int i = lane; i < l.fresh; i += 32) s.tables[r * s.table_stride + l.held + i] = ring(first[r] + i);
+    for (long long i = id0; i < n_pag; i += ids) {
+        const int r = last_at_most(first, s.n_req, i);
+        s.tables[r * s.table_stride + pages_of(cached[r], shift, s.table_width) + (i - first[r])] = ring((int)i);
     }
 }
 
@@ -165,58 +159,165 @@ __device__ __forceinline__ int nf4_code(float norm)
     return best;
 }
 
+// Vectors (one token's keys or values of one head) are numbered token, then keys
+// before values, then head; D / 8 threads hold one, a packed word each.
+struct VectorIndex {
+    int token, head;
+    bool value;
+};
+
+__device__ __forceinline__ VectorIndex vector_index(long long i, int kv_heads, unsigned long long magic)
+{
+    VectorIndex v;
+    v.token = (int)__umul64hi((unsigned long long)i, magic);       // i / (2 kv_heads): magic = 2^64 / (2 kv_heads) + 1, i < 2^42
+    const int hv = (int)(i - (long long)v.token * (2 * kv_heads));
+    v.value = hv >= kv_heads;
+    v.head = v.value ? hv - kv_heads : hv;
+    return v;
+}
+
 struct AppendParams {
     KvLayout l;
     uint8_t* blocks;
     const void *k, *v;
     long long k_tok, k_head, v_tok, v_head;
     const int32_t* slots;
-    long long n;              // vectors: tokens * 2 * kv_heads
+    long long n;                       // vectors: tokens * 2 * kv_heads
+    unsigned long long magic;
 };
 
-// Eight columns (one packed word) a thread, head_dim / 8 threads a vector.
-template <typename T, int FMT, int D>
+// 8 columns of T as loaded, and as fp32
+template <typename T, bool VEC>
+struct Columns {
+    uint4 raw[sizeof(T) / 2];
+    __device__ void load(const T* p)
+    {
+        if (VEC) {
+#pragma unroll
+            for (int i = 0; i < (int)sizeof(T) / 2; ++i) raw[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
+        } else {
+            T* r = reinterpret_cast<T*>(raw);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) r[i] = p[i];
+        }
+    }
+    __device__ float get(int i) const { return kv_float(reinterpret_cast<const T*>(raw)[i]); }
+};
+
+// One packed word of INT4 codes.  The quotient by a product with the reciprocal is
+// within 2 ulp of the fp32 division that defines the code, so a code is taken from
+// it where it lies further than 1e-5 from a tie; the rest, and scales that are no
+// normal fp16 number (there a quotient may pass 8), are divided.
+__device__ __forceinline__ uint32_t int4_word(const float (&x)[8], float s)
+{
+    const float inv = __fdividef(1.0f, s);
+    uint32_t w = 0;
+    float worst = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const float y = x[j] * inv, r = y + 12582912.0f;           // 1.5 * 2^23: the integer nearest to y in the low bits
+        worst = fmaxf(worst, fabsf(y - (r - 12582912.0f)));
+        w |= (__float_as_uint(r) & 15u) << (4 * j);
+        if (isnan(y)) worst = 1.0f;
+    }
+    if (worst < 0.49999f && s >= 6.1035156e-5f && s <= 65504.0f) return w ^ 0x88888888u;   // two's complement to code - 8
+    w = 0;
+#pragma unroll 1
+    for (int j = 0; j < 8; ++j) w |= (uint32_t)int4_code(__fdiv_rn(x[j], s)) << (4 * j);
+    return w;
+}
+
+// One packed word of NF4 codes.  [-1, 1] is cut into 31 bins of 1 / kBins with one boundary
+// between two levels at most; lane b holds bin b's boundary and the level below it
+// (codes below the boundary), so a code is a product, two shuffles and a
+// comparison instead of a scan of 16 levels.  Quotients within 1e-6 of a boundary
+// (and NaN) are divided and scanned as the definition says.
+constexpr float kBins = 15.2f;         // less than the least distance between two boundaries; none lies at a bin's edge
+
+__device__ __forceinline__ uint32_t nf4_word(const float (&x)[8], float s, float boundary, int below)
+{
+    const float inv = __fdividef(1.0f, s);
+    uint32_t w = 0;
+    float worst = 1.0f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const float y = x[j] * inv;
+        const int bin = (int)__float_as_uint(fmaf(y, kBins, 8388608.0f + 16.0f));          // low 5 bits: 16 + the integer nearest to kBins y
+        const float d = y - __shfl_sync(0xffffffffu, boundary, bin);
+        const int c = __shfl_sync(0xffffffffu, below, bin) + (d >= 0.0f);
+        worst = fminf(worst, fabsf(d));
+        if (isnan(y)) worst = 0.0f;
+        w |= (uint32_t)c << (4 * j);
+    }
+    if (worst > 1e-6f && s > 1e-30f && s < 1e30f) return w;
+    w = 0;
+#pragma unroll 1
+    for (int j = 0; j < 8; ++j) w |= (uint32_t)nf4_code(__fdiv_rn(x[j], s)) << (4 * j);
+    return w;
+}
+
+constexpr int kAppendUnroll = 2;       // vectors a thread has in flight
+
+// Bound by memory: 2.1 to 4.5 bytes a column.
+template <typename T, int FMT, int D, bool VEC>
 __global__ void __launch_bounds__(256) kv_append_kernel(const AppendParams p)
 {
-    constexpr int TPV = D / 8;
+    constexpr int TPV = D / 8, per = 256 / TPV;
+    float boundary = 4.0f;
+    int below = 0;
+    if (FMT == B4_KV_NF4) {
+        const int lane = threadIdx.x & 31;
+        const float start = (lane - 16.5f) / kBins, end = (lane - 15.5f) / kBins;
+#pragma unroll
+        for (int c = 0; c < 15; ++c) {
+            const float m = 0.5f * (c_nf4_table[c] + c_nf4_table[c + 1]);
+            if (m < start) below = c + 1;
+            else if (m < end) boundary = m;
+        }
+    }
     kv_begin();
     const int sub = threadIdx.x % TPV;
-    for (long long b = (long long)blockIdx.x * (256 / TPV); b < p.n; b += (long long)gridDim.x * (256 / TPV)) {
-        const long long v = b + threadIdx.x / TPV, i = v < p.n ? v : p.n - 1;   // whole warps take part in the shuffles
-        const int token = (int)(i / (2 * p.l.kv_heads)), hv = (int)(i - (long long)token * (2 * p.l.kv_heads));
-        const bool val = hv >= p.l.kv_heads;
-        const int head = val ? hv - p.l.kv_heads : hv;
-        const int slot = __ldg(p.slots + token);
-        const int page = slot >> p.l.page_shift, row = slot & (p.l.page_size - 1);
-        const bool live = v < p.n && slot >= 0 && page < p.l.n_pages;
-        const T* src = val ? static_cast<const T*>(p.v) + token * p.v_tok + head * p.v_head
-                           : static_cast<const T*>(p.k) + token * p.k_tok + head * p.k_head;
+    const long long first = (long long)blockIdx.x * (kAppendUnroll * per) + threadIdx.x / TPV;
+    Columns<T, VEC> c[kAppendUnroll];
+    uint8_t* block[kAppendUnroll];
+    int at[kAppendUnroll];
+#pragma unroll
+    for (int u = 0; u < kAppendUnroll; ++u) {
+        const long long i = min(first + u * per, p.n - 1);         // whole warps take part in the shuffles
+        const VectorIndex v = vector_index(i, p.l.kv_heads, p.magic);
+        const int slot = __ldg(p.slots + v.token), page = slot >> p.l.page_shift;
+        const bool live = first + u * per < p.n && slot >= 0 && page < p.l.n_pages;
+        const T* src = v.value ? static_cast<const T*>(p.v) + v.token * p.v_tok + v.head * p.v_head
+                               : static_cast<const T*>(p.k) + v.token * p.k_tok + v.head * p.k_head;
+        c[u].load(src + sub * 8);
+        block[u] = live ? p.blocks + ((long long)page * p.l.kv_heads + v.head) * p.l.block : nullptr;
+        at[u] = (v.value ? p.l.page_size : 0) + (slot & (p.l.page_size - 1));
+    }
+#pragma unroll
+    for (int u = 0; u < kAppendUnroll; ++u) {
         float x[8], amax = 0.0f;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            x[j] = live ? kv_float(src[sub * 8 + j]) : 0.0f;
+            x[j] = c[u].get(j);
             amax = fmaxf(amax, fabsf(x[j]));
         }
 #pragma unroll
         for (int o = TPV / 2; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-        if (!live) continue;
-        uint8_t* block = p.blocks + ((long long)page * p.l.kv_heads + head) * p.l.block;
-        uint8_t* codes = block + ((val ? p.l.page_size : 0) + row) * (D / 2);
-        uint8_t* scale = block + p.l.page_size * D + ((val ? p.l.page_size : 0) + row) * (FMT == B4_KV_INT4 ? 2 : 4);
-        uint32_t w = 0;
+        uint32_t w;
+        __half sh;
         if (FMT == B4_KV_INT4) {
-            const __half sh = __float2half_rn(amax > 0.0f ? __fmul_rn(amax, 1.0f / 7.0f) : 1.0f);
-            const float s = __half2float(sh);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) w |= (uint32_t)int4_code(__fdiv_rn(x[j], s)) << (4 * j);
-            if (sub == 0) *reinterpret_cast<__half*>(scale) = sh;
+            sh = __float2half_rn(amax > 0.0f ? __fmul_rn(amax, 1.0f / 7.0f) : 1.0f);
+            w = int4_word(x, __half2float(sh));
         } else {
-            const float s = amax > 0.0f ? amax : 1.0f;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) w |= (uint32_t)nf4_code(__fdiv_rn(x[j], s)) << (4 * j);
-            if (sub == 0) *reinterpret_cast<float*>(scale) = s;
+            if (!(amax > 0.0f)) amax = 1.0f;
+            w = nf4_word(x, amax, boundary, below);
         }
-        reinterpret_cast<uint32_t*>(codes)[sub] = w;
+        if (!block[u]) continue;
+        reinterpret_cast<uint32_t*>(block[u] + at[u] * (D / 2))[sub] = w;
+        if (sub == 0) {
+            if (FMT == B4_KV_INT4) reinterpret_cast<__half*>(block[u] + p.l.page_size * D)[at[u]] = sh;
+            else reinterpret_cast<float*>(block[u] + p.l.page_size * D)[at[u]] = amax;
+        }
     }
 }
 
@@ -226,49 +327,70 @@ struct ReadParams {
     const uint8_t* blocks;
     const int32_t* slots;
     float *k, *v;
-    long long n;              // packed words: tokens * 2 * kv_heads * head_dim / 8
+    long long n;                       // vectors
+    unsigned long long magic;
 };
 
+// Bound by its fp32 stores.
 template <int FMT, int D>
 __global__ void __launch_bounds__(256) kv_read_kernel(const ReadParams p)
 {
-    constexpr int TPV = D / 8;
+    constexpr int TPV = D / 8, per = 256 / TPV;
+    const float level = c_nf4_table[threadIdx.x & 15];
     kv_begin();
-    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < p.n; i += (long long)gridDim.x * 256) {
-        const int sub = (int)(i % TPV);
-        const long long vec = i / TPV;
-        const int token = (int)(vec / (2 * p.l.kv_heads)), hv = (int)(vec - (long long)token * (2 * p.l.kv_heads));
-        const bool val = hv >= p.l.kv_heads;
-        const int head = val ? hv - p.l.kv_heads : hv;
-        const int slot = __ldg(p.slots + token);
-        const int page = slot >> p.l.page_shift, row = slot & (p.l.page_size - 1);
-        float x[8] = {};
-        if (slot >= 0 && page < p.l.n_pages) {
-            const uint8_t* block = p.blocks + ((long long)page * p.l.kv_heads + head) * p.l.block;
-            const int at = (val ? p.l.page_size : 0) + row;
-            const uint32_t w = reinterpret_cast<const uint32_t*>(block + at * (D / 2))[sub];
-            const uint8_t* sp = block + p.l.page_size * D;
-            const float s = FMT == B4_KV_INT4 ? __half2float(reinterpret_cast<const __half*>(sp)[at])
-                                              : reinterpret_cast<const float*>(sp)[at];
+    const int sub = threadIdx.x % TPV;
+    const long long first = (long long)blockIdx.x * (kAppendUnroll * per) + threadIdx.x / TPV;
+    uint32_t w[kAppendUnroll];
+    float s[kAppendUnroll];
+    float* dst[kAppendUnroll];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const int c = (w >> (4 * j)) & 15;
-                x[j] = __fmul_rn(FMT == B4_KV_INT4 ? (float)(c - 8) : c_nf4_table[c], s);
-            }
+    for (int u = 0; u < kAppendUnroll; ++u) {
+        const long long i = min(first + u * per, p.n - 1);
+        const VectorIndex v = vector_index(i, p.l.kv_heads, p.magic);
+        const int slot = __ldg(p.slots + v.token), page = slot >> p.l.page_shift, row = slot & (p.l.page_size - 1);
+        w[u] = FMT == B4_KV_INT4 ? 0x88888888u : 0x77777777u;      // zeros outside the cache
+        s[u] = 0.0f;
+        if (slot >= 0 && page < p.l.n_pages) {
+            const uint8_t* block = p.blocks + ((long long)page * p.l.kv_heads + v.head) * p.l.block;
+            const int at = (v.value ? p.l.page_size : 0) + row;
+            w[u] = reinterpret_cast<const uint32_t*>(block + at * (D / 2))[sub];
+            const uint8_t* sp = block + p.l.page_size * D;
+            s[u] = FMT == B4_KV_INT4 ? __half2float(reinterpret_cast<const __half*>(sp)[at]) : reinterpret_cast<const float*>(sp)[at];
         }
-        float4* o = reinterpret_cast<float4*>((val ? p.v : p.k) + ((long long)token * p.l.kv_heads + head) * D) + 2 * sub;
-        o[0] = make_float4(x[0], x[1], x[2], x[3]);
-        o[1] = make_float4(x[4], x[5], x[6], x[7]);
+        dst[u] = first + u * per < p.n ? (v.value ? p.v : p.k) + ((long long)v.token * p.l.kv_heads + v.head) * D + sub * 8 : nullptr;
+    }
+#pragma unroll
+    for (int u = 0; u < kAppendUnroll; ++u) {
+        float x[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const uint32_t c = w[u] >> (4 * j);
+            x[j] = __fmul_rn(FMT == B4_KV_INT4 ? (float)((int)(c & 15) - 8) : __shfl_sync(0xffffffffu, level, c & 15), s[u]);
+        }
+        if (!dst[u]) continue;
+        reinterpret_cast<float4*>(dst[u])[0] = make_float4(x[0], x[1], x[2], x[3]);
+        reinterpret_cast<float4*>(dst[u])[1] = make_float4(x[4], x[5], x[6], x[7]);
     }
 }
+
+// blocks of a launch over n vectors, and the divisor's magic number
+inline long long vector_blocks(long long n, int head_dim)
+{
+    const int per = kAppendUnroll * 256 / (head_dim / 8);
+    return (n + per - 1) / per;
+}
+
+inline unsigned long long vector_magic(int kv_heads) { return ~0ULL / (2ULL * kv_heads) + 1; }
 
 template <typename T, int FMT>
 cudaError_t append(const AppendParams& p, cudaStream_t st)
 {
-    const int per = 256 / (p.l.head_dim / 8);
-    const dim3 grid((unsigned)std::min<long long>((p.n + per - 1) / per, 148LL * 64));
-    return p.l.head_dim == 64 ? kv_launch(kv_append_kernel<T, FMT, 64>, grid, 256, 0, st, p)
-                              : kv_launch(kv_append_kernel<T, FMT, 128>, grid, 256, 0, st, p);
+    const long long strides = p.k_tok | p.k_head | p.v_tok | p.v_head;
+    const bool vec = kv_aligned(p.k, 16) && kv_aligned(p.v, 16) && strides * (long long)sizeof(T) % 16 == 0;
+    const dim3 grid((unsigned)vector_blocks(p.n, p.l.head_dim));
+    if (p.l.head_dim == 64)
+        return vec ? kv_launch(kv_append_kernel<T, FMT, 64, true>, grid, 256, 0, st, p) : kv_launch(kv_append_kernel<T, FMT, 64, false>, grid, 256, 0, st, p);
+    return vec ? kv_launch(kv_append_kernel<T, FMT, 128, true>, grid, 256, 0, st, p) : kv_launch(kv_append_kernel<T, FMT, 128, false>, grid, 256, 0, st, p);
 }
 
 }  // namespace
@@ -294,14 +416,14 @@ int b4_kv_tables(const b4_kv_step* s, b4_stream_t stream)
     if (s->n_req > 0 && (!s->cached || !s->added || !s->ctx_len || (s->table_width > 0 && !s->tables))) return cudaErrorInvalidValue;
     if ((s->ring_size > 0 && !s->free_pages) || (s->max_tokens > 0 && (!s->slots || !s->positions))) return cudaErrorInvalidValue;
     if (s->free_state_out < s->free_state + 2 && s->free_state < s->free_state_out + 3) return cudaErrorInvalidValue;
-    const size_t smem = 8 * (size_t)s->n_req;
+    const size_t smem = 12 * (size_t)s->n_req;
     if (smem > 48 * 1024) {
-        const cudaError_t e = cudaFuncSetAttribute(kv_tables_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 8 * B4_KV_MAX_REQUESTS);
+        const cudaError_t e = cudaFuncSetAttribute(kv_tables_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 12 * B4_KV_MAX_REQUESTS);
         if (e != cudaSuccess) return e;
     }
-    const long long want = ((long long)s->max_tokens + 4 * kTabThreads - 1) / (4 * kTabThreads);
-    return kv_launch(kv_tables_kernel, dim3((unsigned)std::max<long long>(1, std::min<long long>(want, 148))), kTabThreads, smem,
-                     reinterpret_cast<cudaStream_t>(stream), *s);
+    const long long want = ((long long)s->max_tokens + kTabThreads - 1) / kTabThreads;
+    return kv_launch(kv_tables_kernel, dim3((unsigned)std::max<long long>(1, std::min<long long>(want, kTabGrid))), kTabThreads, smem,
+                     reinterpret_cast<cudaStream_t>(stream), *s, s->page_size == 16 ? 4 : s->page_size == 32 ? 5 : 6);
 }
 
 int b4_kv_append(const b4_kv_cache* cache, const void* k, const void* v, int dtype, long long k_stride_token,
@@ -324,6 +446,8 @@ int b4_kv_append(const b4_kv_cache* cache, const void* k, const void* v, int dty
     p.v_head = v_stride_head;
     p.slots = slots;
     p.n = 2LL * n_tokens * cache->kv_heads;
+    p.magic = vector_magic(cache->kv_heads);
+    if (vector_blocks(p.n, cache->head_dim) > 0x7fffffffLL) return cudaErrorInvalidValue;
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     const bool i4 = cache->fmt == B4_KV_INT4;
     if (dtype == B4_DTYPE_F16) return i4 ? append<__half, B4_KV_INT4>(p, st) : append<__half, B4_KV_NF4>(p, st);
@@ -343,8 +467,10 @@ int b4_kv_read(const b4_kv_cache* cache, const int32_t* slots, int n_tokens, flo
     p.slots = slots;
     p.k = k;
     p.v = v;
-    p.n = 2LL * n_tokens * cache->kv_heads * (cache->head_dim / 8);
-    const dim3 grid((unsigned)std::min<long long>((p.n + 255) / 256, 148LL * 64));
+    p.n = 2LL * n_tokens * cache->kv_heads;
+    p.magic = vector_magic(cache->kv_heads);
+    if (vector_blocks(p.n, cache->head_dim) > 0x7fffffffLL) return cudaErrorInvalidValue;
+    const dim3 grid((unsigned)vector_blocks(p.n, cache->head_dim));
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     if (cache->fmt == B4_KV_INT4)
         return cache->head_dim == 64 ? kv_launch(kv_read_kernel<B4_KV_INT4, 64>, grid, 256, 0, st, p)
