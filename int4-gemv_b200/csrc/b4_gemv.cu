@@ -1688,9 +1688,9 @@ int b4_gemv_multi_ws(int fmt, const b4_gemv_segment* segs, int nseg, const void*
 
 int b4_device_error(int clear)
 {
-    const int a = gemv_tma_device_error(clear), b = xtab_device_error(clear);
-    if (a < 0 || b < 0) return -1;
-    return a | b;
+    const int a = gemv_tma_device_error(clear), b = xtab_device_error(clear), c = kv_attn_device_error(clear);
+    if (a < 0 || b < 0 || c < 0) return -1;
+    return a | b | c;
 }
 
 int b4_empty_launch(b4_stream_t stream)

@@ -68,4 +68,7 @@ void default_config_ws(const GemvProblem& p, b4_gemv_config* cfg);
 // counters.  cudaErrorNotSupported when the rule does not take the shape.
 int launch_xtab_shard(const GemvProblem& p, const float* xgu, int flags, void* ws, cudaStream_t st);
 
+// The device error flag of the cache attention's kernels (b4_device_error).
+int kv_attn_device_error(int clear);
+
 }  // namespace b4

@@ -13,6 +13,8 @@ struct AttnParams {
     const uint8_t* blocks;
     b4_kv_attn a;
     int group;              // query heads that share a kv head
+    int rows_above;         // the tile kernel takes requests of more rows (queries x group) than this, the warp kernel
+    int rows_upto;          // those of at most this many
 };
 
 constexpr int kChunk = 32;  // tokens that a warp takes at a time: one page of 32, two of 16, half of one of 64
@@ -82,6 +84,9 @@ __device__ __forceinline__ void copy_async16(uint32_t dst, const void* src)
 {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
+
+// A maximum that no score has set yet: finite, so that differences with it are.
+constexpr float kNoMax = -1e30f;
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 

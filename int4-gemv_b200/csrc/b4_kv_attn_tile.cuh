@@ -1,0 +1,777 @@
+// b4_kv_attn_tile.cuh -- attention over the 4-bit cache for many queries a request
+// (prompt chunks, long drafts): products of 128 x 128 tiles on the tcgen05 pipe.
+//
+// Mathematics.  The queries that share a kv head (query tokens x heads of the
+// group) are rows; a CTA takes 256 of them (two tiles of 128) through the keys in
+// blocks of 128:
+//   S = Q K^T  (Q, K in shared memory),  O += P V  (P in tensor memory, V in shared)
+// with fp16 operands and fp32 accumulators in tensor memory.  K and V hold the bare
+// levels (INT4: exact integers; NF4: rounded to fp16, kNf4Up), so a token's key
+// scale multiplies a column of S and its value scale a column of P, in fp32.
+// Softmax is the warp kernel's (b4_kv_attn_warp.cuh): a row a thread, a maximum
+// that moves only when a score passes it by 2^8, weights relative to it and to a
+// running power of two of the value scales, rounded to fp16 for the product.
+//
+// Roles.  Warps 0-3 and 4-7: softmax of the two tiles, so that one tile's products
+// run under the other's exponentials.  Warps 8-11: codes to fp16 operands, a token a
+// thread, in the 128-byte swizzle (the same bytes serve K, whose columns are the
+// product's depth, and V, whose rows are).  Warp 12: issues the products.  Warp 13:
+// the schedule.  K and V are double-buffered; S and P of a tile share 128 columns of
+// tensor memory, the two O the other 256.
+//
+// Split.  The (request, row tile, head, key block) units of the whole call, only
+// those that some row sees, form one sequence and every CTA gets an equal run of it;
+// a segment (request, tile, head) that crosses CTAs is joined by the last of them to
+// arrive, in order, as in the warp kernel.
+//
+// Every wait is bounded (2 s): one that runs out raises the device error flag and
+// ends the CTA.
+#pragma once
+
+#include "b4_kv_attn.cuh"
+#include "b4_tma.cuh"
+
+namespace b4 {
+
+constexpr int kTileRows = 256, kTileKeys = 128, kTileThreads = 512;
+
+template <int FMT, int D>
+struct TileCfg {
+    static constexpr int kRow = D / 2, kScale = FMT == B4_KV_INT4 ? 2 : 4;
+    static constexpr int kOperand = 128 * D * 2;                   // bytes of 128 rows of D fp16: D / 64 parts of 128 x 128 bytes
+    // NF4: pairs of levels by byte, 256 rows of 16 copies (2 lanes a copy), at shared address 16384, so that an OR makes
+    // a lookup's address; the operands follow it.  Without it they follow the static part.
+    static constexpr int kTable = 16384, kStatic = 10240;
+    static constexpr int kPiece = kTileRows * (D + 2);             // floats: output, maxima, sums
+    static constexpr int kSmem = 6 * kOperand + (FMT == B4_KV_NF4 ? 2 * kTable - kStatic : 1024);   // kStatic: less than the static part and the system's
+};
+
+struct TileSeg {               // a run's part of a segment
+    int q0, n, ctx, head, tile, r, blk0, blk1;
+    int first, last, end;      // whether it has the segment's first, last block; the run is over
+    long long s0, s1;          // the segment's units
+};
+
+struct TileWs {
+    int* count;
+    float* cross;              // [grid][2] a CTA's part of a segment that began before it / goes on after it
+};
+
+// ---- tcgen05 ----------------------------------------------------------------------
+__device__ __forceinline__ uint64_t umma_desc(uint32_t at, uint32_t lbo, uint32_t sbo)
+{
+    // start, leading and stride byte offsets in 16 bytes; version 1; 128-byte swizzle
+    return (uint64_t)((at >> 4) & 0x3fff) | (uint64_t)((lbo >> 4) & 0x3fff) << 16 | (uint64_t)((sbo >> 4) & 0x3fff) << 32 | 1ULL << 46 | 2ULL << 61;
+}
+
+// fp32 accumulators, fp16 operands; `mn`: the right operand's rows are the product's depth
+__host__ __device__ constexpr uint32_t umma_idesc(int m, int n, bool mn)
+{
+    return 1u << 4 | (mn ? 1u << 16 : 0u) | (uint32_t)(n >> 3) << 17 | (uint32_t)(m >> 4) << 24;
+}
+
+__device__ __forceinline__ void umma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add)
+{
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)
+                 : "memory");
+}
+
+__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add)
+{
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)
+                 : "memory");
+}
+
+__device__ __forceinline__ void umma_commit(uint64_t* bar)
+{
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar)) : "memory");
+}
+
+__device__ __forceinline__ void tmem_before_sync() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tmem_after_sync() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+#define B4_R8(r, i) "=r"((r)[i]), "=r"((r)[i + 1]), "=r"((r)[i + 2]), "=r"((r)[i + 3]), "=r"((r)[i + 4]), "=r"((r)[i + 5]), "=r"((r)[i + 6]), "=r"((r)[i + 7])
+#define B4_W8(r, i) "r"((r)[i]), "r"((r)[i + 1]), "r"((r)[i + 2]), "r"((r)[i + 3]), "r"((r)[i + 4]), "r"((r)[i + 5]), "r"((r)[i + 6]), "r"((r)[i + 7])
+
+// 32 columns of the warp's 32 lanes
+__device__ __forceinline__ void tmem_ld32(uint32_t* r, uint32_t at)
+{
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : B4_R8(r, 0), B4_R8(r, 8), B4_R8(r, 16), B4_R8(r, 24)
+        : "r"(at));
+}
+
+__device__ __forceinline__ void tmem_ld16(uint32_t* r, uint32_t at)
+{
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                 : B4_R8(r, 0), B4_R8(r, 8)
+                 : "r"(at));
+}
+
+__device__ __forceinline__ void tmem_st16(uint32_t at, const uint32_t* r)
+{
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(at),
+                 B4_W8(r, 0), B4_W8(r, 8)
+                 : "memory");
+}
+#undef B4_R8
+#undef B4_W8
+
+__device__ __forceinline__ unsigned long long now_ns()
+{
+    unsigned long long t;
+    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+    return t;
+}
+
+// Waits for a phase; false when the CTA gave up (here or elsewhere).
+__device__ __forceinline__ bool tile_wait(uint64_t* bar, uint32_t phase, volatile int* dead)
+{
+    if (mbar_try_wait(bar, phase)) return true;
+    const unsigned long long t0 = now_ns();
+    for (;;) {
+#pragma unroll 1
+        for (int i = 0; i < 16; ++i)
+            if (mbar_try_wait(bar, phase)) return true;
+        if (*dead) return false;
+        if (now_ns() - t0 > 2000000000ULL) {
+            *dead = 1;
+            atomicOr(&g_device_error, kErrMbarrierTimeout);
+            return false;
+        }
+    }
+}
+
+// ... by a whole warp, with one answer
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t phase, volatile int* dead)
+{
+    return __all_sync(0xffffffffu, tile_wait(bar, phase, dead));
+}
+
+template <int R>
+__device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(R)); }
+template <int R>
+__device__ __forceinline__ void regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(R)); }
+
+// the blocks of keys that some row of a request's tile sees; one even where none is seen
+__device__ __forceinline__ void tile_blocks(const AttnParams& p, int n, int ctx, int tile, int& b0, int& b1)
+{
+    const unsigned g = p.group;
+    const int rows = n * p.group, t0 = (int)((unsigned)(tile * kTileRows) / g), t1 = (int)((unsigned)(min((tile + 1) * kTileRows, rows) - 1) / g);
+    const int end = p.a.flags & B4_KV_FULL ? ctx : max(0, min(ctx, ctx - n + t1 + 1));
+    const int begin = p.a.window > 0 ? max(0, ctx - n + t0 + 1 - p.a.window) : 0;
+    b0 = begin / kTileKeys;
+    b1 = max(b0 + 1, (end + kTileKeys - 1) / kTileKeys);
+}
+
+template <typename T, int FMT, int D>
+__global__ void __launch_bounds__(kTileThreads, 1) kv_attn_tile_kernel(const AttnParams p, const TileWs ws)
+{
+    using C = TileCfg<FMT, D>;
+    extern __shared__ __align__(1024) uint8_t tile_smem[];
+    __shared__ uint64_t seg_full[2], seg_empty[2], q_full[2], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_done[2], scale_full[4], tops, team, drain;
+    __shared__ TileSeg segs[2];
+    __shared__ long long units_before[kTileThreads + 1];
+    __shared__ int tiles_before[kTileThreads + 1];
+    __shared__ long long warp_sum[kTileThreads / 32];
+    __shared__ __align__(16) float key_scale[4][kTileKeys], value_scale[4][kTileKeys];
+    __shared__ int value_exp[4], block_pages[4];
+    __shared__ __align__(16) float value_top[2][4];
+    __shared__ uint32_t tmem_at;
+    __shared__ volatile int dead;
+    __shared__ int joins;
+
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const b4_kv_attn& a = p.a;
+    const uint32_t operands = FMT == B4_KV_NF4 ? 2 * C::kTable : (smem_addr(tile_smem) + 1023) & ~1023u;
+    auto operand = [&](uint32_t i) -> uint32_t { return operands + i * C::kOperand; };          // Q of both tiles, K twice, V twice
+    if (tid == 0) {
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&seg_full[i], 1);
+            mbar_init(&seg_empty[i], 13);
+            mbar_init(&q_full[i], 4);
+            mbar_init(&k_full[i], 4);
+            mbar_init(&k_empty[i], 1);
+            mbar_init(&v_full[i], 4);
+            mbar_init(&v_empty[i], 1);
+            mbar_init(&s_full[i], 1);
+            mbar_init(&p_full[i], 4);
+            mbar_init(&o_done[i], 1);
+        }
+        for (int i = 0; i < 4; ++i) mbar_init(&scale_full[i], 4);
+        mbar_init(&tops, 4);
+        mbar_init(&team, 8);
+        mbar_init(&drain, 1);
+        dead = 0;
+    }
+    if (warp == 12) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_addr(&tmem_at)) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
+    if (FMT == B4_KV_NF4) {
+        for (int i = tid; i < 256 * 4; i += kTileThreads) {
+            const uint32_t v = nf4_pair(i >> 2);
+            asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(C::kTable + i * 16), "r"(v) : "memory");
+        }
+    }
+    fence_mbar_init();
+    kv_begin();
+
+    // ---- the call's units: tiles of all requests, then each tile's heads and blocks ----
+    auto taken = [&](const AttnReq& q) { return q.n * p.group > p.rows_above; };
+    auto tiles_of = [&](int r) {
+        const AttnReq q = attn_request(p, r);
+        return taken(q) ? (q.n * p.group + kTileRows - 1) / kTileRows : 0;
+    };
+    auto scan = [&](long long v) {             // exclusive sums over the threads; the total comes back in all
+        long long inc = v;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long x = __shfl_up_sync(0xffffffffu, inc, o);
+            if (lane >= o) inc += x;
+        }
+        __syncthreads();
+        if (lane == 31) warp_sum[warp] = inc;
+        __syncthreads();
+        long long before = inc - v;
+        for (int w = 0; w < warp; ++w) before += warp_sum[w];
+        return before;
+    };
+    const int per = (a.n_req + kTileThreads - 1) / kTileThreads;
+    {
+        int mine = 0;
+        for (int i = 0; i < per; ++i)
+            if (tid * per + i < a.n_req) mine += tiles_of(tid * per + i);
+        const long long before = scan(mine);
+        tiles_before[tid] = (int)before;
+        if (tid == kTileThreads - 1) tiles_before[kTileThreads] = (int)before + mine;
+        __syncthreads();
+    }
+    const int all_tiles = tiles_before[kTileThreads];
+    // a place in the sequence of tiles
+    struct Cursor {
+        int r, tile, tiles;
+        AttnReq q;
+    };
+    auto seek = [&](int tile) {
+        Cursor c;
+        int lo = 0;
+#pragma unroll 1
+        for (int step = kTileThreads / 2; step > 0; step >>= 1)
+            if (tiles_before[lo + step] <= tile) lo += step;
+        c.r = lo * per;
+        tile -= tiles_before[lo];
+        for (;; ++c.r) {
+            c.tiles = tiles_of(c.r);
+            if (tile < c.tiles || c.r >= a.n_req - 1) break;
+            tile -= c.tiles;
+        }
+        c.tile = tile;
+        c.q = attn_request(p, c.r);
+        return c;
+    };
+    auto next = [&](Cursor& c) {
+        if (++c.tile < c.tiles) return;
+        c.tile = 0;
+        do {
+            c.tiles = ++c.r < a.n_req ? tiles_of(c.r) : 1;
+        } while (c.tiles == 0);
+        if (c.r < a.n_req) c.q = attn_request(p, c.r);
+    };
+    const int t_first = (int)((long long)tid * all_tiles / kTileThreads), t_last = (int)((long long)(tid + 1) * all_tiles / kTileThreads);
+    {
+        long long mine = 0;
+        if (t_first < t_last) {
+            Cursor c = seek(t_first);
+            for (int i = t_first; i < t_last; ++i) {
+                int b0, b1;
+                tile_blocks(p, c.q.n, c.q.ctx, c.tile, b0, b1);
+                mine += (long long)(b1 - b0) * p.l.kv_heads;
+                if (i + 1 < t_last) next(c);
+            }
+        }
+        const long long before = scan(mine);
+        units_before[tid] = before;
+        if (tid == kTileThreads - 1) units_before[kTileThreads] = before + mine;
+        tmem_before_sync();
+        __syncthreads();
+        tmem_after_sync();
+    }
+    const long long total = units_before[kTileThreads];
+    const int ctas = (int)min((long long)gridDim.x, total), cta = blockIdx.x;
+    const long long share = ctas > 0 ? total / ctas : 0, rest = ctas > 0 ? total - share * ctas : 0;
+    const long long u0 = cta < ctas ? cta * share + min((long long)cta, rest) : 0, u1 = cta < ctas ? u0 + share + (cta < rest) : 0;
+    auto owner = [&](long long u) { return (int)(u < rest * (share + 1) ? u / (share + 1) : rest + (u - rest * (share + 1)) / share); };
+    const uint32_t tmem = tmem_at;
+
+    if (warp >= 12) {
+        regs_down<64>();
+        if (warp == 13) {
+            // ---- schedule ----
+            long long u = u0;
+            int k = 0;
+            Cursor c = {};
+            long long at = 0;
+            if (u < u1) {
+                int lo = 0;
+#pragma unroll 1
+                for (int step = kTileThreads / 2; step > 0; step >>= 1)
+                    if (units_before[lo + step] <= u) lo += step;
+                at = units_before[lo];
+                c = seek((int)((long long)lo * all_tiles / kTileThreads));
+            }
+            for (;;) {
+                TileSeg s = {};
+                if (u < u1 && c.r < a.n_req) {
+                    int b0, b1;
+                    tile_blocks(p, c.q.n, c.q.ctx, c.tile, b0, b1);
+                    const long long blocks = b1 - b0;
+                    if (u >= at + blocks * p.l.kv_heads) {
+                        at += blocks * p.l.kv_heads;
+                        next(c);
+                        continue;
+                    }
+                    s.q0 = c.q.q0;
+                    s.n = c.q.n;
+                    s.ctx = c.q.ctx;
+                    s.tile = c.tile;
+                    s.r = c.r;
+                    s.head = (int)((u - at) / blocks);
+                    s.s0 = at + s.head * blocks;
+                    s.s1 = s.s0 + blocks;
+                    s.blk0 = b0 + (int)(u - s.s0);
+                    const long long stop = min(s.s1, u1);
+                    s.blk1 = s.blk0 + (int)(stop - u);
+                    s.first = u == s.s0;
+                    s.last = stop == s.s1;
+                    u = stop;
+                } else {
+                    s.end = 1;
+                }
+                if (k >= 2 && !warp_wait(&seg_empty[k & 1], (k >> 1) + 1 & 1, &dead)) break;
+                if (lane == 0) {
+                    segs[k & 1] = s;
+                    mbar_arrive(&seg_full[k & 1]);
+                }
+                __syncwarp();
+                ++k;
+                if (s.end) break;
+            }
+        } else if (warp == 12) {
+            // ---- products ----
+            if (lane == 0) {
+            int ks = 0, vs = 0, cq[2] = {0, 0}, cp[2] = {0, 0};
+            constexpr uint32_t id_s = umma_idesc(128, kTileKeys, false), id_o = umma_idesc(128, D, true);
+            auto scores = [&](int x, int stage) {
+                const uint64_t q = umma_desc(operand(x), 16, 1024), k = umma_desc(operand(2 + stage), 16, 1024);
+#pragma unroll
+                for (int i = 0; i < D / 16; ++i) {
+                    const uint64_t step = (uint64_t)((i >> 2) * (16384 >> 4) + (i & 3) * 2);
+                    umma_ss(tmem + x * 128, q + step, k + step, id_s, i > 0);
+                }
+                umma_commit(&s_full[x]);
+            };
+            auto outputs = [&](int x, int stage, bool add) {
+                const uint64_t v = umma_desc(operand(4 + stage), 16384, 1024);
+#pragma unroll
+                for (int i = 0; i < kTileKeys / 16; ++i)
+                    umma_ts(tmem + 256 + x * 128, tmem + x * 128 + i * 8, v + (uint64_t)(i * (2048 >> 4)), id_o, add || i > 0);
+                umma_commit(&o_done[x]);
+            };
+            bool ok = true;
+            for (int k = 0; ok; ++k) {
+                if (!(ok = tile_wait(&seg_full[k & 1], k >> 1 & 1, &dead))) break;
+                const int blocks = segs[k & 1].blk1 - segs[k & 1].blk0, end = segs[k & 1].end;
+                const int tiles = segs[k & 1].n * p.group - segs[k & 1].tile * kTileRows > 128 ? 2 : 1;
+                mbar_arrive(&seg_empty[k & 1]);
+                if (end) break;
+                for (int x = 0; x < tiles && ok; ++x) ok = tile_wait(&q_full[x], cq[x]++ & 1, &dead);
+                ok = ok && tile_wait(&k_full[ks & 1], ks >> 1 & 1, &dead);
+                if (!ok) break;
+                tmem_after_sync();
+                for (int x = 0; x < tiles; ++x) scores(x, ks & 1);
+                umma_commit(&k_empty[ks & 1]);
+                ++ks;
+                for (int i = 0; i < blocks && ok; ++i) {
+                    ok = tile_wait(&v_full[vs & 1], vs >> 1 & 1, &dead);
+                    for (int x = 0; x < tiles && ok; ++x) {
+                        if (!(ok = tile_wait(&p_full[x], cp[x]++ & 1, &dead))) break;
+                        tmem_after_sync();
+                        outputs(x, vs & 1, i > 0);
+                        if (x == tiles - 1) umma_commit(&v_empty[vs & 1]);
+                        if (i + 1 < blocks) {
+                            if (x == 0 && !(ok = tile_wait(&k_full[ks & 1], ks >> 1 & 1, &dead))) break;
+                            tmem_after_sync();
+                            scores(x, ks & 1);
+                            if (x == tiles - 1) umma_commit(&k_empty[ks & 1]);
+                        }
+                    }
+                    ++vs;
+                    if (i + 1 < blocks) ++ks;
+                }
+            }
+            umma_commit(&drain);               // nothing in flight when the CTA ends
+            for (int i = 0; i < 1 << 20 && !mbar_try_wait(&drain, 0); ++i) {}
+            }
+            __syncwarp();
+        }
+    } else if (warp >= 8) {
+        // ---- codes to operands: a token a thread ----
+        regs_down<96>();
+        const int t = tid - 256;
+        constexpr int W = D / 8;               // words of a token's codes
+        int ks = 0, vs = 0;
+        bool ok = true;
+        const uint32_t row_at = t * 128, swizzle = (t & 7) << 4;
+        auto write = [&](uint32_t to, const uint4 (&raw)[W / 4]) {
+            const uint32_t* w = reinterpret_cast<const uint32_t*>(raw);
+#pragma unroll
+            for (int i = 0; i < W; ++i) {
+                uint32_t h[4];
+                if (FMT == B4_KV_INT4) {
+                    int4_word_to_half2(w[i], h);
+                } else {
+                    const uint32_t copy = C::kTable | (lane & 15) * 4;
+                    h[0] = lds32((w[i] << 6 & 0x3fc0u) | copy);
+                    h[1] = lds32((w[i] >> 2 & 0x3fc0u) | copy);
+                    h[2] = lds32((w[i] >> 10 & 0x3fc0u) | copy);
+                    h[3] = lds32((w[i] >> 18 & 0x3fc0u) | copy);
+                }
+                asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(to + (i >> 3) * 16384 + row_at + (((i & 7) << 4) ^ swizzle)),
+                             "r"(h[0]), "r"(h[1]), "r"(h[2]), "r"(h[3])
+                             : "memory");
+            }
+            fence_proxy_async();
+            __syncwarp();
+        };
+        for (int k = 0; ok; ++k) {
+            if (!(ok = warp_wait(&seg_full[k & 1], k >> 1 & 1, &dead))) break;
+            const TileSeg s = segs[k & 1];
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&seg_empty[k & 1]);
+            if (s.end) break;
+            const int rows = s.n * p.group, last_row = min((s.tile + 1) * kTileRows, rows) - 1;
+            const int see_end = a.flags & B4_KV_FULL ? s.ctx : min(s.ctx, s.ctx - s.n + last_row / p.group + 1);
+            const int see_begin = a.window > 0 ? s.ctx - s.n + s.tile * kTileRows / p.group + 1 - a.window : 0;
+            const int32_t* ids = a.tables + (long long)s.r * a.table_stride;
+            auto page_id = [&](int blk) {
+                const int token = blk * kTileKeys + t;
+                return blk < s.blk1 && token < s.ctx ? __ldg(ids + (token >> p.l.page_shift)) : -1;
+            };
+            int id = page_id(s.blk0), id_next = page_id(s.blk0 + 1), vexp = -126;
+            uint4 kr[W / 4], vr[W / 4];
+            float ksc, vsc;
+            bool there, there_v;
+            auto block_of = [&](int page) { return p.blocks + ((long long)page * p.l.kv_heads + s.head) * p.l.block; };
+            const int row = t & (p.l.page_size - 1);
+            auto load_k = [&](int page) {
+                there = (unsigned)page < (unsigned)p.l.n_pages;
+#pragma unroll
+                for (int i = 0; i < W / 4; ++i) kr[i] = make_uint4(0, 0, 0, 0);
+                ksc = vsc = 0.0f;
+                if (there) {
+                    const uint8_t* b = block_of(page);
+#pragma unroll
+                    for (int i = 0; i < W / 4; ++i) kr[i] = __ldg(reinterpret_cast<const uint4*>(b + row * C::kRow) + i);
+                    const uint8_t* sp = b + p.l.page_size * D + row * C::kScale;
+                    if (FMT == B4_KV_INT4) {
+                        ksc = __half2float(*reinterpret_cast<const __half*>(sp));
+                        vsc = __half2float(*reinterpret_cast<const __half*>(sp + p.l.page_size * C::kScale));
+                    } else {
+                        ksc = *reinterpret_cast<const float*>(sp);
+                        vsc = *reinterpret_cast<const float*>(sp + p.l.page_size * C::kScale);
+                    }
+                }
+            };
+            auto load_v = [&](int page) {
+                there_v = (unsigned)page < (unsigned)p.l.n_pages;
+#pragma unroll
+                for (int i = 0; i < W / 4; ++i) vr[i] = make_uint4(0, 0, 0, 0);
+                if (there_v) {
+                    const uint8_t* b = block_of(page) + (p.l.page_size + row) * C::kRow;
+#pragma unroll
+                    for (int i = 0; i < W / 4; ++i) vr[i] = __ldg(reinterpret_cast<const uint4*>(b) + i);
+                }
+            };
+            load_k(id);
+            load_v(id);
+            for (int blk = s.blk0; blk < s.blk1 && ok; ++blk) {
+                const int id_after = page_id(blk + 2), ring = ks & 3;
+                // scales: those of tokens that no row sees are 0, the values' relative to a running power of two
+                const int token = blk * kTileKeys + t;
+                const bool seen = there && token < see_end && token >= see_begin;
+                float v = seen ? fminf(vsc, 3.4028235e38f) : 0.0f;
+                const unsigned bits = __reduce_max_sync(0xffffffffu, v < 3.4028235e38f ? __float_as_uint(fabsf(v)) : 0u);
+                const unsigned pages = __ballot_sync(0xffffffffu, there);
+                if (lane == 0) {
+                    value_top[ks & 1][warp - 8] = __uint_as_float(bits);
+                    mbar_arrive(&tops);
+                }
+                __syncwarp();
+                if (!(ok = warp_wait(&tops, ks & 1, &dead))) break;
+                const float4 tv = *reinterpret_cast<const float4*>(value_top[ks & 1]);
+                const float top = fmaxf(fmaxf(tv.x, tv.y), fmaxf(tv.z, tv.w));
+                vexp = max(vexp, min((int)(__float_as_uint(top) >> 23) - 126, 126));
+                key_scale[ring][t] = seen ? ksc : 0.0f;
+                value_scale[ring][t] = v * pow2(-vexp);
+                if (t == 0) value_exp[ring] = vexp;
+                // tokens that are not there lie in whole pages of 16 at least: two bits a warp
+                if (lane == 0) reinterpret_cast<uint8_t*>(&block_pages[ring])[warp - 8] = (uint8_t)((pages & 1) | (pages >> 16 & 1) << 1);
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&scale_full[ring]);
+
+                if (ks >= 2 && !(ok = warp_wait(&k_empty[ks & 1], (ks >> 1) + 1 & 1, &dead))) break;
+                write(operand(2 + (ks & 1)), kr);
+                if (lane == 0) mbar_arrive(&k_full[ks & 1]);
+                ++ks;
+                if (blk + 1 < s.blk1) load_k(id_next);
+                if (vs >= 2 && !(ok = warp_wait(&v_empty[vs & 1], (vs >> 1) + 1 & 1, &dead))) break;
+                write(operand(4 + (vs & 1)), vr);
+                if (lane == 0) mbar_arrive(&v_full[vs & 1]);
+                ++vs;
+                if (blk + 1 < s.blk1) load_v(id_next);
+                id_next = id_after;
+            }
+        }
+    } else {
+        // ---- softmax: a row a thread ----
+        regs_up<176>();
+        const int x = warp >> 2, t = tid & 127;
+        const uint32_t lanes = (uint32_t)(warp & 3) << 21;          // 32 lanes a warp, lane in the upper half
+        const uint32_t s_at = tmem + lanes + x * 128, o_at = tmem + lanes + 256 + x * 128;
+        int cs = 0, ring0 = 0, teams = 0;      // this tile's blocks so far; all blocks so far
+        bool ok = true;
+        for (int k = 0; ok; ++k) {
+            if (!(ok = warp_wait(&seg_full[k & 1], k >> 1 & 1, &dead))) break;
+            const TileSeg s = segs[k & 1];
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&seg_empty[k & 1]);
+            if (s.end) break;
+            const int blocks = s.blk1 - s.blk0, rows = s.n * p.group, row0 = s.tile * kTileRows;
+            const bool two = rows - row0 > 128;
+            const int row = row0 + x * 128 + t;
+            const bool mine = row < rows;
+            const int token = row / p.group, head = s.head * p.group + (row - token * p.group);
+            float m = kNoMax, l = 0.0f;
+            int vexp = -126;
+            if (x == 0 || two) {
+                // the row's query: fp16 in the order of the decoded codes (bf16: times a power of two, as query_operand)
+                const uint4* src = reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + (s.q0 + token) * a.q_stride_token + head * a.q_stride_head);
+                float factor = 1.0f, up = 1.0f;
+                if (std::is_same<T, __nv_bfloat16>::value) {
+                    uint32_t top = 0;
+#pragma unroll 4
+                    for (int i = 0; i < D / 8; ++i) {
+                        const uint4 w = mine ? __ldg(src + i) : make_uint4(0, 0, 0, 0);
+                        const uint32_t y[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) top = max(top, max(y[j] << 16 & 0x7fffffffu, y[j] & 0x7fff0000u));
+                    }
+                    const int e = min(max((int)(top >> 23) - 127, -110), 126);
+                    up = pow2(10 - e);
+                    factor = pow2(e - 10);
+                }
+                const uint32_t sign = a.scale < 0.0f ? 0x80008000u : 0u;
+#pragma unroll 8
+                for (int i = 0; i < D / 8; ++i) {
+                    uint4 w = mine ? __ldg(src + i) : make_uint4(0, 0, 0, 0);
+                    if (std::is_same<T, __nv_bfloat16>::value) {
+                        uint32_t* y = reinterpret_cast<uint32_t*>(&w);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) y[j] = pack_half2(__uint_as_float(y[j] << 16) * up, __uint_as_float(y[j] & 0xffff0000u) * up);
+                    }
+                    if (FMT == B4_KV_INT4) w = int4_pair_order(w);
+                    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(operand(x) + (i >> 3) * 16384 + t * 128 + (((i & 7) ^ (t & 7)) << 4)),
+                                 "r"(w.x ^ sign), "r"(w.y ^ sign), "r"(w.z ^ sign), "r"(w.w ^ sign)
+                                 : "memory");
+                }
+                fence_proxy_async();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&q_full[x]);
+                const float qf = fmaxf(factor * (fabsf(a.scale) * kLog2e) * (FMT == B4_KV_NF4 ? 1.0f / kNf4Up : 1.0f), 1e-30f);
+                const int lim = a.flags & B4_KV_FULL ? s.ctx : min(s.ctx, s.ctx - s.n + token + 1);
+                const int from = a.window > 0 ? lim - a.window : 0;
+
+                for (int i = 0; i < blocks && ok; ++i, ++cs) {
+                    const int ring = (ring0 + i) & 3;
+                    if (!(ok = warp_wait(&scale_full[ring], (ring0 + i) >> 2 & 1, &dead))) break;
+                    if (!(ok = warp_wait(&s_full[x], cs & 1, &dead))) break;
+                    tmem_after_sync();
+                    float sc[kTileKeys];
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) tmem_ld32(reinterpret_cast<uint32_t*>(sc) + 32 * c, s_at + 32 * c);
+                    tmem_wait_ld();
+                    float2* s2 = reinterpret_cast<float2*>(sc);
+#pragma unroll
+                    for (int c = 0; c < kTileKeys / 4; ++c) {
+                        const float4 f = reinterpret_cast<const float4*>(key_scale[ring])[c];
+                        s2[2 * c] = __fmul2_rn(s2[2 * c], make_float2(f.x, f.y));
+                        s2[2 * c + 1] = __fmul2_rn(s2[2 * c + 1], make_float2(f.z, f.w));
+                    }
+                    const int key0 = (s.blk0 + i) * kTileKeys, pages = block_pages[ring];
+                    if (__any_sync(0xffffffffu, key0 + kTileKeys > lim || key0 < from || pages != 0x03030303)) {
+#pragma unroll
+                        for (int c = 0; c < kTileKeys; ++c)
+                            if (key0 + c >= lim || key0 + c < from || !(pages >> (c >> 5) * 8 + (c >> 4 & 1) & 1)) sc[c] = -INFINITY;
+                    }
+                    float top = -INFINITY;
+#pragma unroll
+                    for (int c = 0; c < kTileKeys; c += 2) top = fmaxf(top, fmaxf(sc[c], sc[c + 1]));
+                    const int ve = value_exp[ring];
+                    if (__any_sync(0xffffffffu, top * qf > m + 8.0f) || ve != vexp) {
+                        const float next = top == -INFINITY ? m : fmaxf(m, top * qf), keep_l = fast_exp2(m - next);
+                        const float keep = keep_l * pow2(max(vexp - ve, -126));
+                        m = next;
+                        vexp = ve;
+                        l *= keep_l;
+                        if (i > 0) {
+                            if (!(ok = warp_wait(&o_done[x], (cs - 1) & 1, &dead))) break;
+                            tmem_after_sync();
+#pragma unroll 1
+                            for (int c = 0; c < D; c += 16) {
+                                uint32_t o[16];
+                                tmem_ld16(o, o_at + c);
+                                tmem_wait_ld();
+#pragma unroll
+                                for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * keep);
+                                tmem_st16(o_at + c, o);
+                            }
+                            tmem_wait_st();
+                        }
+                    }
+                    const float2 q2 = make_float2(qf, qf), m2 = make_float2(-m, -m);
+                    float2 l2 = make_float2(0.0f, 0.0f);
+#pragma unroll
+                    for (int c = 0; c < kTileKeys / 32; ++c) {
+                        uint32_t w[16];
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) {
+                            const float4 f = reinterpret_cast<const float4*>(value_scale[ring])[8 * c + j];
+                            float2 e0 = __ffma2_rn(s2[16 * c + 2 * j], q2, m2), e1 = __ffma2_rn(s2[16 * c + 2 * j + 1], q2, m2);
+                            e0 = make_float2(fast_exp2(e0.x), fast_exp2(e0.y));
+                            e1 = make_float2(fast_exp2(e1.x), fast_exp2(e1.y));
+                            l2 = __fadd2_rn(l2, __fadd2_rn(e0, e1));
+                            e0 = __fmul2_rn(e0, make_float2(f.x, f.y));
+                            e1 = __fmul2_rn(e1, make_float2(f.z, f.w));
+                            w[2 * j] = pack_half2(e0.x, e0.y);
+                            w[2 * j + 1] = pack_half2(e1.x, e1.y);
+                        }
+                        tmem_st16(s_at + 16 * c, w);
+                    }
+                    l += l2.x + l2.y;
+                    tmem_wait_st();
+                    tmem_before_sync();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&p_full[x]);
+                }
+                if (!ok) break;
+                if (!(ok = warp_wait(&o_done[x], (cs - 1) & 1, &dead))) break;
+                tmem_after_sync();
+            }
+            ring0 += blocks;
+
+            // ---- the segment's rows, or a piece of them ----
+            const bool whole = s.first && s.last;
+            const float vup = pow2(vexp) * (FMT == B4_KV_NF4 ? 1.0f / kNf4Up : 1.0f);
+            float* piece = ws.cross + ((long long)cta * 2 + s.first) * C::kPiece;
+            if (x == 0 || two) {
+                const float inv = whole ? (l > 0.0f ? vup / l : 0.0f) : vup;
+                T* dst = static_cast<T*>(a.out) + (s.q0 + token) * a.out_stride_token + head * a.out_stride_head;
+#pragma unroll 1
+                for (int c = 0; c < D; c += 16) {
+                    uint32_t o[16];
+                    tmem_ld16(o, o_at + c);
+                    tmem_wait_ld();
+                    float y[16];
+#pragma unroll
+                    for (int j = 0; j < 16; ++j)   // INT4: decoded columns (0, 4, 1, 5, 2, 6, 3, 7) of each eight
+                        y[FMT == B4_KV_INT4 ? (j & 8) | (j >> 1 & 3) | (j & 1) << 2 : j] = __uint_as_float(o[j]) * inv;
+                    if (mine && whole) {
+#pragma unroll
+                        for (int j = 0; j < 16; j += 8) {
+                            uint32_t w[4];
+#pragma unroll
+                            for (int h = 0; h < 4; ++h) {
+                                const T lo = kv_round<T>(y[j + 2 * h]), hi = kv_round<T>(y[j + 2 * h + 1]);
+                                w[h] = (uint32_t)*reinterpret_cast<const uint16_t*>(&lo) | (uint32_t)*reinterpret_cast<const uint16_t*>(&hi) << 16;
+                            }
+                            *reinterpret_cast<uint4*>(dst + c + j) = make_uint4(w[0], w[1], w[2], w[3]);
+                        }
+                    } else if (mine) {
+#pragma unroll
+                        for (int j = 0; j < 16; j += 4)
+                            *reinterpret_cast<float4*>(piece + (x * 128 + t) * D + c + j) = make_float4(y[j], y[j + 1], y[j + 2], y[j + 3]);
+                    }
+                    __syncwarp();
+                }
+                tmem_before_sync();
+                if (whole && mine && a.lse) a.lse[(long long)(s.q0 + token) * a.heads + head] = l > 0.0f ? (m + fast_log2(l)) * kLn2 : -INFINITY;
+                if (!whole) {
+                    piece[kTileRows * D + x * 128 + t] = m;
+                    piece[kTileRows * (D + 1) + x * 128 + t] = l;
+                }
+            }
+            if (whole) continue;
+            // the last of the segment's CTAs joins them, in order: a row a warp
+            const int f = owner(s.s0), parts = owner(s.s1 - 1) - f + 1;
+            auto together = [&]() {            // the eight softmax warps
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&team);
+                return warp_wait(&team, teams++ & 1, &dead);
+            };
+            if (!(ok = together())) break;
+            if (tid == 0) {
+                __threadfence();
+                joins = atomicAdd(ws.count + f, 1) == parts - 1;
+                if (joins) ws.count[f] = 0;
+                __threadfence();
+            }
+            if (!(ok = together())) break;
+            const bool join = joins;
+            if (!(ok = together())) break;     // before the flag is written again
+            if (!join) continue;
+            auto part = [&](int i) -> const float* { return ws.cross + ((long long)(f + i) * 2 + (i == 0)) * C::kPiece; };
+            for (int r = warp; r < kTileRows && row0 + r < rows; r += 8) {
+                float top = kNoMax, sum = 0.0f;
+                for (int i = 0; i < parts; ++i) top = fmaxf(top, __ldcg(part(i) + kTileRows * D + r));
+                constexpr int E = D / 32;
+                float y[E] = {};
+#pragma unroll 2
+                for (int i = 0; i < parts; ++i) {
+                    const float* b = part(i);
+                    const float w = fast_exp2(__ldcg(b + kTileRows * D + r) - top);
+                    sum += w * __ldcg(b + kTileRows * (D + 1) + r);
+                    const float2* z = reinterpret_cast<const float2*>(b + r * D + lane * E);
+#pragma unroll
+                    for (int e = 0; e < E / 2; ++e) {
+                        const float2 v = __ldcg(z + e);
+                        y[2 * e] += w * v.x;
+                        y[2 * e + 1] += w * v.y;
+                    }
+                }
+                const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
+                const int tk = (row0 + r) / p.group, hd = s.head * p.group + (row0 + r - tk * p.group);
+                T* dst = static_cast<T*>(a.out) + (s.q0 + tk) * a.out_stride_token + hd * a.out_stride_head + lane * E;
+#pragma unroll
+                for (int e = 0; e < E; e += 2) {
+                    const T w[2] = {kv_round<T>(y[e] * inv), kv_round<T>(y[e + 1] * inv)};
+                    *reinterpret_cast<uint32_t*>(dst + e) =
+                        (uint32_t)*reinterpret_cast<const uint16_t*>(w) | (uint32_t)*reinterpret_cast<const uint16_t*>(w + 1) << 16;
+                }
+                if (a.lse && lane == 0) a.lse[(long long)(s.q0 + tk) * a.heads + hd] = sum > 0.0f ? (top + fast_log2(sum)) * kLn2 : -INFINITY;
+            }
+        }
+    }
+    tmem_before_sync();
+    __syncthreads();
+    tmem_after_sync();
+    if (warp == 12) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+}
+
+}  // namespace b4

@@ -72,9 +72,6 @@ struct WarpWs {                // the workspace: counters, then pieces that othe
     float* cross;              // [grid][2] a CTA's part of a segment that began before it / goes on after it
 };
 
-// A maximum that no score has set yet: finite, so that differences with it are.
-constexpr float kNoMax = -1e30f;
-
 template <typename T, int FMT, int D, int NT, int PT>
 __global__ void __launch_bounds__(WarpCfg<FMT, D, NT, PT>::kThreads, 1) kv_attn_warp_kernel(const AttnParams p, const WarpWs ws)
 {
@@ -104,7 +101,7 @@ __global__ void __launch_bounds__(WarpCfg<FMT, D, NT, PT>::kThreads, 1) kv_attn_
     kv_begin();
 
     // ---- the call's units, and each warp's run of them ----
-    auto tiles_of = [&](const AttnReq& q) { return (q.n * p.group + C::kCols - 1) / C::kCols; };
+    auto tiles_of = [&](const AttnReq& q) { return q.n * p.group <= p.rows_upto ? (q.n * p.group + C::kCols - 1) / C::kCols : 0; };
     auto units_of = [&](const AttnReq& q) { return (long long)p.l.kv_heads * tiles_of(q) * q.chunks; };
     const int per = (a.n_req + kScan - 1) / kScan;
     {

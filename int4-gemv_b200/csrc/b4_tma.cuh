@@ -46,6 +46,11 @@ __device__ __forceinline__ void mbar_arrive_expect_tx(uint64_t* bar, uint32_t by
                  : "memory");
 }
 
+__device__ __forceinline__ void mbar_arrive(uint64_t* bar)
+{
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(bar)) : "memory");
+}
+
 // 1-D bulk copy of `bytes` (a multiple of 16, both addresses 16-byte aligned)
 // from global memory into this CTA's shared memory; completion is counted on
 // `bar` in bytes.  The source is streamed once: evict-first in L2.
