@@ -130,15 +130,26 @@ __device__ __forceinline__ unsigned long long now_ns()
     return t;
 }
 
+__device__ __forceinline__ bool mbar_try_wait_long(uint64_t* bar, uint32_t phase)
+{
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_addr(bar)), "r"(phase), "r"(20000u)             // the thread may sleep for 20 us
+        : "memory");
+    return ok != 0;
+}
+
 // Waits for a phase; false when the CTA gave up (here or elsewhere).
 __device__ __forceinline__ bool tile_wait(uint64_t* bar, uint32_t phase, volatile int* dead)
 {
     if (mbar_try_wait(bar, phase)) return true;
     const unsigned long long t0 = now_ns();
     for (;;) {
-#pragma unroll 1
-        for (int i = 0; i < 16; ++i)
-            if (mbar_try_wait(bar, phase)) return true;
+        if (mbar_try_wait_long(bar, phase)) return true;
         if (*dead) return false;
         if (now_ns() - t0 > 2000000000ULL) {
             *dead = 1;
@@ -370,7 +381,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attn_tile_kernel(const Att
             constexpr uint32_t id_s = umma_idesc(128, kTileKeys, false), id_o = umma_idesc(128, D, true);
             auto scores = [&](int x, int stage) {
                 const uint64_t q = umma_desc(operand(x), 16, 1024), k = umma_desc(operand(2 + stage), 16, 1024);
-#pragma unroll
+#pragma unroll 1
                 for (int i = 0; i < D / 16; ++i) {
                     const uint64_t step = (uint64_t)((i >> 2) * (16384 >> 4) + (i & 3) * 2);
                     umma_ss(tmem + x * 128, q + step, k + step, id_s, i > 0);
@@ -379,7 +390,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attn_tile_kernel(const Att
             };
             auto outputs = [&](int x, int stage, bool add) {
                 const uint64_t v = umma_desc(operand(4 + stage), 16384, 1024);
-#pragma unroll
+#pragma unroll 1
                 for (int i = 0; i < kTileKeys / 16; ++i)
                     umma_ts(tmem + 256 + x * 128, tmem + x * 128 + i * 8, v + (uint64_t)(i * (2048 >> 4)), id_o, add || i > 0);
                 umma_commit(&o_done[x]);
@@ -422,14 +433,92 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attn_tile_kernel(const Att
             __syncwarp();
         }
     } else if (warp >= 8) {
-        // ---- codes to operands: a token a thread ----
+        // ---- codes to operands: a token a thread; keys, values, keys, ... through one loop, the next operand's codes on
+        // their way while one is written ----
         regs_down<96>();
         const int t = tid - 256;
         constexpr int W = D / 8;               // words of a token's codes
-        int ks = 0, vs = 0;
-        bool ok = true;
         const uint32_t row_at = t * 128, swizzle = (t & 7) << 4;
-        auto write = [&](uint32_t to, const uint4 (&raw)[W / 4]) {
+        const int row = t & (p.l.page_size - 1);
+        TileSeg s;
+        int k = -1, blk = 0, id = -1, id_next = -1, vexp = -126, see_begin = 0, see_end = 0;
+        uint4 raw[W / 4];
+        float ksc = 0.0f, vsc = 0.0f;
+        bool ok = true, there = false;
+        auto page_id = [&](const TileSeg& g, int block) {
+            const int token = block * kTileKeys + t;
+            return token < g.ctx ? __ldg(a.tables + (long long)g.r * a.table_stride + (token >> p.l.page_shift)) : -1;
+        };
+        auto load = [&](int page, int head, int o) {                // o: 0 keys and both scales, 1 values
+            there = (unsigned)page < (unsigned)p.l.n_pages;
+#pragma unroll
+            for (int i = 0; i < W / 4; ++i) raw[i] = make_uint4(0, 0, 0, 0);
+            if (o == 0) ksc = vsc = 0.0f;
+            if (!there) return;
+            const uint8_t* b = p.blocks + ((long long)page * p.l.kv_heads + head) * p.l.block;
+#pragma unroll
+            for (int i = 0; i < W / 4; ++i) raw[i] = __ldg(reinterpret_cast<const uint4*>(b + (o * p.l.page_size + row) * C::kRow) + i);
+            if (o == 0) {
+                const uint8_t* sp = b + p.l.page_size * D + row * C::kScale;
+                if (FMT == B4_KV_INT4) {
+                    ksc = __half2float(*reinterpret_cast<const __half*>(sp));
+                    vsc = __half2float(*reinterpret_cast<const __half*>(sp + p.l.page_size * C::kScale));
+                } else {
+                    ksc = *reinterpret_cast<const float*>(sp);
+                    vsc = *reinterpret_cast<const float*>(sp + p.l.page_size * C::kScale);
+                }
+            }
+        };
+        // the next segment, or the end of the run
+        auto next_segment = [&]() {
+            ++k;
+            if (!(ok = warp_wait(&seg_full[k & 1], k >> 1 & 1, &dead))) return false;
+            s = segs[k & 1];
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&seg_empty[k & 1]);
+            if (s.end) return false;
+            const int last_row = min((s.tile + 1) * kTileRows, s.n * p.group) - 1;
+            see_end = a.flags & B4_KV_FULL ? s.ctx : min(s.ctx, s.ctx - s.n + last_row / p.group + 1);
+            see_begin = a.window > 0 ? s.ctx - s.n + s.tile * kTileRows / p.group + 1 - a.window : 0;
+            return true;
+        };
+        bool more = next_segment();
+        if (more) {
+            blk = s.blk0;
+            id = page_id(s, blk);
+            load(id, s.head, 0);
+        }
+#pragma unroll 1
+        for (int j = 0; more; ++j) {           // j: operands so far; even ones keys
+            const int o = j & 1, b = j >> 1, stage = b & 1;
+            if (o == 0) {
+                // scales: those of tokens that no row sees are 0, the values' relative to a running power of two
+                const int token = blk * kTileKeys + t, ring = b & 3;
+                const bool seen = there && token < see_end && token >= see_begin;
+                if (blk == s.blk0) vexp = -126;
+                const float v = seen ? fminf(vsc, 3.4028235e38f) : 0.0f;
+                const unsigned bits = __reduce_max_sync(0xffffffffu, v < 3.4028235e38f ? __float_as_uint(fabsf(v)) : 0u);
+                const unsigned pages = __ballot_sync(0xffffffffu, there);
+                if (lane == 0) {
+                    value_top[stage][warp - 8] = __uint_as_float(bits);
+                    mbar_arrive(&tops);
+                }
+                __syncwarp();
+                if (!(ok = warp_wait(&tops, stage, &dead))) break;
+                const float4 tv = *reinterpret_cast<const float4*>(value_top[stage]);
+                const float top = fmaxf(fmaxf(tv.x, tv.y), fmaxf(tv.z, tv.w));
+                vexp = max(vexp, min((int)(__float_as_uint(top) >> 23) - 126, 126));
+                key_scale[ring][t] = seen ? ksc : 0.0f;
+                value_scale[ring][t] = v * pow2(-vexp);
+                if (t == 0) value_exp[ring] = vexp;
+                // tokens that are not there lie in whole pages of 16 at least: two bits a warp
+                if (lane == 0) reinterpret_cast<uint8_t*>(&block_pages[ring])[warp - 8] = (uint8_t)((pages & 1) | (pages >> 16 & 1) << 1);
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&scale_full[ring]);
+                if (blk + 1 < s.blk1) id_next = page_id(s, blk + 1);
+            }
+            if (b >= 2 && !(ok = warp_wait(o ? &v_empty[stage] : &k_empty[stage], (b >> 1) + 1 & 1, &dead))) break;
+            const uint32_t to = operand(2 + 2 * o + stage) + row_at;
             const uint32_t* w = reinterpret_cast<const uint32_t*>(raw);
 #pragma unroll
             for (int i = 0; i < W; ++i) {
@@ -443,101 +532,26 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attn_tile_kernel(const Att
                     h[2] = lds32((w[i] >> 10 & 0x3fc0u) | copy);
                     h[3] = lds32((w[i] >> 18 & 0x3fc0u) | copy);
                 }
-                asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(to + (i >> 3) * 16384 + row_at + (((i & 7) << 4) ^ swizzle)),
+                asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(to + (i >> 3) * 16384 + (((i & 7) << 4) ^ swizzle)),
                              "r"(h[0]), "r"(h[1]), "r"(h[2]), "r"(h[3])
                              : "memory");
             }
-            fence_proxy_async();
-            __syncwarp();
-        };
-        for (int k = 0; ok; ++k) {
-            if (!(ok = warp_wait(&seg_full[k & 1], k >> 1 & 1, &dead))) break;
-            const TileSeg s = segs[k & 1];
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&seg_empty[k & 1]);
-            if (s.end) break;
-            const int rows = s.n * p.group, last_row = min((s.tile + 1) * kTileRows, rows) - 1;
-            const int see_end = a.flags & B4_KV_FULL ? s.ctx : min(s.ctx, s.ctx - s.n + last_row / p.group + 1);
-            const int see_begin = a.window > 0 ? s.ctx - s.n + s.tile * kTileRows / p.group + 1 - a.window : 0;
-            const int32_t* ids = a.tables + (long long)s.r * a.table_stride;
-            auto page_id = [&](int blk) {
-                const int token = blk * kTileKeys + t;
-                return blk < s.blk1 && token < s.ctx ? __ldg(ids + (token >> p.l.page_shift)) : -1;
-            };
-            int id = page_id(s.blk0), id_next = page_id(s.blk0 + 1), vexp = -126;
-            uint4 kr[W / 4], vr[W / 4];
-            float ksc, vsc;
-            bool there, there_v;
-            auto block_of = [&](int page) { return p.blocks + ((long long)page * p.l.kv_heads + s.head) * p.l.block; };
-            const int row = t & (p.l.page_size - 1);
-            auto load_k = [&](int page) {
-                there = (unsigned)page < (unsigned)p.l.n_pages;
-#pragma unroll
-                for (int i = 0; i < W / 4; ++i) kr[i] = make_uint4(0, 0, 0, 0);
-                ksc = vsc = 0.0f;
-                if (there) {
-                    const uint8_t* b = block_of(page);
-#pragma unroll
-                    for (int i = 0; i < W / 4; ++i) kr[i] = __ldg(reinterpret_cast<const uint4*>(b + row * C::kRow) + i);
-                    const uint8_t* sp = b + p.l.page_size * D + row * C::kScale;
-                    if (FMT == B4_KV_INT4) {
-                        ksc = __half2float(*reinterpret_cast<const __half*>(sp));
-                        vsc = __half2float(*reinterpret_cast<const __half*>(sp + p.l.page_size * C::kScale));
-                    } else {
-                        ksc = *reinterpret_cast<const float*>(sp);
-                        vsc = *reinterpret_cast<const float*>(sp + p.l.page_size * C::kScale);
+            // the operand after this one
+            if (o == 1) {
+                if (++blk < s.blk1) {
+                    id = id_next;
+                } else {
+                    more = next_segment();
+                    if (more) {
+                        blk = s.blk0;
+                        id = page_id(s, blk);
                     }
                 }
-            };
-            auto load_v = [&](int page) {
-                there_v = (unsigned)page < (unsigned)p.l.n_pages;
-#pragma unroll
-                for (int i = 0; i < W / 4; ++i) vr[i] = make_uint4(0, 0, 0, 0);
-                if (there_v) {
-                    const uint8_t* b = block_of(page) + (p.l.page_size + row) * C::kRow;
-#pragma unroll
-                    for (int i = 0; i < W / 4; ++i) vr[i] = __ldg(reinterpret_cast<const uint4*>(b) + i);
-                }
-            };
-            load_k(id);
-            load_v(id);
-            for (int blk = s.blk0; blk < s.blk1 && ok; ++blk) {
-                const int id_after = page_id(blk + 2), ring = ks & 3;
-                // scales: those of tokens that no row sees are 0, the values' relative to a running power of two
-                const int token = blk * kTileKeys + t;
-                const bool seen = there && token < see_end && token >= see_begin;
-                float v = seen ? fminf(vsc, 3.4028235e38f) : 0.0f;
-                const unsigned bits = __reduce_max_sync(0xffffffffu, v < 3.4028235e38f ? __float_as_uint(fabsf(v)) : 0u);
-                const unsigned pages = __ballot_sync(0xffffffffu, there);
-                if (lane == 0) {
-                    value_top[ks & 1][warp - 8] = __uint_as_float(bits);
-                    mbar_arrive(&tops);
-                }
-                __syncwarp();
-                if (!(ok = warp_wait(&tops, ks & 1, &dead))) break;
-                const float4 tv = *reinterpret_cast<const float4*>(value_top[ks & 1]);
-                const float top = fmaxf(fmaxf(tv.x, tv.y), fmaxf(tv.z, tv.w));
-                vexp = max(vexp, min((int)(__float_as_uint(top) >> 23) - 126, 126));
-                key_scale[ring][t] = seen ? ksc : 0.0f;
-                value_scale[ring][t] = v * pow2(-vexp);
-                if (t == 0) value_exp[ring] = vexp;
-                // tokens that are not there lie in whole pages of 16 at least: two bits a warp
-                if (lane == 0) reinterpret_cast<uint8_t*>(&block_pages[ring])[warp - 8] = (uint8_t)((pages & 1) | (pages >> 16 & 1) << 1);
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&scale_full[ring]);
-
-                if (ks >= 2 && !(ok = warp_wait(&k_empty[ks & 1], (ks >> 1) + 1 & 1, &dead))) break;
-                write(operand(2 + (ks & 1)), kr);
-                if (lane == 0) mbar_arrive(&k_full[ks & 1]);
-                ++ks;
-                if (blk + 1 < s.blk1) load_k(id_next);
-                if (vs >= 2 && !(ok = warp_wait(&v_empty[vs & 1], (vs >> 1) + 1 & 1, &dead))) break;
-                write(operand(4 + (vs & 1)), vr);
-                if (lane == 0) mbar_arrive(&v_full[vs & 1]);
-                ++vs;
-                if (blk + 1 < s.blk1) load_v(id_next);
-                id_next = id_after;
             }
+            if (more) load(id, s.head, 1 - o);
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(o ? &v_full[stage] : &k_full[stage]);
         }
     } else {
         // ---- softmax: a row a thread ----
@@ -547,12 +561,57 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attn_tile_kernel(const Att
         const uint32_t s_at = tmem + lanes + x * 128, o_at = tmem + lanes + 256 + x * 128;
         int cs = 0, ring0 = 0, teams = 0;      // this tile's blocks so far; all blocks so far
         bool ok = true;
-        for (int k = 0; ok; ++k) {
-            if (!(ok = warp_wait(&seg_full[k & 1], k >> 1 & 1, &dead))) break;
-            const TileSeg s = segs[k & 1];
+        TileSeg s, following;
+        auto fetch = [&](int k, TileSeg& g) {
+            if (!(ok = warp_wait(&seg_full[k & 1], k >> 1 & 1, &dead))) return;
+            g = segs[k & 1];
             __syncwarp();
             if (lane == 0) mbar_arrive(&seg_empty[k & 1]);
-            if (s.end) break;
+        };
+        // a segment's query of this thread's row to shared memory: fp16 in the order of the decoded codes (bf16: times a
+        // power of two, as query_operand); returns the factor that a product with it lacks
+        auto put_query = [&](const TileSeg& g) -> float {
+            const int rows = g.n * p.group, row = g.tile * kTileRows + x * 128 + t, token = row / p.group;
+            if (rows - g.tile * kTileRows <= x * 128) return 1.0f;  // no second tile
+            const uint4* src = reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + (g.q0 + token) * a.q_stride_token +
+                                                              (g.head * p.group + (row - token * p.group)) * a.q_stride_head);
+            uint4 w[D / 8];
+#pragma unroll
+            for (int i = 0; i < D / 8; ++i) w[i] = row < rows ? __ldg(src + i) : make_uint4(0, 0, 0, 0);
+            float factor = 1.0f, up = 1.0f;
+            if (std::is_same<T, __nv_bfloat16>::value) {
+                uint32_t top = 0;
+#pragma unroll
+                for (int i = 0; i < D / 8; ++i) {
+                    const uint32_t* y = reinterpret_cast<const uint32_t*>(&w[i]);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) top = max(top, max(y[j] << 16 & 0x7fffffffu, y[j] & 0x7fff0000u));
+                }
+                const int e = min(max((int)(top >> 23) - 127, -110), 126);
+                up = pow2(10 - e);
+                factor = pow2(e - 10);
+            }
+            const uint32_t sign = a.scale < 0.0f ? 0x80008000u : 0u, to = operand(x) + t * 128, swizzle = (t & 7) << 4;
+#pragma unroll
+            for (int i = 0; i < D / 8; ++i) {
+                if (std::is_same<T, __nv_bfloat16>::value) {
+                    uint32_t* y = reinterpret_cast<uint32_t*>(&w[i]);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) y[j] = pack_half2(__uint_as_float(y[j] << 16) * up, __uint_as_float(y[j] & 0xffff0000u) * up);
+                }
+                const uint4 v = FMT == B4_KV_INT4 ? int4_pair_order(w[i]) : w[i];
+                asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(to + (i >> 3) * 16384 + (((i & 7) << 4) ^ swizzle)),
+                             "r"(v.x ^ sign), "r"(v.y ^ sign), "r"(v.z ^ sign), "r"(v.w ^ sign)
+                             : "memory");
+            }
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&q_full[x]);
+            return factor;
+        };
+        fetch(0, s);
+        float factor = ok && !s.end ? put_query(s) : 1.0f;
+        for (int k = 1; ok && !s.end; ++k) {
             const int blocks = s.blk1 - s.blk0, rows = s.n * p.group, row0 = s.tile * kTileRows;
             const bool two = rows - row0 > 128;
             const int row = row0 + x * 128 + t;
@@ -560,69 +619,50 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attn_tile_kernel(const Att
             const int token = row / p.group, head = s.head * p.group + (row - token * p.group);
             float m = kNoMax, l = 0.0f;
             int vexp = -126;
+            const float qf = fmaxf(factor * (fabsf(a.scale) * kLog2e) * (FMT == B4_KV_NF4 ? 1.0f / kNf4Up : 1.0f), 1e-30f);
             if (x == 0 || two) {
-                // the row's query: fp16 in the order of the decoded codes (bf16: times a power of two, as query_operand)
-                const uint4* src = reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + (s.q0 + token) * a.q_stride_token + head * a.q_stride_head);
-                float factor = 1.0f, up = 1.0f;
-                if (std::is_same<T, __nv_bfloat16>::value) {
-                    uint32_t top = 0;
-#pragma unroll 4
-                    for (int i = 0; i < D / 8; ++i) {
-                        const uint4 w = mine ? __ldg(src + i) : make_uint4(0, 0, 0, 0);
-                        const uint32_t y[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) top = max(top, max(y[j] << 16 & 0x7fffffffu, y[j] & 0x7fff0000u));
-                    }
-                    const int e = min(max((int)(top >> 23) - 127, -110), 126);
-                    up = pow2(10 - e);
-                    factor = pow2(e - 10);
-                }
-                const uint32_t sign = a.scale < 0.0f ? 0x80008000u : 0u;
-#pragma unroll 8
-                for (int i = 0; i < D / 8; ++i) {
-                    uint4 w = mine ? __ldg(src + i) : make_uint4(0, 0, 0, 0);
-                    if (std::is_same<T, __nv_bfloat16>::value) {
-                        uint32_t* y = reinterpret_cast<uint32_t*>(&w);
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) y[j] = pack_half2(__uint_as_float(y[j] << 16) * up, __uint_as_float(y[j] & 0xffff0000u) * up);
-                    }
-                    if (FMT == B4_KV_INT4) w = int4_pair_order(w);
-                    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(operand(x) + (i >> 3) * 16384 + t * 128 + (((i & 7) ^ (t & 7)) << 4)),
-                                 "r"(w.x ^ sign), "r"(w.y ^ sign), "r"(w.z ^ sign), "r"(w.w ^ sign)
-                                 : "memory");
-                }
-                fence_proxy_async();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&q_full[x]);
-                const float qf = fmaxf(factor * (fabsf(a.scale) * kLog2e) * (FMT == B4_KV_NF4 ? 1.0f / kNf4Up : 1.0f), 1e-30f);
                 const int lim = a.flags & B4_KV_FULL ? s.ctx : min(s.ctx, s.ctx - s.n + token + 1);
                 const int from = a.window > 0 ? lim - a.window : 0;
-
+#pragma unroll 1
                 for (int i = 0; i < blocks && ok; ++i, ++cs) {
                     const int ring = (ring0 + i) & 3;
-                    if (!(ok = warp_wait(&scale_full[ring], (ring0 + i) >> 2 & 1, &dead))) break;
                     if (!(ok = warp_wait(&s_full[x], cs & 1, &dead))) break;
+                    // after the scores, so that the phase asked for is the last one done whatever this tile has skipped
+                    if (!(ok = warp_wait(&scale_full[ring], (ring0 + i) >> 2 & 1, &dead))) break;
                     tmem_after_sync();
-                    float sc[kTileKeys];
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) tmem_ld32(reinterpret_cast<uint32_t*>(sc) + 32 * c, s_at + 32 * c);
-                    tmem_wait_ld();
-                    float2* s2 = reinterpret_cast<float2*>(sc);
-#pragma unroll
-                    for (int c = 0; c < kTileKeys / 4; ++c) {
-                        const float4 f = reinterpret_cast<const float4*>(key_scale[ring])[c];
-                        s2[2 * c] = __fmul2_rn(s2[2 * c], make_float2(f.x, f.y));
-                        s2[2 * c + 1] = __fmul2_rn(s2[2 * c + 1], make_float2(f.z, f.w));
-                    }
                     const int key0 = (s.blk0 + i) * kTileKeys, pages = block_pages[ring];
-                    if (__any_sync(0xffffffffu, key0 + kTileKeys > lim || key0 < from || pages != 0x03030303)) {
+                    const bool masked = __any_sync(0xffffffffu, key0 + kTileKeys > lim || key0 < from || pages != 0x03030303);
+                    // half of the row's scores: columns times their keys' scales, -infinity where the row does not see
+                    constexpr int kHalf = kTileKeys / 2;
+                    auto scores = [&](int h, float2 (&v)[kHalf / 2]) {
+                        uint32_t* r = reinterpret_cast<uint32_t*>(v);
+                        tmem_ld32(r, s_at + h * kHalf);
+                        tmem_ld32(r + 32, s_at + h * kHalf + 32);
+                        const float4* f4 = reinterpret_cast<const float4*>(key_scale[ring] + h * kHalf);
+                        tmem_wait_ld();
 #pragma unroll
-                        for (int c = 0; c < kTileKeys; ++c)
-                            if (key0 + c >= lim || key0 + c < from || !(pages >> (c >> 5) * 8 + (c >> 4 & 1) & 1)) sc[c] = -INFINITY;
-                    }
+                        for (int c = 0; c < kHalf / 4; ++c) {
+                            const float4 f = f4[c];
+                            v[2 * c] = __fmul2_rn(v[2 * c], make_float2(f.x, f.y));
+                            v[2 * c + 1] = __fmul2_rn(v[2 * c + 1], make_float2(f.z, f.w));
+                        }
+                        if (masked) {
+                            const int hi = lim - key0 - h * kHalf, lo = from - key0 - h * kHalf, bits = pages >> 16 * h;
+#pragma unroll
+                            for (int c = 0; c < kHalf; ++c) {
+                                float& y = c & 1 ? v[c / 2].y : v[c / 2].x;
+                                if (c >= hi || c < lo || !(bits >> ((c >> 5) * 8 + (c >> 4 & 1)) & 1)) y = -INFINITY;
+                            }
+                        }
+                    };
                     float top = -INFINITY;
+#pragma unroll 1
+                    for (int h = 0; h < 2; ++h) {
+                        float2 v[kHalf / 2];
+                        scores(h, v);
 #pragma unroll
-                    for (int c = 0; c < kTileKeys; c += 2) top = fmaxf(top, fmaxf(sc[c], sc[c + 1]));
+                        for (int c = 0; c < kHalf / 2; ++c) top = fmaxf(top, fmaxf(v[c].x, v[c].y));
+                    }
                     const int ve = value_exp[ring];
                     if (__any_sync(0xffffffffu, top * qf > m + 8.0f) || ve != vexp) {
                         const float next = top == -INFINITY ? m : fmaxf(m, top * qf), keep_l = fast_exp2(m - next);
@@ -647,22 +687,29 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attn_tile_kernel(const Att
                     }
                     const float2 q2 = make_float2(qf, qf), m2 = make_float2(-m, -m);
                     float2 l2 = make_float2(0.0f, 0.0f);
+                    // P takes S's first 64 columns: a half's 32 lie in scores that have been read
+#pragma unroll 1
+                    for (int h = 0; h < 2; ++h) {
+                        float2 v[kHalf / 2];
+                        scores(h, v);
+                        const float4* f4 = reinterpret_cast<const float4*>(value_scale[ring] + h * kHalf);
 #pragma unroll
-                    for (int c = 0; c < kTileKeys / 32; ++c) {
-                        uint32_t w[16];
+                        for (int c = 0; c < kHalf / 32; ++c) {
+                            uint32_t w[16];
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) {
-                            const float4 f = reinterpret_cast<const float4*>(value_scale[ring])[8 * c + j];
-                            float2 e0 = __ffma2_rn(s2[16 * c + 2 * j], q2, m2), e1 = __ffma2_rn(s2[16 * c + 2 * j + 1], q2, m2);
-                            e0 = make_float2(fast_exp2(e0.x), fast_exp2(e0.y));
-                            e1 = make_float2(fast_exp2(e1.x), fast_exp2(e1.y));
-                            l2 = __fadd2_rn(l2, __fadd2_rn(e0, e1));
-                            e0 = __fmul2_rn(e0, make_float2(f.x, f.y));
-                            e1 = __fmul2_rn(e1, make_float2(f.z, f.w));
-                            w[2 * j] = pack_half2(e0.x, e0.y);
-                            w[2 * j + 1] = pack_half2(e1.x, e1.y);
+                            for (int j = 0; j < 8; ++j) {
+                                const float4 f = f4[8 * c + j];
+                                float2 e0 = __ffma2_rn(v[16 * c + 2 * j], q2, m2), e1 = __ffma2_rn(v[16 * c + 2 * j + 1], q2, m2);
+                                e0 = make_float2(fast_exp2(e0.x), fast_exp2(e0.y));
+                                e1 = make_float2(fast_exp2(e1.x), fast_exp2(e1.y));
+                                l2 = __fadd2_rn(l2, __fadd2_rn(e0, e1));
+                                e0 = __fmul2_rn(e0, make_float2(f.x, f.y));
+                                e1 = __fmul2_rn(e1, make_float2(f.z, f.w));
+                                w[2 * j] = pack_half2(e0.x, e0.y);
+                                w[2 * j + 1] = pack_half2(e1.x, e1.y);
+                            }
+                            tmem_st16(s_at + 32 * h + 16 * c, w);
                         }
-                        tmem_st16(s_at + 16 * c, w);
                     }
                     l += l2.x + l2.y;
                     tmem_wait_st();
@@ -671,10 +718,16 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attn_tile_kernel(const Att
                     if (lane == 0) mbar_arrive(&p_full[x]);
                 }
                 if (!ok) break;
+            }
+            ring0 += blocks;
+            // the next segment's query, whose scores are then computed under this one's end
+            fetch(k, following);
+            if (!ok) break;
+            if (!following.end) factor = put_query(following);
+            if (x == 0 || two) {
                 if (!(ok = warp_wait(&o_done[x], (cs - 1) & 1, &dead))) break;
                 tmem_after_sync();
             }
-            ring0 += blocks;
 
             // ---- the segment's rows, or a piece of them ----
             const bool whole = s.first && s.last;
@@ -717,9 +770,11 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attn_tile_kernel(const Att
                     piece[kTileRows * (D + 1) + x * 128 + t] = l;
                 }
             }
+            const TileSeg ended = s;
+            s = following;
             if (whole) continue;
             // the last of the segment's CTAs joins them, in order: a row a warp
-            const int f = owner(s.s0), parts = owner(s.s1 - 1) - f + 1;
+            const int f = owner(ended.s0), parts = owner(ended.s1 - 1) - f + 1;
             auto together = [&]() {            // the eight softmax warps
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&team);
@@ -737,34 +792,50 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attn_tile_kernel(const Att
             if (!(ok = together())) break;     // before the flag is written again
             if (!join) continue;
             auto part = [&](int i) -> const float* { return ws.cross + ((long long)(f + i) * 2 + (i == 0)) * C::kPiece; };
-            for (int r = warp; r < kTileRows && row0 + r < rows; r += 8) {
-                float top = kNoMax, sum = 0.0f;
-                for (int i = 0; i < parts; ++i) top = fmaxf(top, __ldcg(part(i) + kTileRows * D + r));
+            if (row0 + warp * 32 >= rows) continue;
+            {
+                // a warp's 32 rows: lane i weighs row i's parts, all lanes add them up row by row
                 constexpr int E = D / 32;
-                float y[E] = {};
-#pragma unroll 2
+                const int r0 = warp * 32;
+                float top = kNoMax, sum = 0.0f;
+                for (int i = 0; i < parts; ++i) top = fmaxf(top, __ldcg(part(i) + kTileRows * D + r0 + lane));
+                float y[32][E];
+#pragma unroll
+                for (int r = 0; r < 32; ++r)
+#pragma unroll
+                    for (int e = 0; e < E; ++e) y[r][e] = 0.0f;
+#pragma unroll 1
                 for (int i = 0; i < parts; ++i) {
                     const float* b = part(i);
-                    const float w = fast_exp2(__ldcg(b + kTileRows * D + r) - top);
-                    sum += w * __ldcg(b + kTileRows * (D + 1) + r);
-                    const float2* z = reinterpret_cast<const float2*>(b + r * D + lane * E);
+                    const float w = fast_exp2(__ldcg(b + kTileRows * D + r0 + lane) - top);
+                    sum += w * __ldcg(b + kTileRows * (D + 1) + r0 + lane);
 #pragma unroll
-                    for (int e = 0; e < E / 2; ++e) {
-                        const float2 v = __ldcg(z + e);
-                        y[2 * e] += w * v.x;
-                        y[2 * e + 1] += w * v.y;
+                    for (int r = 0; r < 32; ++r) {
+                        const float k = __shfl_sync(0xffffffffu, w, r);
+                        const float2* z = reinterpret_cast<const float2*>(b + (r0 + r) * D + lane * E);
+#pragma unroll
+                        for (int e = 0; e < E / 2; ++e) {
+                            const float2 v = row0 + r0 + r < rows ? __ldcg(z + e) : make_float2(0.0f, 0.0f);
+                            y[r][2 * e] += k * v.x;
+                            y[r][2 * e + 1] += k * v.y;
+                        }
                     }
                 }
                 const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
-                const int tk = (row0 + r) / p.group, hd = s.head * p.group + (row0 + r - tk * p.group);
-                T* dst = static_cast<T*>(a.out) + (s.q0 + tk) * a.out_stride_token + hd * a.out_stride_head + lane * E;
 #pragma unroll
-                for (int e = 0; e < E; e += 2) {
-                    const T w[2] = {kv_round<T>(y[e] * inv), kv_round<T>(y[e + 1] * inv)};
-                    *reinterpret_cast<uint32_t*>(dst + e) =
-                        (uint32_t)*reinterpret_cast<const uint16_t*>(w) | (uint32_t)*reinterpret_cast<const uint16_t*>(w + 1) << 16;
+                for (int r = 0; r < 32; ++r) {
+                    const float k = __shfl_sync(0xffffffffu, inv, r);
+                    const int tk = __shfl_sync(0xffffffffu, token, r), hd = __shfl_sync(0xffffffffu, head, r);
+                    if (row0 + r0 + r >= rows) continue;
+                    T* dst = static_cast<T*>(a.out) + (ended.q0 + tk) * a.out_stride_token + hd * a.out_stride_head + lane * E;
+#pragma unroll
+                    for (int e = 0; e < E; e += 2) {
+                        const T w[2] = {kv_round<T>(y[r][e] * k), kv_round<T>(y[r][e + 1] * k)};
+                        *reinterpret_cast<uint32_t*>(dst + e) =
+                            (uint32_t)*reinterpret_cast<const uint16_t*>(w) | (uint32_t)*reinterpret_cast<const uint16_t*>(w + 1) << 16;
+                    }
                 }
-                if (a.lse && lane == 0) a.lse[(long long)(s.q0 + tk) * a.heads + hd] = sum > 0.0f ? (top + fast_log2(sum)) * kLn2 : -INFINITY;
+                if (a.lse && mine) a.lse[(long long)(ended.q0 + token) * a.heads + head] = sum > 0.0f ? (top + fast_log2(sum)) * kLn2 : -INFINITY;
             }
         }
     }
