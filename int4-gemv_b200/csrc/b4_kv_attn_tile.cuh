@@ -3,21 +3,25 @@
 //
 // Mathematics.  The queries that share a kv head (query tokens x heads of the
 // group) are rows; a CTA takes 256 of them (two tiles of 128) through the keys in
-// blocks of 128:
+// blocks of 64:
 //   S = Q K^T  (Q, K in shared memory),  O += P V  (P in tensor memory, V in shared)
-// with fp16 operands and fp32 accumulators in tensor memory.  K and V hold the bare
-// levels (INT4: exact integers; NF4: rounded to fp16, kNf4Up), so a token's key
-// scale multiplies a column of S and its value scale a column of P, in fp32.
-// Softmax is the warp kernel's (b4_kv_attn_warp.cuh): a row a thread, a maximum
-// that moves only when a score passes it by 2^8, weights relative to it and to a
-// running power of two of the value scales, rounded to fp16 for the product.
+// with fp16 operands and fp32 accumulators in tensor memory.  Where a request has
+// 128 rows or fewer, the two tiles are the same rows and take every other block: two
+// streams, joined at the end.  K and V hold the bare levels (INT4: exact integers;
+// NF4: rounded to fp16, kNf4Up), so a token's key scale multiplies a column of S and
+// its value scale a column of P, in fp32.  Softmax is the warp kernel's
+// (b4_kv_attn_warp.cuh): a maximum that moves only when a score passes it by 2^8,
+// weights relative to it and to a running power of two of the value scales, rounded
+// to fp16 for the product.
 //
-// Roles.  Warps 0-3 and 4-7: softmax of the two tiles, so that one tile's products
-// run under the other's exponentials.  Warps 8-11: codes to fp16 operands, a token a
-// thread, in the 128-byte swizzle (the same bytes serve K, whose columns are the
-// product's depth, and V, whose rows are).  Warp 12: issues the products.  Warp 13:
-// the schedule.  K and V are double-buffered; S and P of a tile share 128 columns of
-// tensor memory, the two O the other 256.
+// Roles.  Warps 0-3 and 4-7: softmax of the two tiles, a row a thread.  Warps 8-11:
+// codes to fp16 operands, half a token a thread, in the 128-byte swizzle (the same
+// bytes serve K, whose columns are the product's depth, and V, whose rows are).  Warp
+// 12: issues the products.  Warp 13: the schedule.  K and V are rings of four.  A
+// tile has two S of 64 columns of tensor memory (P takes half of one), so that the
+// next block's scores are there when a block's weights are done: with one S of 128
+// columns a block waited 4.1 us on the chain scores - softmax - outputs - scores,
+// of which the products were 0.5.  The two O take the other 256 columns.
 //
 // Split.  The (request, row tile, head, key block) units of the whole call, only
 // those that some row sees, form one sequence and every CTA gets an equal run of it;
@@ -33,17 +37,18 @@
 
 namespace b4 {
 
-constexpr int kTileRows = 256, kTileKeys = 128, kTileThreads = 512;
+constexpr int kTileRows = 256, kTileKeys = 64, kTileThreads = 512, kTileStages = 4, kScaleRing = 8;
 
 template <int FMT, int D>
 struct TileCfg {
     static constexpr int kRow = D / 2, kScale = FMT == B4_KV_INT4 ? 2 : 4;
-    static constexpr int kOperand = 128 * D * 2;                   // bytes of 128 rows of D fp16: D / 64 parts of 128 x 128 bytes
+    static constexpr int kOperand = 128 * D * 2;                   // bytes of 128 queries of D fp16: D / 64 parts of 128 x 128 bytes
+    static constexpr int kBlock = kTileKeys * D * 2;               // of a block's keys or values: parts of 64 x 128 bytes
     // NF4: pairs of levels by byte, 256 rows of 16 copies (2 lanes a copy), at shared address 16384, so that an OR makes
     // a lookup's address; the operands follow it.  Without it they follow the static part.
     static constexpr int kTable = 16384, kStatic = 10240;
     static constexpr int kPiece = kTileRows * (D + 2);             // floats: output, maxima, sums
-    static constexpr int kSmem = 6 * kOperand + (FMT == B4_KV_NF4 ? 2 * kTable - kStatic : 1024);   // kStatic: less than the static part and the system's
+    static constexpr int kSmem = 2 * kOperand + 2 * kTileStages * kBlock + (FMT == B4_KV_NF4 ? 2 * kTable - kStatic : 1024);   // kStatic: less than the static part and the system's
 };
 
 struct TileSeg {               // a run's part of a segment
@@ -146,17 +151,19 @@ __device__ __forceinline__ bool mbar_try_wait_long(uint64_t* bar, uint32_t phase
 // Waits for a phase; false when the CTA gave up (here or elsewhere).
 __device__ __forceinline__ bool tile_wait(uint64_t* bar, uint32_t phase, volatile int* dead)
 {
-    if (mbar_try_wait(bar, phase)) return true;
-    const unsigned long long t0 = now_ns();
-    for (;;) {
+#pragma unroll 1
+    for (int i = 0; i < 64; ++i)
         if (mbar_try_wait_long(bar, phase)) return true;
-        if (*dead) return false;
+    const unsigned long long t0 = now_ns();
+#pragma unroll 1
+    while (!*dead) {
+        if (mbar_try_wait_long(bar, phase)) return true;
         if (now_ns() - t0 > 2000000000ULL) {
             *dead = 1;
             atomicOr(&g_device_error, kErrMbarrierTimeout);
-            return false;
         }
     }
+    return false;
 }
 
 // ... by a whole warp, with one answer
@@ -186,14 +193,15 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attn_tile_kernel(const Att
 {
     using C = TileCfg<FMT, D>;
     extern __shared__ __align__(1024) uint8_t tile_smem[];
-    __shared__ uint64_t seg_full[2], seg_empty[2], q_full[2], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_done[2], scale_full[4], tops, team, drain;
+    __shared__ uint64_t seg_full[2], seg_empty[2], q_full[2], s_full[2][2], p_full[2][2], o_done[2][2], tops, team, drain;
+    __shared__ uint64_t k_full[kTileStages], k_empty[kTileStages], v_full[kTileStages], v_empty[kTileStages], scale_full[kScaleRing];
     __shared__ TileSeg segs[2];
     __shared__ long long units_before[kTileThreads + 1];
     __shared__ int tiles_before[kTileThreads + 1];
     __shared__ long long warp_sum[kTileThreads / 32];
-    __shared__ __align__(16) float key_scale[4][kTileKeys], value_scale[4][kTileKeys];
-    __shared__ int value_exp[4], block_pages[4];
-    __shared__ __align__(16) float value_top[2][4];
+    __shared__ __align__(16) float key_scale[kScaleRing][kTileKeys], value_scale[kScaleRing][kTileKeys];
+    __shared__ int value_exp[kScaleRing], block_pages[kScaleRing];
+    __shared__ float value_top[2][2];
     __shared__ uint32_t tmem_at;
     __shared__ volatile int dead;
     __shared__ int joins;
@@ -201,22 +209,30 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attn_tile_kernel(const Att
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const b4_kv_attn& a = p.a;
     const uint32_t operands = FMT == B4_KV_NF4 ? 2 * C::kTable : (smem_addr(tile_smem) + 1023) & ~1023u;
-    auto operand = [&](uint32_t i) -> uint32_t { return operands + i * C::kOperand; };          // Q of both tiles, K twice, V twice
+    const uint32_t keys_at = operands + 2 * C::kOperand, values_at = keys_at + kTileStages * C::kBlock;     // after Q of both tiles
+    if (FMT == B4_KV_NF4 && smem_addr(tile_smem) > C::kTable) {       // the static part has outgrown its place
+        if (tid == 0) atomicOr(&g_device_error, kErrMbarrierTimeout);
+        return;
+    }
     if (tid == 0) {
         for (int i = 0; i < 2; ++i) {
             mbar_init(&seg_full[i], 1);
             mbar_init(&seg_empty[i], 13);
             mbar_init(&q_full[i], 4);
+            for (int j = 0; j < 2; ++j) {
+                mbar_init(&s_full[i][j], 1);
+                mbar_init(&p_full[i][j], 4);
+                mbar_init(&o_done[i][j], 1);
+            }
+        }
+        for (int i = 0; i < kTileStages; ++i) {
             mbar_init(&k_full[i], 4);
             mbar_init(&k_empty[i], 1);
             mbar_init(&v_full[i], 4);
             mbar_init(&v_empty[i], 1);
-            mbar_init(&s_full[i], 1);
-            mbar_init(&p_full[i], 4);
-            mbar_init(&o_done[i], 1);
         }
-        for (int i = 0; i < 4; ++i) mbar_init(&scale_full[i], 4);
-        mbar_init(&tops, 4);
+        for (int i = 0; i < kScaleRing; ++i) mbar_init(&scale_full[i], 4);
+        mbar_init(&tops, 2);
         mbar_init(&team, 8);
         mbar_init(&drain, 1);
         dead = 0;
@@ -376,97 +392,104 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attn_tile_kernel(const Att
             }
         } else if (warp == 12) {
             // ---- products ----
-            if (lane == 0) {
-            int ks = 0, vs = 0, cq[2] = {0, 0}, cp[2] = {0, 0};
+            uint32_t leader;
+            asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(leader));
             constexpr uint32_t id_s = umma_idesc(128, kTileKeys, false), id_o = umma_idesc(128, D, true);
-            auto scores = [&](int x, int stage) {
-                const uint64_t q = umma_desc(operand(x), 16, 1024), k = umma_desc(operand(2 + stage), 16, 1024);
-#pragma unroll 1
-                for (int i = 0; i < D / 16; ++i) {
-                    const uint64_t step = (uint64_t)((i >> 2) * (16384 >> 4) + (i & 3) * 2);
-                    umma_ss(tmem + x * 128, q + step, k + step, id_s, i > 0);
-                }
-                umma_commit(&s_full[x]);
-            };
-            auto outputs = [&](int x, int stage, bool add) {
-                const uint64_t v = umma_desc(operand(4 + stage), 16384, 1024);
-#pragma unroll 1
-                for (int i = 0; i < kTileKeys / 16; ++i)
-                    umma_ts(tmem + 256 + x * 128, tmem + x * 128 + i * 8, v + (uint64_t)(i * (2048 >> 4)), id_o, add || i > 0);
-                umma_commit(&o_done[x]);
-            };
+            constexpr uint32_t kPartQ = 128 * 128, kPartB = kTileKeys * 128;       // bytes from 64 columns to the next
+            const uint64_t desc_q = umma_desc(operands, 16, 1024), desc_k = umma_desc(keys_at, 16, 1024);
+            const uint64_t desc_v = umma_desc(values_at, kPartB, 1024);
+            int blocks_before = 0, cq[2] = {0, 0}, cp[2] = {0, 0}, cs[2] = {0, 0};  // the tiles' queries, weights, scores so far
             bool ok = true;
             for (int k = 0; ok; ++k) {
-                if (!(ok = tile_wait(&seg_full[k & 1], k >> 1 & 1, &dead))) break;
+                if (!(ok = warp_wait(&seg_full[k & 1], k >> 1 & 1, &dead))) break;
                 const int blocks = segs[k & 1].blk1 - segs[k & 1].blk0, end = segs[k & 1].end;
-                const int tiles = segs[k & 1].n * p.group - segs[k & 1].tile * kTileRows > 128 ? 2 : 1;
-                mbar_arrive(&seg_empty[k & 1]);
+                const bool two = segs[k & 1].n * p.group - segs[k & 1].tile * kTileRows > 128;
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&seg_empty[k & 1]);
                 if (end) break;
-                for (int x = 0; x < tiles && ok; ++x) ok = tile_wait(&q_full[x], cq[x]++ & 1, &dead);
-                ok = ok && tile_wait(&k_full[ks & 1], ks >> 1 & 1, &dead);
-                if (!ok) break;
-                tmem_after_sync();
-                for (int x = 0; x < tiles; ++x) scores(x, ks & 1);
-                umma_commit(&k_empty[ks & 1]);
-                ++ks;
-                for (int i = 0; i < blocks && ok; ++i) {
-                    ok = tile_wait(&v_full[vs & 1], vs >> 1 & 1, &dead);
-                    for (int x = 0; x < tiles && ok; ++x) {
-                        if (!(ok = tile_wait(&p_full[x], cp[x]++ & 1, &dead))) break;
+                // step st: the outputs of tile st & 1's block, then the scores of its block after next.  Two tiles of rows:
+                // both take every block; one: each takes every other
+                const int steps = two ? 2 * blocks : blocks;
+#pragma unroll 1
+                for (int st = -4; st < steps; ++st) {
+                    const int x = st & 1, pv = two ? st >> 1 : st, sb = two ? (st >> 1) + 2 : st + 4;
+                    const bool leaves = !two || x == 1;            // the block's last use
+                    if (st >= 0) {
+                        const int b = blocks_before + pv, stage = b & (kTileStages - 1), buf = cp[x] & 1;
+                        if (!(ok = warp_wait(&v_full[stage], b / kTileStages & 1, &dead))) break;
+                        if (!(ok = warp_wait(&p_full[x][buf], cp[x] >> 1 & 1, &dead))) break;
+                        ++cp[x];
                         tmem_after_sync();
-                        outputs(x, vs & 1, i > 0);
-                        if (x == tiles - 1) umma_commit(&v_empty[vs & 1]);
-                        if (i + 1 < blocks) {
-                            if (x == 0 && !(ok = tile_wait(&k_full[ks & 1], ks >> 1 & 1, &dead))) break;
-                            tmem_after_sync();
-                            scores(x, ks & 1);
-                            if (x == tiles - 1) umma_commit(&k_empty[ks & 1]);
+                        if (leader) {
+                            const uint32_t o = tmem + 256 + x * 128, pa = tmem + x * 128 + buf * 64;
+                            const uint64_t v = desc_v + (uint64_t)(stage * (C::kBlock >> 4));
+                            const bool add = two ? pv > 0 : pv > 1;
+#pragma unroll
+                            for (int i = 0; i < kTileKeys / 16; ++i)
+                                umma_ts(o, pa + i * 8, v + (uint64_t)(i * (2048 >> 4)), id_o, add || i > 0);
+                            umma_commit(&o_done[x][buf]);
+                            if (leaves) umma_commit(&v_empty[stage]);
                         }
+                        __syncwarp();
                     }
-                    ++vs;
-                    if (i + 1 < blocks) ++ks;
+                    if (sb < blocks) {
+                        const int b = blocks_before + sb, stage = b & (kTileStages - 1), buf = cs[x]++ & 1;
+                        if (!(ok = warp_wait(&k_full[stage], b / kTileStages & 1, &dead))) break;
+                        if (st < -2 && (two || x == 0) && !(ok = warp_wait(&q_full[x], cq[x]++ & 1, &dead))) break;
+                        tmem_after_sync();
+                        if (leader) {
+                            const uint64_t q = desc_q + (uint64_t)((two ? x : 0) * (C::kOperand >> 4));
+                            const uint64_t kd = desc_k + (uint64_t)(stage * (C::kBlock >> 4));
+#pragma unroll
+                            for (int i = 0; i < D / 16; ++i)
+                                umma_ss(tmem + x * 128 + buf * 64, q + (uint64_t)((i >> 2) * (kPartQ >> 4) + (i & 3) * 2),
+                                        kd + (uint64_t)((i >> 2) * (kPartB >> 4) + (i & 3) * 2), id_s, i > 0);
+                            umma_commit(&s_full[x][buf]);
+                            if (leaves) umma_commit(&k_empty[stage]);
+                        }
+                        __syncwarp();
+                    }
                 }
+                blocks_before += blocks;
             }
-            umma_commit(&drain);               // nothing in flight when the CTA ends
-            for (int i = 0; i < 1 << 20 && !mbar_try_wait(&drain, 0); ++i) {}
+            if (leader) {
+                umma_commit(&drain);           // nothing in flight when the CTA ends
+                for (int i = 0; i < 1 << 20 && !mbar_try_wait(&drain, 0); ++i) {}
             }
             __syncwarp();
         }
     } else if (warp >= 8) {
-        // ---- codes to operands: a token a thread; keys, values, keys, ... through one loop, the next operand's codes on
-        // their way while one is written ----
+        // ---- codes to operands: half a token a thread (warps 8, 9 the first columns and the keys' scales, 10, 11 the others
+        // and the values'); keys, values, keys, ... through one loop, the next operand's codes on their way while one is
+        // written ----
         regs_down<96>();
-        const int t = tid - 256;
-        constexpr int W = D / 8;               // words of a token's codes
-        const uint32_t row_at = t * 128, swizzle = (t & 7) << 4;
+        const int t = tid & 63, half = warp >> 1 & 1;
+        constexpr int W = D / 16;              // words of half a token's codes
+        constexpr int kPart = D == 128 ? kTileKeys * 128 : 0;      // D = 64: both halves lie in one part
+        const uint32_t row_at = t * 128 + half * kPart, swizzle = (t & 7) << 4, chunk0 = D == 128 ? 0 : half * W;
         const int row = t & (p.l.page_size - 1);
         TileSeg s;
         int k = -1, blk = 0, id = -1, id_next = -1, vexp = -126, see_begin = 0, see_end = 0;
         uint4 raw[W / 4];
-        float ksc = 0.0f, vsc = 0.0f;
+        float scale = 0.0f;                    // the key's or the value's
         bool ok = true, there = false;
         auto page_id = [&](const TileSeg& g, int block) {
             const int token = block * kTileKeys + t;
             return token < g.ctx ? __ldg(a.tables + (long long)g.r * a.table_stride + (token >> p.l.page_shift)) : -1;
         };
-        auto load = [&](int page, int head, int o) {                // o: 0 keys and both scales, 1 values
+        auto load = [&](int page, int head, int o) {                // o: 0 keys and the scale, 1 values
             there = (unsigned)page < (unsigned)p.l.n_pages;
 #pragma unroll
             for (int i = 0; i < W / 4; ++i) raw[i] = make_uint4(0, 0, 0, 0);
-            if (o == 0) ksc = vsc = 0.0f;
+            if (o == 0) scale = 0.0f;
             if (!there) return;
             const uint8_t* b = p.blocks + ((long long)page * p.l.kv_heads + head) * p.l.block;
+            const uint4* codes = reinterpret_cast<const uint4*>(b + (o * p.l.page_size + row) * C::kRow + half * (C::kRow / 2));
 #pragma unroll
-            for (int i = 0; i < W / 4; ++i) raw[i] = __ldg(reinterpret_cast<const uint4*>(b + (o * p.l.page_size + row) * C::kRow) + i);
+            for (int i = 0; i < W / 4; ++i) raw[i] = __ldg(codes + i);
             if (o == 0) {
-                const uint8_t* sp = b + p.l.page_size * D + row * C::kScale;
-                if (FMT == B4_KV_INT4) {
-                    ksc = __half2float(*reinterpret_cast<const __half*>(sp));
-                    vsc = __half2float(*reinterpret_cast<const __half*>(sp + p.l.page_size * C::kScale));
-                } else {
-                    ksc = *reinterpret_cast<const float*>(sp);
-                    vsc = *reinterpret_cast<const float*>(sp + p.l.page_size * C::kScale);
-                }
+                const uint8_t* sp = b + p.l.page_size * D + (half * p.l.page_size + row) * C::kScale;
+                scale = FMT == B4_KV_INT4 ? __half2float(*reinterpret_cast<const __half*>(sp)) : *reinterpret_cast<const float*>(sp);
             }
         };
         // the next segment, or the end of the run
@@ -490,35 +513,37 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attn_tile_kernel(const Att
         }
 #pragma unroll 1
         for (int j = 0; more; ++j) {           // j: operands so far; even ones keys
-            const int o = j & 1, b = j >> 1, stage = b & 1;
+            const int o = j & 1, b = j >> 1, stage = b & (kTileStages - 1);
             if (o == 0) {
                 // scales: those of tokens that no row sees are 0, the values' relative to a running power of two
-                const int token = blk * kTileKeys + t, ring = b & 3;
+                const int token = blk * kTileKeys + t, ring = b & (kScaleRing - 1);
                 const bool seen = there && token < see_end && token >= see_begin;
-                if (blk == s.blk0) vexp = -126;
-                const float v = seen ? fminf(vsc, 3.4028235e38f) : 0.0f;
-                const unsigned bits = __reduce_max_sync(0xffffffffu, v < 3.4028235e38f ? __float_as_uint(fabsf(v)) : 0u);
-                const unsigned pages = __ballot_sync(0xffffffffu, there);
-                if (lane == 0) {
-                    value_top[stage][warp - 8] = __uint_as_float(bits);
-                    mbar_arrive(&tops);
+                if (half) {
+                    if (blk == s.blk0) vexp = -126;
+                    const float v = seen ? fminf(scale, 3.4028235e38f) : 0.0f;
+                    const unsigned bits = __reduce_max_sync(0xffffffffu, v < 3.4028235e38f ? __float_as_uint(fabsf(v)) : 0u);
+                    if (lane == 0) {
+                        value_top[b & 1][warp & 1] = __uint_as_float(bits);
+                        mbar_arrive(&tops);
+                    }
+                    __syncwarp();
+                    if (!(ok = warp_wait(&tops, b & 1, &dead))) break;
+                    const float top = fmaxf(value_top[b & 1][0], value_top[b & 1][1]);
+                    vexp = max(vexp, min((int)(__float_as_uint(top) >> 23) - 126, 126));
+                    value_scale[ring][t] = v * pow2(-vexp);
+                    if (t == 0) value_exp[ring] = vexp;
+                } else {
+                    key_scale[ring][t] = seen ? scale : 0.0f;
+                    // tokens that are not there lie in whole pages of 16 at least: two bits a warp
+                    const unsigned pages = __ballot_sync(0xffffffffu, there);
+                    if (lane == 0) reinterpret_cast<uint8_t*>(&block_pages[ring])[warp & 1] = (uint8_t)((pages & 1) | (pages >> 16 & 1) << 1);
                 }
-                __syncwarp();
-                if (!(ok = warp_wait(&tops, stage, &dead))) break;
-                const float4 tv = *reinterpret_cast<const float4*>(value_top[stage]);
-                const float top = fmaxf(fmaxf(tv.x, tv.y), fmaxf(tv.z, tv.w));
-                vexp = max(vexp, min((int)(__float_as_uint(top) >> 23) - 126, 126));
-                key_scale[ring][t] = seen ? ksc : 0.0f;
-                value_scale[ring][t] = v * pow2(-vexp);
-                if (t == 0) value_exp[ring] = vexp;
-                // tokens that are not there lie in whole pages of 16 at least: two bits a warp
-                if (lane == 0) reinterpret_cast<uint8_t*>(&block_pages[ring])[warp - 8] = (uint8_t)((pages & 1) | (pages >> 16 & 1) << 1);
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&scale_full[ring]);
                 if (blk + 1 < s.blk1) id_next = page_id(s, blk + 1);
             }
-            if (b >= 2 && !(ok = warp_wait(o ? &v_empty[stage] : &k_empty[stage], (b >> 1) + 1 & 1, &dead))) break;
-            const uint32_t to = operand(2 + 2 * o + stage) + row_at;
+            if (b >= kTileStages && !(ok = warp_wait(o ? &v_empty[stage] : &k_empty[stage], (b / kTileStages + 1) & 1, &dead))) break;
+            const uint32_t to = (o ? values_at : keys_at) + stage * C::kBlock + row_at;
             const uint32_t* w = reinterpret_cast<const uint32_t*>(raw);
 #pragma unroll
             for (int i = 0; i < W; ++i) {
@@ -532,8 +557,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attn_tile_kernel(const Att
                     h[2] = lds32((w[i] >> 10 & 0x3fc0u) | copy);
                     h[3] = lds32((w[i] >> 18 & 0x3fc0u) | copy);
                 }
-                asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(to + (i >> 3) * 16384 + (((i & 7) << 4) ^ swizzle)),
-                             "r"(h[0]), "r"(h[1]), "r"(h[2]), "r"(h[3])
+                asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(to + (((chunk0 + i) << 4) ^ swizzle)), "r"(h[0]), "r"(h[1]), "r"(h[2]),
+                             "r"(h[3])
                              : "memory");
             }
             // the operand after this one
@@ -559,20 +584,15 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attn_tile_kernel(const Att
         const int x = warp >> 2, t = tid & 127;
         const uint32_t lanes = (uint32_t)(warp & 3) << 21;          // 32 lanes a warp, lane in the upper half
         const uint32_t s_at = tmem + lanes + x * 128, o_at = tmem + lanes + 256 + x * 128;
-        int cs = 0, ring0 = 0, teams = 0;      // this tile's blocks so far; all blocks so far
+        int cs = 0, ring0 = 0, teams = 0;      // this tile's blocks so far; all blocks; the joins' barrier's turns
         bool ok = true;
-        TileSeg s, following;
-        auto fetch = [&](int k, TileSeg& g) {
-            if (!(ok = warp_wait(&seg_full[k & 1], k >> 1 & 1, &dead))) return;
-            g = segs[k & 1];
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&seg_empty[k & 1]);
-        };
-        // a segment's query of this thread's row to shared memory: fp16 in the order of the decoded codes (bf16: times a
-        // power of two, as query_operand); returns the factor that a product with it lacks
+        TileSeg s;
+        // A segment's queries to shared memory: fp16 in the order of the decoded codes (bf16: times a power of two, as
+        // query_operand); returns the factor that a product of this thread's row lacks.
         auto put_query = [&](const TileSeg& g) -> float {
-            const int rows = g.n * p.group, row = g.tile * kTileRows + x * 128 + t, token = row / p.group;
-            if (rows - g.tile * kTileRows <= x * 128) return 1.0f;  // no second tile
+            const int rows = g.n * p.group, from = g.tile * kTileRows;
+            const bool two = rows - from > 128;
+            const int row = from + (two ? x * 128 : 0) + t, token = row / p.group;
             const uint4* src = reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + (g.q0 + token) * a.q_stride_token +
                                                               (g.head * p.group + (row - token * p.group)) * a.q_stride_head);
             uint4 w[D / 8];
@@ -591,7 +611,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attn_tile_kernel(const Att
                 up = pow2(10 - e);
                 factor = pow2(e - 10);
             }
-            const uint32_t sign = a.scale < 0.0f ? 0x80008000u : 0u, to = operand(x) + t * 128, swizzle = (t & 7) << 4;
+            if (!two && x == 1) return factor;                     // the first tile's warps put them there
+            const uint32_t sign = a.scale < 0.0f ? 0x80008000u : 0u, to = operands + x * C::kOperand + t * 128, swizzle = (t & 7) << 4;
 #pragma unroll
             for (int i = 0; i < D / 8; ++i) {
                 if (std::is_same<T, __nv_bfloat16>::value) {
@@ -609,172 +630,160 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attn_tile_kernel(const Att
             if (lane == 0) mbar_arrive(&q_full[x]);
             return factor;
         };
-        fetch(0, s);
+        auto fetch = [&](int k) {
+            if (!(ok = warp_wait(&seg_full[k & 1], k >> 1 & 1, &dead))) return;
+            s = segs[k & 1];
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&seg_empty[k & 1]);
+        };
+        fetch(0);
         float factor = ok && !s.end ? put_query(s) : 1.0f;
+#pragma unroll 1
         for (int k = 1; ok && !s.end; ++k) {
             const int blocks = s.blk1 - s.blk0, rows = s.n * p.group, row0 = s.tile * kTileRows;
             const bool two = rows - row0 > 128;
-            const int row = row0 + x * 128 + t;
+            const int row = row0 + (two ? x * 128 : 0) + t;
             const bool mine = row < rows;
-            const int token = row / p.group, head = s.head * p.group + (row - token * p.group);
+            const int token = row / p.group, head = s.head * p.group + (row - token * p.group), q0 = s.q0;
+            const bool whole = s.first && s.last && two, first = s.first;
+            const long long s0 = s.s0, s1 = s.s1;
+            const int lim = a.flags & B4_KV_FULL ? s.ctx : min(s.ctx, s.ctx - s.n + token + 1);
+            const int from = a.window > 0 ? lim - a.window : 0;
+            const float qf = fmaxf(factor * (fabsf(a.scale) * kLog2e) * (FMT == B4_KV_NF4 ? 1.0f / kNf4Up : 1.0f), 1e-30f);
             float m = kNoMax, l = 0.0f;
             int vexp = -126;
-            const float qf = fmaxf(factor * (fabsf(a.scale) * kLog2e) * (FMT == B4_KV_NF4 ? 1.0f / kNf4Up : 1.0f), 1e-30f);
-            if (x == 0 || two) {
-                const int lim = a.flags & B4_KV_FULL ? s.ctx : min(s.ctx, s.ctx - s.n + token + 1);
-                const int from = a.window > 0 ? lim - a.window : 0;
+            bool any = false;                  // whether O holds something
 #pragma unroll 1
-                for (int i = 0; i < blocks && ok; ++i, ++cs) {
-                    const int ring = (ring0 + i) & 3;
-                    if (!(ok = warp_wait(&s_full[x], cs & 1, &dead))) break;
-                    // after the scores, so that the phase asked for is the last one done whatever this tile has skipped
-                    if (!(ok = warp_wait(&scale_full[ring], (ring0 + i) >> 2 & 1, &dead))) break;
-                    tmem_after_sync();
-                    const int key0 = (s.blk0 + i) * kTileKeys, pages = block_pages[ring];
-                    const bool masked = __any_sync(0xffffffffu, key0 + kTileKeys > lim || key0 < from || pages != 0x03030303);
-                    // half of the row's scores: columns times their keys' scales, -infinity where the row does not see
-                    constexpr int kHalf = kTileKeys / 2;
-                    auto scores = [&](int h, float2 (&v)[kHalf / 2]) {
-                        uint32_t* r = reinterpret_cast<uint32_t*>(v);
-                        tmem_ld32(r, s_at + h * kHalf);
-                        tmem_ld32(r + 32, s_at + h * kHalf + 32);
-                        const float4* f4 = reinterpret_cast<const float4*>(key_scale[ring] + h * kHalf);
-                        tmem_wait_ld();
-#pragma unroll
-                        for (int c = 0; c < kHalf / 4; ++c) {
-                            const float4 f = f4[c];
-                            v[2 * c] = __fmul2_rn(v[2 * c], make_float2(f.x, f.y));
-                            v[2 * c + 1] = __fmul2_rn(v[2 * c + 1], make_float2(f.z, f.w));
-                        }
-                        if (masked) {
-                            const int hi = lim - key0 - h * kHalf, lo = from - key0 - h * kHalf, bits = pages >> 16 * h;
-#pragma unroll
-                            for (int c = 0; c < kHalf; ++c) {
-                                float& y = c & 1 ? v[c / 2].y : v[c / 2].x;
-                                if (c >= hi || c < lo || !(bits >> ((c >> 5) * 8 + (c >> 4 & 1)) & 1)) y = -INFINITY;
-                            }
-                        }
-                    };
-                    float top = -INFINITY;
-#pragma unroll 1
-                    for (int h = 0; h < 2; ++h) {
-                        float2 v[kHalf / 2];
-                        scores(h, v);
-#pragma unroll
-                        for (int c = 0; c < kHalf / 2; ++c) top = fmaxf(top, fmaxf(v[c].x, v[c].y));
-                    }
-                    const int ve = value_exp[ring];
-                    if (__any_sync(0xffffffffu, top * qf > m + 8.0f) || ve != vexp) {
-                        const float next = top == -INFINITY ? m : fmaxf(m, top * qf), keep_l = fast_exp2(m - next);
-                        const float keep = keep_l * pow2(max(vexp - ve, -126));
-                        m = next;
-                        vexp = ve;
-                        l *= keep_l;
-                        if (i > 0) {
-                            if (!(ok = warp_wait(&o_done[x], (cs - 1) & 1, &dead))) break;
-                            tmem_after_sync();
-#pragma unroll 1
-                            for (int c = 0; c < D; c += 16) {
-                                uint32_t o[16];
-                                tmem_ld16(o, o_at + c);
-                                tmem_wait_ld();
-#pragma unroll
-                                for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * keep);
-                                tmem_st16(o_at + c, o);
-                            }
-                            tmem_wait_st();
-                        }
-                    }
-                    const float2 q2 = make_float2(qf, qf), m2 = make_float2(-m, -m);
-                    float2 l2 = make_float2(0.0f, 0.0f);
-                    // P takes S's first 64 columns: a half's 32 lie in scores that have been read
-#pragma unroll 1
-                    for (int h = 0; h < 2; ++h) {
-                        float2 v[kHalf / 2];
-                        scores(h, v);
-                        const float4* f4 = reinterpret_cast<const float4*>(value_scale[ring] + h * kHalf);
-#pragma unroll
-                        for (int c = 0; c < kHalf / 32; ++c) {
-                            uint32_t w[16];
-#pragma unroll
-                            for (int j = 0; j < 8; ++j) {
-                                const float4 f = f4[8 * c + j];
-                                float2 e0 = __ffma2_rn(v[16 * c + 2 * j], q2, m2), e1 = __ffma2_rn(v[16 * c + 2 * j + 1], q2, m2);
-                                e0 = make_float2(fast_exp2(e0.x), fast_exp2(e0.y));
-                                e1 = make_float2(fast_exp2(e1.x), fast_exp2(e1.y));
-                                l2 = __fadd2_rn(l2, __fadd2_rn(e0, e1));
-                                e0 = __fmul2_rn(e0, make_float2(f.x, f.y));
-                                e1 = __fmul2_rn(e1, make_float2(f.z, f.w));
-                                w[2 * j] = pack_half2(e0.x, e0.y);
-                                w[2 * j + 1] = pack_half2(e1.x, e1.y);
-                            }
-                            tmem_st16(s_at + 32 * h + 16 * c, w);
-                        }
-                    }
-                    l += l2.x + l2.y;
-                    tmem_wait_st();
-                    tmem_before_sync();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&p_full[x]);
-                }
-                if (!ok) break;
-            }
-            ring0 += blocks;
-            // the next segment's query, whose scores are then computed under this one's end
-            fetch(k, following);
-            if (!ok) break;
-            if (!following.end) factor = put_query(following);
-            if (x == 0 || two) {
-                if (!(ok = warp_wait(&o_done[x], (cs - 1) & 1, &dead))) break;
+            for (int i = two ? 0 : x; i < blocks && ok; i += two ? 1 : 2, ++cs) {
+                const int ring = (ring0 + i) & (kScaleRing - 1), buf = cs & 1;
+                if (!(ok = warp_wait(&s_full[x][buf], cs >> 1 & 1, &dead))) break;
+                // after the scores, so that the phase asked for is the last one done
+                if (!(ok = warp_wait(&scale_full[ring], (ring0 + i) / kScaleRing & 1, &dead))) break;
                 tmem_after_sync();
+                const int key0 = (s.blk0 + i) * kTileKeys, pages = block_pages[ring] & 0xffff, ve = value_exp[ring];
+                const float4* ks = reinterpret_cast<const float4*>(key_scale[ring]);
+                float2 v[kTileKeys / 2];       // the row's scores
+                tmem_ld32(reinterpret_cast<uint32_t*>(v), s_at + buf * 64);
+                tmem_ld32(reinterpret_cast<uint32_t*>(v) + 32, s_at + buf * 64 + 32);
+                tmem_wait_ld();                // nothing between: the registers are the loads' until here
+#pragma unroll
+                for (int j = 0; j < kTileKeys / 4; ++j) {
+                    const float4 f = ks[j];
+                    v[2 * j] = __fmul2_rn(v[2 * j], make_float2(f.x, f.y));
+                    v[2 * j + 1] = __fmul2_rn(v[2 * j + 1], make_float2(f.z, f.w));
+                }
+                if (__any_sync(0xffffffffu, key0 + kTileKeys > lim || key0 < from || pages != 0x0303)) {
+                    const int hi = lim - key0, lo = from - key0;
+#pragma unroll
+                    for (int j = 0; j < kTileKeys; ++j) {
+                        float& y = j & 1 ? v[j / 2].y : v[j / 2].x;
+                        if (j >= hi || j < lo || !(pages >> ((j >> 5) * 8 + (j >> 4 & 1)) & 1)) y = -INFINITY;
+                    }
+                }
+                float tops4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int j = 0; j < kTileKeys / 2; ++j) tops4[j & 3] = fmaxf(tops4[j & 3], fmaxf(v[j].x, v[j].y));
+                const float top = fmaxf(fmaxf(tops4[0], tops4[1]), fmaxf(tops4[2], tops4[3]));
+                if (__any_sync(0xffffffffu, top * qf > m + 8.0f) || ve != vexp) {
+                    const float next = top == -INFINITY ? m : fmaxf(m, top * qf), keep_l = fast_exp2(m - next);
+                    const float keep = keep_l * pow2(max(vexp - ve, -126));
+                    m = next;
+                    vexp = ve;
+                    l *= keep_l;
+                    if (any) {                 // two barriers in turn: the scores at hand say that the block before the last is done
+                        if (!(ok = warp_wait(&o_done[x][cs - 1 & 1], (cs - 1) >> 1 & 1, &dead))) break;
+                        tmem_after_sync();
+#pragma unroll 1
+                        for (int c = 0; c < D; c += 16) {
+                            uint32_t o[16];
+                            tmem_ld16(o, o_at + c);
+                            tmem_wait_ld();
+#pragma unroll
+                            for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * keep);
+                            tmem_st16(o_at + c, o);
+                        }
+                        tmem_wait_st();
+                    }
+                }
+                any = true;
+                const float2 q2 = make_float2(qf, qf), m2 = make_float2(-m, -m);
+                const float4* vs = reinterpret_cast<const float4*>(value_scale[ring]);
+                float2 l2[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+                uint32_t w[kTileKeys / 2];
+#pragma unroll
+                for (int j = 0; j < kTileKeys / 4; ++j) {
+                    const float4 f = vs[j];
+                    float2 e0 = __ffma2_rn(v[2 * j], q2, m2), e1 = __ffma2_rn(v[2 * j + 1], q2, m2);
+                    e0 = make_float2(fast_exp2(e0.x), fast_exp2(e0.y));
+                    e1 = make_float2(fast_exp2(e1.x), fast_exp2(e1.y));
+                    l2[0] = __fadd2_rn(l2[0], e0);
+                    l2[1] = __fadd2_rn(l2[1], e1);
+                    e0 = __fmul2_rn(e0, make_float2(f.x, f.y));
+                    e1 = __fmul2_rn(e1, make_float2(f.z, f.w));
+                    w[2 * j] = pack_half2(e0.x, e0.y);
+                    w[2 * j + 1] = pack_half2(e1.x, e1.y);
+                }
+                // the weights take the first 32 of the scores' 64 columns
+                tmem_st16(s_at + buf * 64, w);
+                tmem_st16(s_at + buf * 64 + 16, w + 16);
+                l += (l2[0].x + l2[0].y) + (l2[1].x + l2[1].y);
+                tmem_wait_st();
+                tmem_before_sync();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&p_full[x][buf]);
             }
+            if (!ok) break;
+            ring0 += blocks;
+            // the next segment's queries, whose scores are then computed under this one's end; where the other stream reads
+            // the same queries, after it has: the outputs' barrier comes after all products issued before them
+            if (!two && any && !(ok = warp_wait(&o_done[x][cs - 1 & 1], (cs - 1) >> 1 & 1, &dead))) break;
+            fetch(k);
+            if (!ok) break;
+            if (!s.end) factor = put_query(s);
+            if (two && !(ok = warp_wait(&o_done[x][cs - 1 & 1], (cs - 1) >> 1 & 1, &dead))) break;
+            tmem_after_sync();
 
             // ---- the segment's rows, or a piece of them ----
-            const bool whole = s.first && s.last;
             const float vup = pow2(vexp) * (FMT == B4_KV_NF4 ? 1.0f / kNf4Up : 1.0f);
-            float* piece = ws.cross + ((long long)cta * 2 + s.first) * C::kPiece;
-            if (x == 0 || two) {
-                const float inv = whole ? (l > 0.0f ? vup / l : 0.0f) : vup;
-                T* dst = static_cast<T*>(a.out) + (s.q0 + token) * a.out_stride_token + head * a.out_stride_head;
+            float* piece = ws.cross + (((long long)cta * 2 + first) * 2 + x) * (C::kPiece / 2);
+            const float inv = whole ? (l > 0.0f ? vup / l : 0.0f) : vup;
+            T* dst = static_cast<T*>(a.out) + (q0 + token) * a.out_stride_token + head * a.out_stride_head;
 #pragma unroll 1
-                for (int c = 0; c < D; c += 16) {
-                    uint32_t o[16];
-                    tmem_ld16(o, o_at + c);
-                    tmem_wait_ld();
-                    float y[16];
+            for (int c = 0; c < D; c += 16) {
+                uint32_t o[16];
+                if (any) tmem_ld16(o, o_at + c);
+                tmem_wait_ld();
+                float y[16];
 #pragma unroll
-                    for (int j = 0; j < 16; ++j)   // INT4: decoded columns (0, 4, 1, 5, 2, 6, 3, 7) of each eight
-                        y[FMT == B4_KV_INT4 ? (j & 8) | (j >> 1 & 3) | (j & 1) << 2 : j] = __uint_as_float(o[j]) * inv;
-                    if (mine && whole) {
+                for (int j = 0; j < 16; ++j)   // INT4: decoded columns (0, 4, 1, 5, 2, 6, 3, 7) of each eight
+                    y[FMT == B4_KV_INT4 ? (j & 8) | (j >> 1 & 3) | (j & 1) << 2 : j] = any ? __uint_as_float(o[j]) * inv : 0.0f;
+                if (mine && whole) {
 #pragma unroll
-                        for (int j = 0; j < 16; j += 8) {
-                            uint32_t w[4];
+                    for (int j = 0; j < 16; j += 8) {
+                        uint32_t w[4];
 #pragma unroll
-                            for (int h = 0; h < 4; ++h) {
-                                const T lo = kv_round<T>(y[j + 2 * h]), hi = kv_round<T>(y[j + 2 * h + 1]);
-                                w[h] = (uint32_t)*reinterpret_cast<const uint16_t*>(&lo) | (uint32_t)*reinterpret_cast<const uint16_t*>(&hi) << 16;
-                            }
-                            *reinterpret_cast<uint4*>(dst + c + j) = make_uint4(w[0], w[1], w[2], w[3]);
+                        for (int e = 0; e < 4; ++e) {
+                            const T lo = kv_round<T>(y[j + 2 * e]), hi = kv_round<T>(y[j + 2 * e + 1]);
+                            w[e] = (uint32_t)*reinterpret_cast<const uint16_t*>(&lo) | (uint32_t)*reinterpret_cast<const uint16_t*>(&hi) << 16;
                         }
-                    } else if (mine) {
-#pragma unroll
-                        for (int j = 0; j < 16; j += 4)
-                            *reinterpret_cast<float4*>(piece + (x * 128 + t) * D + c + j) = make_float4(y[j], y[j + 1], y[j + 2], y[j + 3]);
+                        *reinterpret_cast<uint4*>(dst + c + j) = make_uint4(w[0], w[1], w[2], w[3]);
                     }
-                    __syncwarp();
+                } else if (mine) {
+#pragma unroll
+                    for (int j = 0; j < 16; j += 4)
+                        *reinterpret_cast<float4*>(piece + t * D + c + j) = make_float4(y[j], y[j + 1], y[j + 2], y[j + 3]);
                 }
-                tmem_before_sync();
-                if (whole && mine && a.lse) a.lse[(long long)(s.q0 + token) * a.heads + head] = l > 0.0f ? (m + fast_log2(l)) * kLn2 : -INFINITY;
-                if (!whole) {
-                    piece[kTileRows * D + x * 128 + t] = m;
-                    piece[kTileRows * (D + 1) + x * 128 + t] = l;
-                }
+                __syncwarp();
             }
-            const TileSeg ended = s;
-            s = following;
-            if (whole) continue;
-            // the last of the segment's CTAs joins them, in order: a row a warp
-            const int f = owner(ended.s0), parts = owner(ended.s1 - 1) - f + 1;
+            tmem_before_sync();
+            if (whole) {
+                if (mine && a.lse) a.lse[(long long)(q0 + token) * a.heads + head] = l > 0.0f ? (m + fast_log2(l)) * kLn2 : -INFINITY;
+                continue;
+            }
+            piece[128 * D + t] = m;
+            piece[128 * (D + 1) + t] = l;
+            // the last of the segment's CTAs joins them, in order
+            const int f = owner(s0), parts = owner(s1 - 1) - f + 1;
             auto together = [&]() {            // the eight softmax warps
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&team);
@@ -782,61 +791,71 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attn_tile_kernel(const Att
             };
             if (!(ok = together())) break;
             if (tid == 0) {
+                // the counter is the crossing segment's that begins in CTA f, not that of one inside it
                 __threadfence();
-                joins = atomicAdd(ws.count + f, 1) == parts - 1;
-                if (joins) ws.count[f] = 0;
+                joins = parts == 1 || atomicAdd(ws.count + f, 1) == parts - 1;
+                if (joins && parts > 1) ws.count[f] = 0;
                 __threadfence();
             }
             if (!(ok = together())) break;
             const bool join = joins;
             if (!(ok = together())) break;     // before the flag is written again
             if (!join) continue;
-            auto part = [&](int i) -> const float* { return ws.cross + ((long long)(f + i) * 2 + (i == 0)) * C::kPiece; };
-            if (row0 + warp * 32 >= rows) continue;
-            {
-                // a warp's 32 rows: lane i weighs row i's parts, all lanes add them up row by row
-                constexpr int E = D / 32;
-                const int r0 = warp * 32;
-                float top = kNoMax, sum = 0.0f;
-                for (int i = 0; i < parts; ++i) top = fmaxf(top, __ldcg(part(i) + kTileRows * D + r0 + lane));
-                float y[32][E];
+            // eight rows at a time: lane i weighs row i's parts (two tiles: its CTAs'; one: both streams of each), all lanes
+            // add them up row by row
+            constexpr int E = D / 32;
+            const int n_parts = two ? parts : 2 * parts;
+            auto part = [&](int i) -> const float* {
+                const int c = two ? i : i >> 1, y = two ? x : i & 1;
+                return ws.cross + (((long long)(f + c) * 2 + (c == 0)) * 2 + y) * (C::kPiece / 2);
+            };
+            const int r_first = two ? (warp & 3) * 32 : warp * 16, r_base = row0 + (two ? x * 128 : 0);
+#pragma unroll 1
+            for (int r0 = r_first; r0 < r_first + (two ? 32 : 16) && r_base + r0 < rows; r0 += 8) {
+                float jt = kNoMax, sum = 0.0f, y[8][E];
+                for (int i = 0; i < n_parts; ++i) jt = fmaxf(jt, __ldcg(part(i) + 128 * D + r0 + (lane & 7)));
 #pragma unroll
-                for (int r = 0; r < 32; ++r)
+                for (int r = 0; r < 8; ++r)
 #pragma unroll
                     for (int e = 0; e < E; ++e) y[r][e] = 0.0f;
 #pragma unroll 1
-                for (int i = 0; i < parts; ++i) {
+                for (int i = 0; i < n_parts; ++i) {
                     const float* b = part(i);
-                    const float w = fast_exp2(__ldcg(b + kTileRows * D + r0 + lane) - top);
-                    sum += w * __ldcg(b + kTileRows * (D + 1) + r0 + lane);
+                    const float w = fast_exp2(__ldcg(b + 128 * D + r0 + (lane & 7)) - jt);
+                    sum += w * __ldcg(b + 128 * (D + 1) + r0 + (lane & 7));
 #pragma unroll
-                    for (int r = 0; r < 32; ++r) {
-                        const float k = __shfl_sync(0xffffffffu, w, r);
+                    for (int r = 0; r < 8; ++r) {
+                        const float k8 = __shfl_sync(0xffffffffu, w, r);
                         const float2* z = reinterpret_cast<const float2*>(b + (r0 + r) * D + lane * E);
 #pragma unroll
                         for (int e = 0; e < E / 2; ++e) {
-                            const float2 v = row0 + r0 + r < rows ? __ldcg(z + e) : make_float2(0.0f, 0.0f);
-                            y[r][2 * e] += k * v.x;
-                            y[r][2 * e + 1] += k * v.y;
+                            const float2 v = r_base + r0 + r < rows ? __ldcg(z + e) : make_float2(0.0f, 0.0f);
+                            y[r][2 * e] += k8 * v.x;
+                            y[r][2 * e + 1] += k8 * v.y;
                         }
                     }
                 }
-                const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
+                const int jr = r_base + r0 + (lane & 7), jtk = jr / p.group, jhd = (head / p.group) * p.group + (jr - jtk * p.group);
+                const float jinv = sum > 0.0f ? 1.0f / sum : 0.0f;
 #pragma unroll
-                for (int r = 0; r < 32; ++r) {
-                    const float k = __shfl_sync(0xffffffffu, inv, r);
-                    const int tk = __shfl_sync(0xffffffffu, token, r), hd = __shfl_sync(0xffffffffu, head, r);
-                    if (row0 + r0 + r >= rows) continue;
-                    T* dst = static_cast<T*>(a.out) + (ended.q0 + tk) * a.out_stride_token + hd * a.out_stride_head + lane * E;
+                for (int r = 0; r < 8; ++r) {
+                    const float k8 = __shfl_sync(0xffffffffu, jinv, r);
+                    const int tk = __shfl_sync(0xffffffffu, jtk, r), hd = __shfl_sync(0xffffffffu, jhd, r);
+                    if (r_base + r0 + r < rows) {
+                        T* to = static_cast<T*>(a.out) + (q0 + tk) * a.out_stride_token + hd * a.out_stride_head + lane * E;
 #pragma unroll
-                    for (int e = 0; e < E; e += 2) {
-                        const T w[2] = {kv_round<T>(y[r][e] * k), kv_round<T>(y[r][e + 1] * k)};
-                        *reinterpret_cast<uint32_t*>(dst + e) =
-                            (uint32_t)*reinterpret_cast<const uint16_t*>(w) | (uint32_t)*reinterpret_cast<const uint16_t*>(w + 1) << 16;
+                        for (int e = 0; e < E; e += 2) {
+                            const T w[2] = {kv_round<T>(y[r][e] * k8), kv_round<T>(y[r][e + 1] * k8)};
+                            *reinterpret_cast<uint32_t*>(to + e) =
+                                (uint32_t)*reinterpret_cast<const uint16_t*>(w) | (uint32_t)*reinterpret_cast<const uint16_t*>(w + 1) << 16;
+                        }
                     }
+                    __syncwarp();
                 }
-                if (a.lse && mine) a.lse[(long long)(ended.q0 + token) * a.heads + head] = sum > 0.0f ? (top + fast_log2(sum)) * kLn2 : -INFINITY;
+                if (a.lse && lane < 8 && jr < rows) a.lse[(long long)(q0 + jtk) * a.heads + jhd] = sum > 0.0f ? (jt + fast_log2(sum)) * kLn2 : -INFINITY;
+                __syncwarp();
             }
+            if (!(ok = together())) break;     // before a later segment's pieces take the place of these
         }
     }
     tmem_before_sync();
