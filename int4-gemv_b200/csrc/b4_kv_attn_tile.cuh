@@ -14,10 +14,11 @@
 // weights relative to it and to a running power of two of the value scales, rounded
 // to fp16 for the product.
 //
-// Roles.  Warps 0-3 and 4-7: softmax of the two tiles, a row a thread.  Warps 8-11:
-// codes to fp16 operands, half a token a thread, in the 128-byte swizzle (the same
-// bytes serve K, whose columns are the product's depth, and V, whose rows are).  Warp
-// 12: issues the products.  Warp 13: the schedule.  K and V are rings of four.  A
+// Roles.  Warps 0 and 2: a thread each issues a tile's products (one thread for both
+// took 2.4 us a block over its chain of waits and issues).  Warp 1: the schedule.  Warps 4-7 and 8-11:
+// softmax of the two tiles, a row a thread.  Warps 12-15: codes to fp16 operands, half
+// a token a thread, in the 128-byte swizzle (the same bytes serve K, whose columns are
+// the product's depth, and V, whose rows are).  K and V are rings of four.  A
 // tile has two S of 64 columns of tensor memory (P takes half of one), so that the
 // next block's scores are there when a block's weights are done: with one S of 128
 // columns a block waited 4.1 us on the chain scores - softmax - outputs - scores,
@@ -63,11 +64,11 @@ struct TileWs {
 };
 
 // ---- tcgen05 ----------------------------------------------------------------------
-__device__ __forceinline__ uint64_t umma_desc(uint32_t at, uint32_t lbo, uint32_t sbo)
-{
-    // start, leading and stride byte offsets in 16 bytes; version 1; 128-byte swizzle
-    return (uint64_t)((at >> 4) & 0x3fff) | (uint64_t)((lbo >> 4) & 0x3fff) << 16 | (uint64_t)((sbo >> 4) & 0x3fff) << 32 | 1ULL << 46 | 2ULL << 61;
-}
+// An operand's descriptor: start and leading byte offset in 16 bytes in the lower half;
+// stride byte offset (1024: eight rows of 128 bytes), version 1 and the 128-byte
+// swizzle in the upper.
+__device__ __forceinline__ uint32_t umma_desc(uint32_t at, uint32_t lbo) { return (at >> 4) | (lbo >> 4) << 16; }
+constexpr uint32_t kDescUpper = (1024 >> 4) | 1u << 14 | 2u << 29;
 
 // fp32 accumulators, fp16 operands; `mn`: the right operand's rows are the product's depth
 __host__ __device__ constexpr uint32_t umma_idesc(int m, int n, bool mn)
@@ -75,17 +76,19 @@ __host__ __device__ constexpr uint32_t umma_idesc(int m, int n, bool mn)
     return 1u << 4 | (mn ? 1u << 16 : 0u) | (uint32_t)(n >> 3) << 17 | (uint32_t)(m >> 4) << 24;
 }
 
-__device__ __forceinline__ void umma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add)
+__device__ __forceinline__ void umma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool add)
 {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-                 "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)
+    asm volatile("{\n\t.reg .pred p;\n\t.reg .b64 x, y;\n\tsetp.ne.b32 p, %4, 0;\n\tmov.b64 x, {%1, %5};\n\tmov.b64 y, {%2, %5};\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, p;\n\t}" ::"r"(d), "r"(a), "r"(b), "r"(idesc), "r"((uint32_t)add),
+                 "r"(kDescUpper)
                  : "memory");
 }
 
-__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add)
+__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool add)
 {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)
+    asm volatile("{\n\t.reg .pred p;\n\t.reg .b64 y;\n\tsetp.ne.b32 p, %4, 0;\n\tmov.b64 y, {%2, %5};\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], y, %3, p;\n\t}" ::"r"(d), "r"(a), "r"(b), "r"(idesc), "r"((uint32_t)add),
+                 "r"(kDescUpper)
                  : "memory");
 }
 
@@ -193,7 +196,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attn_tile_kernel(const Att
 {
     using C = TileCfg<FMT, D>;
     extern __shared__ __align__(1024) uint8_t tile_smem[];
-    __shared__ uint64_t seg_full[2], seg_empty[2], q_full[2], s_full[2][2], p_full[2][2], o_done[2][2], tops, team, drain;
+    __shared__ uint64_t seg_full[2], seg_empty[2], q_full[2], s_full[2][2], p_full[2][2], o_done[2][2], q_both, q_free, tops, team, drain[2];
     __shared__ uint64_t k_full[kTileStages], k_empty[kTileStages], v_full[kTileStages], v_empty[kTileStages], scale_full[kScaleRing];
     __shared__ TileSeg segs[2];
     __shared__ long long units_before[kTileThreads + 1];
@@ -217,7 +220,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attn_tile_kernel(const Att
     if (tid == 0) {
         for (int i = 0; i < 2; ++i) {
             mbar_init(&seg_full[i], 1);
-            mbar_init(&seg_empty[i], 13);
+            mbar_init(&seg_empty[i], 14);
             mbar_init(&q_full[i], 4);
             for (int j = 0; j < 2; ++j) {
                 mbar_init(&s_full[i][j], 1);
@@ -227,17 +230,20 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attn_tile_kernel(const Att
         }
         for (int i = 0; i < kTileStages; ++i) {
             mbar_init(&k_full[i], 4);
-            mbar_init(&k_empty[i], 1);
+            mbar_init(&k_empty[i], 2);
             mbar_init(&v_full[i], 4);
-            mbar_init(&v_empty[i], 1);
+            mbar_init(&v_empty[i], 2);
         }
         for (int i = 0; i < kScaleRing; ++i) mbar_init(&scale_full[i], 4);
         mbar_init(&tops, 2);
         mbar_init(&team, 8);
-        mbar_init(&drain, 1);
+        mbar_init(&q_both, 4);
+        mbar_init(&q_free, 1);
+        mbar_init(&drain[0], 1);
+        mbar_init(&drain[1], 1);
         dead = 0;
     }
-    if (warp == 12) {
+    if (warp == 0) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_addr(&tmem_at)) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     }
@@ -337,9 +343,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attn_tile_kernel(const Att
     auto owner = [&](long long u) { return (int)(u < rest * (share + 1) ? u / (share + 1) : rest + (u - rest * (share + 1)) / share); };
     const uint32_t tmem = tmem_at;
 
-    if (warp >= 12) {
+    if (warp < 4) {
         regs_down<64>();
-        if (warp == 13) {
+        if (warp == 1) {
             // ---- schedule ----
             long long u = u0;
             int k = 0;
@@ -390,76 +396,87 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attn_tile_kernel(const Att
                 ++k;
                 if (s.end) break;
             }
-        } else if (warp == 12) {
-            // ---- products ----
+        } else if (warp != 3) {
+            // ---- products: one thread a tile ----
+            const int x = warp >> 1;
             uint32_t leader;
             asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(leader));
-            constexpr uint32_t id_s = umma_idesc(128, kTileKeys, false), id_o = umma_idesc(128, D, true);
-            constexpr uint32_t kPartQ = 128 * 128, kPartB = kTileKeys * 128;       // bytes from 64 columns to the next
-            const uint64_t desc_q = umma_desc(operands, 16, 1024), desc_k = umma_desc(keys_at, 16, 1024);
-            const uint64_t desc_v = umma_desc(values_at, kPartB, 1024);
-            int blocks_before = 0, cq[2] = {0, 0}, cp[2] = {0, 0}, cs[2] = {0, 0};  // the tiles' queries, weights, scores so far
-            bool ok = true;
-            for (int k = 0; ok; ++k) {
-                if (!(ok = warp_wait(&seg_full[k & 1], k >> 1 & 1, &dead))) break;
-                const int blocks = segs[k & 1].blk1 - segs[k & 1].blk0, end = segs[k & 1].end;
-                const bool two = segs[k & 1].n * p.group - segs[k & 1].tile * kTileRows > 128;
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&seg_empty[k & 1]);
-                if (end) break;
-                // step st: the outputs of tile st & 1's block, then the scores of its block after next.  Two tiles of rows:
-                // both take every block; one: each takes every other
-                const int steps = two ? 2 * blocks : blocks;
-#pragma unroll 1
-                for (int st = -4; st < steps; ++st) {
-                    const int x = st & 1, pv = two ? st >> 1 : st, sb = two ? (st >> 1) + 2 : st + 4;
-                    const bool leaves = !two || x == 1;            // the block's last use
-                    if (st >= 0) {
-                        const int b = blocks_before + pv, stage = b & (kTileStages - 1), buf = cp[x] & 1;
-                        if (!(ok = warp_wait(&v_full[stage], b / kTileStages & 1, &dead))) break;
-                        if (!(ok = warp_wait(&p_full[x][buf], cp[x] >> 1 & 1, &dead))) break;
-                        ++cp[x];
-                        tmem_after_sync();
-                        if (leader) {
-                            const uint32_t o = tmem + 256 + x * 128, pa = tmem + x * 128 + buf * 64;
-                            const uint64_t v = desc_v + (uint64_t)(stage * (C::kBlock >> 4));
-                            const bool add = two ? pv > 0 : pv > 1;
-#pragma unroll
-                            for (int i = 0; i < kTileKeys / 16; ++i)
-                                umma_ts(o, pa + i * 8, v + (uint64_t)(i * (2048 >> 4)), id_o, add || i > 0);
-                            umma_commit(&o_done[x][buf]);
-                            if (leaves) umma_commit(&v_empty[stage]);
-                        }
-                        __syncwarp();
-                    }
-                    if (sb < blocks) {
-                        const int b = blocks_before + sb, stage = b & (kTileStages - 1), buf = cs[x]++ & 1;
-                        if (!(ok = warp_wait(&k_full[stage], b / kTileStages & 1, &dead))) break;
-                        if (st < -2 && (two || x == 0) && !(ok = warp_wait(&q_full[x], cq[x]++ & 1, &dead))) break;
-                        tmem_after_sync();
-                        if (leader) {
-                            const uint64_t q = desc_q + (uint64_t)((two ? x : 0) * (C::kOperand >> 4));
-                            const uint64_t kd = desc_k + (uint64_t)(stage * (C::kBlock >> 4));
-#pragma unroll
-                            for (int i = 0; i < D / 16; ++i)
-                                umma_ss(tmem + x * 128 + buf * 64, q + (uint64_t)((i >> 2) * (kPartQ >> 4) + (i & 3) * 2),
-                                        kd + (uint64_t)((i >> 2) * (kPartB >> 4) + (i & 3) * 2), id_s, i > 0);
-                            umma_commit(&s_full[x][buf]);
-                            if (leaves) umma_commit(&k_empty[stage]);
-                        }
-                        __syncwarp();
-                    }
-                }
-                blocks_before += blocks;
-            }
             if (leader) {
-                umma_commit(&drain);           // nothing in flight when the CTA ends
-                for (int i = 0; i < 1 << 20 && !mbar_try_wait(&drain, 0); ++i) {}
+                constexpr uint32_t id_s = umma_idesc(128, kTileKeys, false), id_o = umma_idesc(128, D, true);
+                constexpr uint32_t kPartQ = 128 * 128, kPartB = kTileKeys * 128;   // bytes from 64 columns to the next
+                const uint32_t desc_k = umma_desc(keys_at, 16), desc_v = umma_desc(values_at, kPartB);
+                const uint32_t s_at = tmem + x * 128, o_at = tmem + 256 + x * 128;
+                int blocks_before = 0, cq = 0, shared = 0, cp = 0, cs = 0;     // blocks so far; the tile's queries, shared ones, weights, scores
+                bool ok = true;
+                for (int k = 0; ok; ++k) {
+                    if (!(ok = tile_wait(&seg_full[k & 1], k >> 1 & 1, &dead))) break;
+                    const int blocks = segs[k & 1].blk1 - segs[k & 1].blk0, end = segs[k & 1].end;
+                    const bool two = segs[k & 1].n * p.group - segs[k & 1].tile * kTileRows > 128;
+                    mbar_arrive(&seg_empty[k & 1]);
+                    if (end) break;
+                    // two tiles of rows: each takes every block; one: the tile's thread takes every other, and says so of
+                    // the others once they are there (a block is left when both threads have left it)
+                    const uint32_t desc_q = umma_desc(operands + (two ? x : 0) * C::kOperand, 16);
+                    const int ahead = two ? 2 : 4;
+                    bool queries = two || x == 0, add = false;
+                    if (!two && x == 1) {                          // the first tile's queries
+                        if (!(ok = tile_wait(&q_both, shared++ & 1, &dead))) break;
+                        if (blocks == 1) mbar_arrive(&q_free);
+                    }
+#pragma unroll 1
+                    for (int i = -ahead; i < blocks; ++i) {
+                        const int sb = i + ahead;
+                        const bool taken = two || (i & 1) == x;    // ahead is even: so is the parity of sb
+                        if (i >= 0) {
+                            const int b = blocks_before + i, stage = b & (kTileStages - 1);
+                            if (!(ok = tile_wait(&v_full[stage], b / kTileStages & 1, &dead))) break;
+                            if (taken) {
+                                const int buf = cp & 1;
+                                if (!(ok = tile_wait(&p_full[x][buf], cp >> 1 & 1, &dead))) break;
+                                ++cp;
+                                tmem_after_sync();
+                                const uint32_t pa = s_at + buf * 64, v = desc_v + stage * (C::kBlock >> 4);
+#pragma unroll
+                                for (int j = 0; j < kTileKeys / 16; ++j) umma_ts(o_at, pa + j * 8, v + j * (2048 >> 4), id_o, add || j > 0);
+                                add = true;
+                                umma_commit(&o_done[x][buf]);
+                                umma_commit(&v_empty[stage]);
+                            } else {
+                                mbar_arrive(&v_empty[stage]);
+                            }
+                        }
+                        if (sb < blocks) {
+                            const int b = blocks_before + sb, stage = b & (kTileStages - 1);
+                            if (!(ok = tile_wait(&k_full[stage], b / kTileStages & 1, &dead))) break;
+                            if (taken) {
+                                if (queries) {
+                                    if (!(ok = tile_wait(&q_full[x], cq++ & 1, &dead))) break;
+                                    queries = false;
+                                }
+                                const int buf = cs++ & 1;
+                                tmem_after_sync();
+                                const uint32_t kd = desc_k + stage * (C::kBlock >> 4);
+#pragma unroll
+                                for (int j = 0; j < D / 16; ++j)
+                                    umma_ss(s_at + buf * 64, desc_q + (j >> 2) * (kPartQ >> 4) + (j & 3) * 2,
+                                            kd + (j >> 2) * (kPartB >> 4) + (j & 3) * 2, id_s, j > 0);
+                                umma_commit(&s_full[x][buf]);
+                                umma_commit(&k_empty[stage]);
+                                if (!two && x == 1 && sb + 2 >= blocks) umma_commit(&q_free);
+                            } else {
+                                mbar_arrive(&k_empty[stage]);
+                            }
+                        }
+                    }
+                    blocks_before += blocks;
+                }
+                umma_commit(&drain[x]);        // nothing in flight when the CTA ends
+                for (int i = 0; i < 1 << 20 && !mbar_try_wait(&drain[x], 0); ++i) {}
             }
             __syncwarp();
         }
-    } else if (warp >= 8) {
-        // ---- codes to operands: half a token a thread (warps 8, 9 the first columns and the keys' scales, 10, 11 the others
+    } else if (warp >= 12) {
+        // ---- codes to operands: half a token a thread (warps 12, 13 the first columns and the keys' scales, 14, 15 the others
         // and the values'); keys, values, keys, ... through one loop, the next operand's codes on their way while one is
         // written ----
         regs_down<96>();
@@ -581,10 +598,10 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attn_tile_kernel(const Att
     } else {
         // ---- softmax: a row a thread ----
         regs_up<176>();
-        const int x = warp >> 2, t = tid & 127;
+        const int x = (warp >> 2) - 1, t = tid & 127;
         const uint32_t lanes = (uint32_t)(warp & 3) << 21;          // 32 lanes a warp, lane in the upper half
         const uint32_t s_at = tmem + lanes + x * 128, o_at = tmem + lanes + 256 + x * 128;
-        int cs = 0, ring0 = 0, teams = 0;      // this tile's blocks so far; all blocks; the joins' barrier's turns
+        int cs = 0, ring0 = 0, teams = 0, shared = 0;      // this tile's blocks so far; all blocks; barriers' turns
         bool ok = true;
         TileSeg s;
         // A segment's queries to shared memory: fp16 in the order of the decoded codes (bf16: times a power of two, as
@@ -627,7 +644,10 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attn_tile_kernel(const Att
             }
             fence_proxy_async();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&q_full[x]);
+            if (lane == 0) {
+                mbar_arrive(&q_full[x]);
+                if (!two) mbar_arrive(&q_both);
+            }
             return factor;
         };
         auto fetch = [&](int k) {
@@ -735,12 +755,12 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attn_tile_kernel(const Att
             if (!ok) break;
             ring0 += blocks;
             // the next segment's queries, whose scores are then computed under this one's end; where the other stream reads
-            // the same queries, after it has: the outputs' barrier comes after all products issued before them
-            if (!two && any && !(ok = warp_wait(&o_done[x][cs - 1 & 1], (cs - 1) >> 1 & 1, &dead))) break;
+            // the same queries, after its last scores
+            if (!two && x == 0 && !(ok = warp_wait(&q_free, shared++ & 1, &dead))) break;
             fetch(k);
             if (!ok) break;
             if (!s.end) factor = put_query(s);
-            if (two && !(ok = warp_wait(&o_done[x][cs - 1 & 1], (cs - 1) >> 1 & 1, &dead))) break;
+            if (any && !(ok = warp_wait(&o_done[x][cs - 1 & 1], (cs - 1) >> 1 & 1, &dead))) break;
             tmem_after_sync();
 
             // ---- the segment's rows, or a piece of them ----
@@ -790,7 +810,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attn_tile_kernel(const Att
                 return warp_wait(&team, teams++ & 1, &dead);
             };
             if (!(ok = together())) break;
-            if (tid == 0) {
+            if (tid == 128) {
                 // the counter is the crossing segment's that begins in CTA f, not that of one inside it
                 __threadfence();
                 joins = parts == 1 || atomicAdd(ws.count + f, 1) == parts - 1;
@@ -809,7 +829,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attn_tile_kernel(const Att
                 const int c = two ? i : i >> 1, y = two ? x : i & 1;
                 return ws.cross + (((long long)(f + c) * 2 + (c == 0)) * 2 + y) * (C::kPiece / 2);
             };
-            const int r_first = two ? (warp & 3) * 32 : warp * 16, r_base = row0 + (two ? x * 128 : 0);
+            const int r_first = two ? (warp & 3) * 32 : (warp - 4) * 16, r_base = row0 + (two ? x * 128 : 0);
 #pragma unroll 1
             for (int r0 = r_first; r0 < r_first + (two ? 32 : 16) && r_base + r0 < rows; r0 += 8) {
                 float jt = kNoMax, sum = 0.0f, y[8][E];
@@ -861,7 +881,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attn_tile_kernel(const Att
     tmem_before_sync();
     __syncthreads();
     tmem_after_sync();
-    if (warp == 12) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+    if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
 }
 
 }  // namespace b4
