@@ -38,7 +38,7 @@
 
 namespace b4 {
 
-constexpr int kTileRows = 256, kTileKeys = 64, kTileThreads = 512, kTileStages = 4, kScaleRing = 8;
+constexpr int kTileRows = 256, kTileKeys = 64, kTileThreads = 512, kTileStages = 4;
 
 template <int FMT, int D>
 struct TileCfg {
@@ -47,7 +47,7 @@ struct TileCfg {
     static constexpr int kBlock = kTileKeys * D * 2;               // of a block's keys or values: parts of 64 x 128 bytes
     // NF4: pairs of levels by byte, 256 rows of 16 copies (2 lanes a copy), at shared address 16384, so that an OR makes
     // a lookup's address; the operands follow it.  Without it they follow the static part.
-    static constexpr int kTable = 16384, kStatic = 10240;
+    static constexpr int kTable = 16384, kStatic = 9216;
     static constexpr int kPiece = kTileRows * (D + 2);             // floats: output, maxima, sums
     static constexpr int kSmem = 2 * kOperand + 2 * kTileStages * kBlock + (FMT == B4_KV_NF4 ? 2 * kTable - kStatic : 1024);   // kStatic: less than the static part and the system's
 };
@@ -175,6 +175,13 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t phase, volatil
     return __all_sync(0xffffffffu, tile_wait(bar, phase, dead));
 }
 
+__device__ __forceinline__ bool elect_one()
+{
+    uint32_t one;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
+    return one != 0;
+}
+
 template <int R>
 __device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(R)); }
 template <int R>
@@ -197,23 +204,23 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attn_tile_kernel(const Att
     using C = TileCfg<FMT, D>;
     extern __shared__ __align__(1024) uint8_t tile_smem[];
     __shared__ uint64_t seg_full[2], seg_empty[2], q_full[2], s_full[2][2], p_full[2][2], o_done[2][2], q_both, q_free, tops, team, drain[2];
-    __shared__ uint64_t k_full[kTileStages], k_empty[kTileStages], v_full[kTileStages], v_empty[kTileStages], scale_full[kScaleRing];
+    __shared__ uint64_t full[kTileStages], empty[kTileStages];
     __shared__ TileSeg segs[2];
     __shared__ long long units_before[kTileThreads + 1];
     __shared__ int tiles_before[kTileThreads + 1];
     __shared__ long long warp_sum[kTileThreads / 32];
-    __shared__ __align__(16) float key_scale[kScaleRing][kTileKeys], value_scale[kScaleRing][kTileKeys];
-    __shared__ int value_exp[kScaleRing], block_pages[kScaleRing];
+    __shared__ __align__(16) float key_scale[kTileStages][kTileKeys], value_scale[kTileStages][kTileKeys];
+    __shared__ int value_exp[kTileStages], block_pages[kTileStages];
     __shared__ float value_top[2][2];
     __shared__ uint32_t tmem_at;
     __shared__ volatile int dead;
     __shared__ int joins;
 
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int tid = threadIdx.x, lane = tid & 31, warp_u = __shfl_sync(0xffffffffu, tid >> 5, 0), warp = warp_u;
     const b4_kv_attn& a = p.a;
     const uint32_t operands = FMT == B4_KV_NF4 ? 2 * C::kTable : (smem_addr(tile_smem) + 1023) & ~1023u;
     const uint32_t keys_at = operands + 2 * C::kOperand, values_at = keys_at + kTileStages * C::kBlock;     // after Q of both tiles
-    if (FMT == B4_KV_NF4 && smem_addr(tile_smem) > C::kTable) {       // the static part has outgrown its place
+    if (FMT == B4_KV_NF4 && (smem_addr(tile_smem) > C::kTable || smem_addr(tile_smem) < C::kStatic)) {   // the static part is not as kSmem takes it
         if (tid == 0) atomicOr(&g_device_error, kErrMbarrierTimeout);
         return;
     }
@@ -229,12 +236,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attn_tile_kernel(const Att
             }
         }
         for (int i = 0; i < kTileStages; ++i) {
-            mbar_init(&k_full[i], 4);
-            mbar_init(&k_empty[i], 2);
-            mbar_init(&v_full[i], 4);
-            mbar_init(&v_empty[i], 2);
+            mbar_init(&full[i], 4);
+            mbar_init(&empty[i], 2);
         }
-        for (int i = 0; i < kScaleRing; ++i) mbar_init(&scale_full[i], 4);
         mbar_init(&tops, 2);
         mbar_init(&team, 8);
         mbar_init(&q_both, 4);
@@ -397,79 +401,87 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attn_tile_kernel(const Att
                 if (s.end) break;
             }
         } else if (warp != 3) {
-            // ---- products: one thread a tile ----
-            const int x = warp >> 1;
-            uint32_t leader;
-            asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(leader));
-            if (leader) {
-                constexpr uint32_t id_s = umma_idesc(128, kTileKeys, false), id_o = umma_idesc(128, D, true);
-                constexpr uint32_t kPartQ = 128 * 128, kPartB = kTileKeys * 128;   // bytes from 64 columns to the next
-                const uint32_t desc_k = umma_desc(keys_at, 16), desc_v = umma_desc(values_at, kPartB);
-                const uint32_t s_at = tmem + x * 128, o_at = tmem + 256 + x * 128;
-                int blocks_before = 0, cq = 0, shared = 0, cp = 0, cs = 0;     // blocks so far; the tile's queries, shared ones, weights, scores
-                bool ok = true;
-                for (int k = 0; ok; ++k) {
-                    if (!(ok = tile_wait(&seg_full[k & 1], k >> 1 & 1, &dead))) break;
-                    const int blocks = segs[k & 1].blk1 - segs[k & 1].blk0, end = segs[k & 1].end;
-                    const bool two = segs[k & 1].n * p.group - segs[k & 1].tile * kTileRows > 128;
-                    mbar_arrive(&seg_empty[k & 1]);
-                    if (end) break;
-                    // two tiles of rows: each takes every block; one: the tile's thread takes every other, and says so of
-                    // the others once they are there (a block is left when both threads have left it)
-                    const uint32_t desc_q = umma_desc(operands + (two ? x : 0) * C::kOperand, 16);
-                    const int ahead = two ? 2 : 4;
-                    bool queries = two || x == 0, add = false;
-                    if (!two && x == 1) {                          // the first tile's queries
-                        if (!(ok = tile_wait(&q_both, shared++ & 1, &dead))) break;
-                        if (blocks == 1) mbar_arrive(&q_free);
+            // ---- products: one warp a tile ----
+            // Everything that an instruction takes is the same in all lanes and known to be (values from shared memory come
+            // through a shuffle), so that it sits in uniform registers; one elected lane issues.
+            const int x = warp_u >> 1;
+            constexpr uint32_t id_s = umma_idesc(128, kTileKeys, false), id_o = umma_idesc(128, D, true);
+            constexpr uint32_t kPartQ = 128 * 128, kPartB = kTileKeys * 128;       // bytes from 64 columns to the next
+            const uint32_t desc_k = umma_desc(keys_at, 16), desc_v = umma_desc(values_at, kPartB);
+            const uint32_t tmem_u = __shfl_sync(0xffffffffu, tmem, 0), s_at = tmem_u + x * 128, o_at = tmem_u + 256 + x * 128;
+            int blocks_before = 0, cq = 0, shared = 0, cp = 0, cs = 0;             // blocks so far; the tile's queries, shared ones, weights, scores
+            bool ok = true;
+            for (int k = 0; ok; ++k) {
+                if (!(ok = warp_wait(&seg_full[k & 1], k >> 1 & 1, &dead))) break;
+                const TileSeg& g = segs[k & 1];
+                const int blocks = __shfl_sync(0xffffffffu, g.blk1 - g.blk0, 0), end = __shfl_sync(0xffffffffu, g.end, 0);
+                const bool two = __shfl_sync(0xffffffffu, g.n * p.group - g.tile * kTileRows, 0) > 128;
+                if (elect_one()) mbar_arrive(&seg_empty[k & 1]);
+                __syncwarp();
+                if (end) break;
+                // two tiles of rows: each takes every block; one: the tile's warp takes every other, and says so of the
+                // others once they are there (a block is left when both warps have left it)
+                const uint32_t desc_q = umma_desc(operands + (two ? x : 0) * C::kOperand, 16);
+                const int ahead = two ? 2 : 4;
+                bool queries = two || x == 0, add = false;
+                if (!two && x == 1) {                              // the first tile's queries
+                    if (!(ok = warp_wait(&q_both, shared++ & 1, &dead))) break;
+                    if (blocks == 1) {
+                        if (elect_one()) mbar_arrive(&q_free);
+                        __syncwarp();
                     }
+                }
 #pragma unroll 1
-                    for (int i = -ahead; i < blocks; ++i) {
-                        const int sb = i + ahead;
-                        const bool taken = two || (i & 1) == x;    // ahead is even: so is the parity of sb
-                        if (i >= 0) {
-                            const int b = blocks_before + i, stage = b & (kTileStages - 1);
-                            if (!(ok = tile_wait(&v_full[stage], b / kTileStages & 1, &dead))) break;
+                for (int i = -ahead; i < blocks; ++i) {
+                    const int sb = i + ahead;
+                    const bool taken = two || (i & 1) == x;        // ahead is even: so is the parity of sb
+                    if (i >= 0) {                                  // the block's operands are there since its scores
+                        const int stage = (blocks_before + i) & (kTileStages - 1), buf = cp & 1;
+                        if (taken) {
+                            if (!(ok = warp_wait(&p_full[x][buf], cp >> 1 & 1, &dead))) break;
+                            ++cp;
+                        }
+                        tmem_after_sync();
+                        if (elect_one()) {
                             if (taken) {
-                                const int buf = cp & 1;
-                                if (!(ok = tile_wait(&p_full[x][buf], cp >> 1 & 1, &dead))) break;
-                                ++cp;
-                                tmem_after_sync();
                                 const uint32_t pa = s_at + buf * 64, v = desc_v + stage * (C::kBlock >> 4);
 #pragma unroll
                                 for (int j = 0; j < kTileKeys / 16; ++j) umma_ts(o_at, pa + j * 8, v + j * (2048 >> 4), id_o, add || j > 0);
-                                add = true;
                                 umma_commit(&o_done[x][buf]);
-                                umma_commit(&v_empty[stage]);
+                                umma_commit(&empty[stage]);
                             } else {
-                                mbar_arrive(&v_empty[stage]);
+                                mbar_arrive(&empty[stage]);
                             }
                         }
-                        if (sb < blocks) {
-                            const int b = blocks_before + sb, stage = b & (kTileStages - 1);
-                            if (!(ok = tile_wait(&k_full[stage], b / kTileStages & 1, &dead))) break;
-                            if (taken) {
-                                if (queries) {
-                                    if (!(ok = tile_wait(&q_full[x], cq++ & 1, &dead))) break;
-                                    queries = false;
-                                }
-                                const int buf = cs++ & 1;
-                                tmem_after_sync();
+                        __syncwarp();
+                        add = add || taken;
+                    }
+                    if (sb < blocks) {
+                        const int b = blocks_before + sb, stage = b & (kTileStages - 1), buf = cs & 1;
+                        if (!(ok = warp_wait(&full[stage], b / kTileStages & 1, &dead))) break;
+                        if (taken) {
+                            if (queries) {
+                                if (!(ok = warp_wait(&q_full[x], cq++ & 1, &dead))) break;
+                                queries = false;
+                            }
+                            tmem_after_sync();
+                            if (elect_one()) {
                                 const uint32_t kd = desc_k + stage * (C::kBlock >> 4);
 #pragma unroll
                                 for (int j = 0; j < D / 16; ++j)
                                     umma_ss(s_at + buf * 64, desc_q + (j >> 2) * (kPartQ >> 4) + (j & 3) * 2,
                                             kd + (j >> 2) * (kPartB >> 4) + (j & 3) * 2, id_s, j > 0);
                                 umma_commit(&s_full[x][buf]);
-                                umma_commit(&k_empty[stage]);
                                 if (!two && x == 1 && sb + 2 >= blocks) umma_commit(&q_free);
-                            } else {
-                                mbar_arrive(&k_empty[stage]);
                             }
+                            __syncwarp();
+                            ++cs;
                         }
                     }
-                    blocks_before += blocks;
                 }
+                blocks_before += blocks;
+            }
+            if (elect_one()) {
                 umma_commit(&drain[x]);        // nothing in flight when the CTA ends
                 for (int i = 0; i < 1 << 20 && !mbar_try_wait(&drain[x], 0); ++i) {}
             }
@@ -477,90 +489,42 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attn_tile_kernel(const Att
         }
     } else if (warp >= 12) {
         // ---- codes to operands: half a token a thread (warps 12, 13 the first columns and the keys' scales, 14, 15 the others
-        // and the values'); keys, values, keys, ... through one loop, the next operand's codes on their way while one is
-        // written ----
+        // and the values'); a block's codes are asked for while the one before is written, its page ids a block before that
         regs_down<96>();
         const int t = tid & 63, half = warp >> 1 & 1;
         constexpr int W = D / 16;              // words of half a token's codes
         constexpr int kPart = D == 128 ? kTileKeys * 128 : 0;      // D = 64: both halves lie in one part
         const uint32_t row_at = t * 128 + half * kPart, swizzle = (t & 7) << 4, chunk0 = D == 128 ? 0 : half * W;
         const int row = t & (p.l.page_size - 1);
-        TileSeg s;
-        int k = -1, blk = 0, id = -1, id_next = -1, vexp = -126, see_begin = 0, see_end = 0;
-        uint4 raw[W / 4];
-        float scale = 0.0f;                    // the key's or the value's
-        bool ok = true, there = false;
-        auto page_id = [&](const TileSeg& g, int block) {
+        struct Codes {
+            uint4 k[W / 4], v[W / 4];
+            float scale;                       // the key's or the value's
+            bool there;
+        };
+        TileSeg s = {};
+        int k = -1, blk = 0, vexp = -126, see_begin = 0, see_end = 0;
+        bool ok = true;
+        auto page_id = [&](int block) {
             const int token = block * kTileKeys + t;
-            return token < g.ctx ? __ldg(a.tables + (long long)g.r * a.table_stride + (token >> p.l.page_shift)) : -1;
+            return block < s.blk1 && token < s.ctx ? __ldg(a.tables + (long long)s.r * a.table_stride + (token >> p.l.page_shift)) : -1;
         };
-        auto load = [&](int page, int head, int o) {                // o: 0 keys and the scale, 1 values
-            there = (unsigned)page < (unsigned)p.l.n_pages;
+        auto load = [&](int page, Codes& c) {
+            c.there = (unsigned)page < (unsigned)p.l.n_pages;
 #pragma unroll
-            for (int i = 0; i < W / 4; ++i) raw[i] = make_uint4(0, 0, 0, 0);
-            if (o == 0) scale = 0.0f;
-            if (!there) return;
-            const uint8_t* b = p.blocks + ((long long)page * p.l.kv_heads + head) * p.l.block;
-            const uint4* codes = reinterpret_cast<const uint4*>(b + (o * p.l.page_size + row) * C::kRow + half * (C::kRow / 2));
+            for (int i = 0; i < W / 4; ++i) c.k[i] = c.v[i] = make_uint4(0, 0, 0, 0);
+            c.scale = 0.0f;
+            if (!c.there) return;
+            const uint8_t* b = p.blocks + ((long long)page * p.l.kv_heads + s.head) * p.l.block;
+            const uint8_t* codes = b + row * C::kRow + half * (C::kRow / 2);
 #pragma unroll
-            for (int i = 0; i < W / 4; ++i) raw[i] = __ldg(codes + i);
-            if (o == 0) {
-                const uint8_t* sp = b + p.l.page_size * D + (half * p.l.page_size + row) * C::kScale;
-                scale = FMT == B4_KV_INT4 ? __half2float(*reinterpret_cast<const __half*>(sp)) : *reinterpret_cast<const float*>(sp);
+            for (int i = 0; i < W / 4; ++i) {
+                c.k[i] = __ldg(reinterpret_cast<const uint4*>(codes) + i);
+                c.v[i] = __ldg(reinterpret_cast<const uint4*>(codes + p.l.page_size * C::kRow) + i);
             }
+            const uint8_t* sp = b + p.l.page_size * D + (half * p.l.page_size + row) * C::kScale;
+            c.scale = FMT == B4_KV_INT4 ? __half2float(*reinterpret_cast<const __half*>(sp)) : *reinterpret_cast<const float*>(sp);
         };
-        // the next segment, or the end of the run
-        auto next_segment = [&]() {
-            ++k;
-            if (!(ok = warp_wait(&seg_full[k & 1], k >> 1 & 1, &dead))) return false;
-            s = segs[k & 1];
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&seg_empty[k & 1]);
-            if (s.end) return false;
-            const int last_row = min((s.tile + 1) * kTileRows, s.n * p.group) - 1;
-            see_end = a.flags & B4_KV_FULL ? s.ctx : min(s.ctx, s.ctx - s.n + last_row / p.group + 1);
-            see_begin = a.window > 0 ? s.ctx - s.n + s.tile * kTileRows / p.group + 1 - a.window : 0;
-            return true;
-        };
-        bool more = next_segment();
-        if (more) {
-            blk = s.blk0;
-            id = page_id(s, blk);
-            load(id, s.head, 0);
-        }
-#pragma unroll 1
-        for (int j = 0; more; ++j) {           // j: operands so far; even ones keys
-            const int o = j & 1, b = j >> 1, stage = b & (kTileStages - 1);
-            if (o == 0) {
-                // scales: those of tokens that no row sees are 0, the values' relative to a running power of two
-                const int token = blk * kTileKeys + t, ring = b & (kScaleRing - 1);
-                const bool seen = there && token < see_end && token >= see_begin;
-                if (half) {
-                    if (blk == s.blk0) vexp = -126;
-                    const float v = seen ? fminf(scale, 3.4028235e38f) : 0.0f;
-                    const unsigned bits = __reduce_max_sync(0xffffffffu, v < 3.4028235e38f ? __float_as_uint(fabsf(v)) : 0u);
-                    if (lane == 0) {
-                        value_top[b & 1][warp & 1] = __uint_as_float(bits);
-                        mbar_arrive(&tops);
-                    }
-                    __syncwarp();
-                    if (!(ok = warp_wait(&tops, b & 1, &dead))) break;
-                    const float top = fmaxf(value_top[b & 1][0], value_top[b & 1][1]);
-                    vexp = max(vexp, min((int)(__float_as_uint(top) >> 23) - 126, 126));
-                    value_scale[ring][t] = v * pow2(-vexp);
-                    if (t == 0) value_exp[ring] = vexp;
-                } else {
-                    key_scale[ring][t] = seen ? scale : 0.0f;
-                    // tokens that are not there lie in whole pages of 16 at least: two bits a warp
-                    const unsigned pages = __ballot_sync(0xffffffffu, there);
-                    if (lane == 0) reinterpret_cast<uint8_t*>(&block_pages[ring])[warp & 1] = (uint8_t)((pages & 1) | (pages >> 16 & 1) << 1);
-                }
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&scale_full[ring]);
-                if (blk + 1 < s.blk1) id_next = page_id(s, blk + 1);
-            }
-            if (b >= kTileStages && !(ok = warp_wait(o ? &v_empty[stage] : &k_empty[stage], (b / kTileStages + 1) & 1, &dead))) break;
-            const uint32_t to = (o ? values_at : keys_at) + stage * C::kBlock + row_at;
+        auto write = [&](uint32_t to, const uint4 (&raw)[W / 4]) {
             const uint32_t* w = reinterpret_cast<const uint32_t*>(raw);
 #pragma unroll
             for (int i = 0; i < W; ++i) {
@@ -578,22 +542,77 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attn_tile_kernel(const Att
                              "r"(h[3])
                              : "memory");
             }
-            // the operand after this one
-            if (o == 1) {
-                if (++blk < s.blk1) {
-                    id = id_next;
-                } else {
-                    more = next_segment();
-                    if (more) {
-                        blk = s.blk0;
-                        id = page_id(s, blk);
-                    }
-                }
+        };
+        // the next segment, or the end of the run
+        auto next_segment = [&]() {
+            ++k;
+            if (!(ok = warp_wait(&seg_full[k & 1], k >> 1 & 1, &dead))) return false;
+            s = segs[k & 1];
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&seg_empty[k & 1]);
+            if (s.end) return false;
+            const int last_row = min((s.tile + 1) * kTileRows, s.n * p.group) - 1;
+            see_end = a.flags & B4_KV_FULL ? s.ctx : min(s.ctx, s.ctx - s.n + last_row / p.group + 1);
+            see_begin = a.window > 0 ? s.ctx - s.n + s.tile * kTileRows / p.group + 1 - a.window : 0;
+            return true;
+        };
+        Codes now, next;
+        int id_next = -1;
+        bool more = next_segment();
+        if (more) {
+            blk = s.blk0;
+            const int id = page_id(blk);
+            id_next = page_id(blk + 1);
+            load(id, now);
+        }
+#pragma unroll 1
+        for (int b = 0; more; ++b) {
+            const int stage = b & (kTileStages - 1);
+            if (blk + 1 < s.blk1) {
+                load(id_next, next);
+                id_next = page_id(blk + 2);
             }
-            if (more) load(id, s.head, 1 - o);
+            if (b >= kTileStages && !(ok = warp_wait(&empty[stage], (b / kTileStages + 1) & 1, &dead))) break;
+            // scales: those of tokens that no row sees are 0, the values' relative to a running power of two
+            const int token = blk * kTileKeys + t;
+            const bool seen = now.there && token < see_end && token >= see_begin;
+            if (half) {
+                if (blk == s.blk0) vexp = -126;
+                const float v = seen ? fminf(now.scale, 3.4028235e38f) : 0.0f;
+                const unsigned bits = __reduce_max_sync(0xffffffffu, v < 3.4028235e38f ? __float_as_uint(fabsf(v)) : 0u);
+                if (lane == 0) {
+                    value_top[b & 1][warp & 1] = __uint_as_float(bits);
+                    mbar_arrive(&tops);
+                }
+                __syncwarp();
+                write(values_at + stage * C::kBlock + row_at, now.v);          // while the other warp's maximum comes
+                if (!(ok = warp_wait(&tops, b & 1, &dead))) break;
+                const float top = fmaxf(value_top[b & 1][0], value_top[b & 1][1]);
+                vexp = max(vexp, min((int)(__float_as_uint(top) >> 23) - 126, 126));
+                value_scale[stage][t] = v * pow2(-vexp);
+                if (t == 0) value_exp[stage] = vexp;
+            } else {
+                key_scale[stage][t] = seen ? now.scale : 0.0f;
+                // tokens that are not there lie in whole pages of 16 at least: two bits a warp
+                const unsigned pages = __ballot_sync(0xffffffffu, now.there);
+                if (lane == 0) reinterpret_cast<uint8_t*>(&block_pages[stage])[warp & 1] = (uint8_t)((pages & 1) | (pages >> 16 & 1) << 1);
+                write(values_at + stage * C::kBlock + row_at, now.v);
+            }
+            write(keys_at + stage * C::kBlock + row_at, now.k);
             fence_proxy_async();
             __syncwarp();
-            if (lane == 0) mbar_arrive(o ? &v_full[stage] : &k_full[stage]);
+            if (lane == 0) mbar_arrive(&full[stage]);
+            if (++blk < s.blk1) {
+                now = next;
+            } else {
+                more = next_segment();
+                if (more) {
+                    blk = s.blk0;
+                    const int id = page_id(blk);
+                    id_next = page_id(blk + 1);
+                    load(id, now);
+                }
+            }
         }
     } else {
         // ---- softmax: a row a thread ----
@@ -675,13 +694,13 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attn_tile_kernel(const Att
             bool any = false;                  // whether O holds something
 #pragma unroll 1
             for (int i = two ? 0 : x; i < blocks && ok; i += two ? 1 : 2, ++cs) {
-                const int ring = (ring0 + i) & (kScaleRing - 1), buf = cs & 1;
+                const int stage = (ring0 + i) & (kTileStages - 1), buf = cs & 1;
                 if (!(ok = warp_wait(&s_full[x][buf], cs >> 1 & 1, &dead))) break;
-                // after the scores, so that the phase asked for is the last one done
-                if (!(ok = warp_wait(&scale_full[ring], (ring0 + i) / kScaleRing & 1, &dead))) break;
+                // the scales' writers; after the scores, so that the phase asked for is the last one done
+                if (!(ok = warp_wait(&full[stage], (ring0 + i) / kTileStages & 1, &dead))) break;
                 tmem_after_sync();
-                const int key0 = (s.blk0 + i) * kTileKeys, pages = block_pages[ring] & 0xffff, ve = value_exp[ring];
-                const float4* ks = reinterpret_cast<const float4*>(key_scale[ring]);
+                const int key0 = (s.blk0 + i) * kTileKeys, pages = block_pages[stage] & 0xffff, ve = value_exp[stage];
+                const float4* ks = reinterpret_cast<const float4*>(key_scale[stage]);
                 float2 v[kTileKeys / 2];       // the row's scores
                 tmem_ld32(reinterpret_cast<uint32_t*>(v), s_at + buf * 64);
                 tmem_ld32(reinterpret_cast<uint32_t*>(v) + 32, s_at + buf * 64 + 32);
@@ -727,7 +746,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attn_tile_kernel(const Att
                 }
                 any = true;
                 const float2 q2 = make_float2(qf, qf), m2 = make_float2(-m, -m);
-                const float4* vs = reinterpret_cast<const float4*>(value_scale[ring]);
+                const float4* vs = reinterpret_cast<const float4*>(value_scale[stage]);
                 float2 l2[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
                 uint32_t w[kTileKeys / 2];
 #pragma unroll
