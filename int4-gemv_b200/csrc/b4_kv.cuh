@@ -82,4 +82,17 @@ template <typename T> __device__ __forceinline__ T kv_round(float v);
 template <> __device__ __forceinline__ __half kv_round<__half>(float v) { return __float2half_rn(v); }
 template <> __device__ __forceinline__ __nv_bfloat16 kv_round<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
+// two columns as T, packed
+template <typename T> __device__ __forceinline__ uint32_t kv_round2(float lo, float hi);
+template <> __device__ __forceinline__ uint32_t kv_round2<__half>(float lo, float hi)
+{
+    const __half2 v = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+template <> __device__ __forceinline__ uint32_t kv_round2<__nv_bfloat16>(float lo, float hi)
+{
+    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+
 }  // namespace b4

@@ -47,7 +47,7 @@ struct TileCfg {
     static constexpr int kBlock = kTileKeys * D * 2;               // of a block's keys or values: parts of 64 x 128 bytes
     // NF4: pairs of levels by byte, 256 rows of 16 copies (2 lanes a copy), at shared address 16384, so that an OR makes
     // a lookup's address; the operands follow it.  Without it they follow the static part.
-    static constexpr int kTable = 16384, kStatic = 9216;
+    static constexpr int kTable = 16384, kStatic = 13312;
     static constexpr int kPiece = kTileRows * (D + 2);             // floats: output, maxima, sums
     static constexpr int kSmem = 2 * kOperand + 2 * kTileStages * kBlock + (FMT == B4_KV_NF4 ? 2 * kTable - kStatic : 1024);   // kStatic: less than the static part and the system's
 };
@@ -131,6 +131,19 @@ __device__ __forceinline__ void tmem_st16(uint32_t at, const uint32_t* r)
 #undef B4_R8
 #undef B4_W8
 
+__device__ __forceinline__ uint4 lds128(uint32_t at)
+{
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
+    return v;
+}
+
+// 16 bytes, or zeros
+__device__ __forceinline__ void copy_async16_or_0(uint32_t dst, const void* src, bool there)
+{
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
+}
+
 __device__ __forceinline__ unsigned long long now_ns()
 {
     unsigned long long t;
@@ -212,6 +225,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attn_tile_kernel(const Att
     __shared__ __align__(16) float key_scale[kTileStages][kTileKeys], value_scale[kTileStages][kTileKeys];
     __shared__ int value_exp[kTileStages], block_pages[kTileStages];
     __shared__ float value_top[2][2];
+    __shared__ float q_factor[2][128], stream_max[2][128], stream_sum[2][128], stream_up[2][128];
     __shared__ uint32_t tmem_at;
     __shared__ volatile int dead;
     __shared__ int joins;
@@ -422,11 +436,12 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attn_tile_kernel(const Att
                 // two tiles of rows: each takes every block; one: the tile's warp takes every other, and says so of the
                 // others once they are there (a block is left when both warps have left it)
                 const uint32_t desc_q = umma_desc(operands + (two ? x : 0) * C::kOperand, 16);
-                const int ahead = two ? 2 : 4;
+                // a tile's next block's scores are asked for before its weights are waited for
+                const int ahead = two ? 1 : 2;
                 bool queries = two || x == 0, add = false;
                 if (!two && x == 1) {                              // the first tile's queries
                     if (!(ok = warp_wait(&q_both, shared++ & 1, &dead))) break;
-                    if (blocks == 1) {
+                    if (blocks < 2) {
                         if (elect_one()) mbar_arrive(&q_free);
                         __syncwarp();
                     }
@@ -434,28 +449,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attn_tile_kernel(const Att
 #pragma unroll 1
                 for (int i = -ahead; i < blocks; ++i) {
                     const int sb = i + ahead;
-                    const bool taken = two || (i & 1) == x;        // ahead is even: so is the parity of sb
-                    if (i >= 0) {                                  // the block's operands are there since its scores
-                        const int stage = (blocks_before + i) & (kTileStages - 1), buf = cp & 1;
-                        if (taken) {
-                            if (!(ok = warp_wait(&p_full[x][buf], cp >> 1 & 1, &dead))) break;
-                            ++cp;
-                        }
-                        tmem_after_sync();
-                        if (elect_one()) {
-                            if (taken) {
-                                const uint32_t pa = s_at + buf * 64, v = desc_v + stage * (C::kBlock >> 4);
-#pragma unroll
-                                for (int j = 0; j < kTileKeys / 16; ++j) umma_ts(o_at, pa + j * 8, v + j * (2048 >> 4), id_o, add || j > 0);
-                                umma_commit(&o_done[x][buf]);
-                                umma_commit(&empty[stage]);
-                            } else {
-                                mbar_arrive(&empty[stage]);
-                            }
-                        }
-                        __syncwarp();
-                        add = add || taken;
-                    }
+                    const bool taken = two || (i & 1) == x;        // and so is sb
                     if (sb < blocks) {
                         const int b = blocks_before + sb, stage = b & (kTileStages - 1), buf = cs & 1;
                         if (!(ok = warp_wait(&full[stage], b / kTileStages & 1, &dead))) break;
@@ -477,6 +471,27 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attn_tile_kernel(const Att
                             __syncwarp();
                             ++cs;
                         }
+                    }
+                    if (i >= 0) {                                  // the block's operands are there since its scores
+                        const int stage = (blocks_before + i) & (kTileStages - 1), buf = cp & 1;
+                        if (taken) {
+                            if (!(ok = warp_wait(&p_full[x][buf], cp >> 1 & 1, &dead))) break;
+                            ++cp;
+                        }
+                        tmem_after_sync();
+                        if (elect_one()) {
+                            if (taken) {
+                                const uint32_t pa = s_at + buf * 64, v = desc_v + stage * (C::kBlock >> 4);
+#pragma unroll
+                                for (int j = 0; j < kTileKeys / 16; ++j) umma_ts(o_at, pa + j * 8, v + j * (2048 >> 4), id_o, add || j > 0);
+                                umma_commit(&o_done[x][buf]);
+                                umma_commit(&empty[stage]);
+                            } else {
+                                mbar_arrive(&empty[stage]);
+                            }
+                        }
+                        __syncwarp();
+                        add = add || taken;
                     }
                 }
                 blocks_before += blocks;
@@ -623,43 +638,63 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attn_tile_kernel(const Att
         int cs = 0, ring0 = 0, teams = 0, shared = 0;      // this tile's blocks so far; all blocks; barriers' turns
         bool ok = true;
         TileSeg s;
-        // A segment's queries to shared memory: fp16 in the order of the decoded codes (bf16: times a power of two, as
-        // query_operand); returns the factor that a product of this thread's row lacks.
-        auto put_query = [&](const TileSeg& g) -> float {
+        // A segment's queries to shared memory.  ask: copies in flight, a warp its 32 rows, D / 8 lanes a row.  put: each
+        // thread turns its row into fp16 in the order of the decoded codes (bf16: times a power of two, as query_operand);
+        // the factor that the row's products then lack is returned.  Where both tiles are the same rows, the first one's
+        // warps do it, and the second's find the factors in q_factor.
+        constexpr int kLanes = D / 8;
+        constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
+        auto query_at = [&](int r, int c) { return operands + x * C::kOperand + (c >> 3) * 16384 + r * 128 + (((c & 7) ^ (r & 7)) << 4); };
+        auto ask = [&](const TileSeg& g) {
             const int rows = g.n * p.group, from = g.tile * kTileRows;
             const bool two = rows - from > 128;
+            if (!two && x == 1) return;
             const int row = from + (two ? x * 128 : 0) + t, token = row / p.group;
-            const uint4* src = reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + (g.q0 + token) * a.q_stride_token +
-                                                              (g.head * p.group + (row - token * p.group)) * a.q_stride_head);
-            uint4 w[D / 8];
-#pragma unroll
-            for (int i = 0; i < D / 8; ++i) w[i] = row < rows ? __ldg(src + i) : make_uint4(0, 0, 0, 0);
+            const long long at = (g.q0 + token) * a.q_stride_token + (g.head * p.group + (row - token * p.group)) * a.q_stride_head;
+            const unsigned in = __ballot_sync(0xffffffffu, row < rows);
+#pragma unroll 4
+            for (int i = lane / kLanes; i < 32; i += 32 / kLanes) {
+                const long long src = __shfl_sync(0xffffffffu, at, i);
+                const int ok = in >> i & 1;
+                copy_async16_or_0(query_at((warp & 3) * 32 + i, lane & (kLanes - 1)),
+                                  static_cast<const T*>(a.q) + (ok ? src + (lane & (kLanes - 1)) * 8 : 0), ok);
+            }
+        };
+        auto put = [&](const TileSeg& g) -> float {
+            const bool two = g.n * p.group - g.tile * kTileRows > 128;
+            if (!two && x == 1) return 1.0f;
+            const uint32_t sign = a.scale < 0.0f ? 0x80008000u : 0u;
             float factor = 1.0f, up = 1.0f;
-            if (std::is_same<T, __nv_bfloat16>::value) {
+            asm volatile("cp.async.wait_all;" ::: "memory");
+            __syncwarp();
+            if (kBf16) {
                 uint32_t top = 0;
-#pragma unroll
-                for (int i = 0; i < D / 8; ++i) {
-                    const uint32_t* y = reinterpret_cast<const uint32_t*>(&w[i]);
+#pragma unroll 4
+                for (int c = 0; c < kLanes; ++c) {
+                    const uint4 v = lds128(query_at(t, c));
+                    const uint32_t y[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
                     for (int j = 0; j < 4; ++j) top = max(top, max(y[j] << 16 & 0x7fffffffu, y[j] & 0x7fff0000u));
                 }
                 const int e = min(max((int)(top >> 23) - 127, -110), 126);
                 up = pow2(10 - e);
                 factor = pow2(e - 10);
+                if (!two) q_factor[shared & 1][t] = factor;
             }
-            if (!two && x == 1) return factor;                     // the first tile's warps put them there
-            const uint32_t sign = a.scale < 0.0f ? 0x80008000u : 0u, to = operands + x * C::kOperand + t * 128, swizzle = (t & 7) << 4;
+            if (kBf16 || FMT == B4_KV_INT4 || sign) {
+#pragma unroll 4
+                for (int c = 0; c < kLanes; ++c) {
+                    uint4 v = lds128(query_at(t, c));
+                    if (kBf16) {
+                        uint32_t* y = reinterpret_cast<uint32_t*>(&v);
 #pragma unroll
-            for (int i = 0; i < D / 8; ++i) {
-                if (std::is_same<T, __nv_bfloat16>::value) {
-                    uint32_t* y = reinterpret_cast<uint32_t*>(&w[i]);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) y[j] = pack_half2(__uint_as_float(y[j] << 16) * up, __uint_as_float(y[j] & 0xffff0000u) * up);
+                        for (int j = 0; j < 4; ++j) y[j] = pack_half2(__uint_as_float(y[j] << 16) * up, __uint_as_float(y[j] & 0xffff0000u) * up);
+                    }
+                    if (FMT == B4_KV_INT4) v = int4_pair_order(v);
+                    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(query_at(t, c)), "r"(v.x ^ sign), "r"(v.y ^ sign), "r"(v.z ^ sign),
+                                 "r"(v.w ^ sign)
+                                 : "memory");
                 }
-                const uint4 v = FMT == B4_KV_INT4 ? int4_pair_order(w[i]) : w[i];
-                asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(to + (i >> 3) * 16384 + (((i & 7) << 4) ^ swizzle)),
-                             "r"(v.x ^ sign), "r"(v.y ^ sign), "r"(v.z ^ sign), "r"(v.w ^ sign)
-                             : "memory");
             }
             fence_proxy_async();
             __syncwarp();
@@ -669,6 +704,11 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attn_tile_kernel(const Att
             }
             return factor;
         };
+        auto together = [&]() {                // the eight softmax warps
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&team);
+            return warp_wait(&team, teams++ & 1, &dead);
+        };
         auto fetch = [&](int k) {
             if (!(ok = warp_wait(&seg_full[k & 1], k >> 1 & 1, &dead))) return;
             s = segs[k & 1];
@@ -676,7 +716,11 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attn_tile_kernel(const Att
             if (lane == 0) mbar_arrive(&seg_empty[k & 1]);
         };
         fetch(0);
-        float factor = ok && !s.end ? put_query(s) : 1.0f;
+        float factor = 1.0f;
+        if (ok && !s.end) {
+            ask(s);
+            factor = put(s);
+        }
 #pragma unroll 1
         for (int k = 1; ok && !s.end; ++k) {
             const int blocks = s.blk1 - s.blk0, rows = s.n * p.group, row0 = s.tile * kTileRows;
@@ -684,10 +728,14 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attn_tile_kernel(const Att
             const int row = row0 + (two ? x * 128 : 0) + t;
             const bool mine = row < rows;
             const int token = row / p.group, head = s.head * p.group + (row - token * p.group), q0 = s.q0;
-            const bool whole = s.first && s.last && two, first = s.first;
+            const bool whole = s.first && s.last, first = s.first;
             const long long s0 = s.s0, s1 = s.s1;
             const int lim = a.flags & B4_KV_FULL ? s.ctx : min(s.ctx, s.ctx - s.n + token + 1);
             const int from = a.window > 0 ? lim - a.window : 0;
+            if (kBf16 && !two && x == 1) {
+                if (!(ok = warp_wait(&q_both, shared & 1, &dead))) break;
+                factor = q_factor[shared & 1][t];
+            }
             const float qf = fmaxf(factor * (fabsf(a.scale) * kLog2e) * (FMT == B4_KV_NF4 ? 1.0f / kNf4Up : 1.0f), 1e-30f);
             float m = kNoMax, l = 0.0f;
             int vexp = -126;
@@ -773,128 +821,134 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attn_tile_kernel(const Att
             }
             if (!ok) break;
             ring0 += blocks;
-            // the next segment's queries, whose scores are then computed under this one's end; where the other stream reads
-            // the same queries, after its last scores
-            if (!two && x == 0 && !(ok = warp_wait(&q_free, shared++ & 1, &dead))) break;
+            // The next segment's queries, whose scores are then computed under this one's end.  Their place is free: the
+            // tile's last scores have been read; one tile of rows: and the other stream's are done.
             fetch(k);
             if (!ok) break;
-            if (!s.end) factor = put_query(s);
+            if (!two && !(ok = warp_wait(&q_free, shared++ & 1, &dead))) break;
+            if (!s.end) ask(s);
             if (any && !(ok = warp_wait(&o_done[x][cs - 1 & 1], (cs - 1) >> 1 & 1, &dead))) break;
-            tmem_after_sync();
+            if (!s.end) factor = put(s);
 
-            // ---- the segment's rows, or a piece of them ----
-            const float vup = pow2(vexp) * (FMT == B4_KV_NF4 ? 1.0f / kNf4Up : 1.0f);
-            float* piece = ws.cross + (((long long)cta * 2 + first) * 2 + x) * (C::kPiece / 2);
-            const float inv = whole ? (l > 0.0f ? vup / l : 0.0f) : vup;
-            T* dst = static_cast<T*>(a.out) + (q0 + token) * a.out_stride_token + head * a.out_stride_head;
+            // ---- the segment's rows, or a piece of them: a row a thread; one tile of rows: half a row's columns, of both streams ----
+            const float vup = any ? pow2(vexp) * (FMT == B4_KV_NF4 ? 1.0f / kNf4Up : 1.0f) : 0.0f;
+            float wa = vup, wb = 0.0f;
+            if (!two) {
+                stream_max[x][t] = m;
+                stream_sum[x][t] = l;
+                stream_up[x][t] = vup;
+                if (!(ok = together())) break;
+                const float m0 = stream_max[0][t], m1 = stream_max[1][t];
+                m = fmaxf(m0, m1);
+                wa = fast_exp2(m0 - m);
+                wb = fast_exp2(m1 - m);
+                l = wa * stream_sum[0][t] + wb * stream_sum[1][t];
+                wa *= stream_up[0][t];
+                wb *= stream_up[1][t];
+            }
+            tmem_after_sync();
+            const float inv = !whole ? 1.0f : l > 0.0f ? 1.0f / l : 0.0f;
+            wa *= inv;
+            wb *= inv;
+            const int c_begin = two ? 0 : x * (D / 2), c_end = two ? D : c_begin + D / 2, rows_of = two ? x : 0;
+            auto piece_of = [&](int c, int begins) { return ws.cross + (((long long)c * 2 + begins) * 2 + rows_of) * (C::kPiece / 2); };
+            float* const piece = piece_of(cta, first);             // [D / 4][128][4], maxima, sums
+            T* const out = static_cast<T*>(a.out) + (q0 + token) * a.out_stride_token + head * a.out_stride_head;
+            const uint32_t oa = two ? o_at : tmem + lanes + 256, ob = tmem + lanes + 256 + 128;
+            auto store16 = [&](int c, const float* y) {
+                uint32_t w[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) w[j] = kv_round2<T>(y[2 * j], y[2 * j + 1]);
+                *reinterpret_cast<uint4*>(out + c) = make_uint4(w[0], w[1], w[2], w[3]);
+                *reinterpret_cast<uint4*>(out + c + 8) = make_uint4(w[4], w[5], w[6], w[7]);
+            };
 #pragma unroll 1
-            for (int c = 0; c < D; c += 16) {
+            for (int c = c_begin; c < c_end; c += 16) {
                 uint32_t o[16];
-                if (any) tmem_ld16(o, o_at + c);
-                tmem_wait_ld();
                 float y[16];
+                tmem_ld16(o, oa + c);
+                tmem_wait_ld();
 #pragma unroll
                 for (int j = 0; j < 16; ++j)   // INT4: decoded columns (0, 4, 1, 5, 2, 6, 3, 7) of each eight
-                    y[FMT == B4_KV_INT4 ? (j & 8) | (j >> 1 & 3) | (j & 1) << 2 : j] = any ? __uint_as_float(o[j]) * inv : 0.0f;
-                if (mine && whole) {
+                    y[FMT == B4_KV_INT4 ? (j & 8) | (j >> 1 & 3) | (j & 1) << 2 : j] = __uint_as_float(o[j]) * wa;
+                if (!two && blocks > 1) {
+                    tmem_ld16(o, ob + c);
+                    tmem_wait_ld();
 #pragma unroll
-                    for (int j = 0; j < 16; j += 8) {
-                        uint32_t w[4];
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const T lo = kv_round<T>(y[j + 2 * e]), hi = kv_round<T>(y[j + 2 * e + 1]);
-                            w[e] = (uint32_t)*reinterpret_cast<const uint16_t*>(&lo) | (uint32_t)*reinterpret_cast<const uint16_t*>(&hi) << 16;
-                        }
-                        *reinterpret_cast<uint4*>(dst + c + j) = make_uint4(w[0], w[1], w[2], w[3]);
+                    for (int j = 0; j < 16; ++j) {
+                        float& z = y[FMT == B4_KV_INT4 ? (j & 8) | (j >> 1 & 3) | (j & 1) << 2 : j];
+                        z = fmaf(__uint_as_float(o[j]), wb, z);
                     }
-                } else if (mine) {
+                }
+                if (whole) {
+                    if (mine) store16(c, y);
+                } else {
 #pragma unroll
                     for (int j = 0; j < 16; j += 4)
-                        *reinterpret_cast<float4*>(piece + t * D + c + j) = make_float4(y[j], y[j + 1], y[j + 2], y[j + 3]);
+                        *reinterpret_cast<float4*>(piece + ((c + j) / 4 * 128 + t) * 4) = make_float4(y[j], y[j + 1], y[j + 2], y[j + 3]);
                 }
                 __syncwarp();
             }
             tmem_before_sync();
+            if (!two && !(ok = together())) break;                 // both streams' outputs are read
             if (whole) {
-                if (mine && a.lse) a.lse[(long long)(q0 + token) * a.heads + head] = l > 0.0f ? (m + fast_log2(l)) * kLn2 : -INFINITY;
+                if (mine && rows_of == x && a.lse)
+                    a.lse[(long long)(q0 + token) * a.heads + head] = l > 0.0f ? (m + fast_log2(l)) * kLn2 : -INFINITY;
                 continue;
             }
-            piece[128 * D + t] = m;
-            piece[128 * (D + 1) + t] = l;
+            if (rows_of == x) {
+                piece[128 * D + t] = m;
+                piece[128 * (D + 1) + t] = l;
+            }
             // the last of the segment's CTAs joins them, in order
             const int f = owner(s0), parts = owner(s1 - 1) - f + 1;
-            auto together = [&]() {            // the eight softmax warps
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&team);
-                return warp_wait(&team, teams++ & 1, &dead);
-            };
             if (!(ok = together())) break;
             if (tid == 128) {
-                // the counter is the crossing segment's that begins in CTA f, not that of one inside it
                 __threadfence();
-                joins = parts == 1 || atomicAdd(ws.count + f, 1) == parts - 1;
-                if (joins && parts > 1) ws.count[f] = 0;
+                joins = atomicAdd(ws.count + f, 1) == parts - 1;
+                if (joins) ws.count[f] = 0;
                 __threadfence();
             }
             if (!(ok = together())) break;
             const bool join = joins;
             if (!(ok = together())) break;     // before the flag is written again
             if (!join) continue;
-            // eight rows at a time: lane i weighs row i's parts (two tiles: its CTAs'; one: both streams of each), all lanes
-            // add them up row by row
-            constexpr int E = D / 32;
-            const int n_parts = two ? parts : 2 * parts;
-            auto part = [&](int i) -> const float* {
-                const int c = two ? i : i >> 1, y = two ? x : i & 1;
-                return ws.cross + (((long long)(f + c) * 2 + (c == 0)) * 2 + y) * (C::kPiece / 2);
-            };
-            const int r_first = two ? (warp & 3) * 32 : (warp - 4) * 16, r_base = row0 + (two ? x * 128 : 0);
+            float jt = kNoMax, sum = 0.0f;
+#pragma unroll 4
+            for (int i = 0; i < parts; ++i) jt = fmaxf(jt, __ldcg(piece_of(f + i, i == 0) + 128 * D + t));
+            constexpr int E = D / 2;           // columns at a time
 #pragma unroll 1
-            for (int r0 = r_first; r0 < r_first + (two ? 32 : 16) && r_base + r0 < rows; r0 += 8) {
-                float jt = kNoMax, sum = 0.0f, y[8][E];
-                for (int i = 0; i < n_parts; ++i) jt = fmaxf(jt, __ldcg(part(i) + 128 * D + r0 + (lane & 7)));
+            for (int c = c_begin; c < c_end; c += E) {
+                float y[E];
 #pragma unroll
-                for (int r = 0; r < 8; ++r)
-#pragma unroll
-                    for (int e = 0; e < E; ++e) y[r][e] = 0.0f;
+                for (int e = 0; e < E; ++e) y[e] = 0.0f;
+                sum = 0.0f;
 #pragma unroll 1
-                for (int i = 0; i < n_parts; ++i) {
-                    const float* b = part(i);
-                    const float w = fast_exp2(__ldcg(b + 128 * D + r0 + (lane & 7)) - jt);
-                    sum += w * __ldcg(b + 128 * (D + 1) + r0 + (lane & 7));
+                for (int i = 0; i < parts; ++i) {
+                    const float* b = piece_of(f + i, i == 0);
+                    float4 z[E / 4];
 #pragma unroll
-                    for (int r = 0; r < 8; ++r) {
-                        const float k8 = __shfl_sync(0xffffffffu, w, r);
-                        const float2* z = reinterpret_cast<const float2*>(b + (r0 + r) * D + lane * E);
+                    for (int e = 0; e < E / 4; ++e) z[e] = __ldcg(reinterpret_cast<const float4*>(b) + (c / 4 + e) * 128 + t);
+                    const float w = fast_exp2(__ldcg(b + 128 * D + t) - jt);
+                    sum = fmaf(w, __ldcg(b + 128 * (D + 1) + t), sum);
 #pragma unroll
-                        for (int e = 0; e < E / 2; ++e) {
-                            const float2 v = r_base + r0 + r < rows ? __ldcg(z + e) : make_float2(0.0f, 0.0f);
-                            y[r][2 * e] += k8 * v.x;
-                            y[r][2 * e + 1] += k8 * v.y;
-                        }
+                    for (int e = 0; e < E / 4; ++e) {
+                        y[4 * e] = fmaf(w, z[e].x, y[4 * e]);
+                        y[4 * e + 1] = fmaf(w, z[e].y, y[4 * e + 1]);
+                        y[4 * e + 2] = fmaf(w, z[e].z, y[4 * e + 2]);
+                        y[4 * e + 3] = fmaf(w, z[e].w, y[4 * e + 3]);
                     }
                 }
-                const int jr = r_base + r0 + (lane & 7), jtk = jr / p.group, jhd = (head / p.group) * p.group + (jr - jtk * p.group);
                 const float jinv = sum > 0.0f ? 1.0f / sum : 0.0f;
 #pragma unroll
-                for (int r = 0; r < 8; ++r) {
-                    const float k8 = __shfl_sync(0xffffffffu, jinv, r);
-                    const int tk = __shfl_sync(0xffffffffu, jtk, r), hd = __shfl_sync(0xffffffffu, jhd, r);
-                    if (r_base + r0 + r < rows) {
-                        T* to = static_cast<T*>(a.out) + (q0 + tk) * a.out_stride_token + hd * a.out_stride_head + lane * E;
+                for (int e = 0; e < E; ++e) y[e] *= jinv;
+                if (mine) {
 #pragma unroll
-                        for (int e = 0; e < E; e += 2) {
-                            const T w[2] = {kv_round<T>(y[r][e] * k8), kv_round<T>(y[r][e + 1] * k8)};
-                            *reinterpret_cast<uint32_t*>(to + e) =
-                                (uint32_t)*reinterpret_cast<const uint16_t*>(w) | (uint32_t)*reinterpret_cast<const uint16_t*>(w + 1) << 16;
-                        }
-                    }
-                    __syncwarp();
+                    for (int e = 0; e < E; e += 16) store16(c + e, y + e);
                 }
-                if (a.lse && lane < 8 && jr < rows) a.lse[(long long)(q0 + jtk) * a.heads + jhd] = sum > 0.0f ? (jt + fast_log2(sum)) * kLn2 : -INFINITY;
-                __syncwarp();
             }
-            if (!(ok = together())) break;     // before a later segment's pieces take the place of these
+            if (mine && rows_of == x && a.lse)
+                a.lse[(long long)(q0 + token) * a.heads + head] = sum > 0.0f ? (jt + fast_log2(sum)) * kLn2 : -INFINITY;
         }
     }
     tmem_before_sync();
