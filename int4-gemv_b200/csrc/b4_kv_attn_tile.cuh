@@ -39,6 +39,8 @@
 namespace b4 {
 
 constexpr int kTileRows = 256, kTileKeys = 64, kTileThreads = 512, kTileStages = 4;
+// What a segment (a row tile and head) costs beside its blocks, in blocks' time.
+constexpr int kSegUnits = 4;
 
 template <int FMT, int D>
 struct TileCfg {
@@ -55,7 +57,7 @@ struct TileCfg {
 struct TileSeg {               // a run's part of a segment
     int q0, n, ctx, head, tile, r, blk0, blk1;
     int first, last, end;      // whether it has the segment's first, last block; the run is over
-    long long s0, s1;          // the segment's units
+    long long s0, s1;          // the segment's units of blocks (kSegUnits more follow, with nothing to do)
 };
 
 struct TileWs {
@@ -343,7 +345,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attn_tile_kernel(const Att
             for (int i = t_first; i < t_last; ++i) {
                 int b0, b1;
                 tile_blocks(p, c.q.n, c.q.ctx, c.tile, b0, b1);
-                mine += (long long)(b1 - b0) * p.l.kv_heads;
+                mine += (long long)(b1 - b0 + kSegUnits) * p.l.kv_heads;
                 if (i + 1 < t_last) next(c);
             }
         }
@@ -382,9 +384,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attn_tile_kernel(const Att
                 if (u < u1 && c.r < a.n_req) {
                     int b0, b1;
                     tile_blocks(p, c.q.n, c.q.ctx, c.tile, b0, b1);
-                    const long long blocks = b1 - b0;
-                    if (u >= at + blocks * p.l.kv_heads) {
-                        at += blocks * p.l.kv_heads;
+                    const long long blocks = b1 - b0, units = blocks + kSegUnits;
+                    if (u >= at + units * p.l.kv_heads) {
+                        at += units * p.l.kv_heads;
                         next(c);
                         continue;
                     }
@@ -393,15 +395,19 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attn_tile_kernel(const Att
                     s.ctx = c.q.ctx;
                     s.tile = c.tile;
                     s.r = c.r;
-                    s.head = (int)((u - at) / blocks);
-                    s.s0 = at + s.head * blocks;
+                    s.head = (int)((u - at) / units);
+                    s.s0 = at + s.head * units;
                     s.s1 = s.s0 + blocks;
+                    if (u >= s.s1) {               // only of its end
+                        u = s.s0 + units;
+                        continue;
+                    }
                     s.blk0 = b0 + (int)(u - s.s0);
                     const long long stop = min(s.s1, u1);
                     s.blk1 = s.blk0 + (int)(stop - u);
                     s.first = u == s.s0;
                     s.last = stop == s.s1;
-                    u = stop;
+                    u = s.last ? s.s0 + units : stop;
                 } else {
                     s.end = 1;
                 }
@@ -513,7 +519,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attn_tile_kernel(const Att
         const int row = t & (p.l.page_size - 1);
         struct Codes {
             uint4 k[W / 4], v[W / 4];
-            float scale;                       // the key's or the value's
+            uint32_t scale;                    // the key's or the value's, as it lies there
             bool there;
         };
         TileSeg s = {};
@@ -527,7 +533,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attn_tile_kernel(const Att
             c.there = (unsigned)page < (unsigned)p.l.n_pages;
 #pragma unroll
             for (int i = 0; i < W / 4; ++i) c.k[i] = c.v[i] = make_uint4(0, 0, 0, 0);
-            c.scale = 0.0f;
+            c.scale = 0;
             if (!c.there) return;
             const uint8_t* b = p.blocks + ((long long)page * p.l.kv_heads + s.head) * p.l.block;
             const uint8_t* codes = b + row * C::kRow + half * (C::kRow / 2);
@@ -537,7 +543,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attn_tile_kernel(const Att
                 c.v[i] = __ldg(reinterpret_cast<const uint4*>(codes + p.l.page_size * C::kRow) + i);
             }
             const uint8_t* sp = b + p.l.page_size * D + (half * p.l.page_size + row) * C::kScale;
-            c.scale = FMT == B4_KV_INT4 ? __half2float(*reinterpret_cast<const __half*>(sp)) : *reinterpret_cast<const float*>(sp);
+            c.scale = FMT == B4_KV_INT4 ? __ldg(reinterpret_cast<const uint16_t*>(sp)) : __ldg(reinterpret_cast<const uint32_t*>(sp));
         };
         auto write = [&](uint32_t to, const uint4 (&raw)[W / 4]) {
             const uint32_t* w = reinterpret_cast<const uint32_t*>(raw);
@@ -591,9 +597,10 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attn_tile_kernel(const Att
             // scales: those of tokens that no row sees are 0, the values' relative to a running power of two
             const int token = blk * kTileKeys + t;
             const bool seen = now.there && token < see_end && token >= see_begin;
+            const float scale = !seen ? 0.0f : FMT == B4_KV_INT4 ? __half2float(__ushort_as_half((unsigned short)now.scale)) : __uint_as_float(now.scale);
             if (half) {
                 if (blk == s.blk0) vexp = -126;
-                const float v = seen ? fminf(now.scale, 3.4028235e38f) : 0.0f;
+                const float v = fminf(scale, 3.4028235e38f);
                 const unsigned bits = __reduce_max_sync(0xffffffffu, v < 3.4028235e38f ? __float_as_uint(fabsf(v)) : 0u);
                 if (lane == 0) {
                     value_top[b & 1][warp & 1] = __uint_as_float(bits);
@@ -607,7 +614,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attn_tile_kernel(const Att
                 value_scale[stage][t] = v * pow2(-vexp);
                 if (t == 0) value_exp[stage] = vexp;
             } else {
-                key_scale[stage][t] = seen ? now.scale : 0.0f;
+                key_scale[stage][t] = scale;
                 // tokens that are not there lie in whole pages of 16 at least: two bits a warp
                 const unsigned pages = __ballot_sync(0xffffffffu, now.there);
                 if (lane == 0) reinterpret_cast<uint8_t*>(&block_pages[stage])[warp & 1] = (uint8_t)((pages & 1) | (pages >> 16 & 1) << 1);
