@@ -15,8 +15,12 @@ int sm_count()
     return n;
 }
 
-// Which kernels run.  A request of at most 16 rows (queries x heads that share a kv
-// head) is the warp kernel's, in tiles of 8 or 16; one of more is the tile kernel's.
+// Which kernels run.  The warp kernel takes requests of few rows (queries x heads that
+// share a kv head), in tiles of 8 or 16 that each read the cache, the tile kernel the
+// others, whose time does not depend on the rows up to 128.  24 requests of 4000 tokens,
+// 4 kv heads x 128, INT4: 32 rows 58 us against 68, 48 rows 72 against 68 (NF4: 72 and
+// 83, 93 and 83); 8 kv heads x 64: 48 rows 78 us against 97 (NF4: 94 and 111).  So the
+// warp kernel has up to 32 rows of 128, 48 of 64.
 // max_q says which of the two the call needs: one where every request is of one
 // kind by it, both (each skipping the other's requests) where it cannot be known.
 struct Plan {
@@ -28,7 +32,7 @@ struct Plan {
 Plan plan(const AttnParams& p)
 {
     const long long most = (long long)std::max(1, p.a.max_q) * p.group;
-    if (most <= 16) return {true, false, most <= 8 ? 8 : 16, INT_MAX, INT_MAX};
+    if (most <= (p.l.head_dim == 64 ? 48 : 32)) return {true, false, most <= 8 ? 8 : 16, INT_MAX, INT_MAX};
     if ((long long)p.a.n_req * p.a.max_q <= p.a.total_q || p.group > 16) return {false, true, 0, 0, 0};    // alike, or none of few rows
     const int cols = p.group <= 8 ? 8 : 16;
     return {true, true, cols, cols, cols};
