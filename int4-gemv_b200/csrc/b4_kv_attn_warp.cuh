@@ -711,37 +711,22 @@ __global__ void __launch_bounds__(WarpCfg<FMT, D, NT, PT>::kThreads, 1) kv_attn_
         int f;
         const int n = span(pc, f);
         auto part = [&](int c) -> const float* { return ws.cross + ((long long)(f + c) * 2 + (c == 0)) * C::kPiece; };
-        __syncthreads();
-        for (int col = warp; col < C::kCols; col += kWarps) {
-            float m = kNoMax, l = 0.0f;
-            for (int c = lane; c < n; c += 32) {           // a running pair a lane
-                const float* b = part(c) + C::kCols * D + col;
-                const float mc = __ldcg(b), lc = __ldcg(b + C::kCols), next = fmaxf(m, mc);
-                l = l * fast_exp2(m - next) + lc * fast_exp2(mc - next);
-                m = next;
-            }
-            float top = m;
-#pragma unroll
-            for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-            l *= fast_exp2(m - top);
-#pragma unroll
-            for (int off = 16; off > 0; off >>= 1) l += __shfl_xor_sync(0xffffffffu, l, off);
-            if (lane == 0) joined[col][0] = make_float2(top, l);
-        }
-        __syncthreads();
+        // every thread adds up its own columns' maxima and sums, so that all loads of eight parts are in flight at once
         for (int e = tid * 2; e < C::kCols * D; e += kThreads * 2) {
             const int col = e / D;
-            const float2 ml = joined[col][0];
+            float m = kNoMax, l = 0.0f;
             float2 x = make_float2(0.0f, 0.0f);
 #pragma unroll 8
             for (int c = 0; c < n; ++c) {
                 const float* b = part(c);
-                const float w = fast_exp2(__ldcg(b + C::kCols * D + col) - ml.x);
+                const float mc = __ldcg(b + C::kCols * D + col), lc = __ldcg(b + C::kCols * (D + 1) + col);
                 const float2 y = __ldcg(reinterpret_cast<const float2*>(b + e));
-                x.x += w * y.x;
-                x.y += w * y.y;
+                const float top = fmaxf(m, mc), keep = fast_exp2(m - top), w = fast_exp2(mc - top);
+                l = l * keep + lc * w;
+                x = make_float2(x.x * keep + y.x * w, x.y * keep + y.y * w);
+                m = top;
             }
-            emit(pc, e, x, ml.x, ml.y);
+            emit(pc, e, x, m, l);
         }
     }
 }
