@@ -39,6 +39,9 @@
 
 namespace b4 {
 
+// What a segment (a request's head and column tile) costs a warp beside its chunks, in a chunk's time.
+constexpr int kSegChunks = 2;
+
 // PT: tokens of a page in shared memory, 16 or 32 (half a page of 64 lies there as a page of 32)
 template <int FMT, int D, int NT, int PT>
 struct WarpCfg {
@@ -61,7 +64,7 @@ struct WarpCfg {
 };
 
 struct WarpPiece {
-    long long s0, s1;          // the segment's units
+    long long s0, s1;          // the segment's units of chunks (kSegChunks more follow, with nothing to do)
     int q0, n, head, tile;
     int valid;
 };
@@ -102,7 +105,7 @@ __global__ void __launch_bounds__(WarpCfg<FMT, D, NT, PT>::kThreads, 1) kv_attn_
 
     // ---- the call's units, and each warp's run of them ----
     auto tiles_of = [&](const AttnReq& q) { return q.n * p.group <= p.rows_upto ? (q.n * p.group + C::kCols - 1) / C::kCols : 0; };
-    auto units_of = [&](const AttnReq& q) { return (long long)p.l.kv_heads * tiles_of(q) * q.chunks; };
+    auto units_of = [&](const AttnReq& q) { return (long long)p.l.kv_heads * tiles_of(q) * (q.chunks + kSegChunks); };
     const int per = (a.n_req + kScan - 1) / kScan;
     {
         long long sum = 0;
@@ -169,9 +172,9 @@ __global__ void __launch_bounds__(WarpCfg<FMT, D, NT, PT>::kThreads, 1) kv_attn_
         const long long u = c * share + min((long long)c, rest);
         if (near == 0 || u <= 0 || u >= total) return u;
         long long at;
-        const int chunks = request(find(u, at)).chunks;
-        const long long s0 = at + div64(u - at, chunks) * chunks;
-        return u - s0 <= near ? s0 : s0 + chunks - u <= near ? s0 + chunks : u;
+        const int units = request(find(u, at)).chunks + kSegChunks;
+        const long long s0 = at + div64(u - at, units) * units;
+        return u - s0 <= near ? s0 : s0 + units - u <= near ? s0 + units : u;
     };
     const long long c0 = end_of(cta), c1 = end_of(cta + 1);
     auto run_start = [&](int w) {
@@ -449,15 +452,20 @@ __global__ void __launch_bounds__(WarpCfg<FMT, D, NT, PT>::kThreads, 1) kv_attn_
                 ++r;
                 continue;
             }
-            const int tiles = tiles_of(q), seg = (int)div64(v - at, q.chunks), first = (int)(v - at - (long long)seg * q.chunks);
+            const int tiles = tiles_of(q), seg = (int)div64(v - at, q.chunks + kSegChunks);
+            const long long seg_unit = at + (long long)seg * (q.chunks + kSegChunks), seg_end = min(seg_unit + q.chunks + kSegChunks, v1);
+            const int first = (int)(v - seg_unit);
+            if (first >= q.chunks) {               // only of its end
+                v = seg_end;
+                continue;
+            }
             const int last = (int)min((long long)q.chunks, first + (v1 - v));
             u.q0 = q.q0;
             u.n = q.n;
             u.ctx = q.ctx;
             u.head = seg / tiles;
             u.tile = seg - u.head * tiles;
-            const long long seg_unit = at + (long long)seg * q.chunks;
-            v += last - first;
+            v = last == q.chunks ? seg_end : v1;
 
             // the feed: page ids by 32, `ids` from page `base` on and the 32 after those
             const int32_t* row = a.tables + (long long)r * a.table_stride;
@@ -593,36 +601,37 @@ __global__ void __launch_bounds__(WarpCfg<FMT, D, NT, PT>::kThreads, 1) kv_attn_
     const bool mine = lane < 2 * kWarps && pieces[lane >> 1][lane & 1].valid;
     const long long my_s0 = mine ? pieces[lane >> 1][lane & 1].s0 : -1;
     const uint32_t have = __ballot_sync(0xffffffffu, mine);
-    // the pieces of the segment of piece f
-    auto same = [&](int f) {
-        const long long s0 = __shfl_sync(0xffffffffu, my_s0, f);    // by every lane
-        return __ballot_sync(0xffffffffu, mine && s0 == my_s0);
-    };
+    // the pieces of this lane's segment, which are neighbours in this order but for lanes without a piece: those count,
+    // with nothing, to the segment before them
+    const uint32_t my_list = __match_any_sync(0xffffffffu, my_s0);
+    const uint32_t upto = have & (0xffffffffu >> (31 - lane));
+    const uint32_t its_list = __shfl_sync(0xffffffffu, my_list, upto ? 31 - __clz(upto) : lane);
+    const int lead = upto ? __ffs(its_list) - 1 : lane;
+    const int tail = mine ? 31 - __clz(my_list) : lane;
     // maxima and sums of every segment (at its first piece) and the pieces' factors, a column a warp
     for (int col = warp; col < C::kCols; col += kWarps) {
-        float m = kNoMax, l = 0.0f, f = 0.0f;
+        float m = kNoMax, l = 0.0f;
         if (mine) {
             const float* b = piece_of(lane) + C::kCols * D + col;
             m = b[0];
             l = b[C::kCols];
         }
-        for (uint32_t todo = have; todo;) {
-            const int at = __ffs(todo) - 1;
-            const uint32_t list = same(at);
-            const bool in = list >> lane & 1;
-            float top = in ? m : kNoMax;
+        float top = m;
 #pragma unroll
-            for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-            if (in) f = fast_exp2(m - top);
-            float all = in ? f * l : 0.0f;
-#pragma unroll
-            for (int off = 16; off > 0; off >>= 1) all += __shfl_xor_sync(0xffffffffu, all, off);
-            if (lane == at) {
-                joined[col][at].x = top;
-                joined[col][at].y = all;
-            }
-            todo &= ~list;
+        for (int off = 1; off < 32; off <<= 1) {
+            const float y = __shfl_up_sync(0xffffffffu, top, off);
+            if (lane - off >= lead) top = fmaxf(top, y);
         }
+        top = __shfl_sync(0xffffffffu, top, tail);
+        const float f = mine ? fast_exp2(m - top) : 0.0f;
+        float all = f * l;
+#pragma unroll
+        for (int off = 1; off < 32; off <<= 1) {
+            const float y = __shfl_up_sync(0xffffffffu, all, off);
+            if (lane - off >= lead) all += y;
+        }
+        all = __shfl_sync(0xffffffffu, all, tail);
+        if (mine && lane == lead) joined[col][lane] = make_float2(top, all);
         factor[col][lane] = f;
     }
     __syncthreads();
@@ -637,9 +646,13 @@ __global__ void __launch_bounds__(WarpCfg<FMT, D, NT, PT>::kThreads, 1) kv_attn_
             a.lse[(long long)(pc.q0 + token) * a.heads + head] = l > 0.0f ? (m + fast_log2(l)) * kLn2 : -INFINITY;
     };
     int cross[2] = {-1, -1};                   // the first pieces of the segments that began before this CTA, that go on after it
+    // a warp takes 256 outputs of a segment, eight a lane, so that many short segments join side by side
+    constexpr int kItems = C::kCols * D / 256;
+    static_assert(kItems <= kWarps, "one of a segment's items a warp");
+    int turn = warp;                           // of the kWarps items, the next that is this warp's
     for (uint32_t todo = have; todo;) {
         const int at = __ffs(todo) - 1;
-        const uint32_t list = same(at), lasts = list & 0xaaaaaaaau, firsts = list & 0x55555555u;
+        const uint32_t list = __shfl_sync(0xffffffffu, my_list, at), lasts = list & 0xaaaaaaaau, firsts = list & 0x55555555u;
         todo &= ~list;
         const WarpPiece& pc = pieces[at >> 1][at & 1];
         const bool inside = pc.s0 >= c0 && pc.s1 <= c1, begins = pc.s0 >= c0;
@@ -647,33 +660,42 @@ __global__ void __launch_bounds__(WarpCfg<FMT, D, NT, PT>::kThreads, 1) kv_attn_
             if (begins) cross[1] = at;
             else cross[0] = at;
         }
-        const int w0 = (__ffs(lasts) - 1) >> 1, w1 = (31 - __clz(lasts)) >> 1;
-        for (int e = tid * 2; e < C::kCols * D; e += kThreads * 2) {
-            const int col = e / D;
-            float2 x = make_float2(0.0f, 0.0f);
-            if (lasts) {
+        const int item = turn;
+        turn -= kItems;
+        if (turn < 0) turn += kWarps;
+        if (item >= kItems) continue;
+        const int e0 = item * 256 + lane * 2;
+        float2 x[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[j] = make_float2(0.0f, 0.0f);
+        auto add = [&](const float* b, int i, bool in) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int e = e0 + j * 64;
+                const float k = in ? factor[e / D][i] : 0.0f;
+                const float2 y = *reinterpret_cast<const float2*>(b + e);
+                x[j].x += k * y.x;
+                x[j].y += k * y.y;
+            }
+        };
+        if (lasts) {
+            const int w0 = (__ffs(lasts) - 1) >> 1, w1 = (31 - __clz(lasts)) >> 1;
 #pragma unroll 4
-                for (int w = w0; w <= w1; ++w) {
-                    const bool in = lasts >> (2 * w + 1) & 1;
-                    const float k = in ? factor[col][2 * w + 1] : 0.0f;
-                    const float2 y = *reinterpret_cast<const float2*>(ring_of(in ? w : w0) + e * 4);
-                    x.x += k * y.x;
-                    x.y += k * y.y;
-                }
+            for (int w = w0; w <= w1; ++w) {
+                const bool in = lasts >> (2 * w + 1) & 1;
+                add(reinterpret_cast<const float*>(ring_of(in ? w : w0)), 2 * w + 1, in);
             }
-            if (firsts) {                      // one at most: a run's first piece ends its segment
-                const int i = __ffs(firsts) - 1;
-                const float k = factor[col][i];
-                const float2 y = *reinterpret_cast<const float2*>(piece_of(i) + e);
-                x.x += k * y.x;
-                x.y += k * y.y;
-            }
+        }
+        if (firsts) add(piece_of(__ffs(firsts) - 1), __ffs(firsts) - 1, true);        // one at most: a run's first piece ends its segment
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int e = e0 + j * 64, col = e / D;
             const float2 ml = joined[col][at];
             if (inside) {
-                emit(pc, e, x, ml.x, ml.y);
+                emit(pc, e, x[j], ml.x, ml.y);
             } else {
                 float* dst = ws.cross + ((long long)cta * 2 + begins) * C::kPiece;
-                *reinterpret_cast<float2*>(dst + e) = x;
+                *reinterpret_cast<float2*>(dst + e) = x[j];
                 if (e % D == 0) {
                     dst[C::kCols * D + col] = ml.x;
                     dst[C::kCols * (D + 1) + col] = ml.y;
@@ -686,7 +708,7 @@ __global__ void __launch_bounds__(WarpCfg<FMT, D, NT, PT>::kThreads, 1) kv_attn_
     // ---- segments that cross CTAs: the last to arrive joins them, in CTA order ----
     auto span = [&](const WarpPiece& pc, int& f) {         // the CTAs that hold pieces of the segment
         f = owner(min(pc.s0 + near, total - 1));
-        return max(owner(max(pc.s1 - near - 1, 0LL)) - f, 0) + 1;
+        return max(owner(max(min(pc.s1, pc.s1 + kSegChunks - near) - 1, 0LL)) - f, 0) + 1;
     };
     __syncthreads();
     if (tid < 2) {
