@@ -256,10 +256,13 @@ __device__ __forceinline__ uint32_t nf4_word(const float (&x)[8], float s, float
     return w;
 }
 
-constexpr int kAppendUnroll = 2;       // vectors a thread has in flight
+// Vectors a thread has in flight, U: two where 16-bit rows fill the GPU more than once (20011 tokens x 4 x 128, bf16 to
+// NF4, append and read-back: 43 us against 51 with one), one otherwise (64 tokens x 8 x 128: 4.7 us against 6.7 with
+// two; 6007 x 12 x 64 in fp32: 24.6 against 25.3).
+constexpr long long kFewBlocks = 148 * 8;
 
 // Bound by memory: 2.1 to 4.5 bytes a column.
-template <typename T, int FMT, int D, bool VEC>
+template <typename T, int FMT, int D, bool VEC, int U>
 __global__ void __launch_bounds__(256) kv_append_kernel(const AppendParams p)
 {
     constexpr int TPV = D / 8, per = 256 / TPV;
@@ -277,12 +280,12 @@ __global__ void __launch_bounds__(256) kv_append_kernel(const AppendParams p)
     }
     kv_begin();
     const int sub = threadIdx.x % TPV;
-    const long long first = (long long)blockIdx.x * (kAppendUnroll * per) + threadIdx.x / TPV;
-    Columns<T, VEC> c[kAppendUnroll];
-    uint8_t* block[kAppendUnroll];
-    int at[kAppendUnroll];
+    const long long first = (long long)blockIdx.x * (U * per) + threadIdx.x / TPV;
+    Columns<T, VEC> c[U];
+    uint8_t* block[U];
+    int at[U];
 #pragma unroll
-    for (int u = 0; u < kAppendUnroll; ++u) {
+    for (int u = 0; u < U; ++u) {
         const long long i = min(first + u * per, p.n - 1);         // whole warps take part in the shuffles
         const VectorIndex v = vector_index(i, p.l.kv_heads, p.magic);
         const int slot = __ldg(p.slots + v.token), page = slot >> p.l.page_shift;
@@ -294,7 +297,7 @@ __global__ void __launch_bounds__(256) kv_append_kernel(const AppendParams p)
         at[u] = (v.value ? p.l.page_size : 0) + (slot & (p.l.page_size - 1));
     }
 #pragma unroll
-    for (int u = 0; u < kAppendUnroll; ++u) {
+    for (int u = 0; u < U; ++u) {
         float x[8], amax = 0.0f;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
@@ -332,19 +335,19 @@ struct ReadParams {
 };
 
 // Bound by its fp32 stores.
-template <int FMT, int D>
+template <int FMT, int D, int U>
 __global__ void __launch_bounds__(256) kv_read_kernel(const ReadParams p)
 {
     constexpr int TPV = D / 8, per = 256 / TPV;
     const float level = c_nf4_table[threadIdx.x & 15];
     kv_begin();
     const int sub = threadIdx.x % TPV;
-    const long long first = (long long)blockIdx.x * (kAppendUnroll * per) + threadIdx.x / TPV;
-    uint32_t w[kAppendUnroll];
-    float s[kAppendUnroll];
-    float* dst[kAppendUnroll];
+    const long long first = (long long)blockIdx.x * (U * per) + threadIdx.x / TPV;
+    uint32_t w[U];
+    float s[U];
+    float* dst[U];
 #pragma unroll
-    for (int u = 0; u < kAppendUnroll; ++u) {
+    for (int u = 0; u < U; ++u) {
         const long long i = min(first + u * per, p.n - 1);
         const VectorIndex v = vector_index(i, p.l.kv_heads, p.magic);
         const int slot = __ldg(p.slots + v.token), page = slot >> p.l.page_shift, row = slot & (p.l.page_size - 1);
@@ -360,7 +363,7 @@ __global__ void __launch_bounds__(256) kv_read_kernel(const ReadParams p)
         dst[u] = first + u * per < p.n ? (v.value ? p.v : p.k) + ((long long)v.token * p.l.kv_heads + v.head) * D + sub * 8 : nullptr;
     }
 #pragma unroll
-    for (int u = 0; u < kAppendUnroll; ++u) {
+    for (int u = 0; u < U; ++u) {
         float x[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
@@ -373,24 +376,44 @@ __global__ void __launch_bounds__(256) kv_read_kernel(const ReadParams p)
     }
 }
 
-// blocks of a launch over n vectors, and the divisor's magic number
-inline long long vector_blocks(long long n, int head_dim)
+// blocks of a launch over n vectors, u a thread, and the divisor's magic number
+inline long long vector_blocks(long long n, int head_dim, int u)
 {
-    const int per = kAppendUnroll * 256 / (head_dim / 8);
+    const int per = u * 256 / (head_dim / 8);
     return (n + per - 1) / per;
 }
 
 inline unsigned long long vector_magic(int kv_heads) { return ~0ULL / (2ULL * kv_heads) + 1; }
+
+template <typename T, int FMT, int D, int U>
+cudaError_t append_u(const AppendParams& p, bool vec, cudaStream_t st)
+{
+    const dim3 grid((unsigned)vector_blocks(p.n, D, U));
+    return vec ? kv_launch(kv_append_kernel<T, FMT, D, true, U>, grid, 256, 0, st, p) : kv_launch(kv_append_kernel<T, FMT, D, false, U>, grid, 256, 0, st, p);
+}
+
+template <typename T, int FMT, int D>
+cudaError_t append_d(const AppendParams& p, bool vec, cudaStream_t st)
+{
+    if constexpr (sizeof(T) == 2)
+        if (vector_blocks(p.n, D, 1) > kFewBlocks) return append_u<T, FMT, D, 2>(p, vec, st);
+    return append_u<T, FMT, D, 1>(p, vec, st);
+}
+
+template <int FMT, int D>
+cudaError_t read_d(const ReadParams& p, cudaStream_t st)
+{
+    const long long few = vector_blocks(p.n, D, 1);
+    if (few > kFewBlocks) return kv_launch(kv_read_kernel<FMT, D, 2>, dim3((unsigned)vector_blocks(p.n, D, 2)), 256, 0, st, p);
+    return kv_launch(kv_read_kernel<FMT, D, 1>, dim3((unsigned)few), 256, 0, st, p);
+}
 
 template <typename T, int FMT>
 cudaError_t append(const AppendParams& p, cudaStream_t st)
 {
     const long long strides = p.k_tok | p.k_head | p.v_tok | p.v_head;
     const bool vec = kv_aligned(p.k, 16) && kv_aligned(p.v, 16) && strides * (long long)sizeof(T) % 16 == 0;
-    const dim3 grid((unsigned)vector_blocks(p.n, p.l.head_dim));
-    if (p.l.head_dim == 64)
-        return vec ? kv_launch(kv_append_kernel<T, FMT, 64, true>, grid, 256, 0, st, p) : kv_launch(kv_append_kernel<T, FMT, 64, false>, grid, 256, 0, st, p);
-    return vec ? kv_launch(kv_append_kernel<T, FMT, 128, true>, grid, 256, 0, st, p) : kv_launch(kv_append_kernel<T, FMT, 128, false>, grid, 256, 0, st, p);
+    return p.l.head_dim == 64 ? append_d<T, FMT, 64>(p, vec, st) : append_d<T, FMT, 128>(p, vec, st);
 }
 
 }  // namespace
@@ -447,7 +470,7 @@ int b4_kv_append(const b4_kv_cache* cache, const void* k, const void* v, int dty
     p.slots = slots;
     p.n = 2LL * n_tokens * cache->kv_heads;
     p.magic = vector_magic(cache->kv_heads);
-    if (vector_blocks(p.n, cache->head_dim) > 0x7fffffffLL) return cudaErrorInvalidValue;
+    if (vector_blocks(p.n, cache->head_dim, 1) > 0x7fffffffLL) return cudaErrorInvalidValue;
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     const bool i4 = cache->fmt == B4_KV_INT4;
     if (dtype == B4_DTYPE_F16) return i4 ? append<__half, B4_KV_INT4>(p, st) : append<__half, B4_KV_NF4>(p, st);
@@ -469,14 +492,10 @@ int b4_kv_read(const b4_kv_cache* cache, const int32_t* slots, int n_tokens, flo
     p.v = v;
     p.n = 2LL * n_tokens * cache->kv_heads;
     p.magic = vector_magic(cache->kv_heads);
-    if (vector_blocks(p.n, cache->head_dim) > 0x7fffffffLL) return cudaErrorInvalidValue;
-    const dim3 grid((unsigned)vector_blocks(p.n, cache->head_dim));
+    if (vector_blocks(p.n, cache->head_dim, 1) > 0x7fffffffLL) return cudaErrorInvalidValue;
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-    if (cache->fmt == B4_KV_INT4)
-        return cache->head_dim == 64 ? kv_launch(kv_read_kernel<B4_KV_INT4, 64>, grid, 256, 0, st, p)
-                                     : kv_launch(kv_read_kernel<B4_KV_INT4, 128>, grid, 256, 0, st, p);
-    return cache->head_dim == 64 ? kv_launch(kv_read_kernel<B4_KV_NF4, 64>, grid, 256, 0, st, p)
-                                 : kv_launch(kv_read_kernel<B4_KV_NF4, 128>, grid, 256, 0, st, p);
+    if (cache->fmt == B4_KV_INT4) return cache->head_dim == 64 ? read_d<B4_KV_INT4, 64>(p, st) : read_d<B4_KV_INT4, 128>(p, st);
+    return cache->head_dim == 64 ? read_d<B4_KV_NF4, 64>(p, st) : read_d<B4_KV_NF4, 128>(p, st);
 }
 
 }  // extern "C"
