@@ -431,8 +431,7 @@ const char* b4_nccl_error_string(int status);
  * reference, which stops at the projections.
  *
  * A page holds page_size tokens of every kv head; one kv head's part of a page
- * is a block of contiguous bytes, so that a bulk copy brings it into shared
- * memory whole:
+ * is a block of contiguous bytes, so that a page is read in whole lines:
  *   codes of the keys     [page_size][head_dim / 2]   (packed as the weights are:
  *   codes of the values   [page_size][head_dim / 2]    lower column, low nibble)
  *   scales of the keys    [page_size]
@@ -518,7 +517,8 @@ int b4_kv_read(const b4_kv_cache* cache, const int32_t* slots, int n_tokens, flo
  * columns contiguous, rows 16-byte aligned.  lse (optional): fp32
  * [total_q][heads], the natural logarithm of the sum of exp(scores).
  * max_q: the most queries of one request (chooses the kernels; requests with
- * more are computed all the same).  heads / kv_heads <= 64.
+ * more are computed all the same).  heads / kv_heads <= 64,
+ * total_q * heads / kv_heads < 2^31.
  * ws: b4_kv_attention_workspace bytes of device memory, 16-byte aligned,
  * ZERO-FILLED before its first use; calls leave ready for the next what must be
  * zero.  Not shared with b4_gemv_ws, nor by calls that may run at the same time. */
@@ -539,8 +539,8 @@ int b4_kv_attention(const b4_kv_cache* cache, const b4_kv_attn* attn, void* ws, 
 
 /* Reads (and with clear != 0 resets) the current device's error flags: non-zero
  * after a bounded wait ran out -- 1: a streaming kernel's wait on its copy
- * ring (the kernel then ended early; the cache attention's: carried on), 2: the x-pair table kernel's count-in
- * (it then carried on without it) -- and that launch's output is not valid.
+ * ring or the cache attention's on another warp (the kernel then ended early),
+ * 2: the x-pair table kernel's count-in (it then carried on without it) -- and that launch's output is not valid.
  * Returns the flags, or -1 if they could not be read. */
 int b4_device_error(int clear);
 

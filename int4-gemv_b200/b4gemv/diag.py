@@ -14,6 +14,9 @@ src/diag_aspect.cu on B200): the measurements the dispatch rule is fitted to.
       the benchmark's NF4 decode step, eagerly (the launch list's command).
   python -m b4gemv.diag glue    [--n 28672] [--launches 3]
       the decode layer's elementwise kernels.
+  python -m b4gemv.diag kv      [--fmt nf4|int4] [--requests 16] [--prompt 200] [--tokens 20]
+      the attention half of a decode layer over the 4-bit cache (kvlayer.py): a
+      prompt step, then decode steps, their time.
 Run from int4-gemv_b200/ (or with it on sys.path).
 """
 from __future__ import annotations
@@ -313,6 +316,29 @@ def cmd_glue(args, torch):
     print(f"ran {args.launches} x (swiglu, cast) on {args.n} elements")
 
 
+def cmd_kv(args, torch):
+    """A packed prompt step and `tokens` decode steps of one 28-head layer's
+    attention half, all requests in one batch."""
+    from .kvlayer import CachedAttention
+    fmt = FMT_NF4_B64 if args.fmt == "nf4" else FMT_INT4_G128
+    n, width = args.requests, -(-(args.prompt + args.tokens) // 64)
+    layer = CachedAttention(fmt, 3584, 28, 4, n * width, n, max_context=64 * width)
+    a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+    layer.step(torch.randn((n * args.prompt, 3584), device="cuda").half(), [args.prompt] * n)
+    x = torch.randn((n, 3584), device="cuda").half()
+    for i in range(args.tokens):
+        if i == 3:
+            a.record()
+        layer.step(x, [1] * n)
+    b.record()
+    torch.cuda.synchronize()
+    done, state = layer.cached.tolist(), layer.free_state.tolist()
+    if load().b4_device_error(0) or done != [args.prompt + args.tokens] * n or state[2]:
+        raise RuntimeError(f"kv: lengths {done}, ring {state}")
+    print(f"{n} requests, {args.prompt} + {args.tokens} tokens, {args.fmt}: {a.elapsed_time(b) * 1e3 / max(1, args.tokens - 3):.1f} us a "
+          f"decode step, host launches included; {state[1]} pages left")
+
+
 def cmd_p2p(args, torch):
     """The row-parallel GEMV with the peer-memory all-reduce in its epilogue
     (b4_tp_gemv_p2p_ex) in a world of one rank (its own slots, no peer, no
@@ -375,6 +401,11 @@ def main(argv=None):
     gl = sub.add_parser("glue")
     gl.add_argument("--n", type=int, default=28672)
     gl.add_argument("--launches", type=int, default=3)
+    kv = sub.add_parser("kv")
+    kv.add_argument("--fmt", default="nf4", choices=["nf4", "int4"])
+    kv.add_argument("--requests", type=int, default=16)
+    kv.add_argument("--prompt", type=int, default=200)
+    kv.add_argument("--tokens", type=int, default=20)
     pp = sub.add_parser("p2p")
     pp.add_argument("--fmt", default="nf4", choices=["nf4", "int4"])
     pp.add_argument("--shape", default="tp2_down", choices=list(SHAPES))
@@ -383,7 +414,7 @@ def main(argv=None):
     args = ap.parse_args(argv)
     import torch
     torch.cuda.init()
-    {"sweep": cmd_sweep, "aspect": cmd_aspect, "run": cmd_run, "step": cmd_step, "glue": cmd_glue,
+    {"sweep": cmd_sweep, "aspect": cmd_aspect, "run": cmd_run, "step": cmd_step, "glue": cmd_glue, "kv": cmd_kv,
      "p2p": cmd_p2p}[args.cmd](args, torch)
 
 

@@ -173,12 +173,14 @@ def kv_read(cache: KVCache, slots, k=None, v=None, stream=None):
 _WS, _WS_BYTES = {}, {}
 
 
-def _workspace(index, nbytes: int):
-    """The package's workspace for attention on a device: zero-filled, grown on demand."""
+def _workspace(index, nbytes: int, stream=None):
+    """The package's workspace for attention on a device: zero-filled (before what `stream` does next), grown on demand."""
     ws = _WS.get(index)
     if ws is None or ws.numel() < nbytes:
         ws = _torch.zeros(max(int(nbytes), 1 << 20), dtype=_torch.uint8, device=f"cuda:{index}")
         _WS[index] = ws
+        if stream is not None:
+            stream.wait_stream(_torch.cuda.current_stream(index))
     return ws
 
 
@@ -234,7 +236,7 @@ def kv_attention(cache: KVCache, q, tables, ctx_len, q_starts, max_q: int, scale
         need = _WS_BYTES.get(key)
         if need is None:
             need = _WS_BYTES[key] = _attn_bytes(cache, args)
-        ws = _workspace(cache.index, need)
+        ws = _workspace(cache.index, need, stream)
     status = load().b4_kv_attention(cache._ref, args, ws.data_ptr(), ws.numel(),
                                     stream.cuda_stream if stream is not None else _raw_stream(cache.index))
     if status:

@@ -13,7 +13,7 @@ namespace {
 // between CTAs; then the threads of the grid share the packed tokens and the new
 // table entries, one each where the grid allows, and find their request by binary
 // search in the sums: the time is a handful of dependent loads, whatever the
-// requests' lengths.  A slot in a new page comes straight from the ring, not through
+// requests' lengths (48 requests: 3.7 us; 700 with 175 thousand tokens: 9.0 us, 1.4 MB).  A slot in a new page comes straight from the ring, not through
 // the table, which another CTA may still be writing.
 constexpr int kTabThreads = 256, kTabGrid = 148 * 8;
 
@@ -261,7 +261,8 @@ __device__ __forceinline__ uint32_t nf4_word(const float (&x)[8], float s, float
 // two; 6007 x 12 x 64 in fp32: 24.6 against 25.3).
 constexpr long long kFewBlocks = 148 * 8;
 
-// Bound by memory: 2.1 to 4.5 bytes a column.
+// Bound by memory, 2.1 to 4.5 bytes a column, and at NF4 by the instructions of a code (10): 20011 tokens x 4 x 128 from
+// bf16 in 30 us.
 template <typename T, int FMT, int D, bool VEC, int U>
 __global__ void __launch_bounds__(256) kv_append_kernel(const AppendParams p)
 {
@@ -334,7 +335,7 @@ struct ReadParams {
     unsigned long long magic;
 };
 
-// Bound by its fp32 stores.
+// Bound by its fp32 stores: the same tokens in 20 us, 5.2 TB/s.
 template <int FMT, int D, int U>
 __global__ void __launch_bounds__(256) kv_read_kernel(const ReadParams p)
 {

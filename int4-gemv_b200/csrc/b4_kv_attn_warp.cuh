@@ -31,6 +31,13 @@
 // time, so a warp waits for nothing but its own data.  (Bulk copies measured slower
 // here: a warp that issues one spends some 35 instructions on it, and half a page
 // of 64 takes four.)
+//
+// What bounds it.  INT4: the loop runs at 5.3 TB/s; around it a launch spends 5 us up to
+// its first products (lengths, units, page ids, queries: four loads that wait for one
+// another) and 6 to 9 on the joins.  NF4: the lookups, 96 of some 150 shared-memory
+// cycles per 16 tokens, 4.1 TB/s.  Measured: 32 requests x 8192 tokens, 64 heads over 8
+// x 128, INT4: 68 us, 4.07 TB/s over all; one request of 131071, NF4: 57 us, 2.5 TB/s;
+// 96 of 1 to 6000, 32 heads over 8 x 64, NF4: 68 us, 2.4 TB/s; one of 777, INT4: 11.7 us.
 #pragma once
 
 #include <type_traits>
@@ -39,7 +46,8 @@
 
 namespace b4 {
 
-// What a segment (a request's head and column tile) costs a warp beside its chunks, in a chunk's time.
+// What a segment (a request's head and column tile) costs a warp beside its chunks, in a chunk's time: 96 requests of 1 to
+// 6000 tokens take 78 us without it, 69 with 1, 68 with 2 and with 4.
 constexpr int kSegChunks = 2;
 
 // PT: tokens of a page in shared memory, 16 or 32 (half a page of 64 lies there as a page of 32)
