@@ -9,9 +9,10 @@
 // 8-wide side is the queries and none of it is padding for groups of 8.  A token's
 // scale does not depend on the column, so the key's scale multiplies S and the
 // value's scale P, in fp32; the operands hold the bare levels (INT4: exact
-// integers; NF4: keys rounded to fp16 (kNf4Up), values as fp16 high and low parts
-// in two products, since an output over many tokens is far smaller than its
-// terms, and a level's rounding does not average out as the weights' does).
+// integers; NF4: keys rounded to fp16 (kNf4Up), values so too where the output is
+// bf16, as fp16 high and low parts in two products where it is fp16, since an output
+// over many tokens is far smaller than its terms, and a level's rounding averages out
+// only as far as the codes are spread as kNf4Up takes them).
 // Softmax's maximum and sum run along the tokens, in fp32, private to a warp;
 // the maximum moves only when a score passes it by 2^8, which the weights'
 // range allows.  P goes to fp16 (its rounding is of the size of the output's own),
@@ -204,6 +205,7 @@ __global__ void __launch_bounds__(WarpCfg<FMT, D, NT, PT>::kThreads, 1) kv_attn_
         constexpr int tile1 = PT == 16 ? C::kBlock : 16 * C::kRow;
         const int v_other = t & 1 ? -C::kRow : C::kRow;
         const int s_at = lane / PT * C::kBlock + PT * D + lane % PT * C::kScale;
+        constexpr bool kLow = std::is_same<T, __half>::value;              // NF4 values in two parts
         const uint32_t t_key = C::kTable + lane * 8 + (lane >> 4) * 4, t_val = C::kTable + lane * 8;
 
         float o[NT][D / 16][4];                // m-tile mt: columns 2t, 2t + 1 of d = g * (D / 8) + 2 mt, and of d + 1
@@ -432,13 +434,18 @@ __global__ void __launch_bounds__(WarpCfg<FMT, D, NT, PT>::kThreads, 1) kv_attn_
                             uint2 lo[2], hi[2];
 #pragma unroll
                             for (int j = 0; j < 2; ++j) {
-                                lo[j] = lds64(__byte_perm(e[j], t_val, 0x7604 | b << 4));
-                                hi[j] = lds64(__byte_perm(f[j], t_val, 0x7604 | b << 4));
+                                if (kLow) {
+                                    lo[j] = lds64(__byte_perm(e[j], t_val, 0x7604 | b << 4));
+                                    hi[j] = lds64(__byte_perm(f[j], t_val, 0x7604 | b << 4));
+                                } else {
+                                    lo[j].x = lds32(__byte_perm(e[j], t_key, 0x7604 | b << 4));
+                                    hi[j].x = lds32(__byte_perm(f[j], t_key, 0x7604 | b << 4));
+                                }
                             }
 #pragma unroll
                             for (int nt = 0; nt < NT; ++nt) {
                                 mma_f16(o[nt][4 * i + b], lo[0].x, hi[0].x, lo[1].x, hi[1].x, pb[st][nt][0], pb[st][nt][1]);
-                                mma_f16(o[nt][4 * i + b], lo[0].y, hi[0].y, lo[1].y, hi[1].y, pb[st][nt][0], pb[st][nt][1]);
+                                if (kLow) mma_f16(o[nt][4 * i + b], lo[0].y, hi[0].y, lo[1].y, hi[1].y, pb[st][nt][0], pb[st][nt][1]);
                             }
                         }
                     }

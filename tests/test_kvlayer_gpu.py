@@ -11,7 +11,7 @@ from b4gemv.kvlayer import CachedAttention, rotate
 pytestmark = pytest.mark.gpu
 
 
-@pytest.mark.parametrize("fmt,kv_fmt", [(b4gemv.FMT_INT4_G128, ref.INT4), (b4gemv.FMT_NF4_B64, ref.NF4)])
+@pytest.mark.parametrize("fmt,kv_fmt", [(b4gemv.FMT_INT4_G128, b4gemv.KV_INT4), (b4gemv.FMT_NF4_B64, b4gemv.KV_NF4)])
 @pytest.mark.parametrize("heads,kvh,dim,page", [(4, 2, 128, 16), (8, 1, 64, 32)])
 def test_steps(cuda, fmt, kv_fmt, heads, kvh, dim, page):
     hidden = 512
@@ -31,7 +31,7 @@ def test_steps(cuda, fmt, kv_fmt, heads, kvh, dim, page):
         out, _, (weight, size) = ref.attention(kv_fmt, page, dim, layer.cache.blocks, q.half(), layer.tables[:3], done, starts, dim ** -0.5)
         # q's rounding to fp16 may fall to either side (2^-10 of q, so of the largest score, then twice in a weight), the NF4
         # code book in fp16 3e-4 of a level; weights and outputs are rounded to fp16 once each
-        book = 3e-4 if kv_fmt == ref.NF4 else 0.0
+        book = 3e-4 if kv_fmt == b4gemv.KV_NF4 else 0.0
         tol = weight * (2 ** -11 + book + 2 * size[..., None] * (2.0 ** -10 + book)) + out.abs() * 2 ** -11 + 2.0 ** -20
         got, want = y.double(), out.view(x.shape[0], -1) @ w["o"].T
         assert bool(((got - want).abs() <= tol.view(x.shape[0], -1) @ w["o"].abs().T + 1e-4 * want.abs().max()).all())
@@ -43,7 +43,7 @@ def test_steps(cuda, fmt, kv_fmt, heads, kvh, dim, page):
         slots = torch.from_numpy(table[row, place.cpu().numpy() // page] * page + place.cpu().numpy() % page).int().cuda()
         for a, b in zip(b4gemv.kv_read(layer.cache, slots), (k, v)):
             # half the widest step (INT4: 1 / 14 of the largest column; NF4: 0.152 of it), and what is rounded before
-            step = (1 / 14 if kv_fmt == ref.INT4 else 0.152) * b.abs().amax(-1, keepdim=True)
+            step = (1 / 14 if kv_fmt == b4gemv.KV_INT4 else 0.152) * b.abs().amax(-1, keepdim=True)
             assert bool(((a - b).abs() <= step * 1.01 + 1e-3).all())
     assert layer.free_state.tolist()[2] == 0
     assert b4gemv.load().b4_device_error(0) == 0
