@@ -85,6 +85,15 @@ __device__ __forceinline__ void copy_async16(uint32_t dst, const void* src)
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 
+// Counts in at a segment that crosses CTAs: after it, what the CTAs that counted in before wrote is there.  By one thread,
+// behind a barrier that puts its CTA's writes before it.
+__device__ __forceinline__ int count_in(int* at)
+{
+    int n;
+    asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], 1;" : "=r"(n) : "l"(at) : "memory");
+    return n;
+}
+
 // A maximum that no score has set yet: finite, so that differences with it are.
 constexpr float kNoMax = -1e30f;
 

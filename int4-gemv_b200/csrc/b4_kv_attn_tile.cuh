@@ -929,10 +929,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attn_tile_kernel(const Att
             const int f = owner(s0), parts = owner(s1 - 1) - f + 1;
             if (!(ok = together())) break;
             if (tid == 128) {
-                __threadfence();
-                joins = atomicAdd(ws.count + f, 1) == parts - 1;
+                joins = count_in(ws.count + f) == parts - 1;
                 if (joins) ws.count[f] = 0;
-                __threadfence();
             }
             if (!(ok = together())) break;
             const bool join = joins;

@@ -732,10 +732,8 @@ __global__ void __launch_bounds__(WarpCfg<FMT, D, NT, PT>::kThreads, 1) kv_attn_
         if (at >= 0) {
             int f;
             const int n = span(pieces[at >> 1][at & 1], f);
-            __threadfence();
-            last = atomicAdd(ws.count + f, 1) == n - 1;
+            last = count_in(ws.count + f) == n - 1;
             if (last) ws.count[f] = 0;
-            __threadfence();
         }
         last_cta[tid] = last;
     }
