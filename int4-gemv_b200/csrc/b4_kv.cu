@@ -212,15 +212,15 @@ __device__ __forceinline__ uint32_t int4_word(const float (&x)[8], float s)
 {
     const float inv = __fdividef(1.0f, s);
     uint32_t w = 0;
-    float worst = 0.0f;
+    float worst = 0.0f, nans = 0.0f;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
         const float y = x[j] * inv, r = y + 12582912.0f;           // 1.5 * 2^23: the integer nearest to y in the low bits
         worst = fmaxf(worst, fabsf(y - (r - 12582912.0f)));
         w |= (__float_as_uint(r) & 15u) << (4 * j);
-        if (isnan(y)) worst = 1.0f;
+        nans = fmaf(y, 0.0f, nans);
     }
-    if (worst < 0.49999f && s >= 6.1035156e-5f && s <= 65504.0f) return w ^ 0x88888888u;   // two's complement to code - 8
+    if (worst < 0.49999f && nans == 0.0f && s >= 6.1035156e-5f && s <= 65504.0f) return w ^ 0x88888888u;   // two's complement to code - 8
     w = 0;
 #pragma unroll 1
     for (int j = 0; j < 8; ++j) w |= (uint32_t)int4_code(__fdiv_rn(x[j], s)) << (4 * j);
@@ -238,7 +238,7 @@ __device__ __forceinline__ uint32_t nf4_word(const float (&x)[8], float s, float
 {
     const float inv = __fdividef(1.0f, s);
     uint32_t w = 0;
-    float worst = 1.0f;
+    float worst = 1.0f, nans = 0.0f;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
         const float y = x[j] * inv;
@@ -246,10 +246,10 @@ __device__ __forceinline__ uint32_t nf4_word(const float (&x)[8], float s, float
         const float d = y - __shfl_sync(0xffffffffu, boundary, bin);
         const int c = __shfl_sync(0xffffffffu, below, bin) + (d >= 0.0f);
         worst = fminf(worst, fabsf(d));
-        if (isnan(y)) worst = 0.0f;
+        nans = fmaf(y, 0.0f, nans);
         w |= (uint32_t)c << (4 * j);
     }
-    if (worst > 1e-6f && s > 1e-30f && s < 1e30f) return w;
+    if (worst > 1e-6f && nans == 0.0f && s > 1e-30f && s < 1e30f) return w;
     w = 0;
 #pragma unroll 1
     for (int j = 0; j < 8; ++j) w |= (uint32_t)nf4_code(__fdiv_rn(x[j], s)) << (4 * j);
@@ -272,12 +272,14 @@ __global__ void __launch_bounds__(256) kv_append_kernel(const AppendParams p)
     if (FMT == B4_KV_NF4) {
         const int lane = threadIdx.x & 31;
         const float start = (lane - 16.5f) / kBins, end = (lane - 15.5f) / kBins;
+        // lane c: the boundary above level c; then the first at `start` or above by bisection
+        const float level = c_nf4_table[lane & 15], above = __shfl_down_sync(0xffffffffu, level, 1);
+        const float mid = lane < 15 ? 0.5f * (level + above) : INFINITY;
 #pragma unroll
-        for (int c = 0; c < 15; ++c) {
-            const float m = 0.5f * (c_nf4_table[c] + c_nf4_table[c + 1]);
-            if (m < start) below = c + 1;
-            else if (m < end) boundary = m;
-        }
+        for (int step = 8; step > 0; step >>= 1)
+            if (__shfl_sync(0xffffffffu, mid, below + step - 1) < start) below += step;
+        const float next = __shfl_sync(0xffffffffu, mid, below);
+        if (next < end) boundary = next;
     }
     kv_begin();
     const int sub = threadIdx.x % TPV;
