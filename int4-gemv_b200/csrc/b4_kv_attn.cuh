@@ -100,26 +100,27 @@ constexpr float kNoMax = -1e30f;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 // The NF4 levels as fp16 operands.  fp16 has 11 bits, the levels 24: rounded as
-// they are, the levels are off by 1.6e-4 of the code book's norm.  Times kNf4Up
-// first, all 16 lie nearer to fp16 numbers (9.3e-5 at most, 4e-5 in the mean square),
-// and 1 / kNf4Up goes into a factor that is applied in fp32 anyway.  A level's rounding
-// is the same for every token, so over many tokens it does not average out as the
-// weights' do, while an output gets smaller: of 20 million factors in [1, 2) this one's
-// roundings, weighted by how often a code occurs (normal values under the largest of
-// 64 and of 128; every code alike), sum to the least, 8e-7 of a scale at most (a factor
-// of least rounding, 3.3e-5, leaves 1.1e-5: 0.2 % of an output over 4000 tokens).
-constexpr float kNf4Up = 1.6775788f;
+// they are, the levels are off by 1.6e-4 of the code book's norm.  Times a factor in
+// [1, 2) first, all 16 lie nearer to fp16 numbers, and its reciprocal goes into a
+// factor that is applied in fp32 anyway.  kNf4Least leaves the least, 3.3e-5 in the mean
+// square (6.3e-5 at most): for keys, and where the low parts make the values exact.
+// A value's rounding is the same for every token of its code, so over many tokens it
+// does not average out as the weights' do, while an output gets smaller: of 20 million
+// factors, kNf4Even's roundings (4e-5, 9.3e-5 at most), weighted by how often a code
+// occurs (normal values under the largest of 64 and of 128; every code alike), sum to the
+// least, 8e-7 of a scale (kNf4Least's: 1.1e-5, 0.2 % of an output over 4000 tokens).
+constexpr float kNf4Least = 1.67766535282135f, kNf4Even = 1.6775788f;
 
-__device__ __forceinline__ uint32_t nf4_pair(uint32_t byte)
+__device__ __forceinline__ uint32_t nf4_pair(uint32_t byte, float up)
 {
-    const __half lo = __float2half_rn(c_nf4_table[byte & 15] * kNf4Up), hi = __float2half_rn(c_nf4_table[byte >> 4] * kNf4Up);
+    const __half lo = __float2half_rn(c_nf4_table[byte & 15] * up), hi = __float2half_rn(c_nf4_table[byte >> 4] * up);
     return (uint32_t)__half_as_ushort(lo) | ((uint32_t)__half_as_ushort(hi) << 16);
 }
 
 // What the fp16 parts of nf4_pair leave of the levels: with it they are exact to 2^-22.
-__device__ __forceinline__ uint32_t nf4_pair_low(uint32_t byte)
+__device__ __forceinline__ uint32_t nf4_pair_low(uint32_t byte, float up)
 {
-    const float a = c_nf4_table[byte & 15] * kNf4Up, b = c_nf4_table[byte >> 4] * kNf4Up;
+    const float a = c_nf4_table[byte & 15] * up, b = c_nf4_table[byte >> 4] * up;
     const __half lo = __float2half_rn(a - __half2float(__float2half_rn(a))), hi = __float2half_rn(b - __half2float(__float2half_rn(b)));
     return (uint32_t)__half_as_ushort(lo) | ((uint32_t)__half_as_ushort(hi) << 16);
 }

@@ -8,7 +8,7 @@
 // with fp16 operands and fp32 accumulators in tensor memory.  Where a request has
 // 128 rows or fewer, the two tiles are the same rows and take every other block: two
 // streams, joined at the end.  K and V hold the bare levels (INT4: exact integers;
-// NF4: rounded to fp16, kNf4Up), so a token's key scale multiplies a column of S and
+// NF4: rounded to fp16, kNf4Even), so a token's key scale multiplies a column of S and
 // its value scale a column of P, in fp32.  Softmax is the warp kernel's
 // (b4_kv_attn_warp.cuh): a maximum that moves only when a score passes it by 2^8,
 // weights relative to it and to a running power of two of the value scales, rounded
@@ -287,7 +287,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attn_tile_kernel(const Att
     }
     if (FMT == B4_KV_NF4) {
         for (int i = tid; i < 256 * 4; i += kTileThreads) {
-            const uint32_t v = nf4_pair(i >> 2);
+            const uint32_t v = nf4_pair(i >> 2, kNf4Even);
             asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(C::kTable + i * 16), "r"(v) : "memory");
         }
     }
@@ -761,7 +761,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attn_tile_kernel(const Att
                 if (!(ok = warp_wait(&q_both, shared & 1, &dead))) break;
                 factor = q_factor[shared & 1][t];
             }
-            const float qf = fmaxf(factor * (fabsf(a.scale) * kLog2e) * (FMT == B4_KV_NF4 ? 1.0f / kNf4Up : 1.0f), 1e-30f);
+            const float qf = fmaxf(factor * (fabsf(a.scale) * kLog2e) * (FMT == B4_KV_NF4 ? 1.0f / kNf4Even : 1.0f), 1e-30f);
             float m = kNoMax, l = 0.0f;
             int vexp = -126;
             bool any = false;                  // whether O holds something
@@ -856,7 +856,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attn_tile_kernel(const Att
             if (!s.end) factor = put(s);
 
             // ---- the segment's rows, or a piece of them: a row a thread; one tile of rows: half a row's columns, of both streams ----
-            const float vup = any ? pow2(vexp) * (FMT == B4_KV_NF4 ? 1.0f / kNf4Up : 1.0f) : 0.0f;
+            const float vup = any ? pow2(vexp) * (FMT == B4_KV_NF4 ? 1.0f / kNf4Even : 1.0f) : 0.0f;
             float wa = vup, wb = 0.0f;
             if (!two) {
                 stream_max[x][t] = m;

@@ -9,10 +9,10 @@
 // 8-wide side is the queries and none of it is padding for groups of 8.  A token's
 // scale does not depend on the column, so the key's scale multiplies S and the
 // value's scale P, in fp32; the operands hold the bare levels (INT4: exact
-// integers; NF4: keys rounded to fp16 (kNf4Up), values so too where the output is
+// integers; NF4: keys rounded to fp16 (kNf4Least), values so too where the output is
 // bf16, as fp16 high and low parts in two products where it is fp16, since an output
 // over many tokens is far smaller than its terms, and a level's rounding averages out
-// only as far as the codes are spread as kNf4Up takes them).
+// only as far as the codes are spread as kNf4Even takes them).
 // Softmax's maximum and sum run along the tokens, in fp32, private to a warp;
 // the maximum moves only when a score passes it by 2^8, which the weights'
 // range allows.  P goes to fp16 (its rounding is of the size of the output's own),
@@ -89,6 +89,8 @@ __global__ void __launch_bounds__(WarpCfg<FMT, D, NT, PT>::kThreads, 1) kv_attn_
 {
     using C = WarpCfg<FMT, D, NT, PT>;
     constexpr int kWarps = C::kWarps, kThreads = C::kThreads, kStages = C::kStages, kScan = C::kScan;
+    constexpr bool kLow = std::is_same<T, __half>::value;          // NF4 values in two parts
+    constexpr float kUp = kLow ? kNf4Least : kNf4Even;
     extern __shared__ __align__(1024) uint8_t attn_smem[];
     __shared__ WarpPiece pieces[kWarps][2];
     __shared__ long long scan[kScan + 1], warp_sum[kWarps];
@@ -106,7 +108,7 @@ __global__ void __launch_bounds__(WarpCfg<FMT, D, NT, PT>::kThreads, 1) kv_attn_
         // row b: 32 copies of (high, low) of byte b's two levels, the two swapped in the upper 16 copies: there the
         // high parts alone (keys) lie in the odd banks, and the two products of the values add up to the same
         for (int i = tid; i < 256 * 16; i += kThreads) {
-            const uint32_t b = i >> 4, hi = nf4_pair(b), lo = nf4_pair_low(b);
+            const uint32_t b = i >> 4, hi = nf4_pair(b, kUp), lo = nf4_pair_low(b, kUp);
             reinterpret_cast<uint4*>(attn_smem + C::kTable - smem_at)[i] = (i & 15) < 8 ? make_uint4(hi, lo, hi, lo) : make_uint4(lo, hi, lo, hi);
         }
     }
@@ -205,7 +207,6 @@ __global__ void __launch_bounds__(WarpCfg<FMT, D, NT, PT>::kThreads, 1) kv_attn_
         constexpr int tile1 = PT == 16 ? C::kBlock : 16 * C::kRow;
         const int v_other = t & 1 ? -C::kRow : C::kRow;
         const int s_at = lane / PT * C::kBlock + PT * D + lane % PT * C::kScale;
-        constexpr bool kLow = std::is_same<T, __half>::value;              // NF4 values in two parts
         const uint32_t t_key = C::kTable + lane * 8 + (lane >> 4) * 4, t_val = C::kTable + lane * 8;
 
         float o[NT][D / 16][4];                // m-tile mt: columns 2t, 2t + 1 of d = g * (D / 8) + 2 mt, and of d + 1
@@ -249,7 +250,7 @@ __global__ void __launch_bounds__(WarpCfg<FMT, D, NT, PT>::kThreads, 1) kv_attn_
                 for (int j = 0; j < 2; ++j) {
                     // not 0, so that a masked score's -infinity stays one
                     qf[nt][j] = fmaxf(__shfl_sync(0xffffffffu, factor, (2 * t + j) * 4) * (fabsf(a.scale) * kLog2e) *
-                                          (FMT == B4_KV_NF4 ? 1.0f / kNf4Up : 1.0f), 1e-30f);
+                                          (FMT == B4_KV_NF4 ? 1.0f / kUp : 1.0f), 1e-30f);
                     col_row(nt * 8 + 2 * t + j, token, head);
                     lim[nt][j] = a.flags & B4_KV_FULL ? u.ctx : min(u.ctx, u.ctx - u.n + token + 1);
                     mx[nt][j] = kNoMax;
@@ -545,7 +546,7 @@ __global__ void __launch_bounds__(WarpCfg<FMT, D, NT, PT>::kThreads, 1) kv_attn_
             }
 
             // ---- the end of a segment, or of the run ----
-            const float vup = pow2(vexp) * (FMT == B4_KV_NF4 ? 1.0f / kNf4Up : 1.0f);
+            const float vup = pow2(vexp) * (FMT == B4_KV_NF4 ? 1.0f / kUp : 1.0f);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
