@@ -41,7 +41,7 @@
 // multiply); the rest is the chain of a row's softmax, longest in the two quarters of
 // the SM whose issue slots the products' warps share.  One row tile: the decoding
 // warps, 1.1 us a block.  Measured (chunk of 2048 tokens behind 6000, 28 heads over 4 x
-// 128, INT4): 280 us, 735 TFLOP/s; 24 requests x 5 tokens behind 2500 to 5500: 68 us;
+// 128, INT4): 273 us, 754 TFLOP/s; 24 requests x 5 tokens behind 2500 to 5500: 68 us;
 // the five prompts: 169 us.  Tried and left out: the tiles half a block apart (289 us);
 // the decoding warps in the other two quarters (287 us); scores issued only once the
 // last ones are read (286 us).

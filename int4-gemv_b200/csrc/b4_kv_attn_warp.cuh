@@ -9,8 +9,8 @@
 // 8-wide side is the queries and none of it is padding for groups of 8.  A token's
 // scale does not depend on the column, so the key's scale multiplies S and the
 // value's scale P, in fp32; the operands hold the bare levels (INT4: exact
-// integers; NF4: keys rounded to fp16 (kNf4Least), values so too where the output is
-// bf16, as fp16 high and low parts in two products where it is fp16, since an output
+// integers; NF4: keys rounded to fp16, values so too where the output is bf16, as fp16
+// high and low parts in two products where it is fp16, since an output
 // over many tokens is far smaller than its terms, and a level's rounding averages out
 // only as far as the codes are spread as kNf4Even takes them).
 // Softmax's maximum and sum run along the tokens, in fp32, private to a warp;
@@ -38,7 +38,7 @@
 // another) and 6 to 9 on the joins.  NF4: the lookups, 96 of some 150 shared-memory
 // cycles per 16 tokens, 4.1 TB/s.  Measured: 32 requests x 8192 tokens, 64 heads over 8
 // x 128, INT4: 68 us, 4.07 TB/s over all; one request of 131071, NF4: 57 us, 2.5 TB/s;
-// 96 of 1 to 6000, 32 heads over 8 x 64, NF4: 68 us, 2.4 TB/s; one of 777, INT4: 11.7 us.
+// 96 of 1 to 6000, 32 heads over 8 x 64, NF4: 59 us, 2.8 TB/s; one of 777, INT4: 11.7 us.
 #pragma once
 
 #include <type_traits>
