@@ -257,7 +257,7 @@ __device__ __forceinline__ uint32_t nf4_word(const float (&x)[8], float s, float
 }
 
 // Vectors a thread has in flight, U: two where 16-bit rows fill the GPU more than once (20011 tokens x 4 x 128, bf16 to
-// NF4, append and read-back: 43 us against 51 with one), one otherwise (64 tokens x 8 x 128: 4.7 us against 6.7 with
+// NF4, append and read-back: 40 us against 47 with one), one otherwise (64 tokens x 8 x 128: 4.7 us against 6.7 with
 // two; 6007 x 12 x 64 in fp32: 24.6 against 25.3).
 constexpr long long kFewBlocks = 148 * 8;
 
