@@ -170,17 +170,35 @@ def kv_read(cache: KVCache, slots, k=None, v=None, stream=None):
     return k, v
 
 
-_WS, _WS_BYTES = {}, {}
+_WS = {}
 
 
-def _workspace(index, nbytes: int, stream=None):
-    """The package's workspace for attention on a device: zero-filled (before what `stream` does next), grown on demand."""
+def _workspace_most():
+    """Bytes that serve every attention call on the current device: the tile kernel's, and the warp kernel's 16 columns, of 128."""
+    most = 0
+    for group, queries in ((1, 1 << 20), (16, 1)):
+        cache = KvCache(blocks=16, fmt=KV_INT4, n_pages=1, page_size=16, kv_heads=1, head_dim=128)      # an address that nothing reads
+        n = ctypes.c_size_t(0)
+        check("b4_kv_attention_workspace", load().b4_kv_attention_workspace(
+            ctypes.byref(cache), ctypes.byref(KvAttn(n_req=1, total_q=queries, max_q=queries, heads=group)), ctypes.byref(n)))
+        most = max(most, n.value)
+    return most
+
+
+def _workspace(index, stream=None):
+    """The package's workspace for attention on a device.  Captured graphs and kernels on any stream hold its address, so
+    there is one, of the largest size, made and zeroed once, outside captures, and never replaced."""
     ws = _WS.get(index)
-    if ws is None or ws.numel() < nbytes:
-        ws = _torch.zeros(max(int(nbytes), 1 << 20), dtype=_torch.uint8, device=f"cuda:{index}")
-        _WS[index] = ws
-        if stream is not None:
-            stream.wait_stream(_torch.cuda.current_stream(index))
+    if ws is None:
+        with _torch.cuda.device(index):
+            for s in (None, stream):                           # the caller's and the call's
+                with _torch.cuda.stream(s):
+                    if _torch.cuda.is_current_stream_capturing():
+                        raise ValueError("ws: the first call on a device makes the package's workspace, which a capture would "
+                                         "only record; call once before the capture, or pass ws")
+            ws = _torch.zeros(_workspace_most(), dtype=_torch.uint8, device=f"cuda:{index}")
+            _torch.cuda.current_stream().synchronize()         # zero for every stream from here on
+        ws = _WS.setdefault(index, ws)
     return ws
 
 
@@ -228,15 +246,12 @@ def kv_attention(cache: KVCache, q, tables, ctx_len, q_starts, max_q: int, scale
     request (q_starts).  scale None = head_dim ** -0.5; window 0 = none; lse: an
     fp32 [tokens][heads] tensor that receives the log-sum-exp of the scores.
     ws: a zero-filled uint8 CUDA tensor of kv_attention_workspace() bytes, or
-    None for the package's own of the device (calls that may overlap on the GPU
-    need their own).  Returns out."""
+    None for the package's own of the device (39.4 MB on a B200; the first call
+    makes it and waits for its zeros, and is refused inside a graph capture).
+    Calls that may overlap on the GPU need their own.  Returns out."""
     args, out = _attn(cache, q, tables, ctx_len, q_starts, max_q, scale, window, causal, out, lse)
     if ws is None:
-        key = (q.shape, max_q, cache.kv_heads, ctx_len.numel(), cache.index)     # what the size goes by
-        need = _WS_BYTES.get(key)
-        if need is None:
-            need = _WS_BYTES[key] = _attn_bytes(cache, args)
-        ws = _workspace(cache.index, need, stream)
+        ws = _workspace(cache.index, stream)
     status = load().b4_kv_attention(cache._ref, args, ws.data_ptr(), ws.numel(),
                                     stream.cuda_stream if stream is not None else _raw_stream(cache.index))
     if status:
