@@ -63,7 +63,11 @@ def _table(tables, index, n):
     stride, one = tables.stride()
     if rows < n or (width > 1 and one != 1):
         raise ValueError(f"tables: {n} rows at least, columns contiguous")
-    return width, max(stride, width)
+    if stride < width:
+        if n > 1:                              # expanded or overlapping rows: no stride of such a table's is the library's
+            raise ValueError("tables: rows must not overlap (an expanded table needs contiguous())")
+        stride = width                         # of a single row, that nothing is addressed by
+    return width, stride
 
 
 def kv_block_bytes(fmt: int, page_size: int, head_dim: int) -> int:
