@@ -6,8 +6,8 @@
     kv_append(cache, k, v, step.slots)
     out = kv_attention(cache, q, tables, step.ctx_len, step.q_starts, max_q)
 
-Every call goes to the current stream of the tensors' device (or `stream`) and
-returns without waiting.  Refused arguments raise ValueError before anything is
+Every call goes to the current stream of the tensors' device (or `stream`),
+whichever device is current, and returns without waiting.  Refused arguments raise ValueError before anything is
 launched; what only the library can refuse raises B4Error.
 
 A decode step calls these for every layer, with kernels of a few microseconds:
@@ -30,22 +30,35 @@ _STEP = struct.Struct("@5i4xq10P")
 _ATTN = struct.Struct("@6P5q8if4x")
 assert _STEP.size == ctypes.sizeof(KvStep) and _ATTN.size == ctypes.sizeof(KvAttn)
 
-_torch = _int32 = _float32 = _raw_stream = _codes = None
+_torch = _int32 = _float32 = _raw_stream = _device = _codes = None
 
 
 def _load():
     """torch's names and the library, once."""
-    global _torch, _int32, _float32, _raw_stream, _codes
+    global _torch, _int32, _float32, _raw_stream, _device, _codes
     import torch
     _torch, _int32, _float32 = torch, torch.int32, torch.float32
     _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
         lambda index: torch.cuda.current_stream(index).cuda_stream)
+    _device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
     _codes = {torch.float16: DTYPE_F16, torch.bfloat16: DTYPE_BF16, torch.float32: DTYPE_F32}
     return load()
 
 
 def _lib():
     return load() if _torch is not None else _load()
+
+
+def _launch(name, fn, index, stream, *args):
+    """fn(*args, stream) with device `index` current: the library launches, and counts its SMs, on the current device."""
+    handle = stream.cuda_stream if stream is not None else _raw_stream(index)
+    if _device() == index:
+        status = fn(*args, handle)
+    else:
+        with _torch.cuda.device(index):
+            status = fn(*args, handle)
+    if status:
+        check(name, status)
 
 
 def _ints(name, t, index, least):
@@ -135,9 +148,7 @@ def kv_tables(page_size: int, tables, cached, added, free_pages, free_state, max
     args = _STEP.pack(n, page_size, width, free_pages.numel(), max_tokens, stride, tables.data_ptr(), cached.data_ptr(),
                       added.data_ptr(), free_pages.data_ptr(), free_state.data_ptr(), out[0].data_ptr(), out[1].data_ptr(),
                       out[2].data_ptr(), out[3].data_ptr(), out[4].data_ptr())
-    status = lib.b4_kv_tables(args, stream.cuda_stream if stream is not None else _raw_stream(index))
-    if status:
-        check("b4_kv_tables", status)
+    _launch("b4_kv_tables", lib.b4_kv_tables, index, stream, args)
     return out
 
 
@@ -151,10 +162,8 @@ def kv_append(cache: KVCache, k, v, slots, stream=None) -> None:
     if (code is None or v.dtype is not k.dtype or k.shape != shape or v.shape != shape or k.get_device() != index
             or v.get_device() != index or ks[2] != 1 or vs[2] != 1):
         raise ValueError(f"k and v: {shape}, both fp16, bf16 or fp32, on cuda:{index}, columns contiguous")
-    status = load().b4_kv_append(cache._ref, k.data_ptr(), v.data_ptr(), code, ks[0], ks[1], vs[0], vs[1], slots.data_ptr(), n,
-                                 stream.cuda_stream if stream is not None else _raw_stream(index))
-    if status:
-        check("b4_kv_append", status)
+    _launch("b4_kv_append", load().b4_kv_append, index, stream, cache._ref, k.data_ptr(), v.data_ptr(), code, ks[0], ks[1], vs[0],
+            vs[1], slots.data_ptr(), n)
 
 
 def kv_read(cache: KVCache, slots, k=None, v=None, stream=None):
@@ -167,10 +176,7 @@ def kv_read(cache: KVCache, slots, k=None, v=None, stream=None):
     for x in (k, v):
         if x.shape != shape or x.dtype is not _float32 or x.get_device() != index or not x.is_contiguous():
             raise ValueError(f"k and v: contiguous fp32 {shape} on cuda:{index}")
-    status = load().b4_kv_read(cache._ref, slots.data_ptr(), n, k.data_ptr(), v.data_ptr(),
-                               stream.cuda_stream if stream is not None else _raw_stream(index))
-    if status:
-        check("b4_kv_read", status)
+    _launch("b4_kv_read", load().b4_kv_read, index, stream, cache._ref, slots.data_ptr(), n, k.data_ptr(), v.data_ptr())
     return k, v
 
 
@@ -232,15 +238,13 @@ def _attn(cache, q, tables, ctx_len, q_starts, max_q, scale, window, causal, out
                       code, window, 0 if causal else KV_FULL, dim ** -0.5 if scale is None else scale), out
 
 
-def _attn_bytes(cache, args):
-    n = ctypes.c_size_t(0)
-    check("b4_kv_attention_workspace", load().b4_kv_attention_workspace(cache._ref, args, ctypes.byref(n)))
-    return n.value
-
-
 def kv_attention_workspace(cache: KVCache, q, tables, ctx_len, q_starts, max_q: int) -> int:
     """Bytes of workspace that kv_attention needs for such a call (b4_kv_attention_workspace)."""
-    return _attn_bytes(cache, _attn(cache, q, tables, ctx_len, q_starts, max_q, None, 0, True, q, None)[0])
+    n = ctypes.c_size_t(0)
+    args, _ = _attn(cache, q, tables, ctx_len, q_starts, max_q, None, 0, True, q, None)
+    with _torch.cuda.device(cache.index):      # whose SMs are counted
+        check("b4_kv_attention_workspace", load().b4_kv_attention_workspace(cache._ref, args, ctypes.byref(n)))
+    return n.value
 
 
 def kv_attention(cache: KVCache, q, tables, ctx_len, q_starts, max_q: int, scale: float | None = None, window: int = 0,
@@ -256,8 +260,5 @@ def kv_attention(cache: KVCache, q, tables, ctx_len, q_starts, max_q: int, scale
     args, out = _attn(cache, q, tables, ctx_len, q_starts, max_q, scale, window, causal, out, lse)
     if ws is None:
         ws = _workspace(cache.index, stream)
-    status = load().b4_kv_attention(cache._ref, args, ws.data_ptr(), ws.numel(),
-                                    stream.cuda_stream if stream is not None else _raw_stream(cache.index))
-    if status:
-        check("b4_kv_attention", status)
+    _launch("b4_kv_attention", load().b4_kv_attention, cache.index, stream, cache._ref, args, ws.data_ptr(), ws.numel())
     return out
