@@ -30,14 +30,14 @@ _STEP = struct.Struct("@5i4xq10P")
 _ATTN = struct.Struct("@6P5q8if4x")
 assert _STEP.size == ctypes.sizeof(KvStep) and _ATTN.size == ctypes.sizeof(KvAttn)
 
-_torch = _int32 = _float32 = _raw_stream = _device = _codes = None
+_torch = _int32 = _float32 = _uint8 = _raw_stream = _device = _codes = None
 
 
 def _load():
     """torch's names and the library, once."""
-    global _torch, _int32, _float32, _raw_stream, _device, _codes
+    global _torch, _int32, _float32, _uint8, _raw_stream, _device, _codes
     import torch
-    _torch, _int32, _float32 = torch, torch.int32, torch.float32
+    _torch, _int32, _float32, _uint8 = torch, torch.int32, torch.float32, torch.uint8
     _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
         lambda index: torch.cuda.current_stream(index).cuda_stream)
     _device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
@@ -260,5 +260,7 @@ def kv_attention(cache: KVCache, q, tables, ctx_len, q_starts, max_q: int, scale
     args, out = _attn(cache, q, tables, ctx_len, q_starts, max_q, scale, window, causal, out, lse)
     if ws is None:
         ws = _workspace(cache.index, stream)
+    elif ws.dtype is not _uint8 or ws.get_device() != cache.index or not ws.is_contiguous():
+        raise ValueError(f"ws: a contiguous uint8 tensor on cuda:{cache.index}")
     _launch("b4_kv_attention", load().b4_kv_attention, cache.index, stream, cache._ref, args, ws.data_ptr(), ws.numel())
     return out

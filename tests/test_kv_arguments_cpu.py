@@ -106,3 +106,13 @@ def test_launched_on_the_tensors_device(monkeypatch, index, current):
     assert lib.seen[:4] == [(n, index, 100 + index) for n in names]
     assert lib.seen[4][:2] == ("b4_kv_attention_workspace", index)
     assert lib.current == current
+
+
+@pytest.mark.parametrize("bad", [dict(index=-1), dict(index=1), dict(dtype=torch.float32), dict(stride=(2,))])
+def test_workspaces_refused(monkeypatch, bad):
+    """Of the host, of another device, or counted in something else than bytes."""
+    lib = Library(monkeypatch, 0)
+    q = Fake((8, 4, 64), torch.float16)
+    with pytest.raises(ValueError):
+        kv.kv_attention(fake_cache(0), q, Fake((3, 5)), Fake((3,)), Fake((4,)), 4, out=q, ws=Fake((1 << 20,), **{"dtype": torch.uint8, **bad}))
+    assert not lib.seen
