@@ -16,7 +16,7 @@ class Fake:
     def __init__(self, shape, dtype=INT, stride=None, index=0, at=1 << 20):
         self.shape, self.dtype, self.index, self.at = torch.Size(shape), dtype, index, at
         self.strides = tuple(stride) if stride else tuple(math.prod(shape[i + 1:]) for i in range(len(shape)))
-        self.device, self.is_cuda = torch.device("cuda", index), True
+        self.device, self.is_cuda = torch.device("cuda", index) if index >= 0 else torch.device("cpu"), index >= 0
 
     def get_device(self):
         return self.index
