@@ -512,7 +512,8 @@ int b4_kv_read(const b4_kv_cache* cache, const int32_t* slots, int n_tokens, flo
  * kv head h / (heads / kv_heads).  Request r's queries are rows q_starts[r] ..
  * q_starts[r + 1] of q, the last of its ctx_len[r] tokens: query i of n sees the
  * keys below ctx - n + i + 1 (all ctx with B4_KV_FULL), and with window > 0 only
- * the last `window` of those.  A query that sees no key gets zeros (lse -inf).
+ * the last `window` of those.  Keys past table_width pages are masked, the queries'
+ * places among ctx stay.  A query that sees no key gets zeros (lse -inf).
  * q, out: dtype fp16 or bf16 [total_q][heads][head_dim], strides in elements,
  * columns contiguous, rows 16-byte aligned.  lse (optional): fp32
  * [total_q][heads], the natural logarithm of the sum of exp(scores).

@@ -19,21 +19,24 @@ struct AttnParams {
 
 constexpr int kChunk = 32;  // tokens that a warp takes at a time: one page of 32, two of 16, half of one of 64
 
-// What a launch needs of request r: its queries' first row and number, its tokens
-// (those that the table can hold), and the chunks that any of its queries sees.
+// What a launch needs of request r: its queries' first row and number, its tokens,
+// which place the queries, and the chunks that any of its queries sees.
 struct AttnReq {
     int q0, n, ctx, chunk0, chunks;
 };
+
+// The tokens that the table can hold: whole pages, so that those past it are masked as missing pages are.
+__device__ __forceinline__ int attn_held(const AttnParams& p, int ctx) { return min(ctx, p.a.table_width * p.l.page_size); }
 
 __device__ __forceinline__ int attn_first_chunk(const b4_kv_attn& a, int ctx, int n)
 {
     return a.window > 0 ? max(0, ctx - n + 1 - a.window) / kChunk : 0;
 }
 
-__device__ __forceinline__ AttnReq attn_extent(const b4_kv_attn& a, int q0, int n, int ctx)
+__device__ __forceinline__ AttnReq attn_extent(const AttnParams& p, int q0, int n, int ctx)
 {
-    AttnReq q = {q0, n, ctx, attn_first_chunk(a, ctx, n), 1};
-    q.chunks = max(1, (ctx + kChunk - 1) / kChunk - q.chunk0);      // one even where nothing is seen: zeros are written
+    AttnReq q = {q0, n, ctx, attn_first_chunk(p.a, ctx, n), 1};
+    q.chunks = max(1, (attn_held(p, ctx) + kChunk - 1) / kChunk - q.chunk0);      // one even where nothing is seen: zeros are written
     return q;
 }
 
@@ -42,7 +45,7 @@ __device__ __forceinline__ AttnReq attn_request(const AttnParams& p, int r)
     const b4_kv_attn& a = p.a;
     const int q0 = __ldg(a.q_starts + r), q1 = __ldg(a.q_starts + r + 1), ctx = __ldg(a.ctx_len + r);
     const int from = max(0, min(q0, a.total_q));
-    return attn_extent(a, from, max(0, min(q1, a.total_q) - from), max(0, min(ctx, a.table_width * p.l.page_size)));
+    return attn_extent(p, from, max(0, min(q1, a.total_q) - from), max(0, ctx));
 }
 
 __device__ __forceinline__ float fast_exp2(float x)

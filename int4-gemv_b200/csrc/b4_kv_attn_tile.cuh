@@ -225,7 +225,7 @@ __device__ __forceinline__ void tile_blocks(const AttnParams& p, int n, int ctx,
 {
     const unsigned g = p.group;
     const int rows = n * p.group, t0 = (int)((unsigned)(tile * kTileRows) / g), t1 = (int)((unsigned)(min((tile + 1) * kTileRows, rows) - 1) / g);
-    const int end = p.a.flags & B4_KV_FULL ? ctx : max(0, min(ctx, ctx - n + t1 + 1));
+    const int held = attn_held(p, ctx), end = p.a.flags & B4_KV_FULL ? held : max(0, min(held, ctx - n + t1 + 1));
     const int begin = p.a.window > 0 ? max(0, ctx - n + t0 + 1 - p.a.window) : 0;
     b0 = begin / kTileKeys;
     b1 = max(b0 + 1, (end + kTileKeys - 1) / kTileKeys);
@@ -545,7 +545,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attn_tile_kernel(const Att
         bool ok = true;
         auto page_id = [&](int block) {
             const int token = block * kTileKeys + t;
-            return block < s.blk1 && token < s.ctx ? __ldg(a.tables + (long long)s.r * a.table_stride + (token >> p.l.page_shift)) : -1;
+            return block < s.blk1 && token < attn_held(p, s.ctx) ? __ldg(a.tables + (long long)s.r * a.table_stride + (token >> p.l.page_shift)) : -1;
         };
         auto load = [&](int page, Codes& c) {
             c.there = (unsigned)page < (unsigned)p.l.n_pages;

@@ -148,7 +148,7 @@ __global__ void __launch_bounds__(WarpCfg<FMT, D, NT, PT>::kThreads, 1) kv_attn_
     auto request = [&](int r) {                // from shared memory where all fit there
         if (per > 1) return attn_request(p, r);
         const int4 x = cached[r];
-        return attn_extent(a, x.x, x.y, x.z);
+        return attn_extent(p, x.x, x.y, x.z);
     };
     const long long total = scan[kScan];
     if (total == 0) return;
@@ -488,7 +488,7 @@ __global__ void __launch_bounds__(WarpCfg<FMT, D, NT, PT>::kThreads, 1) kv_attn_
             const uint8_t* blocks = p.blocks + u.head * p.l.block;
             const long long page_bytes = p.l.kv_heads * p.l.block;
             int base = (q.chunk0 + first) * kChunk >> p.l.page_shift, next = q.chunk0 + first, queue = 0;
-            auto load_ids = [&](int page) { return (long long)page << p.l.page_shift < q.ctx ? __ldg(row + page) : -1; };
+            auto load_ids = [&](int page) { return page < a.table_width && (long long)page << p.l.page_shift < q.ctx ? __ldg(row + page) : -1; };
             int ids = load_ids(base + lane), more = load_ids(base + 32 + lane);
             auto issue = [&]() {               // the next chunk, if any, into stage `feed`
                 int there = 0;
