@@ -618,8 +618,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attn_tile_kernel(const Att
             const float scale = !seen ? 0.0f : FMT == B4_KV_INT4 ? __half2float(__ushort_as_half((unsigned short)now.scale)) : __uint_as_float(now.scale);
             if (half) {
                 if (blk == s.blk0) vexp = -126;
-                const float v = fminf(scale, 3.4028235e38f);
-                const unsigned bits = __reduce_max_sync(0xffffffffu, v < 3.4028235e38f ? __float_as_uint(fabsf(v)) : 0u);
+                const unsigned bits = __reduce_max_sync(0xffffffffu, scale < 3.4028235e38f ? __float_as_uint(fabsf(scale)) : 0u);
                 if (lane == 0) {
                     value_top[b & 1][warp & 1] = __uint_as_float(bits);
                     mbar_arrive(&tops);
@@ -629,7 +628,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attn_tile_kernel(const Att
                 if (!(ok = warp_wait(&tops, b & 1, &dead))) break;
                 const float top = fmaxf(value_top[b & 1][0], value_top[b & 1][1]);
                 vexp = max(vexp, min((int)(__float_as_uint(top) >> 23) - 126, 126));
-                value_scale[stage][t] = v * pow2(-vexp);
+                value_scale[stage][t] = fminf(scale * pow2(-vexp), 3.4028235e38f);      // finite, so that a weight of 0 makes 0 of it
                 if (t == 0) value_exp[stage] = vexp;
             } else {
                 key_scale[stage][t] = scale;

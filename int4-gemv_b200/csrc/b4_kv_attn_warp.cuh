@@ -346,8 +346,6 @@ __global__ void __launch_bounds__(WarpCfg<FMT, D, NT, PT>::kThreads, 1) kv_attn_
                     top[nt][j] = fmaxf(fmaxf(s[0][nt][j], s[0][nt][j + 2]), fmaxf(s[1][nt][j], s[1][nt][j + 2]));
                     moved |= top[nt][j] * qf[nt][j] > mx[nt][j] + 8.0f;
                 }
-            // finite, so that a weight of 0 makes 0 of it
-            vs = fminf(vs, 3.4028235e38f);
             const unsigned vbits = __reduce_max_sync(0xffffffffu, vs < 3.4028235e38f ? __float_as_uint(fabsf(vs)) : 0u);
             const int ve = max(vexp, min((int)(vbits >> 23) - 126, 126));
             if (__any_sync(0xffffffffu, moved) || ve != vexp) {
@@ -372,7 +370,7 @@ __global__ void __launch_bounds__(WarpCfg<FMT, D, NT, PT>::kThreads, 1) kv_attn_
                         for (int j = 0; j < 4; ++j) o[nt][mt][j] *= keep[j & 1];
                 }
             }
-            vs *= pow2(-vexp);
+            vs = fminf(vs * pow2(-vexp), 3.4028235e38f);           // finite, so that a weight of 0 makes 0 of it
             // weights as the right operand: tokens along k, a query a lane's row
             uint32_t pb[2][NT][2];
 #pragma unroll
