@@ -100,6 +100,11 @@ __device__ __forceinline__ int count_in(int* at)
 // A maximum that no score has set yet: finite, so that differences with it are.
 constexpr float kNoMax = -1e30f;
 
+// A weight times a value scale goes to fp16 relative to the row's running maximum, which weights pass by 2^8 at most, and to
+// 2^e, the least power above the value scales so far (kNoExp: none yet), times 2^kLift: below 2^15, so that fp16 holds its
+// 11 bits down to 2^-21 of the largest weight times 2^e, and 2^-32 of it below that.
+constexpr int kLift = 7, kNoExp = kLift - 126;
+
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 // The NF4 levels as fp16 operands.  fp16 has 11 bits, the levels 24: rounded as

@@ -541,7 +541,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attn_tile_kernel(const Att
             bool there;
         };
         TileSeg s = {};
-        int k = -1, blk = 0, vexp = -126, see_begin = 0, see_end = 0;
+        int k = -1, blk = 0, vexp = kNoExp, see_begin = 0, see_end = 0;
         bool ok = true;
         auto page_id = [&](int block) {
             const int token = block * kTileKeys + t;
@@ -617,7 +617,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attn_tile_kernel(const Att
             const bool seen = now.there && token < see_end && token >= see_begin;
             const float scale = !seen ? 0.0f : FMT == B4_KV_INT4 ? __half2float(__ushort_as_half((unsigned short)now.scale)) : __uint_as_float(now.scale);
             if (half) {
-                if (blk == s.blk0) vexp = -126;
+                if (blk == s.blk0) vexp = kNoExp;
                 const unsigned bits = __reduce_max_sync(0xffffffffu, scale < 3.4028235e38f ? __float_as_uint(fabsf(scale)) : 0u);
                 if (lane == 0) {
                     value_top[b & 1][warp & 1] = __uint_as_float(bits);
@@ -627,8 +627,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attn_tile_kernel(const Att
                 write(values_at + stage * C::kBlock + row_at, now.v);          // while the other warp's maximum comes
                 if (!(ok = warp_wait(&tops, b & 1, &dead))) break;
                 const float top = fmaxf(value_top[b & 1][0], value_top[b & 1][1]);
-                vexp = max(vexp, min((int)(__float_as_uint(top) >> 23) - 126, 126));
-                value_scale[stage][t] = fminf(scale * pow2(-vexp), 3.4028235e38f);      // finite, so that a weight of 0 makes 0 of it
+                vexp = max(vexp, (int)(__float_as_uint(top) >> 23) - 126);
+                value_scale[stage][t] = fminf(scale * pow2(kLift - vexp), 3.4028235e38f);    // finite, so that a weight of 0 makes 0 of it
                 if (t == 0) value_exp[stage] = vexp;
             } else {
                 key_scale[stage][t] = scale;
@@ -762,7 +762,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attn_tile_kernel(const Att
             }
             const float qf = fmaxf(factor * (fabsf(a.scale) * kLog2e) * (FMT == B4_KV_NF4 ? 1.0f / kNf4Even : 1.0f), 1e-30f);
             float m = kNoMax, l = 0.0f;
-            int vexp = -126;
+            int vexp = kNoExp;
             bool any = false;                  // whether O holds something
 #pragma unroll 1
             for (int i = two ? 0 : x; i < blocks && ok; i += two ? 1 : 2, ++cs) {
@@ -855,7 +855,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attn_tile_kernel(const Att
             if (!s.end) factor = put(s);
 
             // ---- the segment's rows, or a piece of them: a row a thread; one tile of rows: half a row's columns, of both streams ----
-            const float vup = any ? pow2(vexp) * (FMT == B4_KV_NF4 ? 1.0f / kNf4Even : 1.0f) : 0.0f;
+            const float vup = any ? pow2(vexp - kLift) * (FMT == B4_KV_NF4 ? 1.0f / kNf4Even : 1.0f) : 0.0f;
             float wa = vup, wb = 0.0f;
             if (!two) {
                 stream_max[x][t] = m;

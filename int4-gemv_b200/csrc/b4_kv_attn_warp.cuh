@@ -15,9 +15,10 @@
 // only as far as the codes are spread as kNf4Even takes them).
 // Softmax's maximum and sum run along the tokens, in fp32, private to a warp;
 // the maximum moves only when a score passes it by 2^8, which the weights'
-// range allows.  P goes to fp16 (its rounding is of the size of the output's own),
-// relative to that maximum and to a running power of two that bounds the value
-// scales, so small scales lose nothing.
+// range allows.  P times the value scale goes to fp16 (its rounding is of the size of
+// the output's own), relative to that maximum and to a running power of two that
+// bounds the value scales (kLift): a token whose value scale is 2^20 below the largest
+// one keeps its 11 bits if its weight is the largest, so only what hardly counts loses bits.
 //
 // Split.  The (request, kv head, column tile, 32-token chunk) units of the whole
 // call form one sequence; every CTA gets an equal run of it, every warp of a CTA
@@ -261,7 +262,7 @@ __global__ void __launch_bounds__(WarpCfg<FMT, D, NT, PT>::kThreads, 1) kv_attn_
 #pragma unroll
                     for (int j = 0; j < 4; ++j) o[nt][mt][j] = 0.0f;
             }
-            vexp = -126;
+            vexp = kNoExp;
         };
 
         // 32 tokens; `masked` where some column does not see all of them
@@ -347,7 +348,7 @@ __global__ void __launch_bounds__(WarpCfg<FMT, D, NT, PT>::kThreads, 1) kv_attn_
                     moved |= top[nt][j] * qf[nt][j] > mx[nt][j] + 8.0f;
                 }
             const unsigned vbits = __reduce_max_sync(0xffffffffu, vs < 3.4028235e38f ? __float_as_uint(fabsf(vs)) : 0u);
-            const int ve = max(vexp, min((int)(vbits >> 23) - 126, 126));
+            const int ve = max(vexp, (int)(vbits >> 23) - 126);
             if (__any_sync(0xffffffffu, moved) || ve != vexp) {
                 const float vkeep = pow2(max(vexp - ve, -126));
                 vexp = ve;
@@ -370,7 +371,7 @@ __global__ void __launch_bounds__(WarpCfg<FMT, D, NT, PT>::kThreads, 1) kv_attn_
                         for (int j = 0; j < 4; ++j) o[nt][mt][j] *= keep[j & 1];
                 }
             }
-            vs = fminf(vs * pow2(-vexp), 3.4028235e38f);           // finite, so that a weight of 0 makes 0 of it
+            vs = fminf(vs * pow2(kLift - vexp), 3.4028235e38f);   // finite, so that a weight of 0 makes 0 of it
             // weights as the right operand: tokens along k, a query a lane's row
             uint32_t pb[2][NT][2];
 #pragma unroll
@@ -544,7 +545,7 @@ __global__ void __launch_bounds__(WarpCfg<FMT, D, NT, PT>::kThreads, 1) kv_attn_
             }
 
             // ---- the end of a segment, or of the run ----
-            const float vup = pow2(vexp) * (FMT == B4_KV_NF4 ? 1.0f / kUp : 1.0f);
+            const float vup = pow2(vexp - kLift) * (FMT == B4_KV_NF4 ? 1.0f / kUp : 1.0f);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
