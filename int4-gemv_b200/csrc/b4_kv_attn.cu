@@ -111,6 +111,7 @@ int attn_params(const b4_kv_cache* cache, const b4_kv_attn* a, AttnParams* p)
     if (a->table_stride < a->table_width || (long long)a->table_width * p->l.page_size > 0x7fffffffLL) return cudaErrorInvalidValue;
     p->blocks = static_cast<const uint8_t*>(cache->blocks);
     p->a = *a;
+    p->a.window = std::min(a->window, INT_MAX - a->total_q);       // a query's place, ctx - n + i + 1 > -total_q, less it fits an int
     p->group = a->heads / p->l.kv_heads;
     return cudaSuccess;
 }
