@@ -519,7 +519,7 @@ int b4_kv_read(const b4_kv_cache* cache, const int32_t* slots, int n_tokens, flo
  * [total_q][heads], the natural logarithm of the sum of exp(scores).
  * max_q: the most queries of one request (chooses the kernels; requests with
  * more are computed all the same).  heads / kv_heads <= 64,
- * total_q * heads / kv_heads < 2^31.
+ * total_q * heads / kv_heads < 2^31, table_width * page_size <= 2^31 - 64.
  * ws: b4_kv_attention_workspace bytes of device memory, 16-byte aligned,
  * ZERO-FILLED before its first use; calls leave ready for the next what must be
  * zero.  Not shared with b4_gemv_ws, nor by calls that may run at the same time. */

@@ -108,7 +108,8 @@ int attn_params(const b4_kv_cache* cache, const b4_kv_attn* a, AttnParams* p)
     if ((long long)a->total_q * (a->heads / p->l.kv_heads) > 0x7fffffffLL) return cudaErrorInvalidValue;
     if (a->dtype != B4_DTYPE_F16 && a->dtype != B4_DTYPE_BF16) return cudaErrorInvalidValue;
     if (a->flags & ~B4_KV_FULL || (a->flags & B4_KV_FULL && a->window > 0) || !std::isfinite(a->scale)) return cudaErrorInvalidValue;
-    if (a->table_stride < a->table_width || (long long)a->table_width * p->l.page_size > 0x7fffffffLL) return cudaErrorInvalidValue;
+    // the kernels count up to a block of 64 keys past a request's last
+    if (a->table_stride < a->table_width || (long long)a->table_width * p->l.page_size > 0x80000000LL - 64) return cudaErrorInvalidValue;
     p->blocks = static_cast<const uint8_t*>(cache->blocks);
     p->a = *a;
     p->a.window = std::min(a->window, INT_MAX - a->total_q);       // a query's place, ctx - n + i + 1 > -total_q, less it fits an int

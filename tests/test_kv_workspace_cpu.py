@@ -21,3 +21,13 @@ def test_most_serves_every_call(head_dim, group):
                         status = b4gemv.load().b4_kv_attention_workspace(ctypes.byref(cache), ctypes.byref(a), ctypes.byref(n))
                         if total * group <= 0x7fffffff:
                             assert status == 0 and 0 < n.value <= most
+
+
+@pytest.mark.parametrize("page", [16, 32, 64])
+def test_tables_of_the_most_keys(page):
+    """2^31 - 64 keys a request at most: the kernels' counts of keys, rounded up to a block, stay in 32 bits."""
+    n = ctypes.c_size_t(0)
+    cache = _lib.KvCache(4096, 0, 10, page, 2, 128)
+    for width, status in (((2 ** 31 - 64) // page, 0), ((2 ** 31 - 64) // page + 1, 1)):
+        a = _lib.KvAttn(n_req=1, total_q=1, max_q=1, heads=2, table_width=width, table_stride=width)
+        assert b4gemv.load().b4_kv_attention_workspace(ctypes.byref(cache), ctypes.byref(a), ctypes.byref(n)) == status
