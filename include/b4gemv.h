@@ -476,8 +476,8 @@ int b4_kv_block_bytes(int fmt, int page_size, int head_dim, size_t* bytes);
  * and the pages that were missing.  A missing page's entry and slots are -1, and
  * so are the slots past table_width pages; b4_kv_append skips those and
  * b4_kv_attention counts such tokens as masked.  Lengths sum to less than 2^31.
- * table_stride in entries; free_state_out must not overlap free_state, nor the
- * other outputs an input.  n_req <= B4_KV_MAX_REQUESTS. */
+ * table_stride in entries.  No output may overlap an input or another output
+ * (refused: other CTAs may still read what the first one overwrites).  n_req <= B4_KV_MAX_REQUESTS. */
 #define B4_KV_MAX_REQUESTS 16384
 typedef struct b4_kv_step {
     int n_req, page_size, table_width, ring_size, max_tokens;

@@ -129,7 +129,8 @@ def kv_tables(page_size: int, tables, cached, added, free_pages, free_state, max
     """b4_kv_tables: block tables (int32 [requests][width], updated in place),
     slots, positions, starts and lengths of one step.  free_pages is the ring
     of free pages, free_state its (place, pages left); the returned free_state is
-    the next step's.  out: buffers to reuse (free_state must be another one)."""
+    the next step's.  out: buffers to reuse; none of them may be one that the call
+    reads (the last step's ctx_len as `cached`, its free_state)."""
     lib = _lib()
     index, n = tables.get_device(), cached.numel()
     width, stride = _table(tables, index, n)

@@ -388,6 +388,42 @@ inline long long vector_blocks(long long n, int head_dim, int u)
 
 inline unsigned long long vector_magic(int kv_heads) { return ~0ULL / (2ULL * kv_heads) + 1; }
 
+struct Ints {
+    uintptr_t from, to;
+    Ints(const int32_t* at, long long n) : from(reinterpret_cast<uintptr_t>(at)), to(from + 4 * n) {}
+};
+
+inline bool overlap(const Ints& a, const Ints& b) { return a.from < b.to && b.from < a.to && a.from < a.to && b.from < b.to; }
+
+// whether a lies on entries of a step's tables
+inline bool on_tables(const Ints& a, const b4_kv_step* s)
+{
+    if (s->n_req == 0 || s->table_width == 0 || !overlap(a, Ints(s->tables, (s->n_req - 1) * s->table_stride + s->table_width))) return false;
+    const long long row = 4LL * s->table_width, stride = 4 * s->table_stride;
+    const long long from = (long long)(a.from - reinterpret_cast<uintptr_t>(s->tables)), to = from + (long long)(a.to - a.from);
+    const long long r = from < row ? 0 : (from - row) / stride + 1;        // the first row that ends after `from`
+    return r < s->n_req && r * stride < to;
+}
+
+// What a step writes lies apart from what it reads, and from what else it writes: every CTA reads the lengths and the
+// ring's place while the first one may have written its outputs.
+inline bool step_apart(const b4_kv_step* s)
+{
+    const Ints out[] = {{s->ctx_len, s->n_req}, {s->q_starts, s->n_req + 1LL}, {s->slots, s->max_tokens}, {s->positions, s->max_tokens},
+                        {s->free_state_out, 3}};
+    const Ints in[] = {{s->cached, s->n_req}, {s->added, s->n_req}, {s->free_pages, s->ring_size}, {s->free_state, 2}};
+    for (const Ints& o : out) {
+        if (on_tables(o, s)) return false;
+        for (const Ints& i : in)
+            if (overlap(o, i)) return false;
+        for (const Ints& p : out)
+            if (&p < &o && overlap(o, p)) return false;
+    }
+    for (const Ints& i : in)
+        if (on_tables(i, s)) return false;
+    return true;
+}
+
 template <typename T, int FMT, int D, int U>
 cudaError_t append_u(const AppendParams& p, bool vec, cudaStream_t st)
 {
@@ -441,7 +477,7 @@ int b4_kv_tables(const b4_kv_step* s, b4_stream_t stream)
     if (s->table_stride < s->table_width || !s->q_starts || !s->free_state || !s->free_state_out) return cudaErrorInvalidValue;
     if (s->n_req > 0 && (!s->cached || !s->added || !s->ctx_len || (s->table_width > 0 && !s->tables))) return cudaErrorInvalidValue;
     if ((s->ring_size > 0 && !s->free_pages) || (s->max_tokens > 0 && (!s->slots || !s->positions))) return cudaErrorInvalidValue;
-    if (s->free_state_out < s->free_state + 2 && s->free_state < s->free_state_out + 3) return cudaErrorInvalidValue;
+    if (!step_apart(s)) return cudaErrorInvalidValue;
     const size_t smem = 12 * (size_t)s->n_req;
     if (smem > 48 * 1024) {
         const cudaError_t e = cudaFuncSetAttribute(kv_tables_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 12 * B4_KV_MAX_REQUESTS);
