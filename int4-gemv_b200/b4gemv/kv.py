@@ -49,22 +49,10 @@ def _lib():
     return load() if _torch is not None else _load()
 
 
-def _launch(name, fn, index, stream, *args):
-    """fn(*args, stream) with device `index` current: the library launches, and counts its SMs, on the current device."""
-    handle = stream.cuda_stream if stream is not None else _raw_stream(index)
-    if _device() == index:
-        status = fn(*args, handle)
-    else:
-        with _torch.cuda.device(index):
-            status = fn(*args, handle)
-    if status:
-        check(name, status)
-
-
 def _ints(name, t, index, least):
     if t.dtype is not _int32 or t.get_device() != index or not t.is_contiguous():
         raise ValueError(f"{name}: a contiguous int32 tensor on cuda:{index}")
-    if t.numel() < least:
+    if least and t.numel() < least:
         raise ValueError(f"{name}: {least} values at least, got {t.numel()}")
 
 
@@ -146,10 +134,15 @@ def kv_tables(page_size: int, tables, cached, added, free_pages, free_state, max
     else:
         for name, least in (("ctx_len", n), ("q_starts", n + 1), ("slots", max_tokens), ("positions", max_tokens), ("free_state", 3)):
             _ints(name, getattr(out, name), index, least)
+    if _device() != index:
+        with _torch.cuda.device(index):
+            return kv_tables(page_size, tables, cached, added, free_pages, free_state, max_tokens, out, stream)
     args = _STEP.pack(n, page_size, width, free_pages.numel(), max_tokens, stride, tables.data_ptr(), cached.data_ptr(),
                       added.data_ptr(), free_pages.data_ptr(), free_state.data_ptr(), out[0].data_ptr(), out[1].data_ptr(),
                       out[2].data_ptr(), out[3].data_ptr(), out[4].data_ptr())
-    _launch("b4_kv_tables", lib.b4_kv_tables, index, stream, args)
+    status = lib.b4_kv_tables(args, stream.cuda_stream if stream is not None else _raw_stream(index))
+    if status:
+        check("b4_kv_tables", status)
     return out
 
 
@@ -163,8 +156,13 @@ def kv_append(cache: KVCache, k, v, slots, stream=None) -> None:
     if (code is None or v.dtype is not k.dtype or k.shape != shape or v.shape != shape or k.get_device() != index
             or v.get_device() != index or ks[2] != 1 or vs[2] != 1):
         raise ValueError(f"k and v: {shape}, both fp16, bf16 or fp32, on cuda:{index}, columns contiguous")
-    _launch("b4_kv_append", load().b4_kv_append, index, stream, cache._ref, k.data_ptr(), v.data_ptr(), code, ks[0], ks[1], vs[0],
-            vs[1], slots.data_ptr(), n)
+    if _device() != index:                     # the library launches on the current device
+        with _torch.cuda.device(index):
+            return kv_append(cache, k, v, slots, stream)
+    status = load().b4_kv_append(cache._ref, k.data_ptr(), v.data_ptr(), code, ks[0], ks[1], vs[0], vs[1], slots.data_ptr(), n,
+                                 stream.cuda_stream if stream is not None else _raw_stream(index))
+    if status:
+        check("b4_kv_append", status)
 
 
 def kv_read(cache: KVCache, slots, k=None, v=None, stream=None):
@@ -177,7 +175,13 @@ def kv_read(cache: KVCache, slots, k=None, v=None, stream=None):
     for x in (k, v):
         if x.shape != shape or x.dtype is not _float32 or x.get_device() != index or not x.is_contiguous():
             raise ValueError(f"k and v: contiguous fp32 {shape} on cuda:{index}")
-    _launch("b4_kv_read", load().b4_kv_read, index, stream, cache._ref, slots.data_ptr(), n, k.data_ptr(), v.data_ptr())
+    if _device() != index:
+        with _torch.cuda.device(index):
+            return kv_read(cache, slots, k, v, stream)
+    status = load().b4_kv_read(cache._ref, slots.data_ptr(), n, k.data_ptr(), v.data_ptr(),
+                               stream.cuda_stream if stream is not None else _raw_stream(index))
+    if status:
+        check("b4_kv_read", status)
     return k, v
 
 
@@ -263,5 +267,11 @@ def kv_attention(cache: KVCache, q, tables, ctx_len, q_starts, max_q: int, scale
         ws = _workspace(cache.index, stream)
     elif ws.dtype is not _uint8 or ws.get_device() != cache.index or not ws.is_contiguous():
         raise ValueError(f"ws: a contiguous uint8 tensor on cuda:{cache.index}")
-    _launch("b4_kv_attention", load().b4_kv_attention, cache.index, stream, cache._ref, args, ws.data_ptr(), ws.numel())
+    if _device() != cache.index:
+        with _torch.cuda.device(cache.index):
+            return kv_attention(cache, q, tables, ctx_len, q_starts, max_q, scale, window, causal, out, lse, ws, stream)
+    status = load().b4_kv_attention(cache._ref, args, ws.data_ptr(), ws.numel(),
+                                    stream.cuda_stream if stream is not None else _raw_stream(cache.index))
+    if status:
+        check("b4_kv_attention", status)
     return out
