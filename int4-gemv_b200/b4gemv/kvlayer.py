@@ -58,16 +58,18 @@ class CachedAttention:
         return y
 
     def step(self, x, added):
-        """x fp16 [sum(added)][hidden], added: new tokens of each request; returns fp32 [sum(added)][hidden]."""
+        """x fp16 [sum(added)][hidden], added: new tokens of each request (0 or more); returns fp32 [sum(added)][hidden]."""
         import torch
         n, total = len(added), x.shape[0]
-        if total != sum(added) or n > self.cached.numel():
-            raise ValueError(f"x: {sum(added)} rows, {self.cached.numel()} requests at most")
+        if total != sum(added) or n > self.cached.numel() or min(added, default=0) < 0:
+            raise ValueError(f"x: {sum(added)} rows, {self.cached.numel()} requests at most, of 0 tokens or more")
         more = torch.tensor(list(added), dtype=torch.int32, device=x.device)
         step = kv_tables(self.cache.page_size, self.tables[:n], self.cached[:n], more, self.free, self.free_state, total)
-        q, k, v = (self._project(name, x).view(total, -1, self.dim) for name in "qkv")
+        q, k, v = (self._project(name, x).view(total, h, self.dim) for name, h in
+                   (("q", self.heads), ("k", self.kv_heads), ("v", self.kv_heads)))
         kv_append(self.cache, rotate(k, step.positions), v, step.slots)
-        out = kv_attention(self.cache, rotate(q, step.positions).half(), self.tables[:n], step.ctx_len, step.q_starts, max(added))
+        out = kv_attention(self.cache, rotate(q, step.positions).half(), self.tables[:n], step.ctx_len, step.q_starts,
+                           max(added, default=0))
         self.cached[:n] = step.ctx_len
         self.free_state = step.free_state
-        return self._project("o", out.view(total, -1))
+        return self._project("o", out.view(total, self.heads * self.dim))
