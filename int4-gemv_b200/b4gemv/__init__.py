@@ -153,6 +153,7 @@ def gemv(fmt: int, qw, scale, x, y=None, config: dict | None = None, stream=None
 
 _WS_SIZE = {}
 _WS = {}
+_WS_REPLACED = []
 
 
 def workspace_size(fmt: int, in_f: int, out_f: int, m: int = 1, config: dict | None = None, device=None) -> int:
@@ -178,7 +179,8 @@ def workspace_size(fmt: int, in_f: int, out_f: int, m: int = 1, config: dict | N
 
 def workspace(device, nbytes: int):
     """The package's workspace for b4_gemv_ws on `device`: one zero-filled
-    uint8 tensor per device, grown on demand (at least 1 MiB).  Every call
+    uint8 tensor per device, grown on demand (at least 1 MiB; a replaced one is
+    kept, since captured graphs and other streams hold its address).  Every call
     leaves it ready for the next (the x-pair table kernel's running counters
     in the first 256 bytes, the split path's counters zero after them).
     Calls on different streams
@@ -190,6 +192,8 @@ def workspace(device, nbytes: int):
     ws = _WS.get(idx)
     if ws is None or ws.numel() < nbytes:
         ws = torch.zeros(max(int(nbytes), 1 << 20), dtype=torch.uint8, device=f"cuda:{idx}")
+        if idx in _WS:
+            _WS_REPLACED.append(_WS[idx])
         _WS[idx] = ws
     return ws
 
