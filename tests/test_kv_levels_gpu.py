@@ -1,0 +1,51 @@
+"""NF4 values in fp16 outputs of few queries: both fp16 parts of a level count."""
+import numpy as np
+import pytest
+import torch
+
+import b4gemv
+import kv_ref as ref
+from test_kv_gpu import NF4
+
+pytestmark = pytest.mark.gpu
+N = 64                                         # tokens, alike in weight
+
+
+def cancelling(rng, columns):
+    """Codes [N][columns] of three levels a column that sum to nearly nothing, in an order of chance: the output is so small
+    that its own rounding hides nothing, while the levels' roundings, were they those of fp16 alone, leave 1.5e-5."""
+    lev = ref.NF4.astype(np.float64)
+    ups = [1.67766535282135, 1.6775788]        # factors that the levels may be rounded with
+    eps = [(np.float32(u) * ref.NF4).astype(np.float16).astype(np.float64) / np.float32(u) - lev for u in ups]
+    found = []
+    i, j = np.meshgrid(np.arange(1, N), np.arange(1, N), indexing="ij")
+    ok = i + j < N
+    counts = np.stack([i[ok], j[ok], N - i[ok] - j[ok]], 1)
+    for a in range(16):
+        for b in range(a + 1, 16):
+            for c in range(b + 1, 16):
+                mean = counts @ lev[[a, b, c]] / N
+                lost = np.minimum(*(np.abs(counts @ e[[a, b, c]]) / N for e in eps))
+                for n in counts[(np.abs(mean) < 1e-3) & (lost > 1.5e-5)]:
+                    found.append(np.repeat([a, b, c], n))
+    assert len(found) > 100
+    return np.stack([rng.permutation(found[k]) for k in rng.integers(len(found), size=columns)], 1).astype(np.uint8)
+
+
+@pytest.mark.parametrize("group", [1, 8, 16])
+@pytest.mark.parametrize("d,page", [(128, 64), (128, 16), (64, 32)])
+def test_levels_of_values(cuda, group, d, page):
+    rng = np.random.default_rng(d + page + group)
+    kvh, pages = 3, N // page
+    codes = rng.integers(0, 16, (2, pages, kvh, page, d)).astype(np.uint8)
+    v = np.stack([cancelling(rng, d) for _ in range(kvh)])                                  # [head][token][column]
+    codes[1] = v.reshape(kvh, pages, page, d).transpose(1, 0, 2, 3)
+    scales = np.ones((2, pages, kvh, page), np.float32)
+    cache = b4gemv.KVCache(torch.from_numpy(ref.pack_blocks(NF4, codes, scales)).to(cuda), NF4, page, d)
+    t = lambda x: torch.tensor(x, dtype=torch.int32, device=cuda)  # noqa: E731
+    q = torch.zeros((1, kvh * group, d), dtype=torch.float16, device=cuda)
+    got = b4gemv.kv_attention(cache, q, t([list(range(pages))]), t([N]), t([0, 1]), 1)[0].cpu().numpy().astype(np.float64)
+    want = np.repeat(ref.NF4.astype(np.float64)[v].mean(1), group, 0)
+    # a level in two parts is off by 2^-22; a product of 16 tokens adds to a sum of fewer than 32 levels, off by 2^-22 of it,
+    # and N / 8 of them make the sum of N: 2^-20; the output is rounded once
+    assert bool((np.abs(got - want) <= 2.0 ** -22 + 2.0 ** -20 + np.abs(want) * 2.0 ** -11).all())
