@@ -90,7 +90,7 @@ __global__ void __launch_bounds__(WarpCfg<FMT, D, NT, PT>::kThreads, 1) kv_attn_
 {
     using C = WarpCfg<FMT, D, NT, PT>;
     constexpr int kWarps = C::kWarps, kThreads = C::kThreads, kStages = C::kStages, kScan = C::kScan;
-    constexpr bool kLow = std::is_same<T, __half>::value;          // NF4 values in two parts
+    constexpr bool kLow = std::is_same<T, __half>::value;          // NF4 levels in two parts
     constexpr float kUp = kLow ? kNf4Least : kNf4Even;
     extern __shared__ __align__(1024) uint8_t attn_smem[];
     __shared__ WarpPiece pieces[kWarps][2];
@@ -296,6 +296,22 @@ __global__ void __launch_bounds__(WarpCfg<FMT, D, NT, PT>::kThreads, 1) kv_attn_
                     if (FMT == B4_KV_INT4) {
                         int4_word_to_half2(k0[i], x);
                         int4_word_to_half2(k1[i], y);
+                    } else if (kLow) {
+#pragma unroll
+                        for (int c = 0; c < 2; ++c) {
+                            uint2 e[2], f[2];
+#pragma unroll
+                            for (int b = 0; b < 2; ++b) {
+                                e[b] = lds64(__byte_perm(k0[i], t_val, 0x7604 | (2 * c + b) << 4));
+                                f[b] = lds64(__byte_perm(k1[i], t_val, 0x7604 | (2 * c + b) << 4));
+                            }
+#pragma unroll
+                            for (int nt = 0; nt < NT; ++nt) {
+                                mma_f16(s[st][nt], e[0].x, f[0].x, e[1].x, f[1].x, qb[nt][4 * i + 2 * c], qb[nt][4 * i + 2 * c + 1]);
+                                mma_f16(s[st][nt], e[0].y, f[0].y, e[1].y, f[1].y, qb[nt][4 * i + 2 * c], qb[nt][4 * i + 2 * c + 1]);
+                            }
+                        }
+                        continue;
                     } else {
 #pragma unroll
                         for (int b = 0; b < 4; ++b) {
