@@ -67,7 +67,7 @@ cudaError_t launch_warp(const AttnParams& p, void* ws, cudaStream_t st)
 template <typename T, int FMT, int D>
 cudaError_t launch_tile(const AttnParams& p, void* ws, cudaStream_t st)
 {
-    using C = TileCfg<FMT, D>;
+    using C = TileCfg<T, FMT, D>;
     auto fn = kv_attn_tile_kernel<T, FMT, D>;
     const cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
     if (e != cudaSuccess) return e;

@@ -60,13 +60,17 @@ constexpr int kTileRows = 256, kTileKeys = 64, kTileThreads = 512, kTileStages =
 // take 196 us with 2, 170 with 4, 177 with 6.
 constexpr int kSegUnits = 4;
 
-template <int FMT, int D>
+template <typename T, int FMT, int D>
 struct TileCfg {
     static constexpr int kRow = D / 2, kScale = FMT == B4_KV_INT4 ? 2 : 4;
     static constexpr int kOperand = 128 * D * 2;                   // bytes of 128 queries of D fp16: D / 64 parts of 128 x 128 bytes
     static constexpr int kBlock = kTileKeys * D * 2;               // of a block's keys or values: parts of 64 x 128 bytes
-    // NF4: pairs of levels by byte, 256 rows of 16 copies (2 lanes a copy), at shared address 16384, so that an OR makes
-    // a lookup's address; the operands follow it.  Without it they follow the static part.
+    // NF4 with fp16 queries: levels in two fp16 parts, each with its operands and products; half as many stages of twice the size
+    static constexpr int kParts = FMT == B4_KV_NF4 && std::is_same<T, __half>::value ? 2 : 1;
+    static constexpr int kStages = kTileStages / kParts, kStage = kParts * kBlock;
+    static constexpr float kUp = kParts == 2 ? kNf4Least : kNf4Even;
+    // NF4: pairs of levels by byte, 256 rows of 16 copies (2 lanes a copy), or of 8 copies of both parts, at shared address
+    // 16384, so that an OR makes a lookup's address; the operands follow it.  Without it they follow the static part.
     static constexpr int kTable = 16384, kStatic = 13312;
     static constexpr int kPiece = kTileRows * (D + 2);             // floats: output, maxima, sums
     static constexpr int kSmem = 2 * kOperand + 2 * kTileStages * kBlock + (FMT == B4_KV_NF4 ? 2 * kTable - kStatic : 1024);   // kStatic: less than the static part and the system's
@@ -234,7 +238,8 @@ __device__ __forceinline__ void tile_blocks(const AttnParams& p, int n, int ctx,
 template <typename T, int FMT, int D>
 __global__ void __launch_bounds__(kTileThreads, 1) kv_attn_tile_kernel(const AttnParams p, const TileWs ws)
 {
-    using C = TileCfg<FMT, D>;
+    using C = TileCfg<T, FMT, D>;
+    constexpr int kStages = C::kStages;
     extern __shared__ __align__(1024) uint8_t tile_smem[];
     __shared__ uint64_t seg_full[2], seg_empty[2], q_full[2], s_full[2][2], p_full[2][2], o_done[2][2], q_both, q_free, tops, team, drain[2];
     __shared__ uint64_t full[kTileStages], empty[kTileStages];
@@ -253,7 +258,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attn_tile_kernel(const Att
     const int tid = threadIdx.x, lane = tid & 31, warp_u = __shfl_sync(0xffffffffu, tid >> 5, 0), warp = warp_u;
     const b4_kv_attn& a = p.a;
     const uint32_t operands = FMT == B4_KV_NF4 ? 2 * C::kTable : (smem_addr(tile_smem) + 1023) & ~1023u;
-    const uint32_t keys_at = operands + 2 * C::kOperand, values_at = keys_at + kTileStages * C::kBlock;     // after Q of both tiles
+    const uint32_t keys_at = operands + 2 * C::kOperand, values_at = keys_at + kStages * C::kStage;     // after Q of both tiles
     if (FMT == B4_KV_NF4 && (smem_addr(tile_smem) > C::kTable || smem_addr(tile_smem) < C::kStatic)) {   // the static part is not as kSmem takes it
         if (tid == 0) atomicOr(&g_device_error, kErrMbarrierTimeout);
         return;
@@ -269,7 +274,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attn_tile_kernel(const Att
                 mbar_init(&o_done[i][j], 1);
             }
         }
-        for (int i = 0; i < kTileStages; ++i) {
+        for (int i = 0; i < kStages; ++i) {
             mbar_init(&full[i], 4);
             mbar_init(&empty[i], 2);
         }
@@ -287,8 +292,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attn_tile_kernel(const Att
     }
     if (FMT == B4_KV_NF4) {
         for (int i = tid; i < 256 * 4; i += kTileThreads) {
-            const uint32_t v = nf4_pair(i >> 2, kNf4Even);
-            asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(C::kTable + i * 16), "r"(v) : "memory");
+            const uint32_t v = nf4_pair(i >> 2, C::kUp), w = C::kParts == 2 ? nf4_pair_low(i >> 2, C::kUp) : v;
+            asm volatile("st.shared.v4.u32 [%0], {%1, %2, %1, %2};" ::"r"(C::kTable + i * 16), "r"(v), "r"(w) : "memory");
         }
     }
     fence_mbar_init();
@@ -460,8 +465,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attn_tile_kernel(const Att
                 // two tiles of rows: each takes every block; one: the tile's warp takes every other, and says so of the
                 // others once they are there (a block is left when both warps have left it)
                 const uint32_t desc_q = umma_desc(operands + (two ? x : 0) * C::kOperand, 16);
-                // a tile's next block's scores are asked for before its weights are waited for
-                const int ahead = two ? 1 : 2;
+                // a tile's next block's scores are asked for before its weights are waited for, as far as the stages reach
+                const int ahead = two || kStages == 2 ? 1 : 2;
                 bool queries = two || x == 0, add = false;
                 if (!two && x == 1) {                              // the first tile's queries
                     if (!(ok = warp_wait(&q_both, shared++ & 1, &dead))) break;
@@ -473,22 +478,24 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attn_tile_kernel(const Att
 #pragma unroll 1
                 for (int i = -ahead; i < blocks; ++i) {
                     const int sb = i + ahead;
-                    const bool taken = two || (i & 1) == x;        // and so is sb
+                    const bool taken = two || (i & 1) == x;
                     if (sb < blocks) {
-                        const int b = blocks_before + sb, stage = b & (kTileStages - 1), buf = cs & 1;
-                        if (!(ok = warp_wait(&full[stage], b / kTileStages & 1, &dead))) break;
-                        if (taken) {
+                        const int b = blocks_before + sb, stage = b & (kStages - 1), buf = cs & 1;
+                        if (!(ok = warp_wait(&full[stage], b / kStages & 1, &dead))) break;
+                        if (two || (sb & 1) == x) {
                             if (queries) {
                                 if (!(ok = warp_wait(&q_full[x], cq++ & 1, &dead))) break;
                                 queries = false;
                             }
                             tmem_after_sync();
                             if (elect_one()) {
-                                const uint32_t kd = desc_k + stage * (C::kBlock >> 4);
+                                const uint32_t kd = desc_k + stage * (C::kStage >> 4);
 #pragma unroll
-                                for (int j = 0; j < D / 16; ++j)
-                                    umma_ss(s_at + buf * 64, desc_q + (j >> 2) * (kPartQ >> 4) + (j & 3) * 2,
-                                            kd + (j >> 2) * (kPartB >> 4) + (j & 3) * 2, id_s, j > 0);
+                                for (int part = 0; part < C::kParts; ++part)
+#pragma unroll
+                                    for (int j = 0; j < D / 16; ++j)
+                                        umma_ss(s_at + buf * 64, desc_q + (j >> 2) * (kPartQ >> 4) + (j & 3) * 2,
+                                                kd + part * (C::kBlock >> 4) + (j >> 2) * (kPartB >> 4) + (j & 3) * 2, id_s, part > 0 || j > 0);
                                 umma_commit(&s_full[x][buf]);
                                 if (!two && x == 1 && sb + 2 >= blocks) umma_commit(&q_free);
                             }
@@ -497,7 +504,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attn_tile_kernel(const Att
                         }
                     }
                     if (i >= 0) {                                  // the block's operands are there since its scores
-                        const int stage = (blocks_before + i) & (kTileStages - 1), buf = cp & 1;
+                        const int stage = (blocks_before + i) & (kStages - 1), buf = cp & 1;
                         if (taken) {
                             if (!(ok = warp_wait(&p_full[x][buf], cp >> 1 & 1, &dead))) break;
                             ++cp;
@@ -505,9 +512,12 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attn_tile_kernel(const Att
                         tmem_after_sync();
                         if (elect_one()) {
                             if (taken) {
-                                const uint32_t pa = s_at + buf * 64, v = desc_v + stage * (C::kBlock >> 4);
+                                const uint32_t pa = s_at + buf * 64, v = desc_v + stage * (C::kStage >> 4);
 #pragma unroll
-                                for (int j = 0; j < kTileKeys / 16; ++j) umma_ts(o_at, pa + j * 8, v + j * (2048 >> 4), id_o, add || j > 0);
+                                for (int part = 0; part < C::kParts; ++part)
+#pragma unroll
+                                    for (int j = 0; j < kTileKeys / 16; ++j)
+                                        umma_ts(o_at, pa + j * 8, v + part * (C::kBlock >> 4) + j * (2048 >> 4), id_o, add || part > 0 || j > 0);
                                 umma_commit(&o_done[x][buf]);
                                 umma_commit(&empty[stage]);
                             } else {
@@ -567,9 +577,17 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attn_tile_kernel(const Att
             const uint32_t* w = reinterpret_cast<const uint32_t*>(raw);
 #pragma unroll
             for (int i = 0; i < W; ++i) {
-                uint32_t h[4];
+                uint32_t h[4], low[4];
                 if (FMT == B4_KV_INT4) {
                     int4_word_to_half2(w[i], h);
+                } else if (C::kParts == 2) {
+                    const uint32_t copy = C::kTable | (lane & 7) * 8;
+#pragma unroll
+                    for (int b = 0; b < 4; ++b) {
+                        const uint2 x = lds64((b ? w[i] >> (8 * b - 6) : w[i] << 6) & 0x3fc0u | copy);
+                        h[b] = x.x;
+                        low[b] = x.y;
+                    }
                 } else {
                     const uint32_t copy = C::kTable | (lane & 15) * 4;
                     h[0] = lds32((w[i] << 6 & 0x3fc0u) | copy);
@@ -580,6 +598,10 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attn_tile_kernel(const Att
                 asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(to + (((chunk0 + i) << 4) ^ swizzle)), "r"(h[0]), "r"(h[1]), "r"(h[2]),
                              "r"(h[3])
                              : "memory");
+                if (C::kParts == 2)
+                    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(to + C::kBlock + (((chunk0 + i) << 4) ^ swizzle)), "r"(low[0]),
+                                 "r"(low[1]), "r"(low[2]), "r"(low[3])
+                                 : "memory");
             }
         };
         // the next segment, or the end of the run
@@ -606,12 +628,12 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attn_tile_kernel(const Att
         }
 #pragma unroll 1
         for (int b = 0; more; ++b) {
-            const int stage = b & (kTileStages - 1);
+            const int stage = b & (kStages - 1);
             if (blk + 1 < s.blk1) {
                 load(id_next, next);
                 id_next = page_id(blk + 2);
             }
-            if (b >= kTileStages && !(ok = warp_wait(&empty[stage], (b / kTileStages + 1) & 1, &dead))) break;
+            if (b >= kStages && !(ok = warp_wait(&empty[stage], (b / kStages + 1) & 1, &dead))) break;
             // scales: those of tokens that no row sees are 0, the values' relative to a running power of two
             const int token = blk * kTileKeys + t;
             const bool seen = now.there && token < see_end && token >= see_begin;
@@ -624,7 +646,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attn_tile_kernel(const Att
                     mbar_arrive(&tops);
                 }
                 __syncwarp();
-                write(values_at + stage * C::kBlock + row_at, now.v);          // while the other warp's maximum comes
+                write(values_at + stage * C::kStage + row_at, now.v);          // while the other warp's maximum comes
                 if (!(ok = warp_wait(&tops, b & 1, &dead))) break;
                 const float top = fmaxf(value_top[b & 1][0], value_top[b & 1][1]);
                 vexp = max(vexp, (int)(__float_as_uint(top) >> 23) - 126);
@@ -635,9 +657,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attn_tile_kernel(const Att
                 // tokens that are not there lie in whole pages of 16 at least: two bits a warp
                 const unsigned pages = __ballot_sync(0xffffffffu, now.there);
                 if (lane == 0) reinterpret_cast<uint8_t*>(&block_pages[stage])[warp & 1] = (uint8_t)((pages & 1) | (pages >> 16 & 1) << 1);
-                write(values_at + stage * C::kBlock + row_at, now.v);
+                write(values_at + stage * C::kStage + row_at, now.v);
             }
-            write(keys_at + stage * C::kBlock + row_at, now.k);
+            write(keys_at + stage * C::kStage + row_at, now.k);
             fence_proxy_async();
             __syncwarp();
             if (lane == 0) mbar_arrive(&full[stage]);
@@ -760,16 +782,16 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attn_tile_kernel(const Att
                 if (!(ok = warp_wait(&q_both, shared & 1, &dead))) break;
                 factor = q_factor[shared & 1][t];
             }
-            const float qf = fmaxf(factor * (fabsf(a.scale) * kLog2e) * (FMT == B4_KV_NF4 ? 1.0f / kNf4Even : 1.0f), 1e-30f);
+            const float qf = fmaxf(factor * (fabsf(a.scale) * kLog2e) * (FMT == B4_KV_NF4 ? 1.0f / C::kUp : 1.0f), 1e-30f);
             float m = kNoMax, l = 0.0f;
             int vexp = kNoExp;
             bool any = false;                  // whether O holds something
 #pragma unroll 1
             for (int i = two ? 0 : x; i < blocks && ok; i += two ? 1 : 2, ++cs) {
-                const int stage = (ring0 + i) & (kTileStages - 1), buf = cs & 1;
+                const int stage = (ring0 + i) & (kStages - 1), buf = cs & 1;
                 if (!(ok = warp_wait(&s_full[x][buf], cs >> 1 & 1, &dead))) break;
                 // the scales' writers; after the scores, so that the phase asked for is the last one done
-                if (!(ok = warp_wait(&full[stage], (ring0 + i) / kTileStages & 1, &dead))) break;
+                if (!(ok = warp_wait(&full[stage], (ring0 + i) / kStages & 1, &dead))) break;
                 tmem_after_sync();
                 const int key0 = (s.blk0 + i) * kTileKeys, pages = block_pages[stage] & 0xffff, ve = value_exp[stage];
                 const float4* ks = reinterpret_cast<const float4*>(key_scale[stage]);
@@ -855,7 +877,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attn_tile_kernel(const Att
             if (!s.end) factor = put(s);
 
             // ---- the segment's rows, or a piece of them: a row a thread; one tile of rows: half a row's columns, of both streams ----
-            const float vup = any ? pow2(vexp - kLift) * (FMT == B4_KV_NF4 ? 1.0f / kNf4Even : 1.0f) : 0.0f;
+            const float vup = any ? pow2(vexp - kLift) * (FMT == B4_KV_NF4 ? 1.0f / C::kUp : 1.0f) : 0.0f;
             float wa = vup, wb = 0.0f;
             if (!two) {
                 stream_max[x][t] = m;

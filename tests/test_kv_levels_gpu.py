@@ -1,4 +1,4 @@
-"""NF4 values in fp16 outputs of few queries: both fp16 parts of a level count."""
+"""NF4 with fp16 queries: both fp16 parts of a level count, in keys and in values, for few queries and for many."""
 import numpy as np
 import pytest
 import torch
@@ -32,9 +32,9 @@ def cancelling(rng, columns):
     return np.stack([rng.permutation(found[k]) for k in rng.integers(len(found), size=columns)], 1).astype(np.uint8)
 
 
-@pytest.mark.parametrize("group", [1, 8, 16])
+@pytest.mark.parametrize("group,new", [(1, 1), (8, 1), (16, 1), (8, 20), (4, 100)])
 @pytest.mark.parametrize("d,page", [(128, 64), (128, 16), (64, 32)])
-def test_levels_of_values(cuda, group, d, page):
+def test_levels_of_values(cuda, group, new, d, page):
     rng = np.random.default_rng(d + page + group)
     kvh, pages = 3, N // page
     codes = rng.integers(0, 16, (2, pages, kvh, page, d)).astype(np.uint8)
@@ -43,9 +43,28 @@ def test_levels_of_values(cuda, group, d, page):
     scales = np.ones((2, pages, kvh, page), np.float32)
     cache = b4gemv.KVCache(torch.from_numpy(ref.pack_blocks(NF4, codes, scales)).to(cuda), NF4, page, d)
     t = lambda x: torch.tensor(x, dtype=torch.int32, device=cuda)  # noqa: E731
-    q = torch.zeros((1, kvh * group, d), dtype=torch.float16, device=cuda)
-    got = b4gemv.kv_attention(cache, q, t([list(range(pages))]), t([N]), t([0, 1]), 1)[0].cpu().numpy().astype(np.float64)
+    q = torch.zeros((new, kvh * group, d), dtype=torch.float16, device=cuda)
+    got = b4gemv.kv_attention(cache, q, t([list(range(pages))]), t([N]), t([0, new]), new, causal=False).cpu().numpy().astype(np.float64)
     want = np.repeat(ref.NF4.astype(np.float64)[v].mean(1), group, 0)
     # a level in two parts is off by 2^-22; a product of 16 tokens adds to a sum of fewer than 32 levels, off by 2^-22 of it,
     # and N / 8 of them make the sum of N: 2^-20; the output is rounded once
     assert bool((np.abs(got - want) <= 2.0 ** -22 + 2.0 ** -20 + np.abs(want) * 2.0 ** -11).all())
+
+
+@pytest.mark.parametrize("group,new", [(1, 1), (8, 1), (16, 1), (8, 20), (4, 100)])
+@pytest.mark.parametrize("d,page", [(128, 64), (128, 16), (64, 32)])
+def test_levels_of_keys(cuda, group, new, d, page):
+    """Requests of one key: the log-sum-exp is its score, queries of ones make it the sum of its levels."""
+    rng = np.random.default_rng(d + page + group + new)
+    kvh, n = 2, 9
+    codes = rng.integers(0, 16, (2, n, kvh, page, d)).astype(np.uint8)
+    k = np.concatenate([cancelling(rng, n * kvh) for _ in range(d // N)]).T.reshape(n, kvh, d)
+    codes[0, :, :, 0] = k
+    cache = b4gemv.KVCache(torch.from_numpy(ref.pack_blocks(NF4, codes, np.ones((2, n, kvh, page), np.float32))).to(cuda), NF4, page, d)
+    t = lambda x: torch.tensor(x, dtype=torch.int32, device=cuda)  # noqa: E731
+    q = torch.ones((n * new, kvh * group, d), dtype=torch.float16, device=cuda)
+    lse = torch.empty(q.shape[:2], device=cuda)
+    b4gemv.kv_attention(cache, q, t(range(n)).view(n, 1), t([1] * n), t(range(0, n * new + 1, new)), new, scale=1.0, causal=False, lse=lse)
+    want = np.repeat(np.repeat(ref.NF4.astype(np.float64)[k].sum(-1), group, 1), new, 0)
+    # as above, summed: a level 2^-22, D / 8 products 2^-22 of 32 levels each; fp16 alone would leave 1e-3 for 64 columns
+    assert bool((np.abs(lse.cpu().numpy() - want) <= d * 2.0 ** -22 + d / 8 * 32 * 2.0 ** -22 + 2.0 ** -20).all())
