@@ -68,6 +68,9 @@ struct TileCfg {
     // NF4 with fp16 queries: levels in two fp16 parts, each with its operands and products; half as many stages of twice the size
     static constexpr int kParts = FMT == B4_KV_NF4 && std::is_same<T, __half>::value ? 2 : 1;
     static constexpr int kStages = kTileStages / kParts, kStage = kParts * kBlock;
+    // Two stages: keys and values have barriers of their own, so that the keys of the block after next are written under a
+    // block's softmax, its values still in place (chunk of 2048 behind 6000, NF4: 542 us without).
+    static constexpr bool kSplit = kStages == 2;
     static constexpr float kUp = kParts == 2 ? kNf4Least : kNf4Even;
     // NF4: pairs of levels by byte, 256 rows of 16 copies (2 lanes a copy), or of 8 copies of both parts, at shared address
     // 16384, so that an OR makes a lookup's address; the operands follow it.  Without it they follow the static part.
@@ -242,7 +245,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attn_tile_kernel(const Att
     constexpr int kStages = C::kStages;
     extern __shared__ __align__(1024) uint8_t tile_smem[];
     __shared__ uint64_t seg_full[2], seg_empty[2], q_full[2], s_full[2][2], p_full[2][2], o_done[2][2], q_both, q_free, tops, team, drain[2];
-    __shared__ uint64_t full[kTileStages], empty[kTileStages];
+    __shared__ uint64_t full[kTileStages], empty[kTileStages], values_full[2], keys_empty[2];      // the last two: kSplit
     __shared__ TileSeg segs[2];
     __shared__ long long units_before[kTileThreads + 1];
     __shared__ int tiles_before[kTileThreads + 1];
@@ -269,7 +272,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attn_tile_kernel(const Att
             mbar_init(&seg_empty[i], 14);
             mbar_init(&q_full[i], 4);
             for (int j = 0; j < 2; ++j) {
-                mbar_init(&s_full[i][j], 1);
+                mbar_init(&s_full[i][j], C::kSplit ? 2 : 1);
                 mbar_init(&p_full[i][j], 4);
                 mbar_init(&o_done[i][j], 1);
             }
@@ -277,6 +280,10 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attn_tile_kernel(const Att
         for (int i = 0; i < kStages; ++i) {
             mbar_init(&full[i], 4);
             mbar_init(&empty[i], 2);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&values_full[i], 4);
+            mbar_init(&keys_empty[i], 2);
         }
         mbar_init(&tops, 2);
         mbar_init(&team, 8);
@@ -466,7 +473,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attn_tile_kernel(const Att
                 // others once they are there (a block is left when both warps have left it)
                 const uint32_t desc_q = umma_desc(operands + (two ? x : 0) * C::kOperand, 16);
                 // a tile's next block's scores are asked for before its weights are waited for, as far as the stages reach
-                const int ahead = two || kStages == 2 ? 1 : 2;
+                const int ahead = two || C::kSplit ? 1 : 2;
                 bool queries = two || x == 0, add = false;
                 if (!two && x == 1) {                              // the first tile's queries
                     if (!(ok = warp_wait(&q_both, shared++ & 1, &dead))) break;
@@ -497,14 +504,22 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attn_tile_kernel(const Att
                                         umma_ss(s_at + buf * 64, desc_q + (j >> 2) * (kPartQ >> 4) + (j & 3) * 2,
                                                 kd + part * (C::kBlock >> 4) + (j >> 2) * (kPartB >> 4) + (j & 3) * 2, id_s, part > 0 || j > 0);
                                 umma_commit(&s_full[x][buf]);
+                                if (C::kSplit) {
+                                    mbar_arrive(&s_full[x][buf]);  // the scales, too, are there for who waits for the scores
+                                    umma_commit(&keys_empty[stage]);
+                                }
                                 if (!two && x == 1 && sb + 2 >= blocks) umma_commit(&q_free);
                             }
                             __syncwarp();
                             ++cs;
+                        } else if (C::kSplit) {
+                            if (elect_one()) mbar_arrive(&keys_empty[stage]);
+                            __syncwarp();
                         }
                     }
                     if (i >= 0) {                                  // the block's operands are there since its scores
                         const int stage = (blocks_before + i) & (kStages - 1), buf = cp & 1;
+                        if (C::kSplit && !(ok = warp_wait(&values_full[stage], (blocks_before + i) / kStages & 1, &dead))) break;
                         if (taken) {
                             if (!(ok = warp_wait(&p_full[x][buf], cp >> 1 & 1, &dead))) break;
                             ++cp;
@@ -633,7 +648,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attn_tile_kernel(const Att
                 load(id_next, next);
                 id_next = page_id(blk + 2);
             }
-            if (b >= kStages && !(ok = warp_wait(&empty[stage], (b / kStages + 1) & 1, &dead))) break;
+            const int scales = b & (kTileStages - 1);
+            if (b >= kStages && !(ok = warp_wait(C::kSplit ? &keys_empty[stage] : &empty[stage], (b / kStages + 1) & 1, &dead))) break;
             // scales: those of tokens that no row sees are 0, the values' relative to a running power of two
             const int token = blk * kTileKeys + t;
             const bool seen = now.there && token < see_end && token >= see_begin;
@@ -646,23 +662,30 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attn_tile_kernel(const Att
                     mbar_arrive(&tops);
                 }
                 __syncwarp();
-                write(values_at + stage * C::kStage + row_at, now.v);          // while the other warp's maximum comes
+                if (!C::kSplit) write(values_at + stage * C::kStage + row_at, now.v);      // while the other warp's maximum comes
                 if (!(ok = warp_wait(&tops, b & 1, &dead))) break;
                 const float top = fmaxf(value_top[b & 1][0], value_top[b & 1][1]);
                 vexp = max(vexp, (int)(__float_as_uint(top) >> 23) - 126);
-                value_scale[stage][t] = fminf(scale * pow2(kLift - vexp), 3.4028235e38f);    // finite, so that a weight of 0 makes 0 of it
-                if (t == 0) value_exp[stage] = vexp;
+                value_scale[scales][t] = fminf(scale * pow2(kLift - vexp), 3.4028235e38f);    // finite, so that a weight of 0 makes 0 of it
+                if (t == 0) value_exp[scales] = vexp;
             } else {
-                key_scale[stage][t] = scale;
+                key_scale[scales][t] = scale;
                 // tokens that are not there lie in whole pages of 16 at least: two bits a warp
                 const unsigned pages = __ballot_sync(0xffffffffu, now.there);
-                if (lane == 0) reinterpret_cast<uint8_t*>(&block_pages[stage])[warp & 1] = (uint8_t)((pages & 1) | (pages >> 16 & 1) << 1);
-                write(values_at + stage * C::kStage + row_at, now.v);
+                if (lane == 0) reinterpret_cast<uint8_t*>(&block_pages[scales])[warp & 1] = (uint8_t)((pages & 1) | (pages >> 16 & 1) << 1);
+                if (!C::kSplit) write(values_at + stage * C::kStage + row_at, now.v);
             }
             write(keys_at + stage * C::kStage + row_at, now.k);
             fence_proxy_async();
             __syncwarp();
             if (lane == 0) mbar_arrive(&full[stage]);
+            if (C::kSplit) {
+                if (b >= kStages && !(ok = warp_wait(&empty[stage], (b / kStages + 1) & 1, &dead))) break;
+                write(values_at + stage * C::kStage + row_at, now.v);
+                fence_proxy_async();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&values_full[stage]);
+            }
             if (++blk < s.blk1) {
                 now = next;
             } else {
@@ -788,13 +811,14 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attn_tile_kernel(const Att
             bool any = false;                  // whether O holds something
 #pragma unroll 1
             for (int i = two ? 0 : x; i < blocks && ok; i += two ? 1 : 2, ++cs) {
-                const int stage = (ring0 + i) & (kStages - 1), buf = cs & 1;
+                const int scales = (ring0 + i) & (kTileStages - 1), buf = cs & 1;
                 if (!(ok = warp_wait(&s_full[x][buf], cs >> 1 & 1, &dead))) break;
-                // the scales' writers; after the scores, so that the phase asked for is the last one done
-                if (!(ok = warp_wait(&full[stage], (ring0 + i) / kStages & 1, &dead))) break;
+                // the scales' writers; after the scores, so that the phase asked for is the last one done.  kSplit: the next one
+                // may be done too, and the scores' barrier speaks for the scales
+                if (!C::kSplit && !(ok = warp_wait(&full[scales], (ring0 + i) / kStages & 1, &dead))) break;
                 tmem_after_sync();
-                const int key0 = (s.blk0 + i) * kTileKeys, pages = block_pages[stage] & 0xffff, ve = value_exp[stage];
-                const float4* ks = reinterpret_cast<const float4*>(key_scale[stage]);
+                const int key0 = (s.blk0 + i) * kTileKeys, pages = block_pages[scales] & 0xffff, ve = value_exp[scales];
+                const float4* ks = reinterpret_cast<const float4*>(key_scale[scales]);
                 float2 v[kTileKeys / 2];       // the row's scores
                 tmem_ld32(reinterpret_cast<uint32_t*>(v), s_at + buf * 64);
                 tmem_ld32(reinterpret_cast<uint32_t*>(v) + 32, s_at + buf * 64 + 32);
@@ -840,7 +864,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attn_tile_kernel(const Att
                 }
                 any = true;
                 const float2 q2 = make_float2(qf, qf), m2 = make_float2(-m, -m);
-                const float4* vs = reinterpret_cast<const float4*>(value_scale[stage]);
+                const float4* vs = reinterpret_cast<const float4*>(value_scale[scales]);
                 float2 l2[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
                 uint32_t w[kTileKeys / 2];
 #pragma unroll
