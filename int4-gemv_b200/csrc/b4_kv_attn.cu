@@ -17,12 +17,16 @@ int sm_count()
 
 // Which kernels run.  The warp kernel takes requests of few rows (queries x heads that
 // share a kv head), in tiles of 8 or 16 that each read the cache, the tile kernel the
-// others, whose time does not depend on the rows up to 128.  24 requests of 4000 tokens,
-// 4 kv heads x 128, INT4: 32 rows 58 us against 68, 48 rows 72 against 68 (NF4: 72 and
-// 83, 93 and 83); 8 kv heads x 64: 48 rows 78 us against 97 (NF4: 94 and 111).  So the
-// warp kernel has up to 32 rows of 128, 48 of 64.
+// others, whose time does not depend on the rows up to 128.  24 requests of 4000 tokens
+// (INT4 in fp16, NF4 in bf16, NF4 in fp16): 4 kv heads x 128, 48 rows 67, 71 and 100 us
+// against 69, 85 and 120, 64 rows 83, 87 and 125 against 69, 85 and 121; 8 kv heads x 64,
+// 64 rows 83, 87 and 118 us against 96, 118 and 169, 80 rows 101, 105 and 144 against 96,
+// 118 and 169.  So the warp kernel has up to 48 rows of 128, 64 of 64.
 // max_q says which of the two the call needs: one where every request is of one
-// kind by it, both (each skipping the other's requests) where it cannot be known.
+// kind by it, both (each skipping the other's requests) where it cannot be known.  In
+// a call for both the warp kernel takes the smallest tile's rows alone: with tiles of 16
+// and up to 48 rows, 31 single tokens behind 4000 and a chunk of 512 behind 2000 take
+// 103 us for 87, 24 x 5 drafts and the chunk 127 for 110 (28 heads over 4 x 128, INT4).
 struct Plan {
     bool warp, tile;
     int cols;               // the warp kernel's tile: 8 or 16 columns
@@ -32,7 +36,7 @@ struct Plan {
 Plan plan(const AttnParams& p)
 {
     const long long most = (long long)std::max(1, p.a.max_q) * p.group;
-    if (most <= (p.l.head_dim == 64 ? 48 : 32)) return {true, false, most <= 8 ? 8 : 16, INT_MAX, INT_MAX};
+    if (most <= (p.l.head_dim == 64 ? 64 : 48)) return {true, false, most <= 8 ? 8 : 16, INT_MAX, INT_MAX};
     if ((long long)p.a.n_req * p.a.max_q <= p.a.total_q || p.group > 16) return {false, true, 0, 0, 0};    // alike, or none of few rows
     const int cols = p.group <= 8 ? 8 : 16;
     return {true, true, cols, cols, cols};
