@@ -517,12 +517,16 @@ int b4_kv_read(const b4_kv_cache* cache, const int32_t* slots, int n_tokens, flo
  * q, out: dtype fp16 or bf16 [total_q][heads][head_dim], strides in elements,
  * columns contiguous, rows 16-byte aligned.  lse (optional): fp32
  * [total_q][heads], the natural logarithm of the sum of exp(scores).
+ * Scores, maxima, sums and outputs are held in fp32; the weights are rounded to
+ * fp16 for the product with the values, and so are NF4's levels where q is bf16
+ * (with fp16 they are taken in two parts).
  * max_q: the most queries of one request (chooses the kernels; requests with
  * more are computed all the same).  heads / kv_heads <= 64,
  * total_q * heads / kv_heads < 2^31, table_width * page_size <= 2^31 - 64.
  * ws: b4_kv_attention_workspace bytes of device memory, 16-byte aligned,
  * ZERO-FILLED before its first use; calls leave ready for the next what must be
- * zero.  Not shared with b4_gemv_ws, nor by calls that may run at the same time. */
+ * zero (after a device error it has to be zero-filled again).  Not shared with
+ * b4_gemv_ws, nor by calls that may run at the same time. */
 #define B4_KV_FULL 1
 typedef struct b4_kv_attn {
     const void* q;

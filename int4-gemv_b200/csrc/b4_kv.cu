@@ -312,6 +312,7 @@ __global__ void __launch_bounds__(256) kv_append_kernel(const AppendParams p)
         uint32_t w;
         __half sh;
         if (FMT == B4_KV_INT4) {
+            // times fp32's 1/7 as torch divides by a number on the GPU: pages written by such a program have these bytes
             sh = __float2half_rn(amax > 0.0f ? __fmul_rn(amax, 1.0f / 7.0f) : 1.0f);
             w = int4_word(x, __half2float(sh));
         } else {
@@ -337,7 +338,7 @@ struct ReadParams {
     unsigned long long magic;
 };
 
-// Bound by its fp32 stores: the same tokens in 20 us, 5.2 TB/s.
+// Bound by its fp32 stores: the same tokens in 20 us, 4.65 TB/s (92.9 MB).
 template <int FMT, int D, int U>
 __global__ void __launch_bounds__(256) kv_read_kernel(const ReadParams p)
 {

@@ -111,12 +111,13 @@ constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 // they are, the levels are off by 1.6e-4 of the code book's norm.  Times a factor in
 // [1, 2) first, all 16 lie nearer to fp16 numbers, and its reciprocal goes into a
 // factor that is applied in fp32 anyway.  kNf4Least leaves the least, 3.3e-5 in the mean
-// square (6.3e-5 at most): for keys, and where the low parts make the values exact.
-// A value's rounding is the same for every token of its code, so over many tokens it
-// does not average out as the weights' do, while an output gets smaller: of 20 million
-// factors, kNf4Even's roundings (4e-5, 9.3e-5 at most), weighted by how often a code
-// occurs (normal values under the largest of 64 and of 128; every code alike), sum to the
-// least, 8e-7 of a scale (kNf4Least's: 1.1e-5, 0.2 % of an output over 4000 tokens).
+// square (6.3e-5 at most): where a low part follows (fp16 queries), which makes the levels
+// exact to 2^-22.  kNf4Even, where none does (bf16), is off by 4e-5 in the mean square and
+// by 9.3e-5 of a scale at most, whatever the codes; since a value's rounding is the same
+// for every token of its code and does not average out, it is the factor, of 20 million,
+// whose roundings sum to the least over codes as normal values and every code alike give
+// them: 4e-7 to 1.1e-6 of a scale (kNf4Least: 1.1e-5).  Laplace values leave 4.7e-6,
+// exponential ones 1.2e-5, 0.2 % of an output over 4000 tokens, which is bf16's own rounding.
 constexpr float kNf4Least = 1.67766535282135f, kNf4Even = 1.6775788f;
 
 __device__ __forceinline__ uint32_t nf4_pair(uint32_t byte, float up)

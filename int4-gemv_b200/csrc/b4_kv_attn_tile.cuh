@@ -8,7 +8,8 @@
 // with fp16 operands and fp32 accumulators in tensor memory.  Where a request has
 // 128 rows or fewer, the two tiles are the same rows and take every other block: two
 // streams, joined at the end.  K and V hold the bare levels (INT4: exact integers;
-// NF4: rounded to fp16, kNf4Even), so a token's key scale multiplies a column of S and
+// NF4: rounded to fp16 with bf16 queries, in two fp16 parts with fp16 ones, each with its
+// operands and products), so a token's key scale multiplies a column of S and
 // its value scale a column of P, in fp32.  Softmax is the warp kernel's
 // (b4_kv_attn_warp.cuh): a maximum that moves only when a score passes it by 2^8,
 // weights relative to it and to a running power of two of the value scales, rounded
@@ -18,7 +19,8 @@
 // took 2.4 us a block over its chain of waits and issues).  Warp 1: the schedule.  Warps 4-7 and 8-11:
 // softmax of the two tiles, a row a thread.  Warps 12-15: codes to fp16 operands, half
 // a token a thread, in the 128-byte swizzle (the same bytes serve K, whose columns are
-// the product's depth, and V, whose rows are).  K and V are rings of four.  A
+// the product's depth, and V, whose rows are).  K and V are rings of four, of two where
+// levels have two parts.  A
 // tile has two S of 64 columns of tensor memory (P takes half of one), so that the
 // next block's scores are there when a block's weights are done: with one S of 128
 // columns a block waited 4.1 us on the chain scores - softmax - outputs - scores,
@@ -34,15 +36,17 @@
 // a segment (request, tile, head) that crosses CTAs is joined by the last of them to
 // arrive, in order, as in the warp kernel.  A segment also costs what its begin and end
 // cost: counted as kSegUnits blocks, since the first tiles of a prompt are many short
-// segments (five prompts of 200 to 1500 tokens, NF4, 64 heads over 8: 310 us without).
+// segments (five prompts of 200 to 1500 tokens, NF4 in bf16, 64 heads over 8: 310 us without).
 //
 // What bounds it.  Two row tiles: some 1.6 us a block of 64 keys, of which the products
 // are 0.75 (scores with 64 keys a product read Q anew for each: 48 cycles where 32
 // multiply); the rest is the chain of a row's softmax, longest in the two quarters of
 // the SM whose issue slots the products' warps share.  One row tile: the decoding
-// warps, 1.1 us a block.  Measured (chunk of 2048 tokens behind 6000, 28 heads over 4 x
-// 128, INT4): 273 us, 754 TFLOP/s; 24 requests x 5 tokens behind 2500 to 5500: 68 us;
-// the five prompts: 169 us.  Tried and left out: the tiles half a block apart (289 us);
+// warps, 1.1 us a block.  Two parts: the chain from a block's weights over the writing of
+// the values after next, 2.8 us a block (LSU 60 % busy).  Measured (chunk of 2048 tokens
+// behind 6000, 28 heads over 4 x 128, INT4): 272 us, 758 TFLOP/s, NF4 in bf16
+// 300 us, in fp16 471; the five prompts: 168 us, in fp16 219.  Tried and left out (INT4
+// chunk): the tiles half a block apart (289 us);
 // the decoding warps in the other two quarters (287 us); scores issued only once the
 // last ones are read (286 us).
 //
@@ -69,7 +73,7 @@ struct TileCfg {
     static constexpr int kParts = FMT == B4_KV_NF4 && std::is_same<T, __half>::value ? 2 : 1;
     static constexpr int kStages = kTileStages / kParts, kStage = kParts * kBlock;
     // Two stages: keys and values have barriers of their own, so that the keys of the block after next are written under a
-    // block's softmax, its values still in place (chunk of 2048 behind 6000, NF4: 542 us without).
+    // block's softmax, its values still in place (chunk of 2048 behind 6000, NF4 in fp16: 542 us without, 470 to 483 with).
     static constexpr bool kSplit = kStages == 2;
     static constexpr float kUp = kParts == 2 ? kNf4Least : kNf4Even;
     // NF4: pairs of levels by byte, 256 rows of 16 copies (2 lanes a copy), or of 8 copies of both parts, at shared address

@@ -9,15 +9,16 @@
 // 8-wide side is the queries and none of it is padding for groups of 8.  A token's
 // scale does not depend on the column, so the key's scale multiplies S and the
 // value's scale P, in fp32; the operands hold the bare levels (INT4: exact
-// integers; NF4: keys rounded to fp16, values so too where the output is bf16, as fp16
-// high and low parts in two products where it is fp16, since an output
-// over many tokens is far smaller than its terms, and a level's rounding averages out
-// only as far as the codes are spread as kNf4Even takes them).
+// integers; NF4: with bf16 queries rounded to fp16 (kNf4Even), which with bf16's own
+// rounding, 1.7e-3 of an output's norm, makes 1.02 to 1.14 times as much; with fp16
+// queries fp16 high and low parts in two products, since there keys rounded once put
+// outputs 3.5e-4 to 6.1e-4 off, where their own rounding is 2.1e-4).
 // Softmax's maximum and sum run along the tokens, in fp32, private to a warp;
 // the maximum moves only when a score passes it by 2^8, which the weights'
 // range allows.  P times the value scale goes to fp16 (its rounding is of the size of
-// the output's own), relative to that maximum and to a running power of two that
-// bounds the value scales (kLift): a token whose value scale is 2^20 below the largest
+// an fp16 output's own: outputs are 2.2e-4 to 3.1e-4 off, 2.1e-4 without it,
+// a row that one token outweighs up to 5e-4), relative to that maximum and to a running
+// power of two that bounds the value scales (kLift): a token whose value scale is 2^20 below the largest
 // one keeps its 11 bits if its weight is the largest, so only what hardly counts loses bits.
 //
 // Split.  The (request, kv head, column tile, 32-token chunk) units of the whole
@@ -36,10 +37,12 @@
 //
 // What bounds it.  INT4: the loop runs at 5.3 TB/s; around it a launch spends 5 us up to
 // its first products (lengths, units, page ids, queries: four loads that wait for one
-// another) and 6 to 9 on the joins.  NF4: the lookups, 96 of some 150 shared-memory
-// cycles per 16 tokens, 4.1 TB/s.  Measured: 32 requests x 8192 tokens, 64 heads over 8
-// x 128, INT4: 68 us, 4.07 TB/s over all; one request of 131071, NF4: 57 us, 2.5 TB/s;
-// 96 of 1 to 6000, 32 heads over 8 x 64, NF4: 59 us, 2.8 TB/s; one of 777, INT4: 11.7 us.
+// another) and 6 to 9 on the joins.  NF4: the lookups, a shared load of 32 bits a byte of
+// codes, of 64 with two parts (LSU 62 and 69 % busy).  Measured: 32 requests x 8192
+// tokens, 64 heads over 8 x 128, INT4: 69 us, 4.03 TB/s over all; one request of 131071,
+// NF4 in fp16: 64 us, 2.2 TB/s; 96 of 1 to 6000, 32 heads over 8 x 64, NF4 in bf16:
+// 59 us, 2.8 TB/s; 24 x 5 drafts behind 2500 to 5500, 28 heads over 4 x 128, INT4: 68 us;
+// one of 777, INT4: 11.8 us.
 #pragma once
 
 #include <type_traits>
