@@ -5,7 +5,7 @@ import torch
 
 import b4gemv
 import kv_ref as ref
-from test_kv_gpu import NF4
+from test_kv_gpu import F16, NF4, check_attention, make
 
 pytestmark = pytest.mark.gpu
 N = 64                                         # tokens, alike in weight
@@ -68,3 +68,13 @@ def test_levels_of_keys(cuda, group, new, d, page):
     want = np.repeat(np.repeat(ref.NF4.astype(np.float64)[k].sum(-1), group, 1), new, 0)
     # as above, summed: a level 2^-22, D / 8 products 2^-22 of 32 levels each; fp16 alone would leave 1e-3 for 64 columns
     assert bool((np.abs(lse.cpu().numpy() - want) <= d * 2.0 ** -22 + d / 8 * 32 * 2.0 ** -22 + 2.0 ** -20).all())
+
+
+@pytest.mark.parametrize("d,heads,kvh", [(128, 16, 2), (64, 28, 4)])
+@pytest.mark.parametrize("ctx,new", [([9000, 4000], [1, 1]), ([3000, 2000, 700], [5, 70, 300]), ([400] * 20, [9] * 20), ([1500, 90], [1500, 90])])
+def test_same_bits_every_time(cuda, d, heads, kvh, ctx, new):
+    """Levels in two parts have their own order of barriers: the same bits whatever it comes to."""
+    state = make(cuda, NF4, F16, heads, kvh, d, 32, ctx, new)
+    first = check_attention(cuda, NF4, F16, heads, kvh, d, 32, ctx, new, state=state).clone()
+    for _ in range(20):
+        assert torch.equal(first, b4gemv.kv_attention(*state))
