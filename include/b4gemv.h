@@ -542,6 +542,108 @@ typedef struct b4_kv_attn {
 int b4_kv_attention_workspace(const b4_kv_cache* cache, const b4_kv_attn* attn, size_t* bytes);
 int b4_kv_attention(const b4_kv_cache* cache, const b4_kv_attn* attn, void* ws, size_t ws_bytes, b4_stream_t stream);
 
+/* ---- Rotated append ---------------------------------------------------------------
+ * Rotary embedding of a step's queries and keys on the way into the cache, in one
+ * launch: what a decode layer does between its q/k/v projections and attention.
+ * No counterpart in the reference.
+ *
+ * Column pair i of the `dim` first columns of a head turns by the angle
+ *   2 pi * frac(positions[axes[i]][t] * turns[i] / 2^64):   (a, b) -> (a c - b s, b c + a s),
+ * c and s its cosine and sine times `scale`; the other columns stay.  turns[i] is a
+ * position's part of a whole turn as a fraction of 64 bits (b4_rotary_turns makes
+ * them), so that the product's wrap at 2^64 leaves out the whole turns exactly,
+ * however far the position.  Pairs are (i, i + dim / 2), or (2i, 2i + 1) with
+ * B4_ROTARY_ADJACENT.  Several axes (time, height, width): positions holds a row for
+ * each, and axes[i] < n_axes names pair i's (NULL: the first for all).  dim: a
+ * multiple of 16 up to head_dim.  turns and axes are device memory. */
+#define B4_ROTARY_ADJACENT 1
+typedef struct b4_rotary {
+    const uint64_t* turns;        /* [dim / 2] */
+    const uint8_t* axes;          /* [dim / 2] or NULL */
+    int dim, n_axes, flags;
+    float scale;
+} b4_rotary;
+/* Host: turns[i] = the fraction of inv_freq[i] / (2 pi), rounded to 64 bits.  inv_freq in radians a position, finite. */
+int b4_rotary_turns(const double* inv_freq, int n, uint64_t* turns);
+
+/* q_out[t][h] = q rotated, k rotated and v as b4_kv_append writes them at slots[t].
+ * Angles, and the keys' turn, are computed in 64 bits and a key's column is rounded
+ * to fp32 once before it is quantised, so that its code does not depend on how a
+ * machine rounds; queries turn in fp32 and are rounded to out_dtype.
+ * q (NULL with heads 0: keys and values alone), k, v: dtype fp16, bf16 or fp32, any
+ * strides in elements, columns contiguous; out_dtype: fp16 or bf16, dtype's own where
+ * that is 16 bits; q_out's rows 16-byte aligned.  q_out may be q with its strides, and
+ * overlaps nothing else.  Every row of q_out is written, those without a slot too. */
+typedef struct b4_kv_rows {
+    const void *q, *k, *v;
+    void* q_out;
+    const int32_t* positions;     /* [n_axes][position_stride] */
+    const int32_t* slots;         /* [n_tokens] */
+    long long position_stride, q_stride_token, q_stride_head, k_stride_token, k_stride_head, v_stride_token, v_stride_head,
+        out_stride_token, out_stride_head;
+    int n_tokens, heads, dtype, out_dtype;
+} b4_kv_rows;
+int b4_kv_append_rotary(const b4_kv_cache* cache, const b4_rotary* rotary, const b4_kv_rows* rows, b4_stream_t stream);
+
+/* ---- Attention over a choice of pages -----------------------------------------------
+ * For long contexts: each query and kv head reads the pages whose keys can matter to
+ * it most, by a score of one 8-bit product a page (b4_kv_select), instead of all.  No
+ * counterpart in the reference.
+ *
+ * A page's box of one kv head bounds its keys: b4_kv_box_bytes bytes, int8
+ * [head_dim] column maxima, int8 [head_dim] minima, an fp32 scale (the largest of
+ * them in magnitude times fp32's 1/127; 1 where all are 0), 12 bytes of zeros; codes
+ * are the nearest by the fp32 quotient, ties to even.  Keys are the fp32 values of
+ * b4_kv_read; those that are no number take no part, and a box that is not finite
+ * has the scale +infinity.  boxes: uint8 [n_pages][kv_heads][b4_kv_box_bytes], 16-byte aligned. */
+int b4_kv_box_bytes(int head_dim, size_t* bytes);
+/* The boxes of the pages whose last token is among slots[n_tokens] (a step's, after
+ * its append): the pages that the step completed.  Others are left as they are. */
+int b4_kv_boxes(const b4_kv_cache* cache, const int32_t* slots, int n_tokens, void* boxes, b4_stream_t stream);
+
+/* lists[t][h][..keep]: the pages that query t reads for kv head h, in the order of
+ * the context, from its request's pages 0 .. c - 1 up to its own place: all where
+ * c <= keep; else the first `first`, the last `last` (its own is the last of them),
+ * and of the others those of the largest score, ties to the earlier.  -1 after them.
+ *   score = box scale * sum over columns of (above * maximum + below * minimum),
+ * the sum of whole numbers times the scale, rounded to fp32 once: above and below are
+ * the sums over the kv head's queries of max(q, 0) and min(q, 0), in 64 bits, rounded
+ * to fp32, then to int8 in units of the largest of them in magnitude times fp32's
+ * 1/127 (by the fp32 quotient, ties to even).  Without the roundings to 8 bits that
+ * is the least upper bound of the sum of the heads' products with any key in the box.
+ * Boxes whose scale is not finite come first among the others (+infinity), pages
+ * missing from the table last; a query that is not finite scores every page 0.
+ * seen[t]: the tokens that t sees of its list, the last page's up to its own place;
+ * 0 for a query that sees none, -1 for rows of no request (their lists are not
+ * written).  Only boxes of pages before a query's own are read.
+ * Requests, queries and tables as in b4_kv_attn; a table's first table_width pages
+ * count, at most B4_KV_SELECT_MAX_WIDTH of them.  1 <= last, 0 <= first, first + last
+ * <= keep, keep * page_size <= 2^31 - 64, keep <= B4_KV_SELECT_MAX_WIDTH. */
+#define B4_KV_SELECT_MAX_WIDTH 49152
+typedef struct b4_kv_choice {
+    const void* q;                /* fp16 or bf16 [total_q][heads][head_dim], as b4_kv_attn's */
+    const void* boxes;
+    const int32_t* tables;        /* [n_req][table_stride] */
+    const int32_t* ctx_len;       /* [n_req] */
+    const int32_t* q_starts;      /* [n_req + 1] */
+    int32_t* lists;               /* [total_q][kv_heads][keep] */
+    int32_t* seen;                /* [total_q] */
+    long long table_stride, q_stride_token, q_stride_head;
+    int table_width, n_req, total_q, max_q, heads, dtype, keep, first, last;
+} b4_kv_choice;
+int b4_kv_select(const b4_kv_cache* cache, const b4_kv_choice* choice, b4_stream_t stream);
+
+/* out[t][h] = softmax(scale * q[t][h] . K) V over the first seen[t] tokens of the
+ * pages lists[t][kv head], page_size to each in order, entries outside the cache
+ * masked.  As b4_kv_attention otherwise, with these fields of b4_kv_attn read in
+ * their own way: tables = lists, int32 [total_q][kv_heads][table_width], table_stride
+ * and list_stride_head its strides in entries; ctx_len = seen [total_q] (0: zeros are
+ * written, below 0: the row of out and lse is left as it is; more than the list holds:
+ * what it holds).  q_starts, n_req, max_q are not read, window and flags must be 0. */
+int b4_kv_attention_lists_workspace(const b4_kv_cache* cache, const b4_kv_attn* attn, size_t* bytes);
+int b4_kv_attention_lists(const b4_kv_cache* cache, const b4_kv_attn* attn, long long list_stride_head, void* ws, size_t ws_bytes,
+                          b4_stream_t stream);
+
 /* Reads (and with clear != 0 resets) the current device's error flags: non-zero
  * after a bounded wait ran out -- 1: a streaming kernel's wait on its copy
  * ring or the cache attention's on another warp (the kernel then ended early),

@@ -27,6 +27,8 @@ __all__ = [
     "ENGINE_NF4_XTAB", "XTAB_WORKSPACE_BYTES",
     "KV_INT4", "KV_NF4", "KVCache", "KVStep", "kv_block_bytes", "kv_tables", "kv_append", "kv_read", "kv_attention",
     "kv_attention_workspace",
+    "Rotary", "KVLists", "kv_append_rotary", "kv_box_bytes", "kv_new_boxes", "kv_boxes", "kv_select", "kv_attention_lists",
+    "kv_attention_lists_workspace",
 ]
 
 
@@ -374,3 +376,5 @@ def unpack_codes(qw, out=None, stream=None):
 
 from .kv import (KV_INT4, KV_NF4, KVCache, KVStep, kv_append, kv_attention, kv_attention_workspace,  # noqa: E402
                  kv_block_bytes, kv_read, kv_tables)
+from .kvlists import (KVLists, Rotary, kv_append_rotary, kv_attention_lists, kv_attention_lists_workspace,  # noqa: E402
+                      kv_box_bytes, kv_boxes, kv_new_boxes, kv_select)

@@ -110,6 +110,35 @@ class KvAttn(ctypes.Structure):
                 + [("scale", ctypes.c_float)])
 
 
+ROTARY_ADJACENT = 1     # b4_rotary.flags: pairs of neighbouring columns
+
+
+class RotaryTable(ctypes.Structure):
+    """b4_rotary (include/b4gemv.h)."""
+
+    _fields_ = [("turns", ctypes.c_void_p), ("axes", ctypes.c_void_p), ("dim", ctypes.c_int), ("n_axes", ctypes.c_int),
+                ("flags", ctypes.c_int), ("scale", ctypes.c_float)]
+
+
+class KvRows(ctypes.Structure):
+    """b4_kv_rows (include/b4gemv.h)."""
+
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("q", "k", "v", "q_out", "positions", "slots")]
+                + [(n, ctypes.c_longlong) for n in ("position_stride", "q_stride_token", "q_stride_head", "k_stride_token",
+                                                    "k_stride_head", "v_stride_token", "v_stride_head", "out_stride_token",
+                                                    "out_stride_head")]
+                + [(n, ctypes.c_int) for n in ("n_tokens", "heads", "dtype", "out_dtype")])
+
+
+class KvChoice(ctypes.Structure):
+    """b4_kv_choice (include/b4gemv.h)."""
+
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("q", "boxes", "tables", "ctx_len", "q_starts", "lists", "seen")]
+                + [(n, ctypes.c_longlong) for n in ("table_stride", "q_stride_token", "q_stride_head")]
+                + [(n, ctypes.c_int) for n in ("table_width", "n_req", "total_q", "max_q", "heads", "dtype", "keep", "first",
+                                               "last")])
+
+
 _P = ctypes.c_void_p
 _I = ctypes.c_int
 
@@ -164,6 +193,14 @@ SIGNATURES = {
     "b4_kv_read": (_I, [ctypes.POINTER(KvCache), _P, _I, _P, _P, _P]),
     "b4_kv_attention_workspace": (_I, [ctypes.POINTER(KvCache), _P, ctypes.POINTER(ctypes.c_size_t)]),
     "b4_kv_attention": (_I, [ctypes.POINTER(KvCache), _P, _P, ctypes.c_size_t, _P]),
+    # ... and b4_rotary, b4_kv_rows and b4_kv_choice
+    "b4_rotary_turns": (_I, [_P, _I, _P]),
+    "b4_kv_append_rotary": (_I, [ctypes.POINTER(KvCache), _P, _P, _P]),
+    "b4_kv_box_bytes": (_I, [_I, ctypes.POINTER(ctypes.c_size_t)]),
+    "b4_kv_boxes": (_I, [ctypes.POINTER(KvCache), _P, _I, _P, _P]),
+    "b4_kv_select": (_I, [ctypes.POINTER(KvCache), _P, _P]),
+    "b4_kv_attention_lists_workspace": (_I, [ctypes.POINTER(KvCache), _P, ctypes.POINTER(ctypes.c_size_t)]),
+    "b4_kv_attention_lists": (_I, [ctypes.POINTER(KvCache), _P, ctypes.c_longlong, _P, ctypes.c_size_t, _P]),
     "b4_nccl_error_string": (ctypes.c_char_p, [_I]),
     "b4_device_error": (_I, [_I]),
     "b4_status_string": (ctypes.c_char_p, [_I]),

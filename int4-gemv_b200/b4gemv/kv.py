@@ -62,7 +62,7 @@ def _table(tables, index, n):
         raise ValueError("tables: an int32 CUDA tensor [requests][width], on the device of the others")
     rows, width = tables.shape
     stride, one = tables.stride()
-    if rows < n or (width > 1 and one != 1):
+    if rows < n or (n > 0 and width > 1 and one != 1):    # an empty table's strides are any
         raise ValueError(f"tables: {n} rows at least, columns contiguous")
     if stride < width:
         if n > 1:                              # expanded or overlapping rows: no stride of such a table's is the library's

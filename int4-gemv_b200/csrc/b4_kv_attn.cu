@@ -36,6 +36,7 @@ struct Plan {
 Plan plan(const AttnParams& p)
 {
     const long long most = (long long)std::max(1, p.a.max_q) * p.group;
+    if (p.lists) return {true, false, p.group <= 8 ? 8 : 16, INT_MAX, INT_MAX};        // rows of one query's group
     if (most <= (p.l.head_dim == 64 ? 64 : 48)) return {true, false, most <= 8 ? 8 : 16, INT_MAX, INT_MAX};
     if ((long long)p.a.n_req * p.a.max_q <= p.a.total_q || p.group > 16) return {false, true, 0, 0, 0};    // alike, or none of few rows
     const int cols = p.group <= 8 ? 8 : 16;
@@ -118,7 +119,33 @@ int attn_params(const b4_kv_cache* cache, const b4_kv_attn* a, AttnParams* p)
     p->a = *a;
     p->a.window = std::min(a->window, INT_MAX - a->total_q);       // a query's place, ctx - n + i + 1 > -total_q, less it fits an int
     p->group = a->heads / p->l.kv_heads;
+    p->lists = 0;
+    p->list_head = 0;
     return cudaSuccess;
+}
+
+// a query's own lists: each query is a request of one
+int list_params(const b4_kv_cache* cache, const b4_kv_attn* attn, AttnParams* p)
+{
+    if (!attn || attn->window != 0 || attn->flags != 0) return cudaErrorInvalidValue;
+    b4_kv_attn a = *attn;
+    a.n_req = a.total_q;
+    a.max_q = 1;
+    a.q_starts = nullptr;
+    const int e = attn_params(cache, &a, p);
+    p->lists = 1;
+    return e;
+}
+
+int attend(const AttnParams& p, void* ws, size_t ws_bytes, b4_stream_t stream)
+{
+    const b4_kv_attn& a = p.a;
+    if (!a.q || !a.out || !a.ctx_len || (p.lists ? a.table_width > 0 && !a.tables : !a.tables || !a.q_starts)) return cudaErrorInvalidValue;
+    const long long strides = a.q_stride_token | a.q_stride_head | a.out_stride_token | a.out_stride_head;
+    if (!kv_aligned(a.q, 16) || !kv_aligned(a.out, 16) || strides % 8 != 0) return cudaErrorInvalidValue;
+    cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+    if (!ws || !kv_aligned(ws, 16) || ws_bytes < ws_bytes_of(p, sm_count())) return cudaErrorInvalidValue;
+    return a.dtype == B4_DTYPE_F16 ? attention<__half>(p, ws, st) : attention<__nv_bfloat16>(p, ws, st);
 }
 
 }  // namespace
@@ -155,12 +182,29 @@ int b4_kv_attention(const b4_kv_cache* cache, const b4_kv_attn* a, void* ws, siz
     const int e = attn_params(cache, a, &p);
     if (e != cudaSuccess) return e;
     if (a->total_q == 0 || a->n_req == 0) return cudaSuccess;
-    if (!a->q || !a->out || !a->tables || !a->ctx_len || !a->q_starts) return cudaErrorInvalidValue;
-    const long long strides = a->q_stride_token | a->q_stride_head | a->out_stride_token | a->out_stride_head;
-    if (!kv_aligned(a->q, 16) || !kv_aligned(a->out, 16) || strides % 8 != 0) return cudaErrorInvalidValue;
-    cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-    if (!ws || !kv_aligned(ws, 16) || ws_bytes < ws_bytes_of(p, sm_count())) return cudaErrorInvalidValue;
-    return a->dtype == B4_DTYPE_F16 ? attention<__half>(p, ws, st) : attention<__nv_bfloat16>(p, ws, st);
+    return attend(p, ws, ws_bytes, stream);
+}
+
+int b4_kv_attention_lists_workspace(const b4_kv_cache* cache, const b4_kv_attn* a, size_t* bytes)
+{
+    AttnParams p;
+    const int e = list_params(cache, a, &p);
+    if (e != cudaSuccess) return e;
+    if (!bytes) return cudaErrorInvalidValue;
+    *bytes = a->total_q ? ws_bytes_of(p, sm_count()) : 0;
+    return cudaSuccess;
+}
+
+int b4_kv_attention_lists(const b4_kv_cache* cache, const b4_kv_attn* a, long long list_stride_head, void* ws, size_t ws_bytes,
+                          b4_stream_t stream)
+{
+    AttnParams p;
+    const int e = list_params(cache, a, &p);
+    if (e != cudaSuccess) return e;
+    if (list_stride_head < a->table_width) return cudaErrorInvalidValue;
+    if (a->total_q == 0) return cudaSuccess;
+    p.list_head = list_stride_head;
+    return attend(p, ws, ws_bytes, stream);
 }
 
 }  // extern "C"

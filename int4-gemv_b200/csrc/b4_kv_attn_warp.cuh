@@ -502,7 +502,7 @@ __global__ void __launch_bounds__(WarpCfg<FMT, D, NT, PT>::kThreads, 1) kv_attn_
             v = last == q.chunks ? seg_end : v1;
 
             // the feed: page ids by 32, `ids` from page `base` on and the 32 after those
-            const int32_t* row = a.tables + (long long)r * a.table_stride;
+            const int32_t* row = a.tables + (long long)r * a.table_stride + u.head * p.list_head;
             const uint8_t* blocks = p.blocks + u.head * p.l.block;
             const long long page_bytes = p.l.kv_heads * p.l.block;
             int base = (q.chunk0 + first) * kChunk >> p.l.page_shift, next = q.chunk0 + first, queue = 0;

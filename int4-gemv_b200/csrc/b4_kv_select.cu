@@ -1,0 +1,519 @@
+// b4_kv_select.cu -- boxes around the keys of completed pages, and the choice of the
+// pages that a query reads by a bound of its scores over the boxes.
+//
+// Mathematics.  Over a box [lo, hi] the largest q . k is the sum over columns of
+// max(q, 0) hi + min(q, 0) lo; summed over the query heads that share a kv head that is
+// linear in their sums of max(q, 0) and of min(q, 0), so a page costs one product of
+// 2 * head_dim, whatever the group.  Both sides are 8-bit: the sum of products is a whole
+// number below 2 * 128 * 127^2 < 2^24, exact in any order and in fp32, so scores, ties
+// and the pages chosen are the same whatever adds them up.  A query's own scale is
+// common to its pages and left out.
+//
+// Select.  16 boxes are the left operand of m16n8k32, up to 8 tokens of a request its
+// columns: a box's bytes go from memory into the operand as they lie (the product's
+// order of columns is free, so a lane's 16 bytes are its words of two steps).  Scores go
+// to shared memory as ordered integers.  The keep-th largest is found by bisection over
+// their bits, then the lists are written in the context's order by ballots.
+//
+// Split.  A cluster of CTAs takes a tile of tokens and a kv head; its CTAs share the
+// boxes, 16 at a time, and send the scores of token i to CTA i mod the cluster's size,
+// which chooses for it.
+#include <algorithm>
+#include <climits>
+
+#include "b4_kv.cuh"
+
+namespace b4 {
+namespace {
+
+constexpr int kBoxTail = 16;               // scale and padding
+
+__host__ __device__ inline long long box_bytes(int head_dim) { return 2 * head_dim + kBoxTail; }
+
+// ---- boxes --------------------------------------------------------------------------
+struct BoxParams {
+    KvLayout l;
+    const uint8_t* blocks;
+    uint8_t* boxes;
+    const int32_t* slots;
+    int n, per;                            // tokens, and those that a warp looks at
+};
+
+// int8 code of x in units of s, rounded to even
+__device__ __forceinline__ int box_code(float x, float s) { return min(127, max(-127, __float2int_rn(__fdiv_rn(x, s)))); }
+
+// A warp makes the boxes of the completed pages among its tokens, of one kv head: a lane holds the
+// extremes of 8 columns over the tokens of its parity (D = 128; of its rest by 4: D = 64).
+template <int FMT, int D>
+__global__ void __launch_bounds__(256) kv_boxes_kernel(const BoxParams p)
+{
+    constexpr int TPV = D / 8, ROWS = 32 / TPV;
+    const int lane = threadIdx.x & 31, sub = lane % TPV, head = blockIdx.y;
+    const long long first = ((long long)blockIdx.x * 8 + (threadIdx.x >> 5)) * p.per;
+    const float level = c_nf4_table[lane & 15];
+    kv_begin();
+    if (first >= p.n) return;
+    const int slot = lane < p.per && first + lane < p.n ? __ldg(p.slots + first + lane) : -1;
+    const int mask = p.l.page_size - 1;
+    const bool ends = slot >= 0 && (slot & mask) == mask && slot >> p.l.page_shift < p.l.n_pages;
+    for (unsigned todo = __ballot_sync(0xffffffffu, ends); todo; todo &= todo - 1) {
+        const int page = __shfl_sync(0xffffffffu, slot, __ffs(todo) - 1) >> p.l.page_shift;
+        const long long at = (long long)page * p.l.kv_heads + head;
+        const uint8_t* block = p.blocks + at * p.l.block;
+        const uint8_t* scales = block + p.l.page_size * D;
+        float s[2];                        // of tokens lane and lane + 32
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int t = min(lane + 32 * i, mask);
+            s[i] = FMT == B4_KV_INT4 ? __half2float(reinterpret_cast<const __half*>(scales)[t]) : reinterpret_cast<const float*>(scales)[t];
+        }
+        float hi[8], lo[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            hi[j] = -INFINITY;
+            lo[j] = INFINITY;
+        }
+        const uint32_t* codes = reinterpret_cast<const uint32_t*>(block) + lane;           // ROWS tokens of 4 * TPV bytes at a time
+#pragma unroll 8
+        for (int t = 0; t < p.l.page_size; t += ROWS) {
+            const uint32_t w = codes[t * TPV];
+            const int token = t + lane / TPV;
+            const float a = __shfl_sync(0xffffffffu, s[0], token & 31), b = __shfl_sync(0xffffffffu, s[1], token & 31);
+            const float scale = token < 32 ? a : b;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const uint32_t c = w >> (4 * j) & 15;
+                const float v = __fmul_rn(FMT == B4_KV_INT4 ? (float)((int)c - 8) : __shfl_sync(0xffffffffu, level, c), scale);
+                hi[j] = fmaxf(hi[j], v);
+                lo[j] = fminf(lo[j], v);
+            }
+        }
+        float top = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+#pragma unroll
+            for (int o = TPV; o < 32; o <<= 1) {
+                hi[j] = fmaxf(hi[j], __shfl_xor_sync(0xffffffffu, hi[j], o));
+                lo[j] = fminf(lo[j], __shfl_xor_sync(0xffffffffu, lo[j], o));
+            }
+            if (hi[j] < lo[j]) hi[j] = lo[j] = 0.0f;                                       // no number in the column
+            top = fmaxf(top, fmaxf(fabsf(hi[j]), fabsf(lo[j])));
+        }
+#pragma unroll
+        for (int o = TPV / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        const float unit = top > 0.0f ? __fmul_rn(top, 1.0f / 127.0f) : 1.0f;
+        uint8_t* box = p.boxes + at * box_bytes(D);
+        if (lane < TPV) {
+            uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                w[j / 4] |= (uint32_t)(box_code(hi[j], unit) & 255) << (j % 4 * 8);
+                w[2 + j / 4] |= (uint32_t)(box_code(lo[j], unit) & 255) << (j % 4 * 8);
+            }
+            reinterpret_cast<uint2*>(box)[sub] = make_uint2(w[0], w[1]);
+            reinterpret_cast<uint2*>(box + D)[sub] = make_uint2(w[2], w[3]);
+            if (sub == 0) *reinterpret_cast<uint4*>(box + 2 * D) = make_uint4(__float_as_uint(unit), 0, 0, 0);
+        }
+    }
+}
+
+// ---- select -------------------------------------------------------------------------
+struct SelectParams {
+    KvLayout l;
+    b4_kv_choice c;
+    int group, tile, cluster, cap;         // heads of a kv head, tokens of a tile, CTAs of a cluster, scores of a token
+    int direct;                            // a tile index is a request's
+};
+
+constexpr int kSelThreads = 256, kSelWarps = kSelThreads / 32, kSelTile = 8;
+
+__device__ __forceinline__ void mma_s8(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1)
+{
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// larger for larger x; 0 below all of them
+__device__ __forceinline__ uint32_t ordered(float x)
+{
+    const uint32_t u = __float_as_uint(x + 0.0f);                  // -0 as 0
+    return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+
+__device__ __forceinline__ void cluster_sync()
+{
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+__device__ __forceinline__ void store_cluster(uint32_t at, uint32_t rank, uint32_t v)
+{
+    uint32_t there;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(at), "r"(rank));
+    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(there), "r"(v) : "memory");
+}
+
+// What a query sees: its pages, its own the last, and its list's entries and tokens.
+struct Seen {
+    int pages, entries, tokens;
+};
+
+__device__ __forceinline__ Seen seen_of(const SelectParams& p, int ctx, int n, int i)
+{
+    const int place = ctx - n + i;                                 // ctx >= 0: above -2^31
+    const long long room = (long long)p.c.table_width * p.l.page_size;
+    const int visible = place < 0 ? 0 : (int)min((long long)place + 1, room);
+    Seen s = {0, 0, 0};
+    if (visible > 0) {
+        s.pages = ((visible - 1) >> p.l.page_shift) + 1;
+        s.entries = min(s.pages, p.c.keep);
+        s.tokens = (s.entries - 1) * p.l.page_size + visible - (s.pages - 1) * p.l.page_size;
+    }
+    return s;
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kSelThreads) kv_select_kernel(const SelectParams p)
+{
+    constexpr int V = D / 32;                                      // 16-byte words of a box that a lane holds
+    constexpr int kRow = 2 * D + 64;
+    extern __shared__ __align__(16) uint32_t scores[];             // [tokens of this CTA][cap]
+    __shared__ __align__(16) uint8_t query[kSelTile * kRow];       // above, below of a token
+    __shared__ int part[2][kSelWarps];
+    __shared__ int2 counts[kSelWarps];
+
+    const b4_kv_choice& a = p.c;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int rank = blockIdx.x % p.cluster, head = blockIdx.y;
+    const int at_tile = blockIdx.x / p.cluster;
+    kv_begin();
+
+    // ---- the request and its tokens ----
+    auto start = [&](int r) { return max(0, min(__ldg(a.q_starts + r), a.total_q)); };
+    int r = at_tile, tile0 = 0;
+    if (!p.direct) {
+        // request r has the tiles from start / 8 + r on, more than it needs at most: the last that begins at or before this one
+        int lo = 0, n = a.n_req;
+        while (n > 1) {
+            const int step = (n + 31) / 32, probe = lo + lane * step;
+            const bool in = lane * step < n && (lane == 0 || start(probe) / kSelTile + probe <= at_tile);
+            const int last = 31 - __clz(__ballot_sync(0xffffffffu, in));
+            n = min(step, n - last * step);
+            lo += last * step;
+        }
+        r = lo;
+        tile0 = at_tile - (start(r) / kSelTile + r);
+    }
+    const int q0 = start(r), n = max(0, start(r + 1) - q0), ctx = max(0, __ldg(a.ctx_len + r));
+    // rows of no request
+    if (head == 0) {
+        const int end = start(a.n_req);
+        for (long long t = end + (long long)blockIdx.x * kSelThreads + tid; t < a.total_q; t += (long long)gridDim.x * kSelThreads) a.seen[t] = -1;
+        if (const int begin = start(0); begin > 0)
+            for (long long t = (long long)blockIdx.x * kSelThreads + tid; t < begin; t += (long long)gridDim.x * kSelThreads) a.seen[t] = -1;
+    }
+    const int32_t* table = a.tables + (long long)r * a.table_stride;
+
+    for (int i0 = tile0 * p.tile; i0 < n; i0 = p.direct ? i0 + p.tile : n) {
+        const int nt = min(p.tile, n - i0);
+        const Seen most = seen_of(p, ctx, n, i0 + nt - 1);
+        const int m = most.pages > a.keep ? most.pages - a.first - a.last : 0;     // pages to score
+
+        if (m > 0) {
+            // ---- scores: this CTA's boxes, 16 a warp at a time ----
+            const int g = lane >> 2, t = lane & 3;
+            const int groups = (m + 15) / 16;
+            uint4 box[2][V];
+            float unit[2];
+            bool there[2];
+            auto load = [&](int at) {
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const int b = at * 16 + g + 8 * j;
+                    const int id = b < m ? __ldg(table + a.first + b) : -1;
+                    there[j] = (unsigned)id < (unsigned)p.l.n_pages;
+                    const uint8_t* src = static_cast<const uint8_t*>(a.boxes) + ((long long)(there[j] ? id : 0) * p.l.kv_heads + head) * box_bytes(D);
+#pragma unroll
+                    for (int i = 0; i < V; ++i) box[j][i] = __ldg(reinterpret_cast<const uint4*>(src + 64 * i) + t);
+                    unit[j] = __ldg(reinterpret_cast<const float*>(src + 2 * D));
+                }
+            };
+            int at = rank + p.cluster * warp;
+            if (at < groups) load(at);
+
+            // a token a warp: the sums of its heads' parts above and below 0, as int8
+            if (warp < p.tile) {
+                constexpr int C = D / 32;                          // columns of a lane
+                double above[C], below[C];
+#pragma unroll
+                for (int j = 0; j < C; ++j) above[j] = below[j] = 0.0;
+                if (warp < nt) {
+                    const T* src = static_cast<const T*>(a.q) + (q0 + i0 + warp) * a.q_stride_token + (long long)head * p.group * a.q_stride_head + lane * C;
+#pragma unroll 8
+                    for (int h = 0; h < p.group; ++h) {
+                        T x[C];
+                        if (C == 4) *reinterpret_cast<uint2*>(x) = __ldg(reinterpret_cast<const uint2*>(src + h * a.q_stride_head));
+                        else *reinterpret_cast<uint32_t*>(x) = __ldg(reinterpret_cast<const uint32_t*>(src + h * a.q_stride_head));
+#pragma unroll
+                        for (int j = 0; j < C; ++j) {
+                            const float v = kv_float(x[j]);
+                            above[j] += v > 0.0f ? v : 0.0f;
+                            below[j] += v > 0.0f ? 0.0f : v;       // NaN too
+                        }
+                    }
+                }
+                float hi[C], lo[C], top = 0.0f;
+                bool finite = true;
+#pragma unroll
+                for (int j = 0; j < C; ++j) {
+                    hi[j] = (float)above[j];
+                    lo[j] = (float)below[j];
+                    const float x = fmaxf(hi[j], -lo[j]);
+                    finite = finite && hi[j] < INFINITY && lo[j] > -INFINITY;
+                    top = fmaxf(top, x);
+                }
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+                finite = __all_sync(0xffffffffu, finite);
+                const float s = top > 0.0f ? __fmul_rn(top, 1.0f / 127.0f) : 1.0f;
+                uint32_t wh = 0, wl = 0;
+#pragma unroll
+                for (int j = 0; j < C; ++j) {
+                    wh |= (uint32_t)(finite ? box_code(hi[j], s) & 255 : 0) << (8 * j);
+                    wl |= (uint32_t)(finite ? box_code(lo[j], s) & 255 : 0) << (8 * j);
+                }
+                uint8_t* dst = query + warp * kRow + lane * C;
+                if (C == 4) {
+                    *reinterpret_cast<uint32_t*>(dst) = wh;
+                    *reinterpret_cast<uint32_t*>(dst + D) = wl;
+                } else {
+                    *reinterpret_cast<uint16_t*>(dst) = (uint16_t)wh;
+                    *reinterpret_cast<uint16_t*>(dst + D) = (uint16_t)wl;
+                }
+            }
+            if (p.cluster > 1) cluster_sync();                     // the others have begun, or are done with the last tile's scores
+            else __syncthreads();
+
+            uint4 qw[V];
+#pragma unroll
+            for (int i = 0; i < V; ++i)
+                qw[i] = g < p.tile ? *reinterpret_cast<const uint4*>(query + g * kRow + 64 * i + 16 * t) : make_uint4(0, 0, 0, 0);
+            const uint32_t scores_at = (uint32_t)__cvta_generic_to_shared(scores);
+            while (at < groups) {
+                int acc[4] = {0, 0, 0, 0};
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    mma_s8(acc, box[0][i].x, box[1][i].x, box[0][i].y, box[1][i].y, qw[i].x, qw[i].y);
+                    mma_s8(acc, box[0][i].z, box[1][i].z, box[0][i].w, box[1][i].w, qw[i].z, qw[i].w);
+                }
+                float s[2];
+                bool in[2];
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    s[j] = unit[j];
+                    in[j] = there[j];
+                }
+                const int now = at;
+                at += p.cluster * kSelWarps;
+                if (at < groups) load(at);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int token = 2 * t + (j & 1), b = now * 16 + g + 8 * (j >> 1);
+                    if (token >= nt || b >= m) continue;
+                    const float unit = s[j >> 1];
+                    const uint32_t key = !in[j >> 1] ? 0u : ordered(unit < INFINITY ? __fmul_rn((float)acc[j], unit) : INFINITY);
+                    const uint32_t place = (uint32_t)(token / p.cluster) * p.cap + b;
+                    if (p.cluster > 1) store_cluster(scores_at + 4 * place, token % p.cluster, key);
+                    else scores[place] = key;
+                }
+            }
+            if (p.cluster > 1) cluster_sync();
+            else __syncthreads();
+        }
+
+        // ---- the choice: tokens rank, rank + cluster, .. of the tile, by teams of warps ----
+        const int mine = nt > rank ? (nt - rank + p.cluster - 1) / p.cluster : 0;
+        const int tw = mine <= 1 ? 8 : mine <= 2 ? 4 : mine <= 4 ? 2 : 1;          // warps of a team
+        const int team = warp / tw, member = warp % tw;
+        if (team < mine) {
+            const int token = team * p.cluster + rank, threads = tw * 32, i = member * 32 + lane;
+            const Seen s = seen_of(p, ctx, n, i0 + token);
+            int32_t* list = a.lists + ((long long)(q0 + i0 + token) * p.l.kv_heads + head) * a.keep;
+            if (head == 0 && i == 0) a.seen[q0 + i0 + token] = s.tokens;
+            auto entry = [&](int b) {
+                const int id = __ldg(table + b);
+                return (unsigned)id < (unsigned)p.l.n_pages ? id : -1;
+            };
+            if (s.pages <= a.keep) {
+                for (int b = i; b < a.keep; b += threads) list[b] = b < s.pages ? entry(b) : -1;
+            } else {
+                const uint32_t* keys = scores + (size_t)team * p.cap;
+                const int mt = s.pages - a.first - a.last, need = a.keep - a.first - a.last;
+                for (int b = i; b < a.first + a.last; b += threads)
+                    list[b < a.first ? b : b + need] = entry(b < a.first ? b : s.pages - a.last + (b - a.first));
+                auto team_sync = [&]() {
+                    if (tw == 1) __syncwarp();
+                    else asm volatile("bar.sync %0, %1;" ::"r"(1 + team), "r"(threads) : "memory");
+                };
+                int turn = 0;
+                auto total = [&](int x) {                          // over the team
+                    x = __reduce_add_sync(0xffffffffu, x);
+                    if (tw == 1) return x;
+                    if (lane == 0) part[turn][warp] = x;
+                    team_sync();
+                    int all = 0;
+                    for (int w = 0; w < tw; ++w) all += part[turn][team * tw + w];
+                    turn ^= 1;
+                    return all;
+                };
+                if (need > 0) {
+                    // the largest `least` that `need` scores reach
+                    uint32_t least = 0;
+                    for (int bit = 31; bit >= 0; --bit) {
+                        const uint32_t cand = least | 1u << bit;
+                        int x = 0;
+                        for (int b = i; b < mt; b += threads) x += keys[b] >= cand;
+                        x = total(x);
+                        if (x >= need) least = cand;
+                        if (x == need) break;
+                    }
+                    // each member's run of scores: those above it, and those at it, the first of which are taken
+                    const int run = ((mt + threads - 1) / threads) * 32, b0 = member * run, b1 = min(mt, b0 + run);
+                    int above = 0, equal = 0;
+                    for (int b = b0 + lane; b < b1; b += 32) {
+                        above += keys[b] > least;
+                        equal += keys[b] == least;
+                    }
+                    above = __reduce_add_sync(0xffffffffu, above);
+                    equal = __reduce_add_sync(0xffffffffu, equal);
+                    int all_above = above, above0 = 0, equal0 = 0;
+                    if (tw > 1) {
+                        team_sync();
+                        if (lane == 0) counts[warp] = make_int2(above, equal);
+                        team_sync();
+                        all_above = 0;
+                        for (int w = 0; w < tw; ++w) {
+                            const int2 c = counts[team * tw + w];
+                            all_above += c.x;
+                            if (w < member) {
+                                above0 += c.x;
+                                equal0 += c.y;
+                            }
+                        }
+                    }
+                    const int ties = need - all_above;
+                    for (int b = b0; b < b1; b += 32) {
+                        const uint32_t key = b + lane < b1 ? keys[b + lane] : 0;
+                        const unsigned gt = __ballot_sync(0xffffffffu, b + lane < b1 && key > least), eq = __ballot_sync(0xffffffffu, b + lane < b1 && key == least);
+                        const unsigned before = (1u << lane) - 1;
+                        const int e = equal0 + __popc(eq & before);
+                        if (gt >> lane & 1 || (eq >> lane & 1 && e < ties))
+                            list[a.first + above0 + __popc(gt & before) + min(e, ties)] = entry(a.first + b + lane);
+                        above0 += __popc(gt);
+                        equal0 += __popc(eq);
+                    }
+                }
+            }
+        }
+    }
+}
+
+template <typename T, int D>
+cudaError_t launch_select(SelectParams p, cudaStream_t st)
+{
+    auto fn = kv_select_kernel<T, D>;
+    p.tile = p.c.max_q <= 1 ? 1 : kSelTile;
+    p.direct = p.c.max_q <= kSelTile;
+    const long long tiles = p.direct ? p.c.n_req : p.c.total_q / kSelTile + p.c.n_req;
+    if (tiles < 1 || tiles * 8 > INT_MAX) return cudaErrorInvalidValue;
+    p.cap = (p.c.table_width + 15) / 16 * 16;
+    // a CTA's boxes, 16 a warp, where few tiles would leave SMs without one; and shared memory for the scores
+    p.cluster = 1;
+    while (p.cluster < 8 && tiles * p.l.kv_heads * p.cluster < 148 && p.cap > 128 * p.cluster) p.cluster *= 2;
+    auto bytes = [&]() { return (size_t)((p.tile + p.cluster - 1) / p.cluster) * p.cap * 4; };
+    while (p.cluster < 8 && bytes() > 200 * 1024) p.cluster *= 2;
+    const size_t smem = bytes();
+    if (smem > 32 * 1024) {
+        const cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024);
+        if (e != cudaSuccess) return e;
+    }
+    cudaLaunchConfig_t lc = {};
+    lc.gridDim = dim3((unsigned)(tiles * p.cluster), (unsigned)p.l.kv_heads);
+    lc.blockDim = dim3(kSelThreads);
+    lc.dynamicSmemBytes = smem;
+    lc.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = (unsigned)p.cluster;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    lc.attrs = attr;
+    lc.numAttrs = 2;
+    return cudaLaunchKernelEx(&lc, fn, p);
+}
+
+template <int FMT>
+cudaError_t launch_boxes(const BoxParams& p, cudaStream_t st)
+{
+    const dim3 grid((unsigned)((p.n + 8LL * p.per - 1) / (8 * p.per)), (unsigned)p.l.kv_heads);
+    return p.l.head_dim == 64 ? kv_launch(kv_boxes_kernel<FMT, 64>, grid, 256, 0, st, p) : kv_launch(kv_boxes_kernel<FMT, 128>, grid, 256, 0, st, p);
+}
+
+}  // namespace
+}  // namespace b4
+
+using namespace b4;
+
+extern "C" {
+
+int b4_kv_box_bytes(int head_dim, size_t* bytes)
+{
+    if (!bytes || (head_dim != 64 && head_dim != 128)) return cudaErrorInvalidValue;
+    *bytes = (size_t)box_bytes(head_dim);
+    return cudaSuccess;
+}
+
+int b4_kv_boxes(const b4_kv_cache* cache, const int32_t* slots, int n_tokens, void* boxes, b4_stream_t stream)
+{
+    BoxParams p;
+    const int e = kv_layout(cache, &p.l);
+    if (e != cudaSuccess) return e;
+    if (n_tokens < 0) return cudaErrorInvalidValue;
+    if (n_tokens == 0) return cudaSuccess;
+    if (!slots || !boxes || !kv_aligned(slots, 4) || !kv_aligned(boxes, 16)) return cudaErrorInvalidValue;
+    p.blocks = static_cast<const uint8_t*>(cache->blocks);
+    p.boxes = static_cast<uint8_t*>(boxes);
+    p.slots = slots;
+    p.n = n_tokens;
+    p.per = (long long)n_tokens * p.l.kv_heads <= 148 * 32 ? 1 : 16;
+    return p.l.fmt == B4_KV_INT4 ? launch_boxes<B4_KV_INT4>(p, reinterpret_cast<cudaStream_t>(stream))
+                                 : launch_boxes<B4_KV_NF4>(p, reinterpret_cast<cudaStream_t>(stream));
+}
+
+int b4_kv_select(const b4_kv_cache* cache, const b4_kv_choice* c, b4_stream_t stream)
+{
+    SelectParams p;
+    const int e = kv_layout(cache, &p.l);
+    if (e != cudaSuccess) return e;
+    if (!c || c->n_req < 0 || c->total_q < 0 || c->max_q < 0 || c->table_width < 0 || c->table_width > B4_KV_SELECT_MAX_WIDTH ||
+        c->table_stride < c->table_width)
+        return cudaErrorInvalidValue;
+    if (c->heads < 1 || c->heads % p.l.kv_heads || c->heads / p.l.kv_heads > 64) return cudaErrorInvalidValue;
+    if (c->dtype != B4_DTYPE_F16 && c->dtype != B4_DTYPE_BF16) return cudaErrorInvalidValue;
+    if (c->first < 0 || c->last < 1 || c->keep < 1 || c->keep > B4_KV_SELECT_MAX_WIDTH || (long long)c->first + c->last > c->keep ||
+        (long long)c->keep * p.l.page_size > 0x80000000LL - 64)
+        return cudaErrorInvalidValue;
+    if (c->total_q == 0) return cudaSuccess;
+    if (!c->q || !c->boxes || !c->lists || !c->seen || (c->n_req > 0 && (!c->ctx_len || !c->q_starts || (c->table_width > 0 && !c->tables))))
+        return cudaErrorInvalidValue;
+    if (!kv_aligned(c->q, 16) || !kv_aligned(c->boxes, 16) || (c->q_stride_token | c->q_stride_head) % 8 != 0) return cudaErrorInvalidValue;
+    p.c = *c;
+    p.group = c->heads / p.l.kv_heads;
+    cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+    if (c->n_req == 0) return cudaMemsetAsync(c->seen, 0xff, 4 * (size_t)c->total_q, st);
+    if (c->dtype == B4_DTYPE_F16) return p.l.head_dim == 64 ? launch_select<__half, 64>(p, st) : launch_select<__half, 128>(p, st);
+    return p.l.head_dim == 64 ? launch_select<__nv_bfloat16, 64>(p, st) : launch_select<__nv_bfloat16, 128>(p, st);
+}
+
+}  // extern "C"
