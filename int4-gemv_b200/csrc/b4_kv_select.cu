@@ -12,8 +12,8 @@
 // Select.  16 boxes are the left operand of m16n8k32, up to 8 tokens of a request its
 // columns: a box's bytes go from memory into the operand as they lie (the product's
 // order of columns is free, so a lane's 16 bytes are its words of two steps).  Scores go
-// to shared memory as ordered integers.  The keep-th largest is found by bisection over
-// their bits, then the lists are written in the context's order by ballots.
+// to shared memory as ordered integers.  The least that is taken is found by histograms
+// of their bits, then the lists are written in the context's order by ballots.
 //
 // Split.  A cluster of CTAs takes a tile of tokens and a kv head; its CTAs share the
 // boxes, 16 at a time, and send the scores of token i to CTA i mod the cluster's size,
@@ -125,7 +125,7 @@ struct SelectParams {
     int direct;                            // a tile index is a request's
 };
 
-constexpr int kSelThreads = 256, kSelWarps = kSelThreads / 32, kSelTile = 8;
+constexpr int kSelThreads = 256, kSelWarps = kSelThreads / 32, kSelTile = 8, kSelBins = 256;
 
 __device__ __forceinline__ void mma_s8(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1)
 {
@@ -179,8 +179,8 @@ __global__ void __launch_bounds__(kSelThreads) kv_select_kernel(const SelectPara
     constexpr int kRow = 2 * D + 64;
     extern __shared__ __align__(16) uint32_t scores[];             // [tokens of this CTA][cap]
     __shared__ __align__(16) uint8_t query[kSelTile * kRow];       // above, below of a token
-    __shared__ int part[2][kSelWarps];
-    __shared__ int2 counts[kSelWarps];
+    __shared__ __align__(16) int bins[kSelWarps][kSelBins];        // of a team's warps together; then the places of its choice
+    __shared__ int2 part[kSelWarps], found[kSelWarps];
 
     const b4_kv_choice& a = p.c;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -223,23 +223,37 @@ __global__ void __launch_bounds__(kSelThreads) kv_select_kernel(const SelectPara
             // ---- scores: this CTA's boxes, 16 a warp at a time ----
             const int g = lane >> 2, t = lane & 3;
             const int groups = (m + 15) / 16;
-            uint4 box[2][V];
-            float unit[2];
-            bool there[2];
-            auto load = [&](int at) {
+            struct Boxes {                                         // of a step: rows g and g + 8
+                uint4 word[2][V];
+                float unit[2];
+                bool there[2];
+            };
+            const int stride = p.cluster * kSelWarps;
+            int at = rank + p.cluster * warp;
+            auto ids_of = [&](int at, int (&id)[2]) {
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
                     const int b = at * 16 + g + 8 * j;
-                    const int id = b < m ? __ldg(table + a.first + b) : -1;
-                    there[j] = (unsigned)id < (unsigned)p.l.n_pages;
-                    const uint8_t* src = static_cast<const uint8_t*>(a.boxes) + ((long long)(there[j] ? id : 0) * p.l.kv_heads + head) * box_bytes(D);
-#pragma unroll
-                    for (int i = 0; i < V; ++i) box[j][i] = __ldg(reinterpret_cast<const uint4*>(src + 64 * i) + t);
-                    unit[j] = __ldg(reinterpret_cast<const float*>(src + 2 * D));
+                    id[j] = b < m ? __ldg(table + a.first + b) : -1;
                 }
             };
-            int at = rank + p.cluster * warp;
-            if (at < groups) load(at);
+            auto load = [&](const int (&id)[2], Boxes& x) {
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    x.there[j] = (unsigned)id[j] < (unsigned)p.l.n_pages;
+                    const uint8_t* src = static_cast<const uint8_t*>(a.boxes) + ((long long)(x.there[j] ? id[j] : 0) * p.l.kv_heads + head) * box_bytes(D);
+#pragma unroll
+                    for (int i = 0; i < V; ++i) x.word[j][i] = __ldg(reinterpret_cast<const uint4*>(src + 64 * i) + t);
+                    x.unit[j] = __ldg(reinterpret_cast<const float*>(src + 2 * D));
+                }
+            };
+            Boxes x[2];                                            // two steps' boxes and the next one's page ids in flight
+            int id[2], next[2];
+            ids_of(at, id);
+            ids_of(at + stride, next);
+            if (at < groups) load(id, x[0]);
+            if (at + stride < groups) load(next, x[1]);
+            ids_of(at + 2 * stride, id);
 
             // a token a warp: the sums of its heads' parts above and below 0, as int8
             if (warp < p.tile) {
@@ -299,32 +313,31 @@ __global__ void __launch_bounds__(kSelThreads) kv_select_kernel(const SelectPara
             for (int i = 0; i < V; ++i)
                 qw[i] = g < p.tile ? *reinterpret_cast<const uint4*>(query + g * kRow + 64 * i + 16 * t) : make_uint4(0, 0, 0, 0);
             const uint32_t scores_at = (uint32_t)__cvta_generic_to_shared(scores);
-            while (at < groups) {
+            auto score = [&](int at, const Boxes& x) {
                 int acc[4] = {0, 0, 0, 0};
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
-                    mma_s8(acc, box[0][i].x, box[1][i].x, box[0][i].y, box[1][i].y, qw[i].x, qw[i].y);
-                    mma_s8(acc, box[0][i].z, box[1][i].z, box[0][i].w, box[1][i].w, qw[i].z, qw[i].w);
+                    mma_s8(acc, x.word[0][i].x, x.word[1][i].x, x.word[0][i].y, x.word[1][i].y, qw[i].x, qw[i].y);
+                    mma_s8(acc, x.word[0][i].z, x.word[1][i].z, x.word[0][i].w, x.word[1][i].w, qw[i].z, qw[i].w);
                 }
-                float s[2];
-                bool in[2];
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    s[j] = unit[j];
-                    in[j] = there[j];
-                }
-                const int now = at;
-                at += p.cluster * kSelWarps;
-                if (at < groups) load(at);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    const int token = 2 * t + (j & 1), b = now * 16 + g + 8 * (j >> 1);
+                    const int token = 2 * t + (j & 1), b = at * 16 + g + 8 * (j >> 1);
                     if (token >= nt || b >= m) continue;
-                    const float unit = s[j >> 1];
-                    const uint32_t key = !in[j >> 1] ? 0u : ordered(unit < INFINITY ? __fmul_rn((float)acc[j], unit) : INFINITY);
+                    const float unit = x.unit[j >> 1];
+                    const uint32_t key = !x.there[j >> 1] ? 0u : ordered(unit < INFINITY ? __fmul_rn((float)acc[j], unit) : INFINITY);
                     const uint32_t place = (uint32_t)(token / p.cluster) * p.cap + b;
                     if (p.cluster > 1) store_cluster(scores_at + 4 * place, token % p.cluster, key);
                     else scores[place] = key;
+                }
+            };
+            for (; at < groups; at += 2 * stride) {
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    if (at + j * stride >= groups) break;
+                    score(at + j * stride, x[j]);
+                    if (at + (2 + j) * stride < groups) load(id, x[j]);
+                    ids_of(at + (3 + j) * stride, id);
                 }
             }
             if (p.cluster > 1) cluster_sync();
@@ -355,62 +368,119 @@ __global__ void __launch_bounds__(kSelThreads) kv_select_kernel(const SelectPara
                     if (tw == 1) __syncwarp();
                     else asm volatile("bar.sync %0, %1;" ::"r"(1 + team), "r"(threads) : "memory");
                 };
-                int turn = 0;
-                auto total = [&](int x) {                          // over the team
-                    x = __reduce_add_sync(0xffffffffu, x);
-                    if (tw == 1) return x;
-                    if (lane == 0) part[turn][warp] = x;
-                    team_sync();
-                    int all = 0;
-                    for (int w = 0; w < tw; ++w) all += part[turn][team * tw + w];
-                    turn ^= 1;
-                    return all;
-                };
                 if (need > 0) {
-                    // the largest `least` that `need` scores reach
-                    uint32_t least = 0;
-                    for (int bit = 31; bit >= 0; --bit) {
-                        const uint32_t cand = least | 1u << bit;
-                        int x = 0;
-                        for (int b = i; b < mt; b += threads) x += keys[b] >= cand;
-                        x = total(x);
-                        if (x >= need) least = cand;
-                        if (x == need) break;
+                    int* hist = bins[team * tw];
+                    // the range of the scores
+                    uint32_t lo = 0xffffffffu, hi = 0;
+#pragma unroll 8
+                    for (int b = i; b < mt; b += threads) {
+                        lo = min(lo, keys[b]);
+                        hi = max(hi, keys[b]);
                     }
-                    // each member's run of scores: those above it, and those at it, the first of which are taken
-                    const int run = ((mt + threads - 1) / threads) * 32, b0 = member * run, b1 = min(mt, b0 + run);
-                    int above = 0, equal = 0;
-                    for (int b = b0 + lane; b < b1; b += 32) {
-                        above += keys[b] > least;
-                        equal += keys[b] == least;
-                    }
-                    above = __reduce_add_sync(0xffffffffu, above);
-                    equal = __reduce_add_sync(0xffffffffu, equal);
-                    int all_above = above, above0 = 0, equal0 = 0;
+                    lo = __reduce_min_sync(0xffffffffu, lo);
+                    hi = __reduce_max_sync(0xffffffffu, hi);
                     if (tw > 1) {
+                        if (lane == 0) part[warp] = make_int2((int)lo, (int)hi);
                         team_sync();
-                        if (lane == 0) counts[warp] = make_int2(above, equal);
-                        team_sync();
-                        all_above = 0;
                         for (int w = 0; w < tw; ++w) {
-                            const int2 c = counts[team * tw + w];
-                            all_above += c.x;
-                            if (w < member) {
-                                above0 += c.x;
-                                equal0 += c.y;
-                            }
+                            lo = min(lo, (uint32_t)part[team * tw + w].x);
+                            hi = max(hi, (uint32_t)part[team * tw + w].y);
                         }
                     }
-                    const int ties = need - all_above;
+                    // The least score that is taken, and how many of those equal to it: a histogram of the scores in [lo, hi]
+                    // by their upper bits, the bin that holds the `rest`-th largest of them, that bin as the next range
+                    uint32_t least = lo;
+                    for (int rest = need; lo < hi;) {
+                        const int shift = max(0, 32 - __clz(hi - lo) - (31 - __clz(kSelBins * tw)));
+                        reinterpret_cast<int4*>(hist)[2 * i] = reinterpret_cast<int4*>(hist)[2 * i + 1] = make_int4(0, 0, 0, 0);
+                        team_sync();
+#pragma unroll 8
+                        for (int b = i; b < mt; b += threads) {
+                            const uint32_t key = keys[b];
+                            if (key >= lo && key <= hi) atomicAdd(hist + ((key - lo) >> shift), 1);
+                        }
+                        team_sync();
+                        // eight bins a thread, the highest first
+                        const int top = kSelBins * tw - 8 * (i + 1);
+                        int own[8], sum = 0;
+                        *reinterpret_cast<int4*>(own) = reinterpret_cast<const int4*>(hist + top)[0];
+                        *reinterpret_cast<int4*>(own + 4) = reinterpret_cast<const int4*>(hist + top)[1];
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) sum += own[j];
+                        int upto = sum;
+#pragma unroll
+                        for (int o = 1; o < 32; o <<= 1) {
+                            const int x = __shfl_up_sync(0xffffffffu, upto, o);
+                            if (lane >= o) upto += x;
+                        }
+                        if (tw > 1) {
+                            if (lane == 31) part[warp].x = upto;
+                            team_sync();
+                            for (int w = 0; w < member; ++w) upto += part[team * tw + w].x;
+                        }
+                        if (upto - sum < rest && rest <= upto) {
+                            int above = upto - sum;
+#pragma unroll
+                            for (int j = 7; j >= 0; --j) {
+                                if (above < rest && rest <= above + own[j]) found[team] = make_int2(top + j, rest - above == own[j] ? 0 : rest - above);
+                                above += own[j];
+                            }
+                        }
+                        team_sync();
+                        const int2 f = found[team];
+                        least = lo + ((uint32_t)f.x << shift);
+                        rest = f.y;
+                        if (rest == 0 || shift == 0) break;        // the whole bin is taken, or it is one score
+                        hi = least + min(hi - least, (1u << shift) - 1);
+                        lo = least;
+                    }
+                    // each member's run of scores: those above it, and those at it, the first of which are taken
+                    const int run = ((mt + threads - 1) / threads) * 32, b0 = min(mt, member * run), b1 = min(mt, b0 + run);
+                    int above0 = 0, equal0 = 0, ties;
+                    {
+                        int above = 0, equal = 0;
+#pragma unroll 8
+                        for (int b = b0 + lane; b < b1; b += 32) {
+                            above += keys[b] > least;
+                            equal += keys[b] == least;
+                        }
+                        above = __reduce_add_sync(0xffffffffu, above);
+                        equal = __reduce_add_sync(0xffffffffu, equal);
+                        int all = above;
+                        if (tw > 1) {
+                            team_sync();
+                            if (lane == 0) part[warp] = make_int2(above, equal);
+                            team_sync();
+                            all = 0;
+                            for (int w = 0; w < tw; ++w) {
+                                const int2 c = part[team * tw + w];
+                                all += c.x;
+                                if (w < member) {
+                                    above0 += c.x;
+                                    equal0 += c.y;
+                                }
+                            }
+                        }
+                        ties = need - all;
+                    }
+                    // their places in order, by way of shared memory where they fit, so that the table is read all at once
+                    const bool fits = need <= kSelBins * tw;
                     for (int b = b0; b < b1; b += 32) {
                         const uint32_t key = b + lane < b1 ? keys[b + lane] : 0;
                         const unsigned gt = __ballot_sync(0xffffffffu, b + lane < b1 && key > least), eq = __ballot_sync(0xffffffffu, b + lane < b1 && key == least);
                         const unsigned before = (1u << lane) - 1;
                         const int e = equal0 + __popc(eq & before);
-                        if (gt >> lane & 1 || (eq >> lane & 1 && e < ties))
-                            list[a.first + above0 + __popc(gt & before) + min(e, ties)] = entry(a.first + b + lane);
+                        if (gt >> lane & 1 || (eq >> lane & 1 && e < ties)) {
+                            const int place = above0 + __popc(gt & before) + min(e, ties);
+                            if (fits) hist[place] = b + lane;
+                            else list[a.first + place] = entry(a.first + b + lane);
+                        }
                         above0 += __popc(gt);
                         equal0 += __popc(eq);
+                    }
+                    if (fits) {
+                        team_sync();
+                        for (int j = i; j < need; j += threads) list[a.first + j] = entry(a.first + hist[j]);
                     }
                 }
             }
