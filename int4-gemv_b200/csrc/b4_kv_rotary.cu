@@ -8,10 +8,10 @@
 // it lies within 2^-50 of a border, whatever computes it, for 2 DFMA a column of a few
 // heads; queries, whose rounding to 16 bits is next, in fp32.
 //
-// Split.  A CTA takes up to 4 tokens: its threads compute the tokens' angles once,
-// into shared memory, and its warps share the tokens' vectors (heads of q, k, v),
-// 32 * 8 / D of one kind at a time, so that no warp holds two kinds.  The pair's other
-// column is in a lane of the same vector, or in the same thread (adjacent pairs).
+// Split.  A warp takes a token, or a part of its vectors (heads of q, k and v), 32 * 8 / D
+// of one kind at a time, and computes the token's angles itself, one or two a lane: no
+// shared memory, no barrier.  A lane holds four pairs' columns, from both halves of a
+// head (eight neighbours where neighbours pair), so a pair never leaves its lane.
 #include <climits>
 #include <cmath>
 #include <type_traits>
@@ -24,7 +24,7 @@ namespace {
 struct RotaryParams {
     KvLayout l;
     uint8_t* blocks;
-    const void* src[3];                // q, k, v
+    const void* src[3];                // k, v, q
     long long tok[3], head[3];         // their strides
     void* out;
     long long out_tok, out_head;
@@ -32,193 +32,188 @@ struct RotaryParams {
     long long axis_stride;
     const uint64_t* turns;
     const uint8_t* axes;
-    int n, heads, half, adjacent, n_axes;
-    int tokens, parts;                 // of a CTA; CTAs that share a token's vectors
+    int n, heads, half, n_axes;
+    int parts;                         // warps that share a token's vectors
+    bool vec;                          // rows are 16-byte aligned
     float scale;
 };
 
-constexpr int kRotThreads = 256, kRotWarps = kRotThreads / 32, kRotTokens = 4, kRotHalf = 64;
+constexpr int kRotThreads = 256, kRotWarps = kRotThreads / 32;
 
-template <typename T, typename O, int FMT, int D, bool VEC>
-__global__ void __launch_bounds__(kRotThreads) kv_append_rotary_kernel(const RotaryParams p)
+// a lane's 8 columns of T as loaded, four at a and four at b (ADJ: right behind them), and as fp32
+template <typename T, bool ADJ>
+struct Pairs {
+    uint32_t raw[2 * sizeof(T)];
+    __device__ void load(const T* a, const T* b, bool vec)
+    {
+        if (!vec) {
+            T* r = reinterpret_cast<T*>(raw);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                r[i] = a[i];
+                r[4 + i] = b[i];
+            }
+        } else if (sizeof(T) == 4) {
+            *reinterpret_cast<uint4*>(raw) = __ldg(reinterpret_cast<const uint4*>(a));
+            *reinterpret_cast<uint4*>(raw + 4) = __ldg(reinterpret_cast<const uint4*>(b));
+        } else if (ADJ) {
+            *reinterpret_cast<uint4*>(raw) = __ldg(reinterpret_cast<const uint4*>(a));
+        } else {
+            *reinterpret_cast<uint2*>(raw) = __ldg(reinterpret_cast<const uint2*>(a));
+            *reinterpret_cast<uint2*>(raw + 2) = __ldg(reinterpret_cast<const uint2*>(b));
+        }
+    }
+    __device__ float get(int i) const { return kv_float(reinterpret_cast<const T*>(raw)[i]); }
+};
+
+template <typename T, typename O, int FMT, int D, bool ADJ>
+__global__ void __launch_bounds__(kRotThreads, 4) kv_append_rotary_kernel(const RotaryParams p)
 {
     constexpr int TPV = D / 8, VPW = 32 / TPV;         // threads a vector, vectors a warp
-    constexpr int U = sizeof(T) == 2 ? 2 : 1;          // items a warp has in flight
-    // pair i of a token at [i % 8][i / 8] (adjacent: [i % 4][i / 4]), so that lanes of neighbouring columns read neighbours
-    __shared__ double2 turn64[kRotTokens][kRotHalf];
-    __shared__ float2 turn32[kRotTokens][kRotHalf];
+    constexpr int U = sizeof(T) == 2 ? 4 : 2;          // query items in flight
+    constexpr int P = D / 64;                          // pairs whose angles a lane computes
     float boundary = 4.0f;
     int below = 0;
     if (FMT == B4_KV_NF4) nf4_bins(boundary, below);
+    const int lane = threadIdx.x & 31, sub = lane % TPV;
+    const int token = (int)blockIdx.x * kRotWarps + (threadIdx.x >> 5), part = blockIdx.y;
     kv_begin();
+    if (token >= p.n) return;
 
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = lane % TPV;
-    const int t0 = blockIdx.x * p.tokens, n = min(p.tokens, p.n - t0);
-    const int q_items = (p.heads + VPW - 1) / VPW, kv_items = (p.l.kv_heads + VPW - 1) / VPW, all = q_items + 2 * kv_items;
-    const int step = kRotWarps * p.parts, items = n * all;
+    // this lane's columns: pairs i0 .. i0 + 3 where it turns, two groups of four of the others where not
+    const bool turn = sub < p.half / 4;
+    const int i0 = 4 * sub, rest = D - 2 * p.half;
+    const int col_a = ADJ ? 8 * sub : turn ? i0 : p.half + i0;
+    const int col_b = ADJ ? 8 * sub + 4 : turn ? p.half + i0 : p.half + rest / 2 + i0;
+    const int kv_items = (p.l.kv_heads + VPW - 1) / VPW, q_items = (p.heads + VPW - 1) / VPW;
+    auto head_of = [&](int item, int heads) { return min(item * VPW + lane / TPV, heads - 1); };   // whole warps take part in the shuffles
+    auto load = [&](int kind, int head, Pairs<T, ADJ>& x) {
+        const T* src = static_cast<const T*>(p.src[kind]) + token * p.tok[kind] + head * p.head[kind];
+        x.load(src + col_a, src + col_b, p.vec);
+    };
 
-    struct Item {
-        int token, kind, head;
-        bool live;
-    };
-    auto item_of = [&](int i) {
-        Item x;
-        x.token = i / all;
-        int w = i - x.token * all;
-        x.kind = w < q_items ? 0 : w < q_items + kv_items ? 1 : 2;
-        w -= x.kind == 0 ? 0 : x.kind == 1 ? q_items : q_items + kv_items;
-        const int heads = x.kind == 0 ? p.heads : p.l.kv_heads;
-        x.head = w * VPW + lane / TPV;
-        x.live = x.head < heads;
-        x.head = min(x.head, heads - 1);               // whole warps take part in the shuffles
-        return x;
-    };
-    auto load = [&](const Item& x, Columns<T, VEC>& c) {
-        c.load(static_cast<const T*>(p.src[x.kind]) + (t0 + x.token) * p.tok[x.kind] + x.head * p.head[x.kind] + sub * 8);
-    };
-    Item item[U];
-    Columns<T, VEC> c[U];
-    int at = warp * p.parts + blockIdx.y;              // asked for before the angles are computed
+    // ---- keys and values: items 0 .. 2 kv_items - 1 of the token; the first is asked for before the angles are computed ----
+    int at = part;
+    Pairs<T, ADJ> x;
+    if (at < 2 * kv_items) load(at >= kv_items, head_of(at < kv_items ? at : at - kv_items, p.l.kv_heads), x);
+    const int slot = __ldg(p.slots + token), page = slot >> p.l.page_shift;
+
+    double co[P], si[P];                               // pairs P * lane ..
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-        if (at + u * step < items) {
-            item[u] = item_of(at + u * step);
-            load(item[u], c[u]);
-        }
-
-    const int per = p.adjacent ? 4 : 8;
-    for (int e = threadIdx.x; e < n * p.half; e += kRotThreads) {
-        const int token = e / p.half, i = e - token * p.half;
-        const int axis = p.axes ? min((int)__ldg(p.axes + i), p.n_axes - 1) : 0;
-        const long long pos = __ldg(p.positions + axis * p.axis_stride + t0 + token);
-        const uint64_t phase = (uint64_t)pos * __ldg(reinterpret_cast<const unsigned long long*>(p.turns) + i);
-        double s, co;
-        sincospi((double)(int64_t)phase * 0x1p-63, &s, &co);
-        s *= p.scale;
-        co *= p.scale;
-        const int place = i % per * (kRotHalf / 8) * (8 / per) + i / per;
-        turn64[token][place] = make_double2(co, s);
-        turn32[token][place] = make_float2((float)co, (float)s);
+    for (int i = 0; i < P; ++i) {
+        const int pair = min(P * lane + i, p.half - 1);
+        const int axis = p.axes ? min((int)__ldg(p.axes + pair), p.n_axes - 1) : 0;
+        const long long pos = __ldg(p.positions + axis * p.axis_stride + token);
+        const uint64_t phase = (uint64_t)pos * __ldg(reinterpret_cast<const unsigned long long*>(p.turns) + pair);
+        sincospi((double)(int64_t)phase * 0x1p-63, &si[i], &co[i]);
+        si[i] *= p.scale;
+        co[i] *= p.scale;
     }
-    __syncthreads();
+    // pair j of this lane's four
+    auto cos_of = [&](int j) { return __shfl_sync(0xffffffffu, co[j % P], (4 * sub + j) / P & 31); };
+    auto sin_of = [&](int j) { return __shfl_sync(0xffffffffu, si[j % P], (4 * sub + j) / P & 31); };
 
-    // this lane's pairs: halves, h8 lanes hold the first columns and the next h8 the second; adjacent, four pairs a lane
-    const int h8 = p.half / 8;
-    const bool turns = sub < 2 * h8, second = !p.adjacent && sub >= h8;
-    const int other = lane + (p.adjacent || !turns ? 0 : second ? -h8 : h8);
-    const int block = p.adjacent ? sub : second ? sub - h8 : sub;
+    const bool live = slot >= 0 && page < p.l.n_pages;
+    for (; at < 2 * kv_items; at += p.parts) {
+        const bool value = at >= kv_items;
+        const int item = value ? at - kv_items : at;
+        float v[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = x.get(j);
+        if (const int next = at + p.parts; next < 2 * kv_items)
+            load(next >= kv_items, head_of(next < kv_items ? next : next - kv_items, p.l.kv_heads), x);
+        if (!value) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const double c = cos_of(j), s = sin_of(j);
+                float &a = ADJ ? v[2 * j] : v[j], &b = ADJ ? v[2 * j + 1] : v[4 + j];
+                const double da = a, db = b;
+                if (turn) {
+                    a = (float)(da * c - db * s);
+                    b = (float)(db * c + da * s);
+                }
+            }
+        }
+        float scale;
+        __half sh;
+        const uint32_t w = quantised_word<FMT, TPV>(v, boundary, below, scale, sh);
+        const int head = item * VPW + lane / TPV;
+        if (!live || head >= p.l.kv_heads) continue;
+        uint8_t* block = p.blocks + ((long long)page * p.l.kv_heads + head) * p.l.block;
+        const int row = (value ? p.l.page_size : 0) + (slot & (p.l.page_size - 1));
+        if (ADJ) {
+            reinterpret_cast<uint32_t*>(block + row * (D / 2))[sub] = w;
+        } else {
+            *reinterpret_cast<uint16_t*>(block + row * (D / 2) + col_a / 2) = (uint16_t)w;
+            *reinterpret_cast<uint16_t*>(block + row * (D / 2) + col_b / 2) = (uint16_t)(w >> 16);
+        }
+        if (sub == 0) {
+            if (FMT == B4_KV_INT4) reinterpret_cast<__half*>(block + p.l.page_size * D)[row] = sh;
+            else reinterpret_cast<float*>(block + p.l.page_size * D)[row] = scale;
+        }
+    }
 
-    for (; at < items; at += U * step) {
+    // ---- queries ----
+    at -= 2 * kv_items;
+    if (at >= q_items) return;
+    float c[4], s[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        c[j] = (float)cos_of(j);
+        s[j] = (float)sin_of(j);
+    }
+    O* out = static_cast<O*>(p.out) + token * p.out_tok;
+    for (; at < q_items; at += U * p.parts) {
+        Pairs<T, ADJ> x[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (at + u * p.parts < q_items) load(2, head_of(at + u * p.parts, p.heads), x[u]);
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            if (at + u * step >= items) break;
-            const Item x = item[u];
+            const int head = (at + u * p.parts) * VPW + lane / TPV;
+            if (head >= p.heads) continue;
             float v[8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = c[u].get(j);
-            if (x.kind < 2) {
-                float w[8];                            // the pairs' other columns
-                if (!p.adjacent) {
-                    Columns<T, VEC> o;
+            for (int j = 0; j < 8; ++j) v[j] = x[u].get(j);
+            if (turn) {
 #pragma unroll
-                    for (int i = 0; i < (int)sizeof(T) / 2; ++i) {
-                        o.raw[i].x = __shfl_sync(0xffffffffu, c[u].raw[i].x, other);
-                        o.raw[i].y = __shfl_sync(0xffffffffu, c[u].raw[i].y, other);
-                        o.raw[i].z = __shfl_sync(0xffffffffu, c[u].raw[i].z, other);
-                        o.raw[i].w = __shfl_sync(0xffffffffu, c[u].raw[i].w, other);
-                    }
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) w[j] = o.get(j);
-                }
-                if (x.kind == 0 && turns) {
-                    if (p.adjacent) {
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            const float2 t = turn32[x.token][j * 16 + block];
-                            const float a = v[2 * j], b = v[2 * j + 1];
-                            v[2 * j] = a * t.x - b * t.y;
-                            v[2 * j + 1] = b * t.x + a * t.y;
-                        }
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) {
-                            const float2 t = turn32[x.token][j * 8 + block];
-                            v[j] = v[j] * t.x + w[j] * (second ? t.y : -t.y);
-                        }
-                    }
-                }
-                if (x.kind == 1 && turns) {
-                    if (p.adjacent) {
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            const double2 t = turn64[x.token][j * 16 + block];
-                            const double a = v[2 * j], b = v[2 * j + 1];
-                            v[2 * j] = (float)(a * t.x - b * t.y);
-                            v[2 * j + 1] = (float)(b * t.x + a * t.y);
-                        }
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) {
-                            const double2 t = turn64[x.token][j * 8 + block];
-                            v[j] = (float)((double)v[j] * t.x + (double)w[j] * (second ? t.y : -t.y));
-                        }
-                    }
+                for (int j = 0; j < 4; ++j) {
+                    float &a = ADJ ? v[2 * j] : v[j], &b = ADJ ? v[2 * j + 1] : v[4 + j];
+                    const float fa = a, fb = b;
+                    a = fa * c[j] - fb * s[j];
+                    b = fb * c[j] + fa * s[j];
                 }
             }
-            const int token = t0 + x.token;
-            if (x.kind == 0) {
-                if (x.live) {
-                    O* dst = static_cast<O*>(p.out) + token * p.out_tok + x.head * p.out_head + sub * 8;
-                    *reinterpret_cast<uint4*>(dst) = make_uint4(kv_round2<O>(v[0], v[1]), kv_round2<O>(v[2], v[3]), kv_round2<O>(v[4], v[5]),
-                                                                kv_round2<O>(v[6], v[7]));
-                }
+            O* dst = out + head * p.out_head;
+            const uint4 w = make_uint4(kv_round2<O>(v[0], v[1]), kv_round2<O>(v[2], v[3]), kv_round2<O>(v[4], v[5]), kv_round2<O>(v[6], v[7]));
+            if (ADJ) {
+                *reinterpret_cast<uint4*>(dst + col_a) = w;
             } else {
-                float scale;
-                __half sh;
-                const uint32_t w = quantised_word<FMT, TPV>(v, boundary, below, scale, sh);
-                const int slot = __ldg(p.slots + token), page = slot >> p.l.page_shift;
-                if (x.live && slot >= 0 && page < p.l.n_pages) {
-                    uint8_t* b = p.blocks + ((long long)page * p.l.kv_heads + x.head) * p.l.block;
-                    const int row = (x.kind == 2 ? p.l.page_size : 0) + (slot & (p.l.page_size - 1));
-                    reinterpret_cast<uint32_t*>(b + row * (D / 2))[sub] = w;
-                    if (sub == 0) {
-                        if (FMT == B4_KV_INT4) reinterpret_cast<__half*>(b + p.l.page_size * D)[row] = sh;
-                        else reinterpret_cast<float*>(b + p.l.page_size * D)[row] = scale;
-                    }
-                }
-            }
-        }
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int next = at + (U + u) * step;
-            if (next < items) {
-                item[u] = item_of(next);
-                load(item[u], c[u]);
+                *reinterpret_cast<uint2*>(dst + col_a) = make_uint2(w.x, w.y);
+                *reinterpret_cast<uint2*>(dst + col_b) = make_uint2(w.z, w.w);
             }
         }
     }
 }
 
 template <typename T, typename O, int FMT, int D>
-cudaError_t launch(RotaryParams p, bool vec, cudaStream_t st)
+cudaError_t launch(RotaryParams p, bool adjacent, cudaStream_t st)
 {
     constexpr int VPW = 256 / D;
     const int all = (p.heads + VPW - 1) / VPW + 2 * ((p.l.kv_heads + VPW - 1) / VPW);
-    // few tokens: a token's vectors over as many CTAs as give each warp one; many: four tokens a CTA, their angles by one
-    // pass of its threads
-    const bool few = p.n < 148 * kRotTokens;
-    p.tokens = few ? 1 : kRotTokens;
-    p.parts = few ? std::max(1, std::min((all + kRotWarps - 1) / kRotWarps, 148 * 8 / p.n)) : 1;
-    const dim3 grid((unsigned)((p.n + p.tokens - 1) / p.tokens), (unsigned)p.parts);
-    return vec ? kv_launch(kv_append_rotary_kernel<T, O, FMT, D, true>, grid, kRotThreads, 0, st, p)
-               : kv_launch(kv_append_rotary_kernel<T, O, FMT, D, false>, grid, kRotThreads, 0, st, p);
+    // few tokens: a token's vectors over as many warps as fill the GPU.  Each computes the token's angles, some 300
+    // instructions, so no more: 8000 tokens x (28 + 2 x 4) x 128 take 34 us with one warp each, 36 with two, 47 with five
+    p.parts = (int)std::max(1LL, std::min<long long>(all, (148LL * 4 * kRotWarps + p.n - 1) / p.n));
+    const dim3 grid((unsigned)((p.n + kRotWarps - 1LL) / kRotWarps), (unsigned)p.parts);
+    return adjacent ? kv_launch(kv_append_rotary_kernel<T, O, FMT, D, true>, grid, kRotThreads, 0, st, p)
+                    : kv_launch(kv_append_rotary_kernel<T, O, FMT, D, false>, grid, kRotThreads, 0, st, p);
 }
 
 template <typename T, typename O>
-cudaError_t launch(const RotaryParams& p, bool vec, cudaStream_t st)
+cudaError_t launch(const RotaryParams& p, bool adjacent, cudaStream_t st)
 {
-    if (p.l.fmt == B4_KV_INT4) return p.l.head_dim == 64 ? launch<T, O, B4_KV_INT4, 64>(p, vec, st) : launch<T, O, B4_KV_INT4, 128>(p, vec, st);
-    return p.l.head_dim == 64 ? launch<T, O, B4_KV_NF4, 64>(p, vec, st) : launch<T, O, B4_KV_NF4, 128>(p, vec, st);
+    if (p.l.fmt == B4_KV_INT4) return p.l.head_dim == 64 ? launch<T, O, B4_KV_INT4, 64>(p, adjacent, st) : launch<T, O, B4_KV_INT4, 128>(p, adjacent, st);
+    return p.l.head_dim == 64 ? launch<T, O, B4_KV_NF4, 64>(p, adjacent, st) : launch<T, O, B4_KV_NF4, 128>(p, adjacent, st);
 }
 
 }  // namespace
@@ -264,15 +259,15 @@ int b4_kv_append_rotary(const b4_kv_cache* cache, const b4_rotary* r, const b4_k
         return cudaErrorInvalidValue;
     if (r->n_axes > 1 && (!r->axes || x->position_stride < x->n_tokens)) return cudaErrorInvalidValue;
     p.blocks = static_cast<uint8_t*>(cache->blocks);
-    p.src[0] = x->q;
-    p.src[1] = x->k;
-    p.src[2] = x->v;
-    p.tok[0] = x->q_stride_token;
-    p.tok[1] = x->k_stride_token;
-    p.tok[2] = x->v_stride_token;
-    p.head[0] = x->q_stride_head;
-    p.head[1] = x->k_stride_head;
-    p.head[2] = x->v_stride_head;
+    p.src[0] = x->k;
+    p.src[1] = x->v;
+    p.src[2] = x->q;
+    p.tok[0] = x->k_stride_token;
+    p.tok[1] = x->v_stride_token;
+    p.tok[2] = x->q_stride_token;
+    p.head[0] = x->k_stride_head;
+    p.head[1] = x->v_stride_head;
+    p.head[2] = x->q_stride_head;
     p.out = x->q_out;
     p.out_tok = x->out_stride_token;
     p.out_head = x->out_stride_head;
@@ -285,19 +280,19 @@ int b4_kv_append_rotary(const b4_kv_cache* cache, const b4_rotary* r, const b4_k
     p.heads = x->heads;
     p.half = r->dim / 2;
     p.n_axes = r->n_axes;
-    p.adjacent = r->flags & B4_ROTARY_ADJACENT;
     p.scale = r->scale;
-    long long strides = p.tok[1] | p.head[1] | p.tok[2] | p.head[2];
-    bool vec = kv_aligned(x->k, 16) && kv_aligned(x->v, 16);
+    long long strides = p.tok[0] | p.head[0] | p.tok[1] | p.head[1];
+    p.vec = kv_aligned(x->k, 16) && kv_aligned(x->v, 16);
     if (x->heads > 0) {
-        strides |= p.tok[0] | p.head[0];
-        vec = vec && kv_aligned(x->q, 16);
+        strides |= p.tok[2] | p.head[2];
+        p.vec = p.vec && kv_aligned(x->q, 16);
     }
-    vec = vec && strides * (long long)item % 16 == 0;
+    p.vec = p.vec && strides * (long long)item % 16 == 0;
+    const bool adjacent = r->flags & B4_ROTARY_ADJACENT;
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-    if (x->dtype == B4_DTYPE_F16) return launch<__half, __half>(p, vec, st);
-    if (x->dtype == B4_DTYPE_BF16) return launch<__nv_bfloat16, __nv_bfloat16>(p, vec, st);
-    return x->out_dtype == B4_DTYPE_F16 ? launch<float, __half>(p, vec, st) : launch<float, __nv_bfloat16>(p, vec, st);
+    if (x->dtype == B4_DTYPE_F16) return launch<__half, __half>(p, adjacent, st);
+    if (x->dtype == B4_DTYPE_BF16) return launch<__nv_bfloat16, __nv_bfloat16>(p, adjacent, st);
+    return x->out_dtype == B4_DTYPE_F16 ? launch<float, __half>(p, adjacent, st) : launch<float, __nv_bfloat16>(p, adjacent, st);
 }
 
 }  // extern "C"

@@ -36,59 +36,64 @@ struct BoxParams {
     const uint8_t* blocks;
     uint8_t* boxes;
     const int32_t* slots;
-    int n, per;                            // tokens, and those that a warp looks at
+    int n, per;                            // tokens, and those that a CTA looks at
 };
 
 // int8 code of x in units of s, rounded to even
 __device__ __forceinline__ int box_code(float x, float s) { return min(127, max(-127, __float2int_rn(__fdiv_rn(x, s)))); }
 
-// A warp makes the boxes of the completed pages among its tokens, of one kv head: a lane holds the
-// extremes of 8 columns over the tokens of its parity (D = 128; of its rest by 4: D = 64).
+// A CTA makes the boxes of the completed pages among its tokens, of one kv head: its warps share a page's tokens, a
+// lane holds the extremes of 8 columns over those of its rows (every second token, D = 128; fourth, D = 64).
+constexpr int kBoxWarps = 8;
+
 template <int FMT, int D>
-__global__ void __launch_bounds__(256) kv_boxes_kernel(const BoxParams p)
+__global__ void __launch_bounds__(32 * kBoxWarps) kv_boxes_kernel(const BoxParams p)
 {
-    constexpr int TPV = D / 8, ROWS = 32 / TPV;
-    const int lane = threadIdx.x & 31, sub = lane % TPV, head = blockIdx.y;
-    const long long first = ((long long)blockIdx.x * 8 + (threadIdx.x >> 5)) * p.per;
+    constexpr int TPV = D / 8, ROWS = 32 / TPV, STEP = ROWS * kBoxWarps;
+    __shared__ float extreme[kBoxWarps][2][D];
+    __shared__ float tops[D / 32];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, sub = lane % TPV, head = blockIdx.y;
+    const long long first = (long long)blockIdx.x * p.per;
     const float level = c_nf4_table[lane & 15];
     kv_begin();
-    if (first >= p.n) return;
     const int slot = lane < p.per && first + lane < p.n ? __ldg(p.slots + first + lane) : -1;
     const int mask = p.l.page_size - 1;
     const bool ends = slot >= 0 && (slot & mask) == mask && slot >> p.l.page_shift < p.l.n_pages;
-    for (unsigned todo = __ballot_sync(0xffffffffu, ends); todo; todo &= todo - 1) {
+    for (unsigned todo = __ballot_sync(0xffffffffu, ends); todo; todo &= todo - 1) {       // the same in every warp
         const int page = __shfl_sync(0xffffffffu, slot, __ffs(todo) - 1) >> p.l.page_shift;
         const long long at = (long long)page * p.l.kv_heads + head;
         const uint8_t* block = p.blocks + at * p.l.block;
         const uint8_t* scales = block + p.l.page_size * D;
-        float s[2];                        // of tokens lane and lane + 32
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int t = min(lane + 32 * i, mask);
-            s[i] = FMT == B4_KV_INT4 ? __half2float(reinterpret_cast<const __half*>(scales)[t]) : reinterpret_cast<const float*>(scales)[t];
-        }
         float hi[8], lo[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             hi[j] = -INFINITY;
             lo[j] = INFINITY;
         }
-        const uint32_t* codes = reinterpret_cast<const uint32_t*>(block) + lane;           // ROWS tokens of 4 * TPV bytes at a time
-#pragma unroll 8
-        for (int t = 0; t < p.l.page_size; t += ROWS) {
-            const uint32_t w = codes[t * TPV];
-            const int token = t + lane / TPV;
-            const float a = __shfl_sync(0xffffffffu, s[0], token & 31), b = __shfl_sync(0xffffffffu, s[1], token & 31);
-            const float scale = token < 32 ? a : b;
+        uint32_t w[64 / STEP];
+        float s[64 / STEP];
+#pragma unroll
+        for (int i = 0; i < 64 / STEP; ++i) {
+            const int token = i * STEP + warp * ROWS + lane / TPV;
+            w[i] = 0;
+            s[i] = 0.0f;
+            if (token > mask) continue;
+            w[i] = reinterpret_cast<const uint32_t*>(block)[token * TPV + sub];
+            s[i] = FMT == B4_KV_INT4 ? __half2float(reinterpret_cast<const __half*>(scales)[token]) : reinterpret_cast<const float*>(scales)[token];
+        }
+#pragma unroll
+        for (int i = 0; i < 64 / STEP; ++i) {
+            const bool in = i * STEP + warp * ROWS + lane / TPV <= mask;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                const uint32_t c = w >> (4 * j) & 15;
-                const float v = __fmul_rn(FMT == B4_KV_INT4 ? (float)((int)c - 8) : __shfl_sync(0xffffffffu, level, c), scale);
-                hi[j] = fmaxf(hi[j], v);
-                lo[j] = fminf(lo[j], v);
+                const uint32_t c = w[i] >> (4 * j) & 15;
+                const float v = __fmul_rn(FMT == B4_KV_INT4 ? (float)((int)c - 8) : __shfl_sync(0xffffffffu, level, c), s[i]);
+                if (in) {
+                    hi[j] = fmaxf(hi[j], v);
+                    lo[j] = fminf(lo[j], v);
+                }
             }
         }
-        float top = 0.0f;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
 #pragma unroll
@@ -96,23 +101,34 @@ __global__ void __launch_bounds__(256) kv_boxes_kernel(const BoxParams p)
                 hi[j] = fmaxf(hi[j], __shfl_xor_sync(0xffffffffu, hi[j], o));
                 lo[j] = fminf(lo[j], __shfl_xor_sync(0xffffffffu, lo[j], o));
             }
-            if (hi[j] < lo[j]) hi[j] = lo[j] = 0.0f;                                       // no number in the column
-            top = fmaxf(top, fmaxf(fabsf(hi[j]), fabsf(lo[j])));
-        }
-#pragma unroll
-        for (int o = TPV / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        const float unit = top > 0.0f ? __fmul_rn(top, 1.0f / 127.0f) : 1.0f;
-        uint8_t* box = p.boxes + at * box_bytes(D);
-        if (lane < TPV) {
-            uint32_t w[4] = {0, 0, 0, 0};
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                w[j / 4] |= (uint32_t)(box_code(hi[j], unit) & 255) << (j % 4 * 8);
-                w[2 + j / 4] |= (uint32_t)(box_code(lo[j], unit) & 255) << (j % 4 * 8);
+            if (lane < TPV) {
+                extreme[warp][0][8 * sub + j] = hi[j];
+                extreme[warp][1][8 * sub + j] = lo[j];
             }
-            reinterpret_cast<uint2*>(box)[sub] = make_uint2(w[0], w[1]);
-            reinterpret_cast<uint2*>(box + D)[sub] = make_uint2(w[2], w[3]);
-            if (sub == 0) *reinterpret_cast<uint4*>(box + 2 * D) = make_uint4(__float_as_uint(unit), 0, 0, 0);
+        }
+        __syncthreads();
+        float h = -INFINITY, l = INFINITY, top = 0.0f;             // of column tid
+        if (tid < D) {
+#pragma unroll
+            for (int k = 0; k < kBoxWarps; ++k) {
+                h = fmaxf(h, extreme[k][0][tid]);
+                l = fminf(l, extreme[k][1][tid]);
+            }
+            if (h < l) h = l = 0.0f;                               // no number in the column
+            top = fmaxf(fabsf(h), fabsf(l));
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+            if (lane == 0) tops[warp] = top;
+        }
+        __syncthreads();
+        if (tid < D) {
+#pragma unroll
+            for (int k = 0; k < D / 32; ++k) top = fmaxf(top, tops[k]);
+            const float unit = top > 0.0f ? __fmul_rn(top, 1.0f / 127.0f) : 1.0f;
+            uint8_t* box = p.boxes + at * box_bytes(D);
+            box[tid] = (uint8_t)box_code(h, unit);
+            box[D + tid] = (uint8_t)box_code(l, unit);
+            if (tid < 4) reinterpret_cast<uint32_t*>(box + 2 * D)[tid] = tid == 0 ? __float_as_uint(unit) : 0u;
         }
     }
 }
@@ -526,8 +542,9 @@ cudaError_t launch_select(SelectParams p, cudaStream_t st)
 template <int FMT>
 cudaError_t launch_boxes(const BoxParams& p, cudaStream_t st)
 {
-    const dim3 grid((unsigned)((p.n + 8LL * p.per - 1) / (8 * p.per)), (unsigned)p.l.kv_heads);
-    return p.l.head_dim == 64 ? kv_launch(kv_boxes_kernel<FMT, 64>, grid, 256, 0, st, p) : kv_launch(kv_boxes_kernel<FMT, 128>, grid, 256, 0, st, p);
+    const dim3 grid((unsigned)((p.n + (long long)p.per - 1) / p.per), (unsigned)p.l.kv_heads);
+    return p.l.head_dim == 64 ? kv_launch(kv_boxes_kernel<FMT, 64>, grid, 32 * kBoxWarps, 0, st, p)
+                              : kv_launch(kv_boxes_kernel<FMT, 128>, grid, 32 * kBoxWarps, 0, st, p);
 }
 
 }  // namespace
@@ -556,7 +573,7 @@ int b4_kv_boxes(const b4_kv_cache* cache, const int32_t* slots, int n_tokens, vo
     p.boxes = static_cast<uint8_t*>(boxes);
     p.slots = slots;
     p.n = n_tokens;
-    p.per = (long long)n_tokens * p.l.kv_heads <= 148 * 32 ? 1 : 16;
+    p.per = (int)std::max(1LL, std::min(16LL, (long long)n_tokens * p.l.kv_heads / (148 * 8)));
     return p.l.fmt == B4_KV_INT4 ? launch_boxes<B4_KV_INT4>(p, reinterpret_cast<cudaStream_t>(stream))
                                  : launch_boxes<B4_KV_NF4>(p, reinterpret_cast<cudaStream_t>(stream));
 }
