@@ -20,6 +20,7 @@
 // which chooses for it.
 #include <algorithm>
 #include <climits>
+#include <type_traits>
 
 #include "b4_kv.cuh"
 
@@ -137,17 +138,27 @@ __global__ void __launch_bounds__(32 * kBoxWarps) kv_boxes_kernel(const BoxParam
 struct SelectParams {
     KvLayout l;
     b4_kv_choice c;
-    int group, tile, cluster, cap;         // heads of a kv head, tokens of a tile, CTAs of a cluster, scores of a token
+    int group, tile, cap;                  // heads of a kv head, tokens of a tile, words of a token's scores
+    int lg;                                // a cluster has 2^lg CTAs
     int direct;                            // a tile index is a request's
 };
 
-constexpr int kSelThreads = 256, kSelWarps = kSelThreads / 32, kSelTile = 8, kSelBins = 256;
+constexpr int kSelThreads = 256, kSelWarps = kSelThreads / 32, kSelBins = 256;
+constexpr int kSelSmem = 200 * 1024;       // of scores
 
 __device__ __forceinline__ void mma_s8(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1)
 {
     asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// past L1, which keeps the table
+__device__ __forceinline__ uint4 load_once(const uint4* p)
+{
+    uint4 v;
+    asm("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
 }
 
 // larger for larger x; 0 below all of them
@@ -169,6 +180,53 @@ __device__ __forceinline__ void store_cluster(uint32_t at, uint32_t rank, uint32
     asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(there), "r"(v) : "memory");
 }
 
+// sum + err += x exactly, as long as err's own sum is: two numbers of 24 bits hold the sum of 64 fp16 numbers
+__device__ __forceinline__ void add_exact(float& sum, float& err, float x)
+{
+    const float s = __fadd_rn(sum, x), part = __fsub_rn(s, sum);
+    err = __fadd_rn(err, __fadd_rn(__fsub_rn(sum, __fsub_rn(s, part)), __fsub_rn(x, part)));
+    sum = s;
+}
+
+// The codes of C columns of a query's sums above and below 0, from the definition; by whole warps.  Its first 8 heads as loaded.
+template <typename T, int C, typename Raw>
+__device__ void exact_codes(const Raw (&raw)[8], const T* src, int group, long long stride, uint32_t (&w)[2])
+{
+    float sum[2][C], err[2][C], top = 0.0f;
+#pragma unroll
+    for (int j = 0; j < C; ++j) sum[0][j] = sum[1][j] = err[0][j] = err[1][j] = 0.0f;
+    auto add = [&](const Raw& r) {
+#pragma unroll
+        for (int j = 0; j < C; ++j) {
+            const float f = kv_float(reinterpret_cast<const T*>(&r)[j]);
+            add_exact(sum[0][j], err[0][j], f > 0.0f ? f : 0.0f);
+            add_exact(sum[1][j], err[1][j], f > 0.0f ? 0.0f : f);      // NaN too
+        }
+    };
+#pragma unroll
+    for (int h = 0; h < 8; ++h)
+        if (h < group) add(raw[h]);
+    for (int h = 8; h < group; ++h) add(__ldg(reinterpret_cast<const Raw*>(src + h * stride)));
+    bool finite = true;
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+#pragma unroll
+        for (int j = 0; j < C; ++j) {
+            sum[k][j] = __fadd_rn(sum[k][j], err[k][j]);
+            finite = finite && fabsf(sum[k][j]) < INFINITY;
+            top = fmaxf(top, fabsf(sum[k][j]));
+        }
+    top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
+    finite = __all_sync(0xffffffffu, finite);
+    const float unit = top > 0.0f ? __fmul_rn(top, 1.0f / 127.0f) : 1.0f;
+    w[0] = w[1] = 0;
+    if (!finite) return;
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+#pragma unroll
+        for (int j = 0; j < C; ++j) w[k] |= (uint32_t)(box_code(sum[k][j], unit) & 255) << (8 * j);
+}
+
 // What a query sees: its pages, its own the last, and its list's entries and tokens.
 struct Seen {
     int pages, entries, tokens;
@@ -188,70 +246,71 @@ __device__ __forceinline__ Seen seen_of(const SelectParams& p, int ctx, int n, i
     return s;
 }
 
-template <typename T, int D>
-__global__ void __launch_bounds__(kSelThreads) kv_select_kernel(const SelectParams p)
+// NT: eights of tokens in a tile
+template <typename T, int D, int NT>
+__global__ void __launch_bounds__(kSelThreads, 2) kv_select_kernel(const SelectParams p)
 {
     constexpr int V = D / 32;                                      // 16-byte words of a box that a lane holds
+    constexpr int C = D / 32;                                      // columns of a query that a lane holds
     constexpr int kRow = 2 * D + 64;
+    constexpr int kAhead = NT == 1 ? 2 : 1;                        // steps of boxes in flight
     extern __shared__ __align__(16) uint32_t scores[];             // [tokens of this CTA][cap]
-    __shared__ __align__(16) uint8_t query[kSelTile * kRow];       // above, below of a token
-    __shared__ __align__(16) int bins[kSelWarps][kSelBins];        // of a team's warps together; then the places of its choice
-    __shared__ int2 part[kSelWarps], found[kSelWarps];
+    __shared__ __align__(16) uint8_t query[8 * NT * kRow];         // above, below of a token
+    __shared__ __align__(16) int bins[kSelWarps][kSelBins];        // of a team's warps together
+    __shared__ uint2 range[16 * NT * kSelWarps];                    // [tokens of this CTA][CTAs][warps] least and largest score
+    __shared__ int2 part[kSelWarps];
+    __shared__ int4 found[kSelWarps];
+    __shared__ uint32_t tied[kSelWarps][32];
+    __shared__ int ties[kSelWarps];
 
     const b4_kv_choice& a = p.c;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int rank = blockIdx.x % p.cluster, head = blockIdx.y;
-    const int at_tile = blockIdx.x / p.cluster;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
+    const int cluster = 1 << p.lg, rank = blockIdx.x & (cluster - 1), head = blockIdx.y;
+    const int at_tile = blockIdx.x >> p.lg;
+    const int stride = kSelWarps << p.lg, step0 = rank + (warp << p.lg);           // of 16 boxes
     kv_begin();
 
     // ---- the request and its tokens ----
     auto start = [&](int r) { return max(0, min(__ldg(a.q_starts + r), a.total_q)); };
     int r = at_tile, tile0 = 0;
     if (!p.direct) {
-        // request r has the tiles from start / 8 + r on, more than it needs at most: the last that begins at or before this one
+        // request r has the tiles from start / tile + r on, as many as it needs at least: the last that begins at or before this one
         int lo = 0, n = a.n_req;
         while (n > 1) {
             const int step = (n + 31) / 32, probe = lo + lane * step;
-            const bool in = lane * step < n && (lane == 0 || start(probe) / kSelTile + probe <= at_tile);
+            const bool in = lane * step < n && (lane == 0 || start(probe) / (8 * NT) + probe <= at_tile);
             const int last = 31 - __clz(__ballot_sync(0xffffffffu, in));
             n = min(step, n - last * step);
             lo += last * step;
         }
         r = lo;
-        tile0 = at_tile - (start(r) / kSelTile + r);
-    }
-    const int q0 = start(r), n = max(0, start(r + 1) - q0), ctx = max(0, __ldg(a.ctx_len + r));
-    // rows of no request
-    if (head == 0) {
-        const int end = start(a.n_req);
-        for (long long t = end + (long long)blockIdx.x * kSelThreads + tid; t < a.total_q; t += (long long)gridDim.x * kSelThreads) a.seen[t] = -1;
-        if (const int begin = start(0); begin > 0)
-            for (long long t = (long long)blockIdx.x * kSelThreads + tid; t < begin; t += (long long)gridDim.x * kSelThreads) a.seen[t] = -1;
+        tile0 = at_tile - (start(r) / (8 * NT) + r);
     }
     const int32_t* table = a.tables + (long long)r * a.table_stride;
+    auto ids_of = [&](int step, int (&id)[2]) {                    // page ids of rows g and g + 8
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const int b = a.first + step * 16 + g + 8 * j;
+            id[j] = b < a.table_width ? __ldg(table + b) : -1;
+        }
+    };
+    int id[2], next[2];                    // asked for before the request's length is known
+    ids_of(step0, id);
+    ids_of(step0 + stride, next);
+    const int q0 = start(r), n = max(0, start(r + 1) - q0), ctx = max(0, __ldg(a.ctx_len + r));
 
-    for (int i0 = tile0 * p.tile; i0 < n; i0 = p.direct ? i0 + p.tile : n) {
+    for (int i0 = tile0 * p.tile, turn = 0; i0 < n; i0 = p.direct ? i0 + p.tile : n, ++turn) {
         const int nt = min(p.tile, n - i0);
         const Seen most = seen_of(p, ctx, n, i0 + nt - 1);
         const int m = most.pages > a.keep ? most.pages - a.first - a.last : 0;     // pages to score
 
         if (m > 0) {
-            // ---- scores: this CTA's boxes, 16 a warp at a time ----
-            const int g = lane >> 2, t = lane & 3;
+            // ---- scores: this CTA's boxes, 16 a warp at a time, two steps of them in flight ----
             const int groups = (m + 15) / 16;
-            struct Boxes {                                         // of a step: rows g and g + 8
+            struct Boxes {
                 uint4 word[2][V];
                 float unit[2];
                 bool there[2];
-            };
-            const int stride = p.cluster * kSelWarps;
-            int at = rank + p.cluster * warp;
-            auto ids_of = [&](int at, int (&id)[2]) {
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    const int b = at * 16 + g + 8 * j;
-                    id[j] = b < m ? __ldg(table + a.first + b) : -1;
-                }
             };
             auto load = [&](const int (&id)[2], Boxes& x) {
 #pragma unroll
@@ -259,113 +318,179 @@ __global__ void __launch_bounds__(kSelThreads) kv_select_kernel(const SelectPara
                     x.there[j] = (unsigned)id[j] < (unsigned)p.l.n_pages;
                     const uint8_t* src = static_cast<const uint8_t*>(a.boxes) + ((long long)(x.there[j] ? id[j] : 0) * p.l.kv_heads + head) * box_bytes(D);
 #pragma unroll
-                    for (int i = 0; i < V; ++i) x.word[j][i] = __ldg(reinterpret_cast<const uint4*>(src + 64 * i) + t);
+                    for (int i = 0; i < V; ++i) x.word[j][i] = load_once(reinterpret_cast<const uint4*>(src + 64 * i) + t);
                     x.unit[j] = __ldg(reinterpret_cast<const float*>(src + 2 * D));
                 }
             };
-            Boxes x[2];                                            // two steps' boxes and the next one's page ids in flight
-            int id[2], next[2];
-            ids_of(at, id);
-            ids_of(at + stride, next);
-            if (at < groups) load(id, x[0]);
-            if (at + stride < groups) load(next, x[1]);
-            ids_of(at + 2 * stride, id);
-
-            // a token a warp: the sums of its heads' parts above and below 0, as int8
-            if (warp < p.tile) {
-                constexpr int C = D / 32;                          // columns of a lane
-                double above[C], below[C];
+            // a token a warp (and every 8th): its first 8 heads, asked for before the boxes' page ids are waited for
+            using Raw = typename std::conditional<C == 4, uint2, uint32_t>::type;
+            auto row_of = [&](int i) {
+                return static_cast<const T*>(a.q) + (q0 + i0 + i) * a.q_stride_token + (long long)head * p.group * a.q_stride_head + lane * C;
+            };
+            auto heads_of = [&](int i, Raw (&raw)[8]) {
+                if (i < nt) {
+                    const T* src = row_of(i);
 #pragma unroll
-                for (int j = 0; j < C; ++j) above[j] = below[j] = 0.0;
-                if (warp < nt) {
-                    const T* src = static_cast<const T*>(a.q) + (q0 + i0 + warp) * a.q_stride_token + (long long)head * p.group * a.q_stride_head + lane * C;
-#pragma unroll 8
-                    for (int h = 0; h < p.group; ++h) {
-                        T x[C];
-                        if (C == 4) *reinterpret_cast<uint2*>(x) = __ldg(reinterpret_cast<const uint2*>(src + h * a.q_stride_head));
-                        else *reinterpret_cast<uint32_t*>(x) = __ldg(reinterpret_cast<const uint32_t*>(src + h * a.q_stride_head));
+                    for (int h = 0; h < 8; ++h)
+                        if (h < p.group) raw[h] = __ldg(reinterpret_cast<const Raw*>(src + h * a.q_stride_head));
+                }
+            };
+            Raw raw[8];
+            heads_of(warp, raw);
+            if (turn > 0) {
+                ids_of(step0, id);
+                ids_of(step0 + stride, next);
+            }
+            Boxes x[kAhead];
+            int at = step0;
+            if (at < groups) load(id, x[0]);
+
+            // The sums of the heads' parts above and below 0, as int8: from sums in fp32 where every code is further from its
+            // next than those can be off (2^-24 for each of a sum's roundings, in it and in the largest, and 2^-21 of the
+            // scale and the quotient: of 127 units); from exact ones otherwise (6 % of the rows of 8 heads)
+#pragma unroll 1
+            for (int i = warp; i < 8 * NT; i += kSelWarps) {
+                if (i > warp) heads_of(i, raw);
+                uint32_t w[2] = {0, 0};
+                if (i < nt) {
+                    float part[2][C], top = 0.0f;
+                    bool finite = true;
+#pragma unroll
+                    for (int j = 0; j < C; ++j) {
+                        float v[8];
+#pragma unroll
+                        for (int h = 0; h < 8; ++h) v[h] = h < p.group ? kv_float(reinterpret_cast<const T*>(&raw[h])[j]) : 0.0f;
+                        part[0][j] = ((fmaxf(v[0], 0.0f) + fmaxf(v[1], 0.0f)) + (fmaxf(v[2], 0.0f) + fmaxf(v[3], 0.0f))) +
+                                     ((fmaxf(v[4], 0.0f) + fmaxf(v[5], 0.0f)) + (fmaxf(v[6], 0.0f) + fmaxf(v[7], 0.0f)));
+                        part[1][j] = ((fminf(v[0], 0.0f) + fminf(v[1], 0.0f)) + (fminf(v[2], 0.0f) + fminf(v[3], 0.0f))) +
+                                     ((fminf(v[4], 0.0f) + fminf(v[5], 0.0f)) + (fminf(v[6], 0.0f) + fminf(v[7], 0.0f)));
+                        const float sum = ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
+                        finite = finite && fabsf(sum) < INFINITY;                          // NaN too
+                    }
+                    const T* src = row_of(i);
+#pragma unroll 4
+                    for (int h = 8; h < p.group; ++h) {
+                        const Raw r = __ldg(reinterpret_cast<const Raw*>(src + h * a.q_stride_head));
 #pragma unroll
                         for (int j = 0; j < C; ++j) {
-                            const float v = kv_float(x[j]);
-                            above[j] += v > 0.0f ? v : 0.0f;
-                            below[j] += v > 0.0f ? 0.0f : v;       // NaN too
+                            const float v = kv_float(reinterpret_cast<const T*>(&r)[j]);
+                            part[0][j] += fmaxf(v, 0.0f);
+                            part[1][j] += fminf(v, 0.0f);
+                            finite = finite && fabsf(v) < INFINITY;
+                        }
+                    }
+#pragma unroll
+                    for (int j = 0; j < C; ++j) top = fmaxf(top, fmaxf(part[0][j], -part[1][j]));
+                    top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
+                    const float inv = __fdividef(127.0f, top), clear = 0.5f - 8e-5f - 1.6e-5f * (p.group <= 8 ? 3 : p.group);
+                    bool sure = finite && top > 1e-30f && top < 1e30f;
+#pragma unroll
+                    for (int k = 0; k < 2; ++k)
+#pragma unroll
+                        for (int j = 0; j < C; ++j) {
+                            const float y = part[k][j] * inv, r = y + 12582912.0f;         // 1.5 * 2^23: the integer nearest to y in the low bits
+                            sure = sure && fabsf(y - (r - 12582912.0f)) < clear;
+                            w[k] |= (__float_as_uint(r) & 255) << (8 * j);
+                        }
+                    if (!__all_sync(0xffffffffu, sure)) exact_codes<T, C>(raw, src, p.group, a.q_stride_head, w);
+                }
+                uint8_t* dst = query + i * kRow + lane * C;
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    if (C == 4) *reinterpret_cast<uint32_t*>(dst + k * D) = w[k];
+                    else *reinterpret_cast<uint16_t*>(dst + k * D) = (uint16_t)w[k];
+                }
+            }
+            if (kAhead == 2) {
+                if (at + stride < groups) load(next, x[kAhead - 1]);
+                ids_of(at + 2 * stride, next);
+            }
+            if (cluster > 1) cluster_sync();                       // the others have begun, or are done with the last tile's scores
+            else __syncthreads();
+
+            auto query_of = [&](int nt8, int i) { return *reinterpret_cast<const uint4*>(query + (nt8 * 8 + g) * kRow + 64 * i + 16 * t); };
+            const uint32_t scores_at = (uint32_t)__cvta_generic_to_shared(scores);
+            uint32_t lo[NT][2], hi[NT][2];
+#pragma unroll
+            for (int nt8 = 0; nt8 < NT; ++nt8)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    lo[nt8][j] = 0xffffffffu;
+                    hi[nt8][j] = 0;
+                }
+            auto score = [&](int step, const Boxes& x) {
+#pragma unroll
+                for (int nt8 = 0; nt8 < NT; ++nt8) {
+                    if (nt8 * 8 >= nt) break;
+                    int acc[4] = {0, 0, 0, 0};
+#pragma unroll
+                    for (int i = 0; i < V; ++i) {
+                        const uint4 q = query_of(nt8, i);
+                        mma_s8(acc, x.word[0][i].x, x.word[1][i].x, x.word[0][i].y, x.word[1][i].y, q.x, q.y);
+                        mma_s8(acc, x.word[0][i].z, x.word[1][i].z, x.word[0][i].w, x.word[1][i].w, q.z, q.w);
+                    }
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const int token = nt8 * 8 + 2 * t + (j & 1), b = step * 16 + g + 8 * (j >> 1);
+                        if (token >= nt || b >= m) continue;
+                        const float unit = x.unit[j >> 1];
+                        const uint32_t key = !x.there[j >> 1] ? 0u : ordered(unit < INFINITY ? __fmul_rn((float)acc[j], unit) : INFINITY);
+                        lo[nt8][j & 1] = min(lo[nt8][j & 1], key);
+                        hi[nt8][j & 1] = max(hi[nt8][j & 1], key);
+                        const uint32_t place = (uint32_t)(token >> p.lg) * p.cap + b;
+                        if (cluster > 1) store_cluster(scores_at + 4 * place, token & (cluster - 1), key);
+                        else scores[place] = key;
+                    }
+                }
+            };
+            // `next` holds the ids of the step after those in flight
+            for (; at < groups; at += kAhead * stride) {
+#pragma unroll
+                for (int j = 0; j < kAhead; ++j) {
+                    if (at + j * stride >= groups) break;
+                    score(at + j * stride, x[j]);
+                    if (at + (kAhead + j) * stride < groups) load(next, x[j]);
+                    ids_of(at + (kAhead + 1 + j) * stride, next);
+                }
+            }
+            const uint32_t range_at = (uint32_t)__cvta_generic_to_shared(range);
+#pragma unroll
+            for (int nt8 = 0; nt8 < NT; ++nt8)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+#pragma unroll
+                    for (int o = 4; o < 32; o <<= 1) {
+                        lo[nt8][j] = min(lo[nt8][j], __shfl_xor_sync(0xffffffffu, lo[nt8][j], o));
+                        hi[nt8][j] = max(hi[nt8][j], __shfl_xor_sync(0xffffffffu, hi[nt8][j], o));
+                    }
+                    const int token = nt8 * 8 + 2 * t + j;
+                    if (g == 0 && token < nt) {
+                        const int place = (((token >> p.lg) << p.lg) + rank) * kSelWarps + warp;
+                        if (cluster > 1) {
+                            store_cluster(range_at + 8 * place, token & (cluster - 1), lo[nt8][j]);
+                            store_cluster(range_at + 8 * place + 4, token & (cluster - 1), hi[nt8][j]);
+                        } else {
+                            range[place] = make_uint2(lo[nt8][j], hi[nt8][j]);
                         }
                     }
                 }
-                float hi[C], lo[C], top = 0.0f;
-                bool finite = true;
-#pragma unroll
-                for (int j = 0; j < C; ++j) {
-                    hi[j] = (float)above[j];
-                    lo[j] = (float)below[j];
-                    const float x = fmaxf(hi[j], -lo[j]);
-                    finite = finite && hi[j] < INFINITY && lo[j] > -INFINITY;
-                    top = fmaxf(top, x);
-                }
-#pragma unroll
-                for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-                finite = __all_sync(0xffffffffu, finite);
-                const float s = top > 0.0f ? __fmul_rn(top, 1.0f / 127.0f) : 1.0f;
-                uint32_t wh = 0, wl = 0;
-#pragma unroll
-                for (int j = 0; j < C; ++j) {
-                    wh |= (uint32_t)(finite ? box_code(hi[j], s) & 255 : 0) << (8 * j);
-                    wl |= (uint32_t)(finite ? box_code(lo[j], s) & 255 : 0) << (8 * j);
-                }
-                uint8_t* dst = query + warp * kRow + lane * C;
-                if (C == 4) {
-                    *reinterpret_cast<uint32_t*>(dst) = wh;
-                    *reinterpret_cast<uint32_t*>(dst + D) = wl;
-                } else {
-                    *reinterpret_cast<uint16_t*>(dst) = (uint16_t)wh;
-                    *reinterpret_cast<uint16_t*>(dst + D) = (uint16_t)wl;
-                }
-            }
-            if (p.cluster > 1) cluster_sync();                     // the others have begun, or are done with the last tile's scores
-            else __syncthreads();
-
-            uint4 qw[V];
-#pragma unroll
-            for (int i = 0; i < V; ++i)
-                qw[i] = g < p.tile ? *reinterpret_cast<const uint4*>(query + g * kRow + 64 * i + 16 * t) : make_uint4(0, 0, 0, 0);
-            const uint32_t scores_at = (uint32_t)__cvta_generic_to_shared(scores);
-            auto score = [&](int at, const Boxes& x) {
-                int acc[4] = {0, 0, 0, 0};
-#pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    mma_s8(acc, x.word[0][i].x, x.word[1][i].x, x.word[0][i].y, x.word[1][i].y, qw[i].x, qw[i].y);
-                    mma_s8(acc, x.word[0][i].z, x.word[1][i].z, x.word[0][i].w, x.word[1][i].w, qw[i].z, qw[i].w);
-                }
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int token = 2 * t + (j & 1), b = at * 16 + g + 8 * (j >> 1);
-                    if (token >= nt || b >= m) continue;
-                    const float unit = x.unit[j >> 1];
-                    const uint32_t key = !x.there[j >> 1] ? 0u : ordered(unit < INFINITY ? __fmul_rn((float)acc[j], unit) : INFINITY);
-                    const uint32_t place = (uint32_t)(token / p.cluster) * p.cap + b;
-                    if (p.cluster > 1) store_cluster(scores_at + 4 * place, token % p.cluster, key);
-                    else scores[place] = key;
-                }
-            };
-            for (; at < groups; at += 2 * stride) {
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    if (at + j * stride >= groups) break;
-                    score(at + j * stride, x[j]);
-                    if (at + (2 + j) * stride < groups) load(id, x[j]);
-                    ids_of(at + (3 + j) * stride, id);
-                }
-            }
-            if (p.cluster > 1) cluster_sync();
+            if (cluster > 1) cluster_sync();
             else __syncthreads();
         }
 
         // ---- the choice: tokens rank, rank + cluster, .. of the tile, by teams of warps ----
-        const int mine = nt > rank ? (nt - rank + p.cluster - 1) / p.cluster : 0;
-        const int tw = mine <= 1 ? 8 : mine <= 2 ? 4 : mine <= 4 ? 2 : 1;          // warps of a team
-        const int team = warp / tw, member = warp % tw;
-        if (team < mine) {
-            const int token = team * p.cluster + rank, threads = tw * 32, i = member * 32 + lane;
+        const int mine = nt > rank ? (nt - rank + cluster - 1) >> p.lg : 0;
+        const int most_lg = mine <= 1 ? 3 : mine <= 2 ? 2 : mine <= 4 ? 1 : 0;
+        int lg = 0;                                                // 2^lg warps in a team: more where scores are many
+        while (lg < most_lg && m > 64 << lg) ++lg;
+        const int tw = 1 << lg, team = warp >> lg, member = warp & (tw - 1), threads = 32 << lg, i = member * 32 + lane;
+        auto team_sync = [&]() {
+            if (tw == 1) __syncwarp();
+            else asm volatile("bar.sync %0, %1;" ::"r"(1 + team), "r"(threads) : "memory");
+        };
+        int* hist = bins[team << lg];
+        for (int slot = team; slot < mine; slot += kSelWarps >> lg) {
+            const int token = (slot << p.lg) + rank;
             const Seen s = seen_of(p, ctx, n, i0 + token);
             int32_t* list = a.lists + ((long long)(q0 + i0 + token) * p.l.kv_heads + head) * a.keep;
             if (head == 0 && i == 0) a.seen[q0 + i0 + token] = s.tokens;
@@ -374,169 +499,219 @@ __global__ void __launch_bounds__(kSelThreads) kv_select_kernel(const SelectPara
                 return (unsigned)id < (unsigned)p.l.n_pages ? id : -1;
             };
             if (s.pages <= a.keep) {
+#pragma unroll 4
                 for (int b = i; b < a.keep; b += threads) list[b] = b < s.pages ? entry(b) : -1;
-            } else {
-                const uint32_t* keys = scores + (size_t)team * p.cap;
-                const int mt = s.pages - a.first - a.last, need = a.keep - a.first - a.last;
-                for (int b = i; b < a.first + a.last; b += threads)
-                    list[b < a.first ? b : b + need] = entry(b < a.first ? b : s.pages - a.last + (b - a.first));
-                auto team_sync = [&]() {
-                    if (tw == 1) __syncwarp();
-                    else asm volatile("bar.sync %0, %1;" ::"r"(1 + team), "r"(threads) : "memory");
-                };
-                if (need > 0) {
-                    int* hist = bins[team * tw];
-                    // the range of the scores
-                    uint32_t lo = 0xffffffffu, hi = 0;
-#pragma unroll 8
-                    for (int b = i; b < mt; b += threads) {
-                        lo = min(lo, keys[b]);
-                        hi = max(hi, keys[b]);
-                    }
-                    lo = __reduce_min_sync(0xffffffffu, lo);
-                    hi = __reduce_max_sync(0xffffffffu, hi);
-                    if (tw > 1) {
-                        if (lane == 0) part[warp] = make_int2((int)lo, (int)hi);
-                        team_sync();
-                        for (int w = 0; w < tw; ++w) {
-                            lo = min(lo, (uint32_t)part[team * tw + w].x);
-                            hi = max(hi, (uint32_t)part[team * tw + w].y);
-                        }
-                    }
-                    // The least score that is taken, and how many of those equal to it: a histogram of the scores in [lo, hi]
-                    // by their upper bits, the bin that holds the `rest`-th largest of them, that bin as the next range
-                    uint32_t least = lo;
-                    for (int rest = need; lo < hi;) {
-                        const int shift = max(0, 32 - __clz(hi - lo) - (31 - __clz(kSelBins * tw)));
-                        reinterpret_cast<int4*>(hist)[2 * i] = reinterpret_cast<int4*>(hist)[2 * i + 1] = make_int4(0, 0, 0, 0);
-                        team_sync();
-#pragma unroll 8
-                        for (int b = i; b < mt; b += threads) {
-                            const uint32_t key = keys[b];
-                            if (key >= lo && key <= hi) atomicAdd(hist + ((key - lo) >> shift), 1);
-                        }
-                        team_sync();
-                        // eight bins a thread, the highest first
-                        const int top = kSelBins * tw - 8 * (i + 1);
-                        int own[8], sum = 0;
-                        *reinterpret_cast<int4*>(own) = reinterpret_cast<const int4*>(hist + top)[0];
-                        *reinterpret_cast<int4*>(own + 4) = reinterpret_cast<const int4*>(hist + top)[1];
+                continue;
+            }
+            const uint32_t* keys = scores + (size_t)slot * p.cap;
+            const int mt = s.pages - a.first - a.last, need = a.keep - a.first - a.last;
+            for (int j = i; j < a.first + a.last; j += threads)
+                list[j < a.first ? j : j + need] = entry(j < a.first ? j : s.pages - a.first - a.last + j);
+            if (need == 0) continue;
+
+            // the range of the tile's scores, which is that of this token's at least
+            uint32_t lo = 0xffffffffu, hi = 0;
+            for (int e = lane; e < cluster * kSelWarps; e += 32) {
+                const uint2 x = range[(slot << p.lg) * kSelWarps + e];
+                lo = min(lo, x.x);
+                hi = max(hi, x.y);
+            }
+            lo = __reduce_min_sync(0xffffffffu, lo);
+            hi = __reduce_max_sync(0xffffffffu, hi);
+            // The least score that is taken, and how many of those equal to it: a histogram of the scores in [lo, hi] by their
+            // upper bits; the bin that holds the `rest`-th largest of them; its scores, ranked by a warp where 32 hold
+            // them, or that bin as the next range
+            uint32_t least = lo;
+            int rest = need, equal_taken;
+            while (true) {
+                const int shift = lo == hi ? 0 : max(0, 32 - __clz(hi - lo) - (8 + lg));
+                reinterpret_cast<int4*>(hist)[2 * i] = reinterpret_cast<int4*>(hist)[2 * i + 1] = make_int4(0, 0, 0, 0);
+                if (i == 0) ties[team] = 0;
+                team_sync();
+#pragma unroll 4
+                for (int b = i; b < mt; b += threads) {
+                    const uint32_t key = keys[b];
+                    if (key >= lo && key <= hi) atomicAdd(hist + ((key - lo) >> shift), 1);
+                }
+                team_sync();
+                // eight bins a thread, the highest first
+                const int top = (kSelBins << lg) - 8 * (i + 1);
+                int own[8], sum = 0;
+                *reinterpret_cast<int4*>(own) = reinterpret_cast<const int4*>(hist + top)[0];
+                *reinterpret_cast<int4*>(own + 4) = reinterpret_cast<const int4*>(hist + top)[1];
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) sum += own[j];
-                        int upto = sum;
+                for (int j = 0; j < 8; ++j) sum += own[j];
+                int upto = sum;
 #pragma unroll
-                        for (int o = 1; o < 32; o <<= 1) {
-                            const int x = __shfl_up_sync(0xffffffffu, upto, o);
-                            if (lane >= o) upto += x;
-                        }
-                        if (tw > 1) {
-                            if (lane == 31) part[warp].x = upto;
-                            team_sync();
-                            for (int w = 0; w < member; ++w) upto += part[team * tw + w].x;
-                        }
-                        if (upto - sum < rest && rest <= upto) {
-                            int above = upto - sum;
+                for (int o = 1; o < 32; o <<= 1) {
+                    const int x = __shfl_up_sync(0xffffffffu, upto, o);
+                    if (lane >= o) upto += x;
+                }
+                if (tw > 1) {
+                    if (lane == 31) part[warp].x = upto;
+                    team_sync();
+                    upto += __reduce_add_sync(0xffffffffu, lane < member ? part[(team << lg) + lane].x : 0);
+                }
+                if (upto - sum < rest && rest <= upto) {
+                    int above = upto - sum;
 #pragma unroll
-                            for (int j = 7; j >= 0; --j) {
-                                if (above < rest && rest <= above + own[j]) found[team] = make_int2(top + j, rest - above == own[j] ? 0 : rest - above);
-                                above += own[j];
-                            }
-                        }
-                        team_sync();
-                        const int2 f = found[team];
-                        least = lo + ((uint32_t)f.x << shift);
-                        rest = f.y;
-                        if (rest == 0 || shift == 0) break;        // the whole bin is taken, or it is one score
-                        hi = least + min(hi - least, (1u << shift) - 1);
-                        lo = least;
-                    }
-                    // each member's run of scores: those above it, and those at it, the first of which are taken
-                    const int run = ((mt + threads - 1) / threads) * 32, b0 = min(mt, member * run), b1 = min(mt, b0 + run);
-                    int above0 = 0, equal0 = 0, ties;
-                    {
-                        int above = 0, equal = 0;
-#pragma unroll 8
-                        for (int b = b0 + lane; b < b1; b += 32) {
-                            above += keys[b] > least;
-                            equal += keys[b] == least;
-                        }
-                        above = __reduce_add_sync(0xffffffffu, above);
-                        equal = __reduce_add_sync(0xffffffffu, equal);
-                        int all = above;
-                        if (tw > 1) {
-                            team_sync();
-                            if (lane == 0) part[warp] = make_int2(above, equal);
-                            team_sync();
-                            all = 0;
-                            for (int w = 0; w < tw; ++w) {
-                                const int2 c = part[team * tw + w];
-                                all += c.x;
-                                if (w < member) {
-                                    above0 += c.x;
-                                    equal0 += c.y;
-                                }
-                            }
-                        }
-                        ties = need - all;
-                    }
-                    // their places in order, by way of shared memory where they fit, so that the table is read all at once
-                    const bool fits = need <= kSelBins * tw;
-                    for (int b = b0; b < b1; b += 32) {
-                        const uint32_t key = b + lane < b1 ? keys[b + lane] : 0;
-                        const unsigned gt = __ballot_sync(0xffffffffu, b + lane < b1 && key > least), eq = __ballot_sync(0xffffffffu, b + lane < b1 && key == least);
-                        const unsigned before = (1u << lane) - 1;
-                        const int e = equal0 + __popc(eq & before);
-                        if (gt >> lane & 1 || (eq >> lane & 1 && e < ties)) {
-                            const int place = above0 + __popc(gt & before) + min(e, ties);
-                            if (fits) hist[place] = b + lane;
-                            else list[a.first + place] = entry(a.first + b + lane);
-                        }
-                        above0 += __popc(gt);
-                        equal0 += __popc(eq);
-                    }
-                    if (fits) {
-                        team_sync();
-                        for (int j = i; j < need; j += threads) list[a.first + j] = entry(a.first + hist[j]);
+                    for (int j = 7; j >= 0; --j) {
+                        if (above < rest && rest <= above + own[j]) found[team] = make_int4(top + j, rest - above, own[j], 0);
+                        above += own[j];
                     }
                 }
+                team_sync();
+                const int4 f = found[team];
+                least = lo + ((uint32_t)f.x << shift);
+                rest = f.y;
+                equal_taken = rest;
+                if (rest == f.z) {                                 // the whole bin: those at its least too
+                    equal_taken = INT_MAX;
+                    break;
+                }
+                if (shift == 0) break;                             // it is one score
+                hi = least + min(hi - least, (1u << shift) - 1);
+                lo = least;
+                if (f.z <= 32) {
+#pragma unroll 4
+                    for (int b = i; b < mt; b += threads) {
+                        const uint32_t key = keys[b];
+                        if (key >= lo && key <= hi) tied[team][atomicAdd(ties + team, 1)] = key;
+                    }
+                    team_sync();
+                    const uint32_t key = lane < f.z ? tied[team][lane] : 0;
+                    int larger = 0;
+                    for (int j = 0; j < f.z; ++j) larger += __shfl_sync(0xffffffffu, key, j) > key;
+                    least = __reduce_min_sync(0xffffffffu, lane < f.z && larger < rest ? key : 0xffffffffu);
+                    equal_taken = rest - __popc(__ballot_sync(0xffffffffu, lane < f.z && key > least));
+                    break;
+                }
             }
+            // In order: each thread's run of scores, of odd length, so that a warp's lie in different banks; their places go by
+            // way of shared memory where they fit there, so that the table is read all at once
+            const bool by_way = need <= kSelBins << lg;
+            const int per = min(31, ((mt + threads - 1) >> (5 + lg)) | 1);
+            team_sync();
+            for (int from = 0, above0 = 0, equal0 = 0; from < mt; from += per * threads) {
+                const int b0 = from + i * per, size = min(per, mt - b0);
+                uint32_t above = 0, equal = 0;
+#pragma unroll 4
+                for (int j = 0; j < size; ++j) {
+                    const uint32_t key = keys[b0 + j];
+                    above |= (key > least ? 1u : 0u) << j;
+                    equal |= (key == least ? 1u : 0u) << j;
+                }
+                const int mine = __popc(above) + (__popc(equal) << 16);            // below 2^13 each over the team
+                int upto = mine;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const int x = __shfl_up_sync(0xffffffffu, upto, o);
+                    if (lane >= o) upto += x;
+                }
+                int all = __shfl_sync(0xffffffffu, upto, 31);
+                if (tw > 1) {
+                    if (lane == 0) part[warp].y = all;
+                    team_sync();
+                    const int x = lane < tw ? part[(team << lg) + lane].y : 0;
+                    upto += __reduce_add_sync(0xffffffffu, lane < member ? x : 0);
+                    all = __reduce_add_sync(0xffffffffu, x);
+                }
+                const int e = equal0 + ((upto - mine) >> 16);
+                for (int drop = __popc(equal) - max(0, min(__popc(equal), equal_taken - e)); drop > 0; --drop) equal &= ~(0x80000000u >> __clz(equal));
+                int place = above0 + ((upto - mine) & 0xffff) + min(e, equal_taken);
+                for (uint32_t left = above | equal; left; left &= left - 1, ++place) {
+                    const int b = b0 + __ffs(left) - 1;
+                    if (by_way) hist[place] = b;
+                    else list[a.first + place] = entry(a.first + b);
+                }
+                above0 += all & 0xffff;
+                equal0 += all >> 16;
+                if (tw > 1 && from + per * threads < mt) team_sync();
+            }
+            if (by_way) {
+                team_sync();
+#pragma unroll 4
+                for (int j = i; j < need; j += threads) list[a.first + j] = entry(a.first + hist[j]);
+            }
+            team_sync();                                           // before the next token's
         }
+    }
+
+    // rows of no request
+    if (head == 0) {
+        const int end = start(a.n_req);
+        for (long long t = end + (long long)blockIdx.x * kSelThreads + tid; t < a.total_q; t += (long long)gridDim.x * kSelThreads) a.seen[t] = -1;
+        if (const int begin = start(0); begin > 0)
+            for (long long t = (long long)blockIdx.x * kSelThreads + tid; t < begin; t += (long long)gridDim.x * kSelThreads) a.seen[t] = -1;
     }
 }
 
-template <typename T, int D>
-cudaError_t launch_select(SelectParams p, cudaStream_t st)
+template <typename T, int D, int NT>
+cudaError_t launch_tiles(SelectParams& p, long long tiles, cudaStream_t st)
 {
-    auto fn = kv_select_kernel<T, D>;
-    p.tile = p.c.max_q <= 1 ? 1 : kSelTile;
-    p.direct = p.c.max_q <= kSelTile;
-    const long long tiles = p.direct ? p.c.n_req : p.c.total_q / kSelTile + p.c.n_req;
-    if (tiles < 1 || tiles * 8 > INT_MAX) return cudaErrorInvalidValue;
-    p.cap = (p.c.table_width + 15) / 16 * 16;
-    // a CTA's boxes, 16 a warp, where few tiles would leave SMs without one; and shared memory for the scores
-    p.cluster = 1;
-    while (p.cluster < 8 && tiles * p.l.kv_heads * p.cluster < 148 && p.cap > 128 * p.cluster) p.cluster *= 2;
-    auto bytes = [&]() { return (size_t)((p.tile + p.cluster - 1) / p.cluster) * p.cap * 4; };
-    while (p.cluster < 8 && bytes() > 200 * 1024) p.cluster *= 2;
-    const size_t smem = bytes();
-    if (smem > 32 * 1024) {
-        const cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024);
+    auto fn = kv_select_kernel<T, D, NT>;
+    const size_t smem = (size_t)((p.tile + (1 << p.lg) - 1) >> p.lg) * p.cap * 4;
+    if (smem > 24 * 1024) {
+        const cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, kSelSmem);
         if (e != cudaSuccess) return e;
     }
     cudaLaunchConfig_t lc = {};
-    lc.gridDim = dim3((unsigned)(tiles * p.cluster), (unsigned)p.l.kv_heads);
     lc.blockDim = dim3(kSelThreads);
     lc.dynamicSmemBytes = smem;
     lc.stream = st;
     cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = (unsigned)p.cluster;
-    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
     lc.attrs = attr;
+    auto grid = [&]() {
+        attr[0].val.clusterDim.x = 1u << p.lg;
+        lc.gridDim = dim3((unsigned)(tiles << p.lg), (unsigned)p.l.kv_heads);
+    };
+    if (p.lg > 3) {                                                // a size that a GPU need not take
+        const cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+        if (e != cudaSuccess) return e;
+        int n = 0;
+        lc.numAttrs = 1;
+        grid();
+        if (cudaOccupancyMaxActiveClusters(&n, fn, &lc) != cudaSuccess || n < 1) {
+            cudaGetLastError();
+            p.lg = 3;
+        }
+    }
+    if (tiles < 1 || tiles << p.lg > INT_MAX) return cudaErrorInvalidValue;
     lc.numAttrs = 2;
+    grid();
     return cudaLaunchKernelEx(&lc, fn, p);
+}
+
+// Tiles and clusters.  Tiles of 16 tokens read the boxes half as often as those of 8, which fill the GPU with fewer tokens:
+// a chunk of 1024 behind 30000 (8 kv heads, pages of 64) takes 46 us with 16, 60 with 8; one of 100 behind 8000 12.5 and
+// 10.9.  A cluster's CTAs share a tile's boxes, 16 a warp at a time, where there are fewer tiles than SMs: one token behind
+// 32000 in pages of 16 (4 kv heads) takes 26.4 us with one CTA, 18.6 with 2, 14.0 with 4, 11.4 with 8, 10.9 with 16; one
+// behind 131000 86 to 24.5 and 20.8; where tiles fill the GPU, more CTAs only add their own 5 us (32 tokens x 8 heads: 13.9
+// us with one, 20.6 with 2).
+template <typename T, int D>
+cudaError_t launch_select(SelectParams p, cudaStream_t st)
+{
+    p.cap = (p.c.table_width + 3) / 4 * 4;
+    p.direct = p.c.max_q <= 8;
+    auto bytes = [&]() { return (size_t)((p.tile + (1 << p.lg) - 1) >> p.lg) * p.cap * 4; };
+    const long long rows = (long long)p.c.total_q * p.l.kv_heads;
+    p.lg = 0;
+    if (!p.direct && p.c.total_q > 16LL * p.c.n_req && rows > 8 * 2 * 148) {
+        p.tile = 16;
+        while (p.lg < 3 && bytes() > 64 * 1024) ++p.lg;
+        if (bytes() <= kSelSmem) return launch_tiles<T, D, 2>(p, p.c.total_q / 16 + (long long)p.c.n_req, st);
+        p.lg = 0;
+    }
+    p.tile = p.c.max_q <= 1 ? 1 : 8;
+    const long long tiles = p.direct ? p.c.n_req : p.c.total_q / 8 + (long long)p.c.n_req;
+    while (p.lg < 3 && tiles * p.l.kv_heads << p.lg < 148 && p.cap > 128 << p.lg) ++p.lg;
+    if (p.lg == 3 && tiles * p.l.kv_heads << 4 <= 148 && p.cap > 1024) p.lg = 4;
+    while (p.lg < 3 && bytes() > kSelSmem) ++p.lg;
+    return launch_tiles<T, D, 1>(p, tiles, st);
 }
 
 template <int FMT>
