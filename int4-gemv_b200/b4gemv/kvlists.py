@@ -188,8 +188,7 @@ def kv_select(cache, boxes, q, tables, ctx_len, q_starts, max_q: int, keep: int,
     _ints("q_starts", q_starts, index, n + 1)
     _boxes(cache, boxes)
     if out is None:
-        empty = _kv._torch.empty
-        out = KVLists(empty((total, cache.kv_heads, keep), dtype=_kv._int32, device=q.device), empty(total, dtype=_kv._int32, device=q.device))
+        out = KVLists(ctx_len.new_empty((total, cache.kv_heads, keep)), ctx_len.new_empty(total))
     else:
         _ints("out.pages", out.pages, index, 0)
         _ints("out.seen", out.seen, index, total)

@@ -2,6 +2,7 @@
 #include <climits>
 #include <cmath>
 
+#include "b4_kv_attn_lists.cuh"
 #include "b4_kv_attn_tile.cuh"
 #include "b4_kv_attn_warp.cuh"
 
@@ -36,20 +37,20 @@ struct Plan {
 Plan plan(const AttnParams& p)
 {
     const long long most = (long long)std::max(1, p.a.max_q) * p.group;
-    if (p.lists) return {true, false, p.group <= 8 ? 8 : 16, INT_MAX, INT_MAX};        // rows of one query's group
     if (most <= (p.l.head_dim == 64 ? 64 : 48)) return {true, false, most <= 8 ? 8 : 16, INT_MAX, INT_MAX};
     if ((long long)p.a.n_req * p.a.max_q <= p.a.total_q || p.group > 16) return {false, true, 0, 0, 0};    // alike, or none of few rows
     const int cols = p.group <= 8 ? 8 : 16;
     return {true, true, cols, cols, cols};
 }
 
-// Workspace: the two kernels' counters, then the pieces of the one that runs
-// ([CTA][warp] first, [CTA][2] crossing; [CTA][2] crossing), one CTA an SM.
-constexpr int kMaxWarps = 16, kCounters = 4096;
+// Workspace: the kernels' counters, then the pieces of the one that runs ([CTA][warp] first, [CTA][2] crossing; [CTA][2]
+// crossing; lists: one for each team of warps), one CTA an SM.
+constexpr int kMaxWarps = 16, kCounters = 4096, kListTeams = 2;
 size_t ws_bytes_of(const AttnParams& p, int sms)
 {
-    const Plan w = plan(p);
     const size_t row = (size_t)(p.l.head_dim + 2) * 4;
+    if (p.lists) return 2 * kCounters + (size_t)(kListTeams * sms) * (p.group <= 8 ? 8 : 16) * row;
+    const Plan w = plan(p);
     const size_t warp = w.warp ? (kMaxWarps + 2) * w.cols * row : 0, tile = w.tile ? 2 * kTileRows * row : 0;
     return 2 * kCounters + (size_t)sms * std::max(warp, tile);
 }
@@ -69,6 +70,41 @@ cudaError_t launch_warp(const AttnParams& p, void* ws, cudaStream_t st)
     return kv_launch(fn, dim3((unsigned)sms), C::kThreads, C::kSmem, st, p, w);
 }
 
+// Teams of warps that share a list: as many as bring the rounds of all lists to their least time, a round's beginning and
+// end counted as kListChunks chunks' time of a warp, the join of several teams as another.
+constexpr int kListChunks = 2;
+int list_parts(long long lists, int teams, int chunks, int warps)
+{
+    int best = 1;
+    long long least = LLONG_MAX;
+    const int most = lists >= teams ? 1 : std::min((chunks + warps - 1) / warps, (int)(teams / lists));
+    for (int n = 1; n <= most; ++n) {
+        const long long rounds = (lists * n + teams - 1) / teams, time = rounds * ((chunks + n * warps - 1) / (n * warps) + kListChunks + (n > 1));
+        if (time < least) {
+            least = time;
+            best = n;
+        }
+    }
+    return best;
+}
+
+template <typename T, int FMT, int D, int NT, int PT>
+cudaError_t launch_lists(AttnParams p, void* ws, cudaStream_t st)
+{
+    using C = WarpCfg<FMT, D, NT, PT>;
+    auto fn = kv_attn_lists_kernel<T, FMT, D, NT, PT>;
+    const cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
+    if (e != cudaSuccess) return e;
+    const int sms = sm_count();
+    const long long lists = (long long)p.a.total_q * p.l.kv_heads * ((p.group + C::kCols - 1) / C::kCols);
+    const long long chunks = ((long long)p.a.table_width * p.l.page_size + kChunk - 1) / kChunk;
+    p.parts = list_parts(lists, kListTeams * sms, (int)std::max(1LL, chunks), C::kWarps / kListTeams);
+    ListWs w;
+    w.count = static_cast<int*>(ws);
+    w.pieces = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + 2 * kCounters);
+    return kv_launch(fn, dim3((unsigned)std::min<long long>(sms, lists * p.parts)), C::kThreads, C::kSmem, st, p, w);
+}
+
 template <typename T, int FMT, int D>
 cudaError_t launch_tile(const AttnParams& p, void* ws, cudaStream_t st)
 {
@@ -85,6 +121,10 @@ cudaError_t launch_tile(const AttnParams& p, void* ws, cudaStream_t st)
 template <typename T, int FMT, int D>
 cudaError_t launch(AttnParams p, void* ws, cudaStream_t st)
 {
+    if (p.lists) {
+        if (p.l.page_size == 16) return p.group <= 8 ? launch_lists<T, FMT, D, 1, 16>(p, ws, st) : launch_lists<T, FMT, D, 2, 16>(p, ws, st);
+        return p.group <= 8 ? launch_lists<T, FMT, D, 1, 32>(p, ws, st) : launch_lists<T, FMT, D, 2, 32>(p, ws, st);
+    }
     const Plan w = plan(p);
     p.rows_above = w.above;
     p.rows_upto = w.upto;
@@ -119,7 +159,8 @@ int attn_params(const b4_kv_cache* cache, const b4_kv_attn* a, AttnParams* p)
     p->a = *a;
     p->a.window = std::min(a->window, INT_MAX - a->total_q);       // a query's place, ctx - n + i + 1 > -total_q, less it fits an int
     p->group = a->heads / p->l.kv_heads;
-    p->lists = 0;
+    p->lists = false;
+    p->parts = 1;
     p->list_head = 0;
     return cudaSuccess;
 }
@@ -133,7 +174,7 @@ int list_params(const b4_kv_cache* cache, const b4_kv_attn* attn, AttnParams* p)
     a.max_q = 1;
     a.q_starts = nullptr;
     const int e = attn_params(cache, &a, p);
-    p->lists = 1;
+    p->lists = true;
     return e;
 }
 

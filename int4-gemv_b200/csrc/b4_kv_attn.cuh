@@ -15,8 +15,11 @@ struct AttnParams {
     int group;              // query heads that share a kv head
     int rows_above;         // the tile kernel takes requests of more rows (queries x group) than this, the warp kernel
     int rows_upto;          // those of at most this many
-    int lists;              // tables hold a list of pages for each query and kv head, list_head entries from one head's to
-    long long list_head;    // the next's; a query is a request of its own, of ctx_len tokens (below 0: of no query)
+    // lists of pages: tables hold one for each query and kv head, list_head entries from one head's to the next's, ctx_len
+    // the tokens that a query sees of its list (below 0: no query); `parts` teams of warps share a list
+    bool lists;
+    int parts;
+    long long list_head;
 };
 
 constexpr int kChunk = 32;  // tokens that a warp takes at a time: one page of 32, two of 16, half of one of 64
@@ -45,10 +48,6 @@ __device__ __forceinline__ AttnReq attn_extent(const AttnParams& p, int q0, int 
 __device__ __forceinline__ AttnReq attn_request(const AttnParams& p, int r)
 {
     const b4_kv_attn& a = p.a;
-    if (p.lists) {
-        const int seen = __ldg(a.ctx_len + r);
-        return attn_extent(p, r, seen >= 0, max(0, seen));
-    }
     const int q0 = __ldg(a.q_starts + r), q1 = __ldg(a.q_starts + r + 1), ctx = __ldg(a.ctx_len + r);
     const int from = max(0, min(q0, a.total_q));
     return attn_extent(p, from, max(0, min(q1, a.total_q) - from), max(0, ctx));

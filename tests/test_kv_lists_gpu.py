@@ -136,7 +136,8 @@ def test_strides_streams_and_repeats(cuda):
 
 
 def test_equal_to_attention_over_the_whole_context(cuda):
-    """Lists that hold a request's every page are its context."""
+    """Lists that hold a request's every page are its context.  The two kernels add in orders of their own; each is within its
+    bound of the exact values, so they are within twice that of one another."""
     page, kvh, d = 16, 2, 128
     cache = filled(cuda, NF4, 60, kvh, page, d)
     ctx, order = [1, 100, 333, 480], torch.randperm(60).int()
@@ -148,8 +149,11 @@ def test_equal_to_attention_over_the_whole_context(cuda):
     tab = tab.to(cuda)
     q = torch.randn((4, 16, d), device=cuda).bfloat16()
     a = b4gemv.kv_attention(cache, q, tab, ints(ctx, cuda), ints(range(5), cuda), 1)
-    b = b4gemv.kv_attention_lists(cache, q, b4gemv.KVLists(tab[:, None].expand(4, kvh, 30).contiguous(), ints(ctx, cuda)))
-    assert torch.equal(a, b)
+    lists = tab[:, None].expand(4, kvh, 30).contiguous()
+    b = b4gemv.kv_attention_lists(cache, q, b4gemv.KVLists(lists, ints(ctx, cuda)))
+    want, wl, aux = lists_ref.attention(NF4, page, d, cache.blocks, q, lists.cpu().numpy(), np.array(ctx), d ** -0.5)
+    tol, _ = bounds(NF4, BF16, want, wl, aux, 480)
+    assert bool(((a.double() - b.double()).abs() <= 2 * tol).all())
 
 
 def test_no_queries(cuda):
