@@ -45,7 +45,7 @@ Plan plan(const AttnParams& p)
 
 // Workspace: the kernels' counters, then the pieces of the one that runs ([CTA][warp] first, [CTA][2] crossing; [CTA][2]
 // crossing; lists: one for each team of warps), one CTA an SM.
-constexpr int kMaxWarps = 16, kCounters = 4096, kListTeams = 2;
+constexpr int kMaxWarps = 16, kCounters = 4096, kListTeams = 4;
 size_t ws_bytes_of(const AttnParams& p, int sms)
 {
     const size_t row = (size_t)(p.l.head_dim + 2) * 4;
@@ -70,39 +70,59 @@ cudaError_t launch_warp(const AttnParams& p, void* ws, cudaStream_t st)
     return kv_launch(fn, dim3((unsigned)sms), C::kThreads, C::kSmem, st, p, w);
 }
 
-// Teams of warps that share a list: as many as bring the rounds of all lists to their least time, a round's beginning and
-// end counted as kListChunks chunks' time of a warp, the join of several teams as another.
-constexpr int kListChunks = 2;
-int list_parts(long long lists, int teams, int chunks, int warps)
+// How lists go to the teams of warps of every SM's CTA: whole ones round by round, each of those left for the last to as many
+// teams as bring its time down; two teams or four, whichever takes less.  Times in hundreds of cycles as a profile has them:
+// a chunk 20 where a warp has its scheduler for itself, 32 where four share it, a list's beginning and end 57, the join of
+// several teams 30.  64 heads over 8 x 128, INT4, pages of 64: 8 lists of 64 pages take 10.5 us with two teams, 19.3 with
+// four, 192 37.3 and 32.6, 256 of 32 22.7 and 26.7; 3200 of 16 (32 heads over 8 x 64) 82 and 69.
+struct ListPlan {
+    long long whole;
+    int parts;
+    double time;
+};
+
+ListPlan list_plan(long long lists, int teams, int chunks, int warps)
 {
-    int best = 1;
-    long long least = LLONG_MAX;
-    const int most = lists >= teams ? 1 : std::min((chunks + warps - 1) / warps, (int)(teams / lists));
-    for (int n = 1; n <= most; ++n) {
-        const long long rounds = (lists * n + teams - 1) / teams, time = rounds * ((chunks + n * warps - 1) / (n * warps) + kListChunks + (n > 1));
-        if (time < least) {
+    const long long rounds = lists / teams;
+    ListPlan best = {rounds * teams, 1, 0.0};
+    const int rest = (int)(lists - best.whole);
+    double least = 0.0;
+    for (int n = 1; rest > 0 && n <= std::min((chunks + warps - 1) / warps, teams / rest); ++n) {
+        const double each = (chunks + n * warps - 1) / (n * warps), time = each * (20.0 + 12.0 * rest * n / teams) + 57.0 + (n > 1 ? 30.0 : 0.0);
+        if (n == 1 || time < least) {
             least = time;
-            best = n;
+            best.parts = n;
         }
     }
+    best.time = rounds * ((chunks + warps - 1) / warps * 32.0 + 57.0) + least;
     return best;
 }
 
-template <typename T, int FMT, int D, int NT, int PT>
-cudaError_t launch_lists(AttnParams p, void* ws, cudaStream_t st)
+template <typename T, int FMT, int D, int NT, int PT, int TEAMS>
+cudaError_t launch_teams(AttnParams p, const ListPlan& plan, long long lists, int sms, void* ws, cudaStream_t st)
 {
     using C = WarpCfg<FMT, D, NT, PT>;
-    auto fn = kv_attn_lists_kernel<T, FMT, D, NT, PT>;
+    auto fn = kv_attn_lists_kernel<T, FMT, D, NT, PT, TEAMS>;
     const cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
     if (e != cudaSuccess) return e;
-    const int sms = sm_count();
-    const long long lists = (long long)p.a.total_q * p.l.kv_heads * ((p.group + C::kCols - 1) / C::kCols);
-    const long long chunks = ((long long)p.a.table_width * p.l.page_size + kChunk - 1) / kChunk;
-    p.parts = list_parts(lists, kListTeams * sms, (int)std::max(1LL, chunks), C::kWarps / kListTeams);
+    p.whole = plan.whole;
+    p.parts = plan.parts;
     ListWs w;
     w.count = static_cast<int*>(ws);
     w.pieces = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + 2 * kCounters);
-    return kv_launch(fn, dim3((unsigned)std::min<long long>(sms, lists * p.parts)), C::kThreads, C::kSmem, st, p, w);
+    return kv_launch(fn, dim3((unsigned)std::min<long long>(sms, p.whole + (lists - p.whole) * p.parts)), C::kThreads, C::kSmem, st, p, w);
+}
+
+template <typename T, int FMT, int D, int NT, int PT>
+cudaError_t launch_lists(const AttnParams& p, void* ws, cudaStream_t st)
+{
+    constexpr int kWarps = WarpCfg<FMT, D, NT, PT>::kWarps;
+    const int sms = sm_count();
+    const long long lists = (long long)p.a.total_q * p.l.kv_heads * ((p.group + 8 * NT - 1) / (8 * NT));
+    const int chunks = (int)std::min<long long>(std::max(1LL, ((long long)p.a.table_width * p.l.page_size + kChunk - 1) / kChunk), 1 << 20);
+    const ListPlan two = list_plan(lists, 2 * sms, chunks, kWarps / 2), four = list_plan(lists, kListTeams * sms, chunks, kWarps / kListTeams);
+    return four.time < two.time ? launch_teams<T, FMT, D, NT, PT, kListTeams>(p, four, lists, sms, ws, st)
+                                : launch_teams<T, FMT, D, NT, PT, 2>(p, two, lists, sms, ws, st);
 }
 
 template <typename T, int FMT, int D>
@@ -161,6 +181,7 @@ int attn_params(const b4_kv_cache* cache, const b4_kv_attn* a, AttnParams* p)
     p->group = a->heads / p->l.kv_heads;
     p->lists = false;
     p->parts = 1;
+    p->whole = 0;
     p->list_head = 0;
     return cudaSuccess;
 }

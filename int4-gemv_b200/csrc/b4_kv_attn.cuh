@@ -16,10 +16,11 @@ struct AttnParams {
     int rows_above;         // the tile kernel takes requests of more rows (queries x group) than this, the warp kernel
     int rows_upto;          // those of at most this many
     // lists of pages: tables hold one for each query and kv head, list_head entries from one head's to the next's, ctx_len
-    // the tokens that a query sees of its list (below 0: no query); `parts` teams of warps share a list
+    // the tokens that a query sees of its list (below 0: no query); a team of warps takes each of the first `whole`, `parts`
+    // teams share each of the others
     bool lists;
     int parts;
-    long long list_head;
+    long long whole, list_head;
 };
 
 constexpr int kChunk = 32;  // tokens that a warp takes at a time: one page of 32, two of 16, half of one of 64

@@ -344,30 +344,51 @@ struct WarpTile {
         }
     }
 
-    // Chunks first .. last - 1, counted from chunk0, of the segment u, whose page ids are `row`
-    __device__ __forceinline__ void walk(const int32_t* row, int chunk0, int first, int last)
+    // A run of a segment's chunks: its page ids by 32, `ids` from page `base` on and the 32 after those; the segment's queries.
+    struct Run {
+        const int32_t* row;
+        int first, last, base, ids, more;
+        uint4 queries[NT][W];
+    };
+
+    __device__ __forceinline__ int load_id(const Run& r, int page) const
     {
-        // the feed: page ids by 32, `ids` from page `base` on and the 32 after those
+        return page < a.table_width && (long long)page << p.l.page_shift < u.ctx ? __ldg(r.row + page) : -1;
+    }
+
+    // chunks first .. last - 1 of the segment u, whose page ids are `row`: asks for what walk() needs first
+    __device__ __forceinline__ void open(Run& r, const int32_t* row, int first, int last)
+    {
+        r.row = row;
+        r.first = first;
+        r.last = last;
+        r.base = first * kChunk >> p.l.page_shift;
+        r.ids = load_id(r, r.base + lane);
+        r.more = load_id(r, r.base + 32 + lane);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) load_queries(nt, r.queries[nt]);
+    }
+
+    __device__ __forceinline__ void walk(Run& r)
+    {
         const uint8_t* blocks = p.blocks + u.head * p.l.block;
         const long long page_bytes = p.l.kv_heads * p.l.block;
-        int base = (chunk0 + first) * kChunk >> p.l.page_shift, next = chunk0 + first, queue = 0;
-        auto load_ids = [&](int page) { return page < a.table_width && (long long)page << p.l.page_shift < u.ctx ? __ldg(row + page) : -1; };
-        int ids = load_ids(base + lane), more = load_ids(base + 32 + lane);
+        int next = r.first, queue = 0;
         auto issue = [&]() {               // the next chunk, if any, into stage `feed`
             int there = 0;
-            if (next < chunk0 + last) {
+            if (next < r.last) {
                 const int page = next * kChunk >> p.l.page_shift;
-                if (page - base >= 32) {
-                    ids = more;
-                    base += 32;
-                    more = load_ids(base + 32 + lane);
+                if (page - r.base >= 32) {
+                    r.ids = r.more;
+                    r.base += 32;
+                    r.more = load_id(r, r.base + 32 + lane);
                 }
                 const int half = PT == 32 ? next * kChunk & (p.l.page_size - 1) : 0;       // of a page of 64
                 const uint32_t dst = ring_at + feed * C::kStage;
 #pragma unroll
                 for (int i = 0; i < C::kPages; ++i) {
                     // a chunk of two pages begins at an even place of the 32: its second page is among them
-                    const int id = __shfl_sync(0xffffffffu, ids, page - base + i);
+                    const int id = __shfl_sync(0xffffffffu, r.ids, page - r.base + i);
                     if ((unsigned)id >= (unsigned)p.l.n_pages) continue;
                     there |= 1 << i;
                     const uint8_t* src = blocks + id * page_bytes;
@@ -386,19 +407,16 @@ struct WarpTile {
             asm volatile("cp.async.commit_group;" ::: "memory");
             queue = queue << 2 | there;
         };
-        uint4 queries[NT][W];              // asked for before the feed waits for its page ids
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) load_queries(nt, queries[nt]);
 #pragma unroll 1
         for (int i = 0; i < kStages; ++i) issue();
-        begin_segment(queries);
+        begin_segment(r.queries);
 
         // every key of a chunk is seen by every column where the chunk lies in [clear, seen)
         const int seen = ONE || a.flags & B4_KV_FULL ? u.ctx : min(u.ctx, u.ctx - u.n + 1 + u.tile * C::kCols / p.group);
         const int clear = !ONE && a.window > 0 ? u.ctx - a.window : 0;
 #pragma unroll 1
-        for (int c = first; c < last; ++c) {
-            u.token = (chunk0 + c) * kChunk;
+        for (int c = r.first; c < r.last; ++c) {
+            u.token = c * kChunk;
             const int there = queue >> (2 * kStages - 2) & 3;
             asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
             __syncwarp();

@@ -196,7 +196,9 @@ __global__ void __launch_bounds__(WarpCfg<FMT, D, NT, PT>::kThreads, 1) kv_attn_
             u.tile = seg - u.head * tiles;
             v = last == q.chunks ? seg_end : v1;
 
-            tile.walk(a.tables + (long long)r * a.table_stride, q.chunk0, first, last);
+            typename WarpTile<T, FMT, D, NT, PT, false>::Run run;
+            tile.open(run, a.tables + (long long)r * a.table_stride, q.chunk0 + first, q.chunk0 + last);
+            tile.walk(run);
 
             // ---- the end of a segment, or of the run ----
             const float vup = tile.finish();
