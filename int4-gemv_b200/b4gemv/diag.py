@@ -14,9 +14,10 @@ src/diag_aspect.cu on B200): the measurements the dispatch rule is fitted to.
       the benchmark's NF4 decode step, eagerly (the launch list's command).
   python -m b4gemv.diag glue    [--n 28672] [--launches 3]
       the decode layer's elementwise kernels.
-  python -m b4gemv.diag kv      [--fmt nf4|int4] [--requests 16] [--prompt 200] [--tokens 20]
+  python -m b4gemv.diag kv      [--fmt nf4|int4] [--requests 16] [--prompt 200] [--tokens 20] [--rotary] [--keep 0]
       the attention half of a decode layer over the 4-bit cache (kvlayer.py): a
-      prompt step, then decode steps, their time.
+      prompt step, then decode steps, their time; --rotary: the rotation in the
+      append's launch, --keep: pages that a query chooses to read.
 Run from int4-gemv_b200/ (or with it on sys.path).
 """
 from __future__ import annotations
@@ -319,10 +320,12 @@ def cmd_glue(args, torch):
 def cmd_kv(args, torch):
     """A packed prompt step and `tokens` decode steps of one 28-head layer's
     attention half, all requests in one batch."""
+    from . import Rotary
     from .kvlayer import CachedAttention
     fmt = FMT_NF4_B64 if args.fmt == "nf4" else FMT_INT4_G128
     n, width = args.requests, -(-(args.prompt + args.tokens) // 64)
-    layer = CachedAttention(fmt, 3584, 28, 4, n * width, n, max_context=64 * width)
+    layer = CachedAttention(fmt, 3584, 28, 4, n * width, n, max_context=64 * width, rotary=Rotary(128) if args.rotary else None,
+                            keep=args.keep)
     a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
     layer.step(torch.randn((n * args.prompt, 3584), device="cuda").half(), [args.prompt] * n)
     x = torch.randn((n, 3584), device="cuda").half()
@@ -406,6 +409,8 @@ def main(argv=None):
     kv.add_argument("--requests", type=int, default=16)
     kv.add_argument("--prompt", type=int, default=200)
     kv.add_argument("--tokens", type=int, default=20)
+    kv.add_argument("--rotary", action="store_true")
+    kv.add_argument("--keep", type=int, default=0)
     pp = sub.add_parser("p2p")
     pp.add_argument("--fmt", default="nf4", choices=["nf4", "int4"])
     pp.add_argument("--shape", default="tp2_down", choices=list(SHAPES))

@@ -74,6 +74,8 @@ class Rotary:
         self.turns = torch.tensor([t - (1 << 64) if t >> 63 else t for t in turns], dtype=torch.int64, device=device)
         self.axes = torch.tensor(axes, dtype=torch.uint8, device=device) if n_axes > 1 else None
         self.index = self.turns.get_device()
+        if self.index >= 0:
+            torch.cuda.current_stream(self.index).synchronize()        # there for every stream from here on
         self._c = RotaryTable(self.turns.data_ptr(), self.axes.data_ptr() if self.axes is not None else None, dim, n_axes,
                               ROTARY_ADJACENT if adjacent else 0, scale)
         self._ref = ctypes.byref(self._c)

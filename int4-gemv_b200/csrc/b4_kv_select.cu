@@ -714,6 +714,12 @@ cudaError_t launch_select(SelectParams p, cudaStream_t st)
     return launch_tiles<T, D, 1>(p, tiles, st);
 }
 
+struct Span {                              // of int32 values
+    uintptr_t from, to;
+    Span(const int32_t* at, long long n) : from(reinterpret_cast<uintptr_t>(at)), to(from + 4 * n) {}
+    bool meets(const Span& o) const { return from < o.to && o.from < to && from < to && o.from < o.to; }
+};
+
 template <int FMT>
 cudaError_t launch_boxes(const BoxParams& p, cudaStream_t st)
 {
@@ -769,6 +775,12 @@ int b4_kv_select(const b4_kv_cache* cache, const b4_kv_choice* c, b4_stream_t st
     if (c->total_q == 0) return cudaSuccess;
     if (!c->q || !c->boxes || !c->lists || !c->seen || (c->n_req > 0 && (!c->ctx_len || !c->q_starts || (c->table_width > 0 && !c->tables))))
         return cudaErrorInvalidValue;
+    // every CTA reads the lengths and tables while others write what they chose
+    const Span lists(c->lists, (long long)c->total_q * p.l.kv_heads * c->keep), seen(c->seen, c->total_q);
+    const Span reads[] = {{c->tables, c->n_req > 0 ? (c->n_req - 1) * c->table_stride + c->table_width : 0}, {c->ctx_len, c->n_req}, {c->q_starts, c->n_req + 1LL}};
+    if (lists.meets(seen)) return cudaErrorInvalidValue;
+    for (const Span& r : reads)
+        if (r.meets(lists) || r.meets(seen)) return cudaErrorInvalidValue;
     if (!kv_aligned(c->q, 16) || !kv_aligned(c->boxes, 16) || (c->q_stride_token | c->q_stride_head) % 8 != 0) return cudaErrorInvalidValue;
     p.c = *c;
     p.group = c->heads / p.l.kv_heads;

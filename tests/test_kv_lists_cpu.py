@@ -217,8 +217,13 @@ def test_library_refuses_boxes_and_choices():
     for args in ((4096, -1, 4096), (None, 8, 4096), (4096, 8, None), (4096, 8, 4104), (4098, 8, 4096)):
         assert refused("b4_kv_boxes", byref(cache()), *args, None)
     assert lib.b4_kv_boxes(byref(cache()), None, 0, None, None) == 0
-    good = dict(q=4096, boxes=4096, tables=4096, ctx_len=4096, q_starts=4096, lists=4096, seen=4096, table_stride=5, q_stride_token=256, q_stride_head=64,
+    good = dict(q=4096, boxes=4096, tables=8192, ctx_len=16384, q_starts=20480, lists=24576, seen=28672, table_stride=5, q_stride_token=256, q_stride_head=64,
                 table_width=5, n_req=3, total_q=8, max_q=4, heads=4, dtype=0, keep=4, first=1, last=1)
+    # lists of 256 bytes and seen of 32 on what the call reads, or on one another
+    for at in (8192, 8192 + 56, 8192 - 252, 16384, 16384 + 8, 16384 - 252, 20480, 20480 + 12):
+        assert refused("b4_kv_select", byref(cache()), byref(_lib.KvChoice(**{**good, "lists": at})), None), at
+    for at in (8192, 8192 + 56, 8192 - 28, 16384, 16384 + 8, 20480 + 12, 24576, 24576 + 252, 24576 - 28):
+        assert refused("b4_kv_select", byref(cache()), byref(_lib.KvChoice(**{**good, "seen": at})), None), at
     for bad in (dict(n_req=-1), dict(total_q=-1), dict(max_q=-1), dict(table_width=-1), dict(table_width=49153, table_stride=49153), dict(table_stride=4),
                 dict(heads=3), dict(heads=0), dict(heads=130), dict(dtype=2), dict(keep=0), dict(first=-1), dict(last=0), dict(first=3, last=2),
                 dict(keep=49153), dict(first=2 ** 31 - 1, last=2 ** 31 - 1), dict(q=None), dict(q=4104), dict(boxes=None), dict(boxes=4104), dict(tables=None), dict(ctx_len=None),
