@@ -30,6 +30,19 @@ _CHOICE = struct.Struct("@7P3q9i4x")
 _ATTN = struct.Struct("@6P5q8if4x")
 assert _ROWS.size == ctypes.sizeof(KvRows) and _CHOICE.size == ctypes.sizeof(KvChoice) and _ATTN.size == ctypes.sizeof(KvAttn)
 
+# torch's names, as kv.py has them once it is loaded: a call looks each up once
+_torch = _int32 = _float32 = _uint8 = _float16 = _codes = None
+
+
+def _lib():
+    """The library; torch's names, once."""
+    global _torch, _int32, _float32, _uint8, _float16, _codes
+    lib = _kv._lib()
+    if _torch is None:
+        _torch, _int32, _float32, _uint8, _codes = _kv._torch, _kv._int32, _kv._float32, _kv._uint8, _kv._codes
+        _float16 = _torch.float16
+    return lib
+
 
 class Rotary:
     """The angles of b4_kv_append_rotary: the first `dim` columns of a head turn, in pairs.
@@ -41,8 +54,8 @@ class Rotary:
 
     def __init__(self, dim: int, base: float = 1e6, inv_freq=None, sections=None, axes=None, adjacent: bool = False, scale: float = 1.0,
                  device="cuda"):
-        lib = _kv._lib()
-        torch = _kv._torch
+        lib = _lib()
+        torch = _torch
         if dim < 16 or dim % 16 or dim > 128:
             raise ValueError(f"dim: a multiple of 16 up to 128, got {dim}")
         half = dim // 2
@@ -86,21 +99,22 @@ def kv_append_rotary(cache, rotary: Rotary, q, k, v, positions, slots, out=None,
     k and v quantised into the cache at slots.  q, k, v: all fp16, bf16 or fp32, any token and head strides, columns
     contiguous.  positions: int32 [tokens], or [axes][tokens] where the rotary has several.  Returns the rotated q:
     out, which may be q itself, or a new tensor of q's type (fp16 for fp32)."""
-    lib = _kv._lib()
-    index, n, dim = cache.index, slots.numel(), cache.head_dim
-    _ints("slots", slots, index, 0)
-    code = _kv._codes.get(k.dtype)
+    lib = _lib()
+    index, n, dim, dtype = cache.index, slots.numel(), cache.head_dim, k.dtype
+    if slots.dtype is not _int32 or slots.get_device() != index or not slots.is_contiguous():
+        raise ValueError(f"slots: a contiguous int32 tensor on cuda:{index}")
+    code = _codes.get(dtype)
     shape, ks, vs = (n, cache.kv_heads, dim), k.stride(), v.stride()
-    if (code is None or v.dtype is not k.dtype or k.shape != shape or v.shape != shape or k.get_device() != index
+    if (code is None or v.dtype is not dtype or k.shape != shape or v.shape != shape or k.get_device() != index
             or v.get_device() != index or ks[2] != 1 or vs[2] != 1):
         raise ValueError(f"k and v: {shape}, both fp16, bf16 or fp32, on cuda:{index}, columns contiguous")
     if rotary.index != index or rotary.dim > dim:
         raise ValueError(f"rotary: {dim} columns at most, on cuda:{index}")
-    axes = rotary.n_axes
-    if (positions.dtype is not _kv._int32 or positions.get_device() != index or positions.shape != ((n,) if axes == 1 and positions.dim() == 1 else (axes, n))
-            or (n > 1 and positions.stride(-1) != 1)):
+    axes, along = rotary.n_axes, positions.stride()
+    if (positions.dtype is not _int32 or positions.get_device() != index
+            or positions.shape != ((n,) if axes == 1 and len(along) == 1 else (axes, n)) or (n > 1 and along[-1] != 1)):
         raise ValueError(f"positions: int32 [{axes}][{n}] on cuda:{index}, an axis contiguous")
-    along = positions.stride(0) if axes > 1 else n
+    along = along[0] if axes > 1 else n
     if along < n:
         raise ValueError("positions: axes must not overlap (an expanded tensor needs contiguous())")
     if q is None:
@@ -108,18 +122,19 @@ def kv_append_rotary(cache, rotary: Rotary, q, k, v, positions, slots, out=None,
             raise ValueError("out: without q nothing is rotated into it")
         heads, qs, os, out_code, q_at, out_at = 0, (0, 0), (0, 0), DTYPE_F16 if code == DTYPE_F32 else code, 0, 0
     else:
-        if q.dtype is not k.dtype or q.dim() != 3 or q.shape[0] != n or q.shape[2] != dim or q.get_device() != index or q.stride(2) != 1:
+        of_q, qs = q.shape, q.stride()
+        if (len(of_q) != 3 or q.dtype is not dtype or of_q[0] != n or of_q[2] != dim or q.get_device() != index or qs[2] != 1):
             raise ValueError(f"q: [{n}][heads][{dim}] of k's type on cuda:{index}, columns contiguous")
-        heads = q.shape[1]
+        heads = of_q[1]
         if out is None:
-            out = _kv._torch.empty(q.shape, dtype=_kv._torch.float16 if code == DTYPE_F32 else q.dtype, device=q.device)
-        out_code = _kv._codes.get(out.dtype)
-        if (out.shape != q.shape or out_code not in (DTYPE_F16, DTYPE_BF16) or (code != DTYPE_F32 and out_code != code)
-                or out.get_device() != index or out.stride(2) != 1):
+            out = _torch.empty(of_q, dtype=_float16 if code == DTYPE_F32 else dtype, device=q.device)
+        out_code, os = _codes.get(out.dtype), out.stride()
+        if (out.shape != of_q or out_code not in (DTYPE_F16, DTYPE_BF16) or (code != DTYPE_F32 and out_code != code)
+                or out.get_device() != index or os[2] != 1):
             raise ValueError("out: as q, of its type (fp16 or bf16 for fp32), columns contiguous")
-        qs, os, q_at, out_at = q.stride(), out.stride(), q.data_ptr(), out.data_ptr()
+        q_at, out_at = q.data_ptr(), out.data_ptr()
     if _kv._device() != index:                 # the library launches on the current device
-        with _kv._torch.cuda.device(index):
+        with _torch.cuda.device(index):
             return kv_append_rotary(cache, rotary, q, k, v, positions, slots, out, stream)
     args = _ROWS.pack(q_at, k.data_ptr(), v.data_ptr(), out_at, positions.data_ptr(), slots.data_ptr(), along, qs[0], qs[1], ks[0], ks[1],
                       vs[0], vs[1], os[0], os[1], n, heads, code, out_code)
@@ -139,24 +154,25 @@ def kv_box_bytes(head_dim: int) -> int:
 
 def kv_new_boxes(cache):
     """Room for the boxes of a cache's pages: zeros, uint8 [pages][kv_heads][kv_box_bytes]."""
-    _kv._lib()
-    return _kv._torch.zeros((cache.n_pages, cache.kv_heads, kv_box_bytes(cache.head_dim)), dtype=_kv._torch.uint8, device=cache.device)
+    _lib()
+    return _torch.zeros((cache.n_pages, cache.kv_heads, kv_box_bytes(cache.head_dim)), dtype=_torch.uint8, device=cache.device)
 
 
 def _boxes(cache, boxes):
-    if (boxes.dtype is not _kv._uint8 or boxes.shape != (cache.n_pages, cache.kv_heads, 2 * cache.head_dim + 16)
+    if (boxes.dtype is not _uint8 or boxes.shape != (cache.n_pages, cache.kv_heads, 2 * cache.head_dim + 16)
             or boxes.get_device() != cache.index or not boxes.is_contiguous()):
         raise ValueError(f"boxes: as kv_new_boxes makes them, on cuda:{cache.index}")
 
 
 def kv_boxes(cache, boxes, slots, stream=None) -> None:
     """b4_kv_boxes: the boxes of the pages whose last token is among slots, into boxes (kv_new_boxes)."""
-    lib = _kv._lib()
+    lib = _lib()
     index = cache.index
-    _ints("slots", slots, index, 0)
+    if slots.dtype is not _int32 or slots.get_device() != index or not slots.is_contiguous():
+        raise ValueError(f"slots: a contiguous int32 tensor on cuda:{index}")
     _boxes(cache, boxes)
     if _kv._device() != index:
-        with _kv._torch.cuda.device(index):
+        with _torch.cuda.device(index):
             return kv_boxes(cache, boxes, slots, stream)
     status = lib.b4_kv_boxes(cache._ref, slots.data_ptr(), slots.numel(), boxes.data_ptr(),
                              stream.cuda_stream if stream is not None else _kv._raw_stream(index))
@@ -170,36 +186,40 @@ class KVLists(NamedTuple):
     seen: object
 
 
+_new_lists = tuple.__new__
+
+
 def kv_select(cache, boxes, q, tables, ctx_len, q_starts, max_q: int, keep: int, first: int = 1, last: int = 1, out: KVLists | None = None,
               stream=None) -> KVLists:
     """b4_kv_select: for every query and kv head the `keep` pages that it reads: the first `first` and the last `last` of its
     request's up to its own place, and of the others those whose boxes bound its scores highest.  q, tables, ctx_len,
     q_starts and max_q as kv_attention takes them; out: buffers to reuse."""
-    lib = _kv._lib()
-    index, dim, n = cache.index, cache.head_dim, ctx_len.numel()
-    code = _kv._codes.get(q.dtype)
-    if (code is None or code == DTYPE_F32 or q.dim() != 3 or q.get_device() != index or q.shape[2] != dim or q.stride(2) != 1):
+    lib = _lib()
+    index, dim, kv_heads, n = cache.index, cache.head_dim, cache.kv_heads, ctx_len.numel()
+    code, shape, qs = _codes.get(q.dtype), q.shape, q.stride()
+    if code is None or code == DTYPE_F32 or len(shape) != 3 or q.get_device() != index or shape[2] != dim or qs[2] != 1:
         raise ValueError(f"q: fp16 or bf16 [tokens][heads][{dim}] on cuda:{index}, columns contiguous")
-    total, heads, _ = q.shape
-    if heads % cache.kv_heads:
-        raise ValueError(f"heads: a multiple of {cache.kv_heads}, got {heads}")
+    total, heads, _ = shape
+    if heads % kv_heads:
+        raise ValueError(f"heads: a multiple of {kv_heads}, got {heads}")
     if keep < 1 or first < 0 or last < 1 or first + last > keep:
         raise ValueError(f"keep {keep}: at least first {first} (0 or more) and last {last} (1 or more)")
     width, stride = _table(tables, index, n)
-    _ints("ctx_len", ctx_len, index, 0)
-    _ints("q_starts", q_starts, index, n + 1)
+    if (ctx_len.dtype is not _int32 or ctx_len.get_device() != index or not ctx_len.is_contiguous() or q_starts.dtype is not _int32
+            or q_starts.get_device() != index or not q_starts.is_contiguous() or q_starts.numel() <= n):
+        raise ValueError(f"ctx_len and q_starts: contiguous int32 tensors on cuda:{index}, q_starts of {n + 1} values at least")
     _boxes(cache, boxes)
     if out is None:
-        out = KVLists(ctx_len.new_empty((total, cache.kv_heads, keep)), ctx_len.new_empty(total))
+        # (empty_like is the quickest: single tokens have as many rows as requests)
+        out = _new_lists(KVLists, (ctx_len.new_empty((total, kv_heads, keep)), _torch.empty_like(ctx_len) if total == n else ctx_len.new_empty(total)))
     else:
         _ints("out.pages", out.pages, index, 0)
         _ints("out.seen", out.seen, index, total)
-        if out.pages.shape != (total, cache.kv_heads, keep):
-            raise ValueError(f"out.pages: [{total}][{cache.kv_heads}][{keep}]")
+        if out.pages.shape != (total, kv_heads, keep):
+            raise ValueError(f"out.pages: [{total}][{kv_heads}][{keep}]")
     if _kv._device() != index:
-        with _kv._torch.cuda.device(index):
+        with _torch.cuda.device(index):
             return kv_select(cache, boxes, q, tables, ctx_len, q_starts, max_q, keep, first, last, out, stream)
-    qs = q.stride()
     args = _CHOICE.pack(q.data_ptr(), boxes.data_ptr(), tables.data_ptr(), ctx_len.data_ptr(), q_starts.data_ptr(), out[0].data_ptr(),
                         out[1].data_ptr(), stride, qs[0], qs[1], width, n, total, max_q, heads, code, keep, first, last)
     status = lib.b4_kv_select(cache._ref, args, stream.cuda_stream if stream is not None else _kv._raw_stream(index))
@@ -210,29 +230,31 @@ def kv_select(cache, boxes, q, tables, ctx_len, q_starts, max_q: int, keep: int,
 
 def _list_attn(cache, q, lists, scale, out, lse):
     """A call's b4_kv_attn, packed, the lists' head stride, and its output."""
-    index, dim = cache.index, cache.head_dim
-    code = _kv._codes.get(q.dtype)
-    if (code is None or code == DTYPE_F32 or q.dim() != 3 or q.get_device() != index or q.shape[2] != dim or q.stride(2) != 1):
+    index, dim, kv_heads = cache.index, cache.head_dim, cache.kv_heads
+    code, shape, qs = _codes.get(q.dtype), q.shape, q.stride()
+    if code is None or code == DTYPE_F32 or len(shape) != 3 or q.get_device() != index or shape[2] != dim or qs[2] != 1:
         raise ValueError(f"q: fp16 or bf16 [tokens][heads][{dim}] on cuda:{index}, columns contiguous")
-    total, heads, _ = q.shape
-    if heads % cache.kv_heads:
-        raise ValueError(f"heads: a multiple of {cache.kv_heads}, got {heads}")
+    total, heads, _ = shape
+    if heads % kv_heads:
+        raise ValueError(f"heads: a multiple of {kv_heads}, got {heads}")
     pages, seen = lists
-    if pages.dtype is not _kv._int32 or pages.get_device() != index or pages.dim() != 3 or pages.shape[:2] != (total, cache.kv_heads):
-        raise ValueError(f"lists.pages: int32 [{total}][{cache.kv_heads}][pages] on cuda:{index}")
-    width = pages.shape[2]
+    of_lists = pages.shape
+    if pages.dtype is not _int32 or pages.get_device() != index or len(of_lists) != 3 or of_lists[0] != total or of_lists[1] != kv_heads:
+        raise ValueError(f"lists.pages: int32 [{total}][{kv_heads}][pages] on cuda:{index}")
+    width = of_lists[2]
     along, across, one = pages.stride()
-    if (width > 1 and one != 1) or (cache.kv_heads > 1 and across < width) or (total > 1 and along < width):
+    if (width > 1 and one != 1) or (kv_heads > 1 and across < width) or (total > 1 and along < width):
         raise ValueError("lists.pages: entries contiguous, rows that do not overlap")
-    _ints("lists.seen", seen, index, total)
+    if seen.dtype is not _int32 or seen.get_device() != index or not seen.is_contiguous() or seen.numel() < total:
+        raise ValueError(f"lists.seen: a contiguous int32 tensor on cuda:{index}, {total} values at least")
     if out is None:
-        out = _kv._torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    elif out.shape != q.shape or out.dtype is not q.dtype or out.get_device() != index or out.stride(2) != 1:
+        out = _torch.empty_like(q) if q.is_contiguous() else _torch.empty(shape, dtype=q.dtype, device=q.device)
+    elif out.shape != shape or out.dtype is not q.dtype or out.get_device() != index or out.stride(2) != 1:
         raise ValueError("out: as q, columns contiguous")
-    if lse is not None and (lse.shape != (total, heads) or lse.dtype is not _kv._float32 or lse.get_device() != index
+    if lse is not None and (lse.shape != (total, heads) or lse.dtype is not _float32 or lse.get_device() != index
                             or not lse.is_contiguous()):
         raise ValueError("lse: contiguous fp32 [tokens][heads]")
-    qs, os = q.stride(), out.stride()
+    os = out.stride()
     args = _ATTN.pack(q.data_ptr(), out.data_ptr(), lse.data_ptr() if lse is not None else 0, pages.data_ptr(), seen.data_ptr(), 0,
                       max(along, width), qs[0], qs[1], os[0], os[1], width, total, total, 1, heads, code, 0, 0,
                       dim ** -0.5 if scale is None else scale)
@@ -241,10 +263,10 @@ def _list_attn(cache, q, lists, scale, out, lse):
 
 def kv_attention_lists_workspace(cache, q, lists: KVLists) -> int:
     """Bytes of workspace that kv_attention_lists needs for such a call (b4_kv_attention_lists_workspace)."""
-    lib = _kv._lib()
+    lib = _lib()
     n = ctypes.c_size_t(0)
     args, _, _ = _list_attn(cache, q, lists, None, q, None)
-    with _kv._torch.cuda.device(cache.index):  # whose SMs are counted
+    with _torch.cuda.device(cache.index):  # whose SMs are counted
         check("b4_kv_attention_lists_workspace", lib.b4_kv_attention_lists_workspace(cache._ref, args, ctypes.byref(n)))
     return n.value
 
@@ -254,14 +276,14 @@ def kv_attention_lists(cache, q, lists: KVLists, scale: float | None = None, out
     others: page ids of the cache in the order of the tokens, of which the first lists.seen are seen).  The rest is as
     kv_attention: q and out [tokens][heads][head_dim] fp16 or bf16, scale None = head_dim ** -0.5, lse, ws and the package's
     workspace of the device.  Rows whose lists.seen is below 0 are left as they are.  Returns out."""
-    lib = _kv._lib()
+    lib = _lib()
     args, across, out = _list_attn(cache, q, lists, scale, out, lse)
     if ws is None:
         ws = _workspace(cache.index, stream)
-    elif ws.dtype is not _kv._uint8 or ws.get_device() != cache.index or not ws.is_contiguous():
+    elif ws.dtype is not _uint8 or ws.get_device() != cache.index or not ws.is_contiguous():
         raise ValueError(f"ws: a contiguous uint8 tensor on cuda:{cache.index}")
     if _kv._device() != cache.index:
-        with _kv._torch.cuda.device(cache.index):
+        with _torch.cuda.device(cache.index):
             return kv_attention_lists(cache, q, lists, scale, out, lse, ws, stream)
     status = lib.b4_kv_attention_lists(cache._ref, args, across, ws.data_ptr(), ws.numel(),
                                        stream.cuda_stream if stream is not None else _kv._raw_stream(cache.index))

@@ -11,6 +11,14 @@
 // 8 x 128, 32 queries, INT4: 28.9 us).  Lists that are too few for one more round of all
 // halves are shared by several, whose pieces the last to arrive joins in the list's
 // order: the same bits every time.
+//
+// What bounds it.  Many lists: the products, a chunk's 600 instructions at 2.4 a cycle (16
+// warps an SM, 2000 cycles for a warp alone, 3200 with three beside it on a scheduler), and
+// 5700 cycles a list around them, half of which the other teams' products hide.  32 queries
+// over 32 pages of 64 (64 heads over 8 x 128, INT4) take 22.7 us, 69 MB, 3.0 TB/s; 64 over
+// 64 pages 69 us, 275 MB, 4.0 TB/s; 96 over up to 64 pages of 16 (32 heads over 8 x 64, NF4
+// in bf16) 24.3 us; a chunk of 300 over 32 pages of 32 (28 heads over 4 x 128, INT4) 47.9 us,
+// whose lists' 162 MB come from L2.  Few: latency, one query over 16 pages of 64 7.6 us.
 #pragma once
 
 #include "b4_kv_attn_cols.cuh"
