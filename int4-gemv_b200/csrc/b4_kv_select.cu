@@ -269,7 +269,7 @@ __global__ void __launch_bounds__(kSelThreads, 2) kv_select_kernel(const SelectP
     extern __shared__ __align__(16) uint32_t scores[];             // [tokens of this CTA][cap]
     __shared__ __align__(16) uint8_t query[8 * NT * kRow];         // above, below of a token
     __shared__ __align__(16) int bins[kSelWarps][kSelBins];        // of a team's warps together
-    __shared__ uint2 range[16 * NT * kSelWarps];                    // [tokens of this CTA][CTAs][warps] least and largest score
+    __shared__ uint2 range[16 * kSelWarps];                        // [CTAs][warps] least and largest score of the tile's tokens
     __shared__ int2 part[kSelWarps];
     __shared__ int4 found[kSelWarps];
     __shared__ uint32_t tied[kSelWarps][32];
@@ -422,16 +422,9 @@ __global__ void __launch_bounds__(kSelThreads, 2) kv_select_kernel(const SelectP
 
             auto query_of = [&](int nt8, int i) { return *reinterpret_cast<const uint4*>(query + (nt8 * 8 + g) * kRow + 64 * i + 16 * t); };
             const uint32_t scores_at = (uint32_t)__cvta_generic_to_shared(scores);
-            uint32_t lo[NT][2], hi[NT][2];
-#pragma unroll
-            for (int nt8 = 0; nt8 < NT; ++nt8)
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    lo[nt8][j] = 0xffffffffu;
-                    hi[nt8][j] = 0;
-                }
+            uint32_t lo = 0xffffffffu, hi = 0;
             auto score = [&](int step, const Boxes& x) {
-#pragma unroll
+#pragma unroll 1
                 for (int nt8 = 0; nt8 < NT; ++nt8) {
                     if (nt8 * 8 >= nt) break;
                     int acc[4] = {0, 0, 0, 0};
@@ -447,8 +440,8 @@ __global__ void __launch_bounds__(kSelThreads, 2) kv_select_kernel(const SelectP
                         if (token >= nt || b >= m) continue;
                         const float unit = x.unit[j >> 1];
                         const uint32_t key = !x.there[j >> 1] ? 0u : ordered(unit < INFINITY ? __fmul_rn((float)acc[j], unit) : INFINITY);
-                        lo[nt8][j & 1] = min(lo[nt8][j & 1], key);
-                        hi[nt8][j & 1] = max(hi[nt8][j & 1], key);
+                        lo = min(lo, key);
+                        hi = max(hi, key);
                         const uint32_t place = (uint32_t)(token >> p.lg) * p.cap + b;
                         if (cluster > 1) store_cluster(scores_at + 4 * place, token & (cluster - 1), key);
                         else scores[place] = key;
@@ -465,27 +458,17 @@ __global__ void __launch_bounds__(kSelThreads, 2) kv_select_kernel(const SelectP
                     ids_of(at + (kAhead + 1 + j) * stride, next);
                 }
             }
-            const uint32_t range_at = (uint32_t)__cvta_generic_to_shared(range);
-#pragma unroll
-            for (int nt8 = 0; nt8 < NT; ++nt8)
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {
-#pragma unroll
-                    for (int o = 4; o < 32; o <<= 1) {
-                        lo[nt8][j] = min(lo[nt8][j], __shfl_xor_sync(0xffffffffu, lo[nt8][j], o));
-                        hi[nt8][j] = max(hi[nt8][j], __shfl_xor_sync(0xffffffffu, hi[nt8][j], o));
-                    }
-                    const int token = nt8 * 8 + 2 * t + j;
-                    if (g == 0 && token < nt) {
-                        const int place = (((token >> p.lg) << p.lg) + rank) * kSelWarps + warp;
-                        if (cluster > 1) {
-                            store_cluster(range_at + 8 * place, token & (cluster - 1), lo[nt8][j]);
-                            store_cluster(range_at + 8 * place + 4, token & (cluster - 1), hi[nt8][j]);
-                        } else {
-                            range[place] = make_uint2(lo[nt8][j], hi[nt8][j]);
-                        }
-                    }
+            lo = __reduce_min_sync(0xffffffffu, lo);
+            hi = __reduce_max_sync(0xffffffffu, hi);
+            if (cluster > 1) {
+                const uint32_t at = (uint32_t)__cvta_generic_to_shared(range + rank * kSelWarps + warp);
+                if (lane < cluster) {
+                    store_cluster(at, lane, lo);
+                    store_cluster(at + 4, lane, hi);
                 }
+            } else if (lane == 0) {
+                range[warp] = make_uint2(lo, hi);
+            }
             if (cluster > 1) cluster_sync();
             else __syncthreads();
         }
@@ -521,10 +504,10 @@ __global__ void __launch_bounds__(kSelThreads, 2) kv_select_kernel(const SelectP
                 list[j < a.first ? j : j + need] = entry(j < a.first ? j : s.pages - a.first - a.last + j);
             if (need == 0) continue;
 
-            // the range of the tile's scores, which is that of this token's at least
+            // the range of all the tile's scores: queries are in units of their largest, so their scores are of one size
             uint32_t lo = 0xffffffffu, hi = 0;
             for (int e = lane; e < cluster * kSelWarps; e += 32) {
-                const uint2 x = range[(slot << p.lg) * kSelWarps + e];
+                const uint2 x = range[e];
                 lo = min(lo, x.x);
                 hi = max(hi, x.y);
             }
