@@ -12,6 +12,7 @@ Streams, devices and refusals are as in kv.py.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import math
 import struct
@@ -42,6 +43,14 @@ def _lib():
         _torch, _int32, _float32, _uint8, _codes = _kv._torch, _kv._int32, _kv._float32, _kv._uint8, _kv._codes
         _float16 = _torch.float16
     return lib
+
+
+def _on(stream):
+    """Where a call's own outputs are allocated: on the stream that writes them, whose memory no other stream still uses."""
+    return _torch.cuda.stream(stream) if stream is not None else _here
+
+
+_here = contextlib.nullcontext()
 
 
 class Rotary:
@@ -127,7 +136,8 @@ def kv_append_rotary(cache, rotary: Rotary, q, k, v, positions, slots, out=None,
             raise ValueError(f"q: [{n}][heads][{dim}] of k's type on cuda:{index}, columns contiguous")
         heads = of_q[1]
         if out is None:
-            out = _torch.empty(of_q, dtype=_float16 if code == DTYPE_F32 else dtype, device=q.device)
+            with _on(stream):
+                out = _torch.empty(of_q, dtype=_float16 if code == DTYPE_F32 else dtype, device=q.device)
         out_code, os = _codes.get(out.dtype), out.stride()
         if (out.shape != of_q or out_code not in (DTYPE_F16, DTYPE_BF16) or (code != DTYPE_F32 and out_code != code)
                 or out.get_device() != index or os[2] != 1):
@@ -211,7 +221,8 @@ def kv_select(cache, boxes, q, tables, ctx_len, q_starts, max_q: int, keep: int,
     _boxes(cache, boxes)
     if out is None:
         # (empty_like is the quickest: single tokens have as many rows as requests)
-        out = _new_lists(KVLists, (ctx_len.new_empty((total, kv_heads, keep)), _torch.empty_like(ctx_len) if total == n else ctx_len.new_empty(total)))
+        with _on(stream):
+            out = _new_lists(KVLists, (ctx_len.new_empty((total, kv_heads, keep)), _torch.empty_like(ctx_len) if total == n else ctx_len.new_empty(total)))
     else:
         _ints("out.pages", out.pages, index, 0)
         _ints("out.seen", out.seen, index, total)
@@ -228,7 +239,7 @@ def kv_select(cache, boxes, q, tables, ctx_len, q_starts, max_q: int, keep: int,
     return out
 
 
-def _list_attn(cache, q, lists, scale, out, lse):
+def _list_attn(cache, q, lists, scale, out, lse, stream=None):
     """A call's b4_kv_attn, packed, the lists' head stride, and its output."""
     index, dim, kv_heads = cache.index, cache.head_dim, cache.kv_heads
     code, shape, qs = _codes.get(q.dtype), q.shape, q.stride()
@@ -248,7 +259,8 @@ def _list_attn(cache, q, lists, scale, out, lse):
     if seen.dtype is not _int32 or seen.get_device() != index or not seen.is_contiguous() or seen.numel() < total:
         raise ValueError(f"lists.seen: a contiguous int32 tensor on cuda:{index}, {total} values at least")
     if out is None:
-        out = _torch.empty_like(q) if q.is_contiguous() else _torch.empty(shape, dtype=q.dtype, device=q.device)
+        with _on(stream):
+            out = _torch.empty_like(q) if q.is_contiguous() else _torch.empty(shape, dtype=q.dtype, device=q.device)
     elif out.shape != shape or out.dtype is not q.dtype or out.get_device() != index or out.stride(2) != 1:
         raise ValueError("out: as q, columns contiguous")
     if lse is not None and (lse.shape != (total, heads) or lse.dtype is not _float32 or lse.get_device() != index
@@ -277,7 +289,7 @@ def kv_attention_lists(cache, q, lists: KVLists, scale: float | None = None, out
     kv_attention: q and out [tokens][heads][head_dim] fp16 or bf16, scale None = head_dim ** -0.5, lse, ws and the package's
     workspace of the device.  Rows whose lists.seen is below 0 are left as they are.  Returns out."""
     lib = _lib()
-    args, across, out = _list_attn(cache, q, lists, scale, out, lse)
+    args, across, out = _list_attn(cache, q, lists, scale, out, lse, stream)
     if ws is None:
         ws = _workspace(cache.index, stream)
     elif ws.dtype is not _uint8 or ws.get_device() != cache.index or not ws.is_contiguous():

@@ -165,6 +165,32 @@ def test_no_queries(cuda):
     assert not bool(b4gemv.kv_attention_lists(cache, q, lists).any())                    # of no pages
 
 
+def test_calls_at_once_on_two_streams(cuda):
+    """Choices and attention of two layers side by side, with outputs of their own streams and workspaces of their own."""
+    layers, want = [], []
+    for seed in range(2):
+        cache = filled(cuda, INT4, 300, 2, 16, 128, seed)
+        boxes = b4gemv.kv_new_boxes(cache)
+        b4gemv.kv_boxes(cache, boxes, torch.arange(300 * 16, dtype=torch.int32, device=cuda))
+        q = torch.randn((3, 14, 128), generator=torch.Generator(device=cuda).manual_seed(seed), device=cuda).half()
+        tab = torch.randperm(300, generator=torch.Generator(device=cuda).manual_seed(seed), device=cuda).int().view(3, 100)
+        ctx, starts = ints([1600, 900, 1333], cuda), ints(range(4), cuda)
+        lists = b4gemv.kv_select(cache, boxes, q, tab, ctx, starts, 1, 40)
+        ws = torch.zeros(b4gemv.kv_attention_lists_workspace(cache, q, lists), dtype=torch.uint8, device=cuda)
+        layers.append((cache, boxes, q, tab, ctx, starts, ws))
+        want.append((lists.pages.clone(), b4gemv.kv_attention_lists(cache, q, lists)))
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = []
+    for _ in range(20):
+        for stream, (cache, boxes, q, tab, ctx, starts, ws) in zip(streams, layers):
+            lists = b4gemv.kv_select(cache, boxes, q, tab, ctx, starts, 1, 40, stream=stream)
+            got.append((lists.pages, b4gemv.kv_attention_lists(cache, q, lists, ws=ws, stream=stream)))
+    torch.cuda.synchronize()
+    for i, (pages, out) in enumerate(got):
+        assert torch.equal(pages, want[i % 2][0]) and torch.equal(out, want[i % 2][1])
+
+
 # ---- together -------------------------------------------------------------------------
 
 class Layer:
