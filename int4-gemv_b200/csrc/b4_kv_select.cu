@@ -177,7 +177,7 @@ __device__ __forceinline__ uint4 load_once(const uint4* p)
 __device__ __forceinline__ uint32_t ordered(float x)
 {
     const uint32_t u = __float_as_uint(x + 0.0f);                  // -0 as 0
-    return u & 0x80000000u ? ~u : u | 0x80000000u;
+    return u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u);
 }
 
 __device__ __forceinline__ void cluster_sync()
@@ -321,17 +321,17 @@ __global__ void __launch_bounds__(kSelThreads, 2) kv_select_kernel(const SelectP
             const int groups = (m + 15) / 16;
             struct Boxes {
                 uint4 word[2][V];
-                float unit[2];
-                bool there[2];
+                float unit[2];                                     // NaN: the page is missing
             };
             auto load = [&](const int (&id)[2], Boxes& x) {
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
-                    x.there[j] = (unsigned)id[j] < (unsigned)p.l.n_pages;
-                    const uint8_t* src = static_cast<const uint8_t*>(a.boxes) + ((long long)(x.there[j] ? id[j] : 0) * p.l.kv_heads + head) * box_bytes(D);
+                    const bool there = (unsigned)id[j] < (unsigned)p.l.n_pages;
+                    const uint8_t* src = static_cast<const uint8_t*>(a.boxes) + ((long long)(there ? id[j] : 0) * p.l.kv_heads + head) * box_bytes(D);
 #pragma unroll
                     for (int i = 0; i < V; ++i) x.word[j][i] = load_once(reinterpret_cast<const uint4*>(src + 64 * i) + t);
-                    x.unit[j] = __ldg(reinterpret_cast<const float*>(src + 2 * D));
+                    const float unit = __ldg(reinterpret_cast<const float*>(src + 2 * D));
+                    x.unit[j] = !there ? __uint_as_float(0x7fffffffu) : unit < INFINITY ? unit : INFINITY;
                 }
             };
             // a token a warp (and every 8th): its first 8 heads, asked for before the boxes' page ids are waited for
@@ -358,8 +358,9 @@ __global__ void __launch_bounds__(kSelThreads, 2) kv_select_kernel(const SelectP
             if (at < groups) load(id, x[0]);
 
             // The sums of the heads' parts above and below 0, as int8: from sums in fp32 where every code is further from its
-            // next than those can be off (2^-24 for each of a sum's roundings, in it and in the largest, and 2^-21 of the
-            // scale and the quotient: of 127 units); from exact ones otherwise (6 % of the rows of 8 heads)
+            // next than those can be off; from exact ones otherwise (5 % of the rows of 8 heads).  Off by 2^-24 of 127 units for
+            // each rounding: a sum's, in it and in the largest (1.6e-5 for the two), the exact sums' own, the two units, the
+            // reciprocal and the two quotients (7, 5.3e-5)
 #pragma unroll 1
             for (int i = warp; i < 8 * NT; i += kSelWarps) {
                 if (i > warp) heads_of(i, raw);
@@ -394,7 +395,7 @@ __global__ void __launch_bounds__(kSelThreads, 2) kv_select_kernel(const SelectP
 #pragma unroll
                     for (int j = 0; j < C; ++j) top = fmaxf(top, fmaxf(part[0][j], -part[1][j]));
                     top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
-                    const float inv = __fdividef(127.0f, top), clear = 0.5f - 8e-5f - 1.6e-5f * (p.group <= 8 ? 3 : p.group);
+                    const float inv = __frcp_rn(__fmul_rn(top, 1.0f / 127.0f)), clear = 0.5f - 5.6e-5f - 1.6e-5f * (p.group <= 8 ? 3 : p.group);
                     bool sure = finite && top > 1e-30f && top < 1e30f;
 #pragma unroll
                     for (int k = 0; k < 2; ++k)
@@ -424,6 +425,9 @@ __global__ void __launch_bounds__(kSelThreads, 2) kv_select_kernel(const SelectP
             const uint32_t scores_at = (uint32_t)__cvta_generic_to_shared(scores);
             uint32_t lo = 0xffffffffu, hi = 0;
             auto score = [&](int step, const Boxes& x) {
+                const int b = step * 16 + g;
+                // every row is a page with a finite box, but at the list's end and beside pages that are not
+                const bool plain = __all_sync(0xffffffffu, step * 16 + 16 <= m && x.unit[0] < INFINITY && x.unit[1] < INFINITY);
 #pragma unroll 1
                 for (int nt8 = 0; nt8 < NT; ++nt8) {
                     if (nt8 * 8 >= nt) break;
@@ -435,16 +439,24 @@ __global__ void __launch_bounds__(kSelThreads, 2) kv_select_kernel(const SelectP
                         mma_s8(acc, x.word[0][i].z, x.word[1][i].z, x.word[0][i].w, x.word[1][i].w, q.z, q.w);
                     }
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const int token = nt8 * 8 + 2 * t + (j & 1), b = step * 16 + g + 8 * (j >> 1);
-                        if (token >= nt || b >= m) continue;
-                        const float unit = x.unit[j >> 1];
-                        const uint32_t key = !x.there[j >> 1] ? 0u : ordered(unit < INFINITY ? __fmul_rn((float)acc[j], unit) : INFINITY);
-                        lo = min(lo, key);
-                        hi = max(hi, key);
+                    for (int c = 0; c < 2; ++c) {
+                        const int token = nt8 * 8 + 2 * t + c;
+                        if (token >= nt) continue;
                         const uint32_t place = (uint32_t)(token >> p.lg) * p.cap + b;
-                        if (cluster > 1) store_cluster(scores_at + 4 * place, token & (cluster - 1), key);
-                        else scores[place] = key;
+#pragma unroll
+                        for (int r = 0; r < 2; ++r) {
+                            uint32_t key;
+                            if (plain) {
+                                key = ordered(__fmul_rn((float)acc[2 * r + c], x.unit[r]));
+                            } else {
+                                if (b + 8 * r >= m) continue;
+                                key = x.unit[r] < INFINITY ? ordered(__fmul_rn((float)acc[2 * r + c], x.unit[r])) : x.unit[r] == INFINITY ? ordered(INFINITY) : 0u;
+                            }
+                            lo = min(lo, key);
+                            hi = max(hi, key);
+                            if (cluster > 1) store_cluster(scores_at + 4 * (place + 8 * r), token & (cluster - 1), key);
+                            else scores[place + 8 * r] = key;
+                        }
                     }
                 }
             };
@@ -568,10 +580,22 @@ __global__ void __launch_bounds__(kSelThreads, 2) kv_select_kernel(const SelectP
                 hi = least + min(hi - least, (1u << shift) - 1);
                 lo = least;
                 if (f.z <= 32) {
+                    if (tw == 1) {                                 // by ballots, which wait less than counts in memory
+                        int at = 0;
 #pragma unroll 4
-                    for (int b = i; b < mt; b += threads) {
-                        const uint32_t key = keys[b];
-                        if (key >= lo && key <= hi) tied[team][atomicAdd(ties + team, 1)] = key;
+                        for (int b0 = 0; b0 < mt; b0 += 32) {
+                            const uint32_t key = b0 + lane < mt ? keys[b0 + lane] : 0;
+                            const bool in = b0 + lane < mt && key >= lo && key <= hi;
+                            const unsigned mask = __ballot_sync(0xffffffffu, in);
+                            if (in) tied[team][at + __popc(mask & ((1u << lane) - 1))] = key;
+                            at += __popc(mask);
+                        }
+                    } else {
+#pragma unroll 4
+                        for (int b = i; b < mt; b += threads) {
+                            const uint32_t key = keys[b];
+                            if (key >= lo && key <= hi) tied[team][atomicAdd(ties + team, 1)] = key;
+                        }
                     }
                     team_sync();
                     const uint32_t key = lane < f.z ? tied[team][lane] : 0;
