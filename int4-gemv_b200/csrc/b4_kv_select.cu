@@ -20,14 +20,14 @@
 // which chooses for it.
 //
 // What bounds it.  A step of single tokens: a chain of waits.  One token behind 9000 in
-// pages of 16 (4 kv heads) takes 8.1 us: 0.5 for the lengths, 0.8 for page ids, 1.1 for the
+// pages of 16 (4 kv heads) takes 8.0 us: 0.5 for the lengths, 0.8 for page ids, 1.1 for the
 // queries, 1.5 for boxes and their products, 0.6 for the cluster's barriers, 2.6 for the
 // choice, 0.5 of it the table again.  Code that runs once costs some 5 cycles an instruction
 // here, whatever its kind, so the choice is short loops over shared memory, not unrolled
 // registers (a bisection with 16 scores a lane in registers: 450 cycles a bit).  32 tokens
-// behind 8 to 32 thousand in pages of 64 (8 kv heads): 14.0 us, of which the 21 MB of boxes
-// take 6; one behind 131000 in pages of 16: 22.4 us, 17.8 MB; a chunk of 1024 behind 30000:
-// 45.8 us for 8192 choices among 480 boxes, 14 of 46 us the scores, the rest the choices.
+// behind 8 to 32 thousand in pages of 64 (8 kv heads): 13.5 us, of which the 21 MB of boxes
+// take 6; one behind 131000 in pages of 16: 20.9 us, 17.8 MB; a chunk of 1024 behind 30000:
+// 44.8 us for 8192 choices among 480 boxes, 13 of 45 us the scores, the rest the choices.
 #include <algorithm>
 #include <climits>
 #include <type_traits>
@@ -56,7 +56,8 @@ __device__ __forceinline__ int box_code(float x, float s) { return min(127, max(
 // A CTA makes the boxes of the completed pages among its tokens, of one kv head: its warps share a page's tokens, a
 // lane holds the extremes of 8 columns over those of its rows (every second token, D = 128; fourth, D = 64).
 // Bound by latency: 16 pages of 64 x 8 heads 4.1 us (a warp a page: 10.7); none completed, as in most steps of single tokens,
-// 1.1 us.
+// 1.1 us.  A CTA looks at 1 to 16 tokens, 8 CTAs an SM before it takes more: 1024 tokens x 8 heads 4.4 us (9.9 with one each),
+// 16384 14.9 (137).
 constexpr int kBoxWarps = 8;
 
 template <int FMT, int D>
@@ -535,7 +536,7 @@ __global__ void __launch_bounds__(kSelThreads, 2) kv_select_kernel(const SelectP
                 reinterpret_cast<int4*>(hist)[2 * i] = reinterpret_cast<int4*>(hist)[2 * i + 1] = make_int4(0, 0, 0, 0);
                 if (i == 0) ties[team] = 0;
                 team_sync();
-#pragma unroll 4
+#pragma unroll 8
                 for (int b = i; b < mt; b += threads) {
                     const uint32_t key = keys[b];
                     if (key >= lo && key <= hi) atomicAdd(hist + ((key - lo) >> shift), 1);
@@ -591,7 +592,7 @@ __global__ void __launch_bounds__(kSelThreads, 2) kv_select_kernel(const SelectP
                             at += __popc(mask);
                         }
                     } else {
-#pragma unroll 4
+#pragma unroll 8
                         for (int b = i; b < mt; b += threads) {
                             const uint32_t key = keys[b];
                             if (key >= lo && key <= hi) tied[team][atomicAdd(ties + team, 1)] = key;
@@ -614,7 +615,7 @@ __global__ void __launch_bounds__(kSelThreads, 2) kv_select_kernel(const SelectP
             for (int from = 0, above0 = 0, equal0 = 0; from < mt; from += per * threads) {
                 const int b0 = from + i * per, size = min(per, mt - b0);
                 uint32_t above = 0, equal = 0;
-#pragma unroll 4
+#pragma unroll 8
                 for (int j = 0; j < size; ++j) {
                     const uint32_t key = keys[b0 + j];
                     above |= (key > least ? 1u : 0u) << j;
@@ -706,15 +707,16 @@ cudaError_t launch_tiles(SelectParams& p, long long tiles, cudaStream_t st)
 }
 
 // Tiles and clusters.  Tiles of 16 tokens read the boxes half as often as those of 8, which fill the GPU with fewer tokens:
-// a chunk of 1024 behind 30000 (8 kv heads, pages of 64) takes 46 us with 16, 60 with 8; one of 100 behind 8000 12.5 and
-// 10.9.  A cluster's CTAs share a tile's boxes, 16 a warp at a time, where there are fewer tiles than SMs: one token behind
+// a chunk of 1024 behind 30000 (8 kv heads, pages of 64) takes 45 us with 16, 60 with 8; one of 100 behind 8000 12.5 and
+// 10.7.  A cluster's CTAs share a tile's boxes, 16 a warp at a time, where there are fewer tiles than SMs: one token behind
 // 32000 in pages of 16 (4 kv heads) takes 26.4 us with one CTA, 18.6 with 2, 14.0 with 4, 11.4 with 8, 10.9 with 16; one
-// behind 131000 86 to 24.5 and 20.8; where tiles fill the GPU, more CTAs only add their own 5 us (32 tokens x 8 heads: 13.9
-// us with one, 20.6 with 2).
+// behind 131000 86 to 24.5 and 19.3; where tiles fill the GPU, more CTAs only add their own 5 us (32 tokens x 8 heads: 13.9
+// us with one, 20.6 with 2).  They pay from 128 pages a CTA for one token (127 of them 7.7 us with one CTA, 8.0 with 2), 120
+// for several (5 tokens, 94 to 96 pages 8.3 and 8.7; 251 with 2 and 4 9.2 and 8.8).
 template <typename T, int D>
 cudaError_t launch_select(SelectParams p, cudaStream_t st)
 {
-    p.cap = (p.c.table_width + 3) / 4 * 4;
+    p.cap = (p.c.table_width + 11) / 16 * 16 + 4;                  // the scores of a lane's neighbours in other banks
     p.direct = p.c.max_q <= 8;
     auto bytes = [&]() { return (size_t)((p.tile + (1 << p.lg) - 1) >> p.lg) * p.cap * 4; };
     const long long rows = (long long)p.c.total_q * p.l.kv_heads;
@@ -726,9 +728,10 @@ cudaError_t launch_select(SelectParams p, cudaStream_t st)
         p.lg = 0;
     }
     p.tile = p.c.max_q <= 1 ? 1 : 8;
+    const int least = p.tile == 1 ? 128 : 120;
     const long long tiles = p.direct ? p.c.n_req : p.c.total_q / 8 + (long long)p.c.n_req;
-    while (p.lg < 3 && tiles * p.l.kv_heads << p.lg < 148 && p.cap > 128 << p.lg) ++p.lg;
-    if (p.lg == 3 && tiles * p.l.kv_heads << 4 <= 148 && p.cap > 1024) p.lg = 4;
+    while (p.lg < 3 && tiles * p.l.kv_heads << p.lg < 148 && p.c.table_width > least << p.lg) ++p.lg;
+    if (p.lg == 3 && tiles * p.l.kv_heads << 4 <= 148 && p.c.table_width > 1024) p.lg = 4;
     while (p.lg < 3 && bytes() > kSelSmem) ++p.lg;
     return launch_tiles<T, D, 1>(p, tiles, st);
 }
