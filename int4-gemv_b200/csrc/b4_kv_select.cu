@@ -27,7 +27,7 @@
 // registers (a bisection with 16 scores a lane in registers: 450 cycles a bit).  32 tokens
 // behind 8 to 32 thousand in pages of 64 (8 kv heads): 13.5 us, of which the 21 MB of boxes
 // take 6; one behind 131000 in pages of 16: 20.9 us, 17.8 MB; a chunk of 1024 behind 30000:
-// 44.8 us for 8192 choices among 480 boxes, 13 of 45 us the scores, the rest the choices.
+// 44.4 us for 8192 choices among 480 boxes, 13 of 45 us the scores, the rest the choices.
 #include <algorithm>
 #include <climits>
 #include <type_traits>
@@ -259,9 +259,9 @@ __device__ __forceinline__ Seen seen_of(const SelectParams& p, int ctx, int n, i
     return s;
 }
 
-// NT: eights of tokens in a tile
-template <typename T, int D, int NT>
-__global__ void __launch_bounds__(kSelThreads, 2) kv_select_kernel(const SelectParams p)
+// NT: eights of tokens in a tile; CTAS: of them on an SM
+template <typename T, int D, int NT, int CTAS>
+__global__ void __launch_bounds__(kSelThreads, CTAS) kv_select_kernel(const SelectParams p)
 {
     constexpr int V = D / 32;                                      // 16-byte words of a box that a lane holds
     constexpr int C = D / 32;                                      // columns of a query that a lane holds
@@ -429,7 +429,7 @@ __global__ void __launch_bounds__(kSelThreads, 2) kv_select_kernel(const SelectP
                 const int b = step * 16 + g;
                 // every row is a page with a finite box, but at the list's end and beside pages that are not
                 const bool plain = __all_sync(0xffffffffu, step * 16 + 16 <= m && x.unit[0] < INFINITY && x.unit[1] < INFINITY);
-#pragma unroll 1
+#pragma unroll
                 for (int nt8 = 0; nt8 < NT; ++nt8) {
                     if (nt8 * 8 >= nt) break;
                     int acc[4] = {0, 0, 0, 0};
@@ -666,10 +666,17 @@ __global__ void __launch_bounds__(kSelThreads, 2) kv_select_kernel(const SelectP
     }
 }
 
+// Two CTAs on an SM, with registers for the boxes ahead; with heads of 64 four, with half the registers, where there are so
+// many that more at once pay: 64 tokens behind 8000 in pages of 32 (8 kv heads) 13.8 us (16.0 with two), 1024 behind 30000 34.8
+// (38.4); 40 of them, 320 CTAs, 13.4 (11.5).  With heads of 128 even three spill: 58.7 us for 44.4.
 template <typename T, int D, int NT>
 cudaError_t launch_tiles(SelectParams& p, long long tiles, cudaStream_t st)
 {
-    auto fn = kv_select_kernel<T, D, NT>;
+    auto fn = kv_select_kernel<T, D, NT, 2>;
+    if constexpr (D == 64) {
+        const long long likely = p.direct ? tiles : tiles - p.c.n_req / 2;                 // a request's last tile half full
+        if (likely * p.l.kv_heads << p.lg > 148 * 5 / 2) fn = kv_select_kernel<T, D, NT, 4>;
+    }
     const size_t smem = (size_t)((p.tile + (1 << p.lg) - 1) >> p.lg) * p.cap * 4;
     if (smem > 24 * 1024) {
         const cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, kSelSmem);
@@ -707,7 +714,7 @@ cudaError_t launch_tiles(SelectParams& p, long long tiles, cudaStream_t st)
 }
 
 // Tiles and clusters.  Tiles of 16 tokens read the boxes half as often as those of 8, which fill the GPU with fewer tokens:
-// a chunk of 1024 behind 30000 (8 kv heads, pages of 64) takes 45 us with 16, 60 with 8; one of 100 behind 8000 12.5 and
+// a chunk of 1024 behind 30000 (8 kv heads, pages of 64) takes 44 us with 16, 60 with 8; one of 100 behind 8000 12.5 and
 // 10.7.  A cluster's CTAs share a tile's boxes, 16 a warp at a time, where there are fewer tiles than SMs: one token behind
 // 32000 in pages of 16 (4 kv heads) takes 26.4 us with one CTA, 18.6 with 2, 14.0 with 4, 11.4 with 8, 10.9 with 16; one
 // behind 131000 86 to 24.5 and 19.3; where tiles fill the GPU, more CTAs only add their own 5 us (32 tokens x 8 heads: 13.9

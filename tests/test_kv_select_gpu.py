@@ -158,6 +158,20 @@ def test_many_requests(cuda):
         check(cuda, make(cuda, F16, 4, 2, 64, 16, ctx, new, extra=3), 6, 1, 1)
 
 
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_more_than_fit_at_once(cuda, dtype, d):
+    """More CTAs than the GPU holds: of a token each, of several, of 16."""
+    rng = np.random.default_rng(d)
+    for n, new in ((150, 1), (130, 4), (2, 300)):
+        s = make(cuda, dtype, 8, 4 if n > 2 else 8, d, 16, (new + rng.integers(0, 2500, n)).tolist(), [new] * n)
+        check(cuda, s, 24, 1, 2)
+        if n > 2:
+            s["box"][::11, :, 2 * d: 2 * d + 4] = np.float32([np.nan]).view(np.uint8)
+            s["tab"][::3, ::5] = -1
+            check(cuda, s, 24, 1, 2)
+
+
 @pytest.mark.parametrize("new", [1, 5, 12])
 def test_ties_go_to_the_earlier(cuda, new):
     """Boxes that are all alike, or of three kinds, and queries of zeros."""
