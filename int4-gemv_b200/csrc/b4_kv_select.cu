@@ -287,7 +287,8 @@ __global__ void __launch_bounds__(kSelThreads, CTAS) kv_select_kernel(const Sele
     auto start = [&](int r) { return max(0, min(__ldg(a.q_starts + r), a.total_q)); };
     int r = at_tile, tile0 = 0;
     if (!p.direct) {
-        // request r has the tiles from start / tile + r on, as many as it needs at least: the last that begins at or before this one
+        // request r has the tiles from start / tile + r on, as many as it needs at least: the last that begins at or before this
+        // one.  Tiles before the first request's, where it does not begin at row 0, have no tokens
         int lo = 0, n = a.n_req;
         while (n > 1) {
             const int step = (n + 31) / 32, probe = lo + lane * step;
@@ -312,7 +313,7 @@ __global__ void __launch_bounds__(kSelThreads, CTAS) kv_select_kernel(const Sele
     ids_of(step0 + stride, next);
     const int q0 = start(r), n = max(0, start(r + 1) - q0), ctx = max(0, __ldg(a.ctx_len + r));
 
-    for (int i0 = tile0 * p.tile, turn = 0; i0 < n; i0 = p.direct ? i0 + p.tile : n, ++turn) {
+    for (int i0 = tile0 < 0 ? n : tile0 * p.tile, turn = 0; i0 < n; i0 = p.direct ? i0 + p.tile : n, ++turn) {
         const int nt = min(p.tile, n - i0);
         const Seen most = seen_of(p, ctx, n, i0 + nt - 1);
         const int m = most.pages > a.keep ? most.pages - a.first - a.last : 0;     // pages to score
