@@ -607,10 +607,11 @@ int b4_kv_boxes(const b4_kv_cache* cache, const int32_t* slots, int n_tokens, vo
  * and of the others those of the largest score, ties to the earlier.  -1 after them.
  *   score = box scale * sum over columns of (above * maximum + below * minimum),
  * the sum of whole numbers times the scale, rounded to fp32 once: above and below are
- * the sums over the kv head's queries of max(q, 0) and min(q, 0), in 64 bits, rounded
- * to fp32, then to int8 in units of the largest of them in magnitude times fp32's
- * 1/127 (by the fp32 quotient, ties to even).  Without the roundings to 8 bits that
- * is the least upper bound of the sum of the heads' products with any key in the box.
+ * the sums over the kv head's queries of max(q, 0) and min(q, 0), in 64 bits (head
+ * after head, which matters to bf16 numbers far apart), rounded to fp32, then to int8
+ * in units of the largest of them in magnitude times fp32's 1/127 (by the fp32
+ * quotient, ties to even).  Without the roundings to 8 bits that is the least upper
+ * bound of the sum of the heads' products with any key in the box.
  * Boxes whose scale is not finite come first among the others (+infinity), pages
  * missing from the table last; a query that is not finite scores every page 0.
  * seen[t]: the tokens that t sees of its list, the last page's up to its own place;

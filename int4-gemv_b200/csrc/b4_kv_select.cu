@@ -193,27 +193,22 @@ __device__ __forceinline__ void store_cluster(uint32_t at, uint32_t rank, uint32
     asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(there), "r"(v) : "memory");
 }
 
-// sum + err += x exactly, as long as err's own sum is: two numbers of 24 bits hold the sum of 64 fp16 numbers
-__device__ __forceinline__ void add_exact(float& sum, float& err, float x)
-{
-    const float s = __fadd_rn(sum, x), part = __fsub_rn(s, sum);
-    err = __fadd_rn(err, __fadd_rn(__fsub_rn(sum, __fsub_rn(s, part)), __fsub_rn(x, part)));
-    sum = s;
-}
-
 // The codes of C columns of a query's sums above and below 0, from the definition; by whole warps.  Its first 8 heads as loaded.
+// In 64 bits, one head after the other: exact for fp16 numbers, whose sums of 64 take 46 bits at most; bf16 numbers may lie
+// further apart than any sum holds (two fp32 numbers in its place lost 2^-48 beside 2.5, and with it the side of a border).
 template <typename T, int C, typename Raw>
 __device__ void exact_codes(const Raw (&raw)[8], const T* src, int group, long long stride, uint32_t (&w)[2])
 {
-    float sum[2][C], err[2][C], top = 0.0f;
+    double sum[2][C];
+    float part[2][C], top = 0.0f;
 #pragma unroll
-    for (int j = 0; j < C; ++j) sum[0][j] = sum[1][j] = err[0][j] = err[1][j] = 0.0f;
+    for (int j = 0; j < C; ++j) sum[0][j] = sum[1][j] = 0.0;
     auto add = [&](const Raw& r) {
 #pragma unroll
         for (int j = 0; j < C; ++j) {
             const float f = kv_float(reinterpret_cast<const T*>(&r)[j]);
-            add_exact(sum[0][j], err[0][j], f > 0.0f ? f : 0.0f);
-            add_exact(sum[1][j], err[1][j], f > 0.0f ? 0.0f : f);      // NaN too
+            sum[0][j] += f > 0.0f ? f : 0.0f;
+            sum[1][j] += f > 0.0f ? 0.0f : f;                      // NaN too
         }
     };
 #pragma unroll
@@ -225,9 +220,9 @@ __device__ void exact_codes(const Raw (&raw)[8], const T* src, int group, long l
     for (int k = 0; k < 2; ++k)
 #pragma unroll
         for (int j = 0; j < C; ++j) {
-            sum[k][j] = __fadd_rn(sum[k][j], err[k][j]);
-            finite = finite && fabsf(sum[k][j]) < INFINITY;
-            top = fmaxf(top, fabsf(sum[k][j]));
+            part[k][j] = __double2float_rn(sum[k][j]);
+            finite = finite && fabsf(part[k][j]) < INFINITY;
+            top = fmaxf(top, fabsf(part[k][j]));
         }
     top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
     finite = __all_sync(0xffffffffu, finite);
@@ -237,7 +232,7 @@ __device__ void exact_codes(const Raw (&raw)[8], const T* src, int group, long l
 #pragma unroll
     for (int k = 0; k < 2; ++k)
 #pragma unroll
-        for (int j = 0; j < C; ++j) w[k] |= (uint32_t)(box_code(sum[k][j], unit) & 255) << (8 * j);
+        for (int j = 0; j < C; ++j) w[k] |= (uint32_t)(box_code(part[k][j], unit) & 255) << (8 * j);
 }
 
 // What a query sees: its pages, its own the last, and its list's entries and tokens.
