@@ -572,8 +572,11 @@ int b4_rotary_turns(const double* inv_freq, int n, uint64_t* turns);
  * machine rounds; queries turn in fp32 and are rounded to out_dtype.
  * q (NULL with heads 0: keys and values alone), k, v: dtype fp16, bf16 or fp32, any
  * strides in elements, columns contiguous; out_dtype: fp16 or bf16, dtype's own where
- * that is 16 bits; q_out's rows 16-byte aligned.  q_out may be q with its strides, and
- * overlaps nothing else.  Every row of q_out is written, those without a slot too. */
+ * that is 16 bits; q_out's rows 16-byte aligned.  q_out may be q with its strides and type,
+ * and lies on nothing else that the call reads or writes: columns of the rows that hold q,
+ * k and v in one token stride are told apart, rows that lie between one another in other
+ * ways are refused as overlaps are, and so are two rows of q_out in one place.  Every row
+ * of q_out is written, those without a slot too. */
 typedef struct b4_kv_rows {
     const void *q, *k, *v;
     void* q_out;

@@ -24,6 +24,7 @@
 #include <cmath>
 #include <type_traits>
 
+#include "b4_kv_overlap.h"
 #include "b4_kv_quant.cuh"
 
 namespace b4 {
@@ -217,6 +218,21 @@ cudaError_t launch(RotaryParams p, bool adjacent, cudaStream_t st)
                     : kv_launch(kv_append_rotary_kernel<T, O, FMT, D, false>, grid, kRotThreads, 0, st, p);
 }
 
+// q_out on what other warps read, or two of its rows on one another: q itself alone may be where it is
+bool out_in_the_way(const b4_kv_cache* cache, const KvLayout& l, const b4_rotary* r, const b4_kv_rows* x)
+{
+    const long long n = x->n_tokens, item = x->dtype == B4_DTYPE_F32 ? 4 : 2, d = l.head_dim;
+    const RowSet out = row_set(x->q_out, 2, x->out_stride_token, x->out_stride_head, n, x->heads, d);
+    const bool in_place = x->q_out == x->q && item == 2 && (n == 1 || x->out_stride_token == x->q_stride_token) &&
+                          (x->heads == 1 || x->out_stride_head == x->q_stride_head);
+    return rows_overlap(out) || (!in_place && rows_meet(out, row_set(x->q, item, x->q_stride_token, x->q_stride_head, n, x->heads, d))) ||
+           rows_meet(out, row_set(x->k, item, x->k_stride_token, x->k_stride_head, n, l.kv_heads, d)) ||
+           rows_meet(out, row_set(x->v, item, x->v_stride_token, x->v_stride_head, n, l.kv_heads, d)) ||
+           rows_meet(out, row_set(x->positions, 4, x->position_stride, 0, r->axes ? r->n_axes : 1, 1, n)) ||
+           rows_meet(out, row_set(x->slots, 4, n)) || rows_meet(out, row_set(r->turns, 8, r->dim / 2)) ||
+           (r->axes && rows_meet(out, row_set(r->axes, 1, r->dim / 2))) || rows_meet(out, row_set(cache->blocks, l.block, (long long)l.n_pages * l.kv_heads));
+}
+
 template <typename T, typename O>
 cudaError_t launch(const RotaryParams& p, bool adjacent, cudaStream_t st)
 {
@@ -266,6 +282,7 @@ int b4_kv_append_rotary(const b4_kv_cache* cache, const b4_rotary* r, const b4_k
     if (x->heads > 0 && (!kv_aligned(x->q, item) || !kv_aligned(x->q_out, 16) || (x->out_stride_token | x->out_stride_head) % 8 != 0))
         return cudaErrorInvalidValue;
     if (r->n_axes > 1 && (!r->axes || x->position_stride < x->n_tokens)) return cudaErrorInvalidValue;
+    if (x->heads > 0 && out_in_the_way(cache, p.l, r, x)) return cudaErrorInvalidValue;
     p.blocks = static_cast<uint8_t*>(cache->blocks);
     p.src[0] = x->k;
     p.src[1] = x->v;
