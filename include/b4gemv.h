@@ -622,8 +622,8 @@ int b4_kv_boxes(const b4_kv_cache* cache, const int32_t* slots, int n_tokens, vo
  * written).  Only boxes of pages before a query's own are read.
  * Requests, queries and tables as in b4_kv_attn; a table's first table_width pages
  * count, at most B4_KV_SELECT_MAX_WIDTH of them.  lists and seen overlap neither
- * one another nor tables, ctx_len or q_starts (refused).  1 <= last, 0 <= first, first + last
- * <= keep, keep * page_size <= 2^31 - 64, keep <= B4_KV_SELECT_MAX_WIDTH. */
+ * one another nor q, boxes, tables, ctx_len or q_starts (refused).  1 <= last,
+ * 0 <= first, first + last <= keep, keep * page_size <= 2^31 - 64, keep <= B4_KV_SELECT_MAX_WIDTH. */
 #define B4_KV_SELECT_MAX_WIDTH 49152
 typedef struct b4_kv_choice {
     const void* q;                /* fp16 or bf16 [total_q][heads][head_dim], as b4_kv_attn's */

@@ -33,6 +33,7 @@
 #include <type_traits>
 
 #include "b4_kv.cuh"
+#include "b4_kv_overlap.h"
 
 namespace b4 {
 namespace {
@@ -739,12 +740,6 @@ cudaError_t launch_select(SelectParams p, cudaStream_t st)
     return launch_tiles<T, D, 1>(p, tiles, st);
 }
 
-struct Span {                              // of int32 values
-    uintptr_t from, to;
-    Span(const int32_t* at, long long n) : from(reinterpret_cast<uintptr_t>(at)), to(from + 4 * n) {}
-    bool meets(const Span& o) const { return from < o.to && o.from < to && from < to && o.from < o.to; }
-};
-
 template <int FMT>
 cudaError_t launch_boxes(const BoxParams& p, cudaStream_t st)
 {
@@ -800,12 +795,14 @@ int b4_kv_select(const b4_kv_cache* cache, const b4_kv_choice* c, b4_stream_t st
     if (c->total_q == 0) return cudaSuccess;
     if (!c->q || !c->boxes || !c->lists || !c->seen || (c->n_req > 0 && (!c->ctx_len || !c->q_starts || (c->table_width > 0 && !c->tables))))
         return cudaErrorInvalidValue;
-    // every CTA reads the lengths and tables while others write what they chose
-    const Span lists(c->lists, (long long)c->total_q * p.l.kv_heads * c->keep), seen(c->seen, c->total_q);
-    const Span reads[] = {{c->tables, c->n_req > 0 ? (c->n_req - 1) * c->table_stride + c->table_width : 0}, {c->ctx_len, c->n_req}, {c->q_starts, c->n_req + 1LL}};
-    if (lists.meets(seen)) return cudaErrorInvalidValue;
-    for (const Span& r : reads)
-        if (r.meets(lists) || r.meets(seen)) return cudaErrorInvalidValue;
+    // every CTA reads these while others write what they chose
+    const RowSet lists = row_set(c->lists, 4, (long long)c->total_q * p.l.kv_heads * c->keep), seen = row_set(c->seen, 4, c->total_q);
+    const RowSet reads[] = {row_set(c->tables, 4, c->n_req > 0 ? (c->n_req - 1) * c->table_stride + c->table_width : 0), row_set(c->ctx_len, 4, c->n_req),
+                            row_set(c->q_starts, 4, c->n_req + 1LL), row_set(c->boxes, box_bytes(p.l.head_dim), (long long)p.l.n_pages * p.l.kv_heads),
+                            row_set(c->q, 2, c->q_stride_token, c->q_stride_head, c->total_q, c->heads, p.l.head_dim)};
+    if (rows_meet(lists, seen)) return cudaErrorInvalidValue;
+    for (const RowSet& r : reads)
+        if (rows_meet(r, lists) || rows_meet(r, seen)) return cudaErrorInvalidValue;
     if (!kv_aligned(c->q, 16) || !kv_aligned(c->boxes, 16) || (c->q_stride_token | c->q_stride_head) % 8 != 0) return cudaErrorInvalidValue;
     p.c = *c;
     p.group = c->heads / p.l.kv_heads;

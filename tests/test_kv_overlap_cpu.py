@@ -94,3 +94,16 @@ ROWS = dict(q=1 << 30, k=1 << 31, v=1 << 32, q_out=1 << 33, positions=1 << 34, s
 def test_outputs_on_inputs_are_refused(bad):
     """Rotated queries on keys, values, other queries, positions, slots, angles, the cache, or on one another."""
     assert refused("b4_kv_append_rotary", byref(cache()), byref(_lib.RotaryTable(**ROTARY)), byref(_lib.KvRows(**{**ROWS, **bad})), None)
+
+
+CHOICE = dict(q=1 << 30, boxes=1 << 31, tables=1 << 32, ctx_len=1 << 33, q_starts=1 << 34, lists=1 << 35, seen=1 << 36, table_stride=5, q_stride_token=512,
+              q_stride_head=64, table_width=5, n_req=3, total_q=8, max_q=4, heads=4, dtype=0, keep=4, first=1, last=1)
+
+
+@pytest.mark.parametrize("bad", [
+    dict(lists=1 << 30), dict(lists=(1 << 30) + 7 * 1024 + 508), dict(lists=(1 << 30) - 252), dict(lists=1 << 31), dict(lists=(1 << 31) + 4 * 2 * 144 - 4),
+    dict(seen=1 << 30), dict(seen=(1 << 30) + 1024), dict(seen=(1 << 30) + 512 - 4), dict(seen=(1 << 31) - 28), dict(seen=(1 << 31) + 4 * 2 * 144 - 4),
+    dict(seen=1 << 35), dict(seen=(1 << 32) + 14 * 4), dict(lists=(1 << 34) + 12)])
+def test_choices_on_what_is_read_are_refused(bad):
+    """Lists and seen on queries or boxes too, which other CTAs read while they are written."""
+    assert refused("b4_kv_select", byref(cache()), byref(_lib.KvChoice(**{**CHOICE, **bad})), None)
