@@ -644,7 +644,9 @@ int b4_kv_select(const b4_kv_cache* cache, const b4_kv_choice* choice, b4_stream
  * their own way: tables = lists, int32 [total_q][kv_heads][table_width], table_stride
  * and list_stride_head its strides in entries; ctx_len = seen [total_q] (0: zeros are
  * written, below 0: the row of out and lse is left as it is; more than the list holds:
- * what it holds).  q_starts, n_req, max_q are not read, window and flags must be 0. */
+ * what it holds).  q_starts, n_req, max_q are not read, window and flags must be 0.
+ * out may be q with its strides; else out and lse overlap neither one another nor
+ * what the call reads (refused, as in b4_kv_append_rotary). */
 int b4_kv_attention_lists_workspace(const b4_kv_cache* cache, const b4_kv_attn* attn, size_t* bytes);
 int b4_kv_attention_lists(const b4_kv_cache* cache, const b4_kv_attn* attn, long long list_stride_head, void* ws, size_t ws_bytes,
                           b4_stream_t stream);

@@ -5,6 +5,7 @@
 #include "b4_kv_attn_lists.cuh"
 #include "b4_kv_attn_tile.cuh"
 #include "b4_kv_attn_warp.cuh"
+#include "b4_kv_overlap.h"
 
 namespace b4 {
 namespace {
@@ -199,6 +200,22 @@ int list_params(const b4_kv_cache* cache, const b4_kv_attn* attn, AttnParams* p)
     return e;
 }
 
+// outputs on what other teams read, or on one another: a query's own row alone may be where its output goes
+bool outputs_in_the_way(const b4_kv_cache* cache, const AttnParams& p)
+{
+    const b4_kv_attn& a = p.a;
+    const long long n = a.total_q, d = p.l.head_dim;
+    const RowSet out = row_set(a.out, 2, a.out_stride_token, a.out_stride_head, n, a.heads, d), lse = row_set(a.lse, 4, a.lse ? n * a.heads : 0);
+    const RowSet q = row_set(a.q, 2, a.q_stride_token, a.q_stride_head, n, a.heads, d);
+    const bool in_place = a.out == a.q && (n == 1 || a.out_stride_token == a.q_stride_token) && (a.heads == 1 || a.out_stride_head == a.q_stride_head);
+    if (rows_overlap(out) || rows_meet(out, lse) || (!in_place && rows_meet(out, q)) || rows_meet(lse, q)) return true;
+    const RowSet reads[] = {row_set(a.tables, 4, a.table_stride, p.list_head, n, p.l.kv_heads, a.table_width), row_set(a.ctx_len, 4, n),
+                            row_set(cache->blocks, p.l.block, (long long)p.l.n_pages * p.l.kv_heads)};
+    for (const RowSet& r : reads)
+        if (rows_meet(out, r) || rows_meet(lse, r)) return true;
+    return false;
+}
+
 int attend(const AttnParams& p, void* ws, size_t ws_bytes, b4_stream_t stream)
 {
     const b4_kv_attn& a = p.a;
@@ -266,6 +283,7 @@ int b4_kv_attention_lists(const b4_kv_cache* cache, const b4_kv_attn* a, long lo
     if (list_stride_head < a->table_width) return cudaErrorInvalidValue;
     if (a->total_q == 0) return cudaSuccess;
     p.list_head = list_stride_head;
+    if (outputs_in_the_way(cache, p)) return cudaErrorInvalidValue;
     return attend(p, ws, ws_bytes, stream);
 }
 

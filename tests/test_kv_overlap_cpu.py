@@ -107,3 +107,16 @@ CHOICE = dict(q=1 << 30, boxes=1 << 31, tables=1 << 32, ctx_len=1 << 33, q_start
 def test_choices_on_what_is_read_are_refused(bad):
     """Lists and seen on queries or boxes too, which other CTAs read while they are written."""
     assert refused("b4_kv_select", byref(cache()), byref(_lib.KvChoice(**{**CHOICE, **bad})), None)
+
+
+LISTS = dict(q=1 << 30, out=1 << 31, lse=1 << 32, tables=1 << 33, ctx_len=1 << 34, q_starts=None, table_stride=8, q_stride_token=256, q_stride_head=64,
+             out_stride_token=256, out_stride_head=64, table_width=4, n_req=0, total_q=8, max_q=0, heads=4, dtype=0, window=0, flags=0, scale=0.125)
+
+
+@pytest.mark.parametrize("bad", [
+    dict(out=1 << 33), dict(out=(1 << 33) + 7 * 32 + 16), dict(out=(1 << 33) - 8 * 512 + 16), dict(out=1 << 34), dict(out=(1 << 34) - 8 * 512 + 16), dict(out=4096),
+    dict(out=(1 << 30) + 128), dict(out=1 << 30, out_stride_token=512), dict(out=(1 << 32) - 16), dict(lse=(1 << 31) + 512), dict(lse=1 << 33), dict(lse=(1 << 34) - 124),
+    dict(lse=1 << 30), dict(lse=(1 << 30) + 8 * 512 - 4), dict(lse=4096), dict(out_stride_token=0), dict(out_stride_head=0), dict(out_stride_head=56)])
+def test_attention_on_what_is_read_is_refused(bad):
+    """Outputs on lists, seen, the cache, queries that are not the row's own, or on one another."""
+    assert refused("b4_kv_attention_lists", byref(cache()), byref(_lib.KvAttn(**{**LISTS, **bad})), 4, 1 << 44, 1 << 40, None)

@@ -1,5 +1,5 @@
-"""Where the rotated append may write its queries: in place among fused rows of queries, keys and values, whatever their order."""
-import numpy as np
+"""Where outputs may lie: the rotated append in place among fused rows of queries, keys and values, whatever their order; attention
+over its own queries."""
 import pytest
 import torch
 
@@ -53,3 +53,22 @@ def test_outputs_on_inputs_are_refused(cuda):
     assert torch.equal(fused, before) and not bool(cache.blocks.any())
     b4gemv.kv_append_rotary(cache, rotary, q, k, v, at, at, out=fused[:, 8:])
     assert torch.equal(fused[:, :8], before[:, :8]) and not torch.equal(fused[:, 8:], before[:, 8:])
+
+
+def test_attention_in_place(cuda):
+    """Over its own queries; a few heads off is refused."""
+    for total, keep in ((3, 40), (200, 6)):                        # lists shared by teams, and not
+        g = torch.Generator(device=cuda).manual_seed(total)
+        cache = b4gemv.KVCache.alloc(INT4, 60, 2, 16, 128, cuda)
+        at = torch.arange(60 * 16, dtype=torch.int32, device=cuda)
+        b4gemv.kv_append(cache, *(torch.randn((60 * 16, 2, 128), generator=g, device=cuda) for _ in range(2)), at)
+        room = torch.randn((total, 24, 128), generator=g, device=cuda).half()
+        q = room[:, 2:22]
+        lists = b4gemv.KVLists(torch.randint(0, 60, (total, 2, keep), generator=g, device=cuda).int(), torch.randint(0, 16 * keep + 1, (total,), generator=g, device=cuda).int())
+        want, before = b4gemv.kv_attention_lists(cache, q.clone(), lists), room.clone()
+        for out in (room[:, 1:21], room[:, 4:], room[:, 2:3].expand(total, 20, 128)):
+            with pytest.raises(b4gemv.B4Error):
+                b4gemv.kv_attention_lists(cache, q, lists, out=out)
+        assert torch.equal(room, before)
+        b4gemv.kv_attention_lists(cache, q, lists, out=q)
+        assert torch.equal(q, want) and torch.equal(room[:, :2], before[:, :2]) and torch.equal(room[:, 22:], before[:, 22:])
