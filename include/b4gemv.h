@@ -563,7 +563,10 @@ typedef struct b4_rotary {
     int dim, n_axes, flags;
     float scale;
 } b4_rotary;
-/* Host: turns[i] = the fraction of inv_freq[i] / (2 pi), rounded to 64 bits.  inv_freq in radians a position, finite. */
+/* Host: turns[i] = the fraction of the fp64 quotient inv_freq[i] / 2 pi, rounded to 64 bits.  inv_freq in radians a
+ * position, finite.  2 pi and the quotient are rounded to fp64, so a turn is off by 2^-52 of inv_freq / (2 pi) at most, and an
+ * angle from position * inv_freq by 2^-52 of that product (1e-10 of a radian at position 500000 for a frequency of 1):
+ * what is exact here is exact relative to turns. */
 int b4_rotary_turns(const double* inv_freq, int n, uint64_t* turns);
 
 /* q_out[t][h] = q rotated, k rotated and v as b4_kv_append writes them at slots[t].

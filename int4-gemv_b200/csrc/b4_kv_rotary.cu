@@ -2,11 +2,12 @@
 // keys on the way.
 //
 // Mathematics.  A position's angle is position * turns mod 2^64, in whole steps of
-// 2^-64 turn: exact for any position, so what is rounded is the angle itself (to
-// 2^-53 of half a turn), its sine and cosine, and the rotated column, once.  Keys are
-// rotated in fp64: their 4-bit codes are then those of the exact rotation but where
-// it lies within 2^-50 of a border, whatever computes it, for 2 DFMA a column of a few
-// heads; queries, whose rounding to 16 bits is next, in fp32.
+// 2^-64 turn: exact relative to the table for any position (the table is off by 2^-52 of a
+// frequency at most), so what is rounded is the angle itself (to 2^-53 of half a turn), its
+// sine and cosine, and the rotated column, once.  Keys are rotated in fp64: their 4-bit
+// codes are then those of the exact rotation by the table's angles but where it lies
+// within 2^-50 of a border, whatever computes it, for 2 DFMA a column of a few heads;
+// queries, whose rounding to 16 bits is next, in fp32.
 //
 // Split.  A warp takes a token, or a part of its vectors (heads of q, k and v), 32 * 8 / D
 // of one kind at a time, and computes the token's angles itself, one or two a lane: no
@@ -254,7 +255,7 @@ int b4_rotary_turns(const double* inv_freq, int n, uint64_t* turns)
         if (!std::isfinite(inv_freq[i])) return cudaErrorInvalidValue;
     for (int i = 0; i < n; ++i) {
         const double f = std::fabs(inv_freq[i] / 6.283185307179586476925287), part = f - std::floor(f);
-        // 64 bits of the part: the upper 32, then what they leave, rounded; all else is exact
+        // 64 bits of the quotient's part: the upper 32, then what they leave, rounded; all but the quotient is exact
         const double hi = std::floor(part * 0x1p32), lo = std::nearbyint((part * 0x1p32 - hi) * 0x1p32);
         const uint64_t t = ((uint64_t)hi << 32) + (uint64_t)lo;
         turns[i] = inv_freq[i] < 0.0 ? 0 - t : t;
