@@ -36,7 +36,8 @@ def rotate(x, positions, base: float = 1e6):
 
 class CachedAttention:
     """rotary: the rotation in the append's launch (kv_append_rotary) instead of rotate()'s torch operations; keep: pages of
-    each kv head that a query reads, the first `first` and the last `last` of its context among them (0: all)."""
+    each kv head that a query reads, the first `first` and the last `last` of its context among them (0: all).  Every step then
+    goes through the choice, prompts too, which gain only where contexts are five or six times what is kept."""
 
     def __init__(self, fmt: int, hidden: int, heads: int, kv_heads: int, n_pages: int, max_requests: int, head_dim: int = 128,
                  page_size: int = 64, max_context: int = 4096, seed: int = 0, device="cuda", rotary: Rotary | None = None, keep: int = 0,

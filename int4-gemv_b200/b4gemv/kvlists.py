@@ -107,7 +107,7 @@ def kv_append_rotary(cache, rotary: Rotary, q, k, v, positions, slots, out=None,
     """b4_kv_append_rotary: q [tokens][heads][head_dim] (or None) and k [tokens][kv_heads][head_dim] rotated by positions,
     k and v quantised into the cache at slots.  q, k, v: all fp16, bf16 or fp32, any token and head strides, columns
     contiguous.  positions: int32 [tokens], or [axes][tokens] where the rotary has several.  Returns the rotated q:
-    out, which may be q itself, or a new tensor of q's type (fp16 for fp32)."""
+    out, which may be q itself but lies on nothing else that the call reads, or a new tensor of q's type (fp16 for fp32)."""
     lib = _lib()
     index, n, dim, dtype = cache.index, slots.numel(), cache.head_dim, k.dtype
     if slots.dtype is not _int32 or slots.get_device() != index or not slots.is_contiguous():
@@ -203,7 +203,8 @@ def kv_select(cache, boxes, q, tables, ctx_len, q_starts, max_q: int, keep: int,
               stream=None) -> KVLists:
     """b4_kv_select: for every query and kv head the `keep` pages that it reads: the first `first` and the last `last` of its
     request's up to its own place, and of the others those whose boxes bound its scores highest.  q, tables, ctx_len,
-    q_starts and max_q as kv_attention takes them; out: buffers to reuse."""
+    q_starts and max_q as kv_attention takes them; out: buffers to reuse, none that the call reads.  Its time follows the
+    tables' width: pass tables[:, :pages] where that is far beyond the longest context."""
     lib = _lib()
     index, dim, kv_heads, n = cache.index, cache.head_dim, cache.kv_heads, ctx_len.numel()
     code, shape, qs = _codes.get(q.dtype), q.shape, q.stride()
@@ -287,7 +288,8 @@ def kv_attention_lists(cache, q, lists: KVLists, scale: float | None = None, out
     """b4_kv_attention_lists: every query's attention over its own lists of pages, one for each kv head (kv_select's, or any
     others: page ids of the cache in the order of the tokens, of which the first lists.seen are seen).  The rest is as
     kv_attention: q and out [tokens][heads][head_dim] fp16 or bf16, scale None = head_dim ** -0.5, lse, ws and the package's
-    workspace of the device.  Rows whose lists.seen is below 0 are left as they are.  Returns out."""
+    workspace of the device.  Rows whose lists.seen is below 0 are left as they are.  Returns out, which may be q itself but
+    lies on nothing else that the call reads."""
     lib = _lib()
     args, across, out = _list_attn(cache, q, lists, scale, out, lse, stream)
     if ws is None:

@@ -2,23 +2,25 @@
 // head: the products and the softmax of b4_kv_attn_cols.cuh, with a schedule for lists.
 //
 // Split.  A list is short (tens of pages) and there are many, of lengths that are alike
-// (a choice keeps as many pages for every query), so a list goes to half a CTA's warps,
-// which share its chunks in runs and join what they leave in shared memory: the two
-// halves of an SM's CTA work on lists of their own, one through its beginning and end
-// while the other multiplies.  The kernel over block tables gives every warp an equal
-// run of all chunks instead: even for any lengths, for searches before and joins across
-// CTAs after that cost lists of 32 pages of 64 as much as their products (64 heads over
-// 8 x 128, 32 queries, INT4: 28.9 us).  Lists that are too few for one more round of all
-// halves are shared by several, whose pieces the last to arrive joins in the list's
-// order: the same bits every time.
+// (a choice keeps as many pages for every query), so a list goes to a team of warps, a
+// half or a quarter of a CTA's (TEAMS = 2 or 4, by the host's model of their times), which
+// share its chunks in runs and join what they leave in shared memory: the teams of an SM's
+// CTA work on lists of their own, one through its beginning and end while the others
+// multiply.  The kernel over block tables gives every warp an equal run of all chunks
+// instead: even for any lengths, for searches before and joins across CTAs after that cost
+// lists of 32 pages of 64 as much as their products (64 heads over 8 x 128, 32 queries,
+// INT4: 28.9 us).  Lists that are too few for one more round of all teams are shared by
+// several, whose pieces the last to arrive joins in the list's order: the same bits every
+// time.
 //
 // What bounds it.  Many lists: the products, a chunk's 600 instructions at 2.4 a cycle (16
 // warps an SM, 2000 cycles for a warp alone, 3200 with three beside it on a scheduler), and
-// 5700 cycles a list around them, half of which the other teams' products hide.  32 queries
-// over 32 pages of 64 (64 heads over 8 x 128, INT4) take 22.7 us, 69 MB, 3.0 TB/s; 64 over
-// 64 pages 69 us, 275 MB, 4.0 TB/s; 96 over up to 64 pages of 16 (32 heads over 8 x 64, NF4
-// in bf16) 24.3 us; a chunk of 300 over 32 pages of 32 (28 heads over 4 x 128, INT4) 47.9 us,
-// whose lists' 162 MB come from L2.  Few: latency, one query over 16 pages of 64 7.6 us.
+// 5700 cycles a list around them, half of which the other teams' products hide.  In two teams
+// 32 queries over 32 pages of 64 (64 heads over 8 x 128, INT4) take 22.7 us, 69 MB, 3.0 TB/s;
+// in four 64 over 64 pages 68.8 us, 275 MB, 4.0 TB/s, 96 over up to 64 pages of 16 (32 heads over
+// 8 x 64, NF4 in bf16) 24.3 us, a chunk of 300 over 32 pages of 32 (28 heads over 4 x 128,
+// INT4) 48.0 us, whose lists' 162 MB come from L2.  Few: latency, one query over 16 pages of
+// 64 7.7 us.
 #pragma once
 
 #include "b4_kv_attn_cols.cuh"

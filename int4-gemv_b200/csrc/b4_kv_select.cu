@@ -25,9 +25,9 @@
 // choice, 0.5 of it the table again.  Code that runs once costs some 5 cycles an instruction
 // here, whatever its kind, so the choice is short loops over shared memory, not unrolled
 // registers (a bisection with 16 scores a lane in registers: 450 cycles a bit).  32 tokens
-// behind 8 to 32 thousand in pages of 64 (8 kv heads): 13.5 us, of which the 21 MB of boxes
-// take 6; one behind 131000 in pages of 16: 20.9 us, 17.8 MB; a chunk of 1024 behind 30000:
-// 44.4 us for 8192 choices among 480 boxes, 13 of 45 us the scores, the rest the choices.
+// behind 8 to 32 thousand in pages of 64 (8 kv heads): 13.3 us, of which the 21 MB of boxes
+// take 6; one behind 131000 in pages of 16: 21.0 us, 17.8 MB; a chunk of 1024 behind 30000:
+// 43.9 us for 8192 choices among 480 boxes, 13 of them the scores, the rest the choices.
 #include <algorithm>
 #include <climits>
 #include <type_traits>
@@ -664,8 +664,9 @@ __global__ void __launch_bounds__(kSelThreads, CTAS) kv_select_kernel(const Sele
 }
 
 // Two CTAs on an SM, with registers for the boxes ahead; with heads of 64 four, with half the registers, where there are so
-// many that more at once pay: 64 tokens behind 8000 in pages of 32 (8 kv heads) 13.8 us (16.0 with two), 1024 behind 30000 34.8
-// (38.4); 40 of them, 320 CTAs, 13.4 (11.5).  With heads of 128 even three spill: 58.7 us for 44.4.
+// many that more at once pay, above 370: 64 tokens behind 8000 in pages of 32 (8 kv heads) 13.6 us (15.9 with two), 1024 behind
+// 30000 34.7 (38.0); 320 CTAs of 40 requests with 1 to 9 drafts behind up to 6000 13.2 (11.4), though 40 single tokens behind
+// 8000 13.2 (14.7).  With heads of 128 even three spill: 58.7 us for 44.4.
 template <typename T, int D, int NT>
 cudaError_t launch_tiles(SelectParams& p, long long tiles, cudaStream_t st)
 {
@@ -711,12 +712,16 @@ cudaError_t launch_tiles(SelectParams& p, long long tiles, cudaStream_t st)
 }
 
 // Tiles and clusters.  Tiles of 16 tokens read the boxes half as often as those of 8, which fill the GPU with fewer tokens:
-// a chunk of 1024 behind 30000 (8 kv heads, pages of 64) takes 44 us with 16, 60 with 8; one of 100 behind 8000 12.5 and
-// 10.7.  A cluster's CTAs share a tile's boxes, 16 a warp at a time, where there are fewer tiles than SMs: one token behind
-// 32000 in pages of 16 (4 kv heads) takes 26.4 us with one CTA, 18.6 with 2, 14.0 with 4, 11.4 with 8, 10.9 with 16; one
-// behind 131000 86 to 24.5 and 19.3; where tiles fill the GPU, more CTAs only add their own 5 us (32 tokens x 8 heads: 13.9
-// us with one, 20.6 with 2).  They pay from 128 pages a CTA for one token (127 of them 7.7 us with one CTA, 8.0 with 2), 120
-// for several (5 tokens, 94 to 96 pages 8.3 and 8.7; 251 with 2 and 4 9.2 and 8.8).
+// a chunk of 1024 behind 30000 (8 kv heads, pages of 64) takes 43.8 us with 16, 57.3 with 8; one of 100 behind 8000 14.1 and
+// 10.4.  A cluster's CTAs share a tile's boxes, 16 a warp at a time, where there are fewer tiles than SMs: one token behind
+// 32000 in pages of 16 (4 kv heads) takes 20.2 us with one CTA, 15.6 with 2, 12.7 with 4, 11.0 with 8, 10.6 with 16; one
+// behind 131000 80.9 to 23.0 and 19.5; where tiles fill the GPU, more CTAs only add their own 7 us (32 tokens x 8 heads: 13.4
+// us with one, 20.4 with 2).  They pay from 128 pages a CTA for one token (128 of them 7.3 us with one CTA, 7.8 with 2; 157
+// 7.6 and 7.5), 120 for several (5 tokens, 94 pages 8.1 and 8.5; 251 with 2 and 4 9.1 and 8.6).
+// Pages are counted by the table's width, for lengths are on the device: short contexts in wide tables get clusters and
+// score rows that they do not need.  Single tokens behind 2000 lose 0 to 1.5 us to a table of 8192 pages; tiles of several
+// tokens, whose score rows then fill an SM, much more: 32 requests x 4 tokens 34.5 us for 11.2, a chunk of 512 80.4 for 15.9.
+// The counts of SMs and CTAs here are a whole B200's.
 template <typename T, int D>
 cudaError_t launch_select(SelectParams p, cudaStream_t st)
 {
