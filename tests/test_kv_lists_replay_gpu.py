@@ -11,10 +11,11 @@ INT4, NF4 = 0, 1
 F16, BF16 = torch.float16, torch.bfloat16
 
 
-@pytest.mark.parametrize("fmt,dtype,d,pages", [(INT4, F16, 128, 60), (NF4, BF16, 64, 60), (INT4, BF16, 128, 700)])
+@pytest.mark.parametrize("fmt,dtype,d,pages", [(INT4, F16, 128, 60), (NF4, BF16, 64, 60), (INT4, BF16, 128, 700), (NF4, F16, 64, 1100)])
 @pytest.mark.parametrize("prompts,new,steps", [([1, 1, 1], 1, 130), ([300, 40, 95], 1, 40), ([300, 40, 95], 5, 12)])
 def test_steps_replayed_past_what_is_kept(cuda, fmt, dtype, d, pages, prompts, new, steps):
-    """Of 4 pages of 16: single tokens from the first on and behind prompts, drafts; tables of 700 pages are shared by clusters."""
+    """Of 4 pages of 16: single tokens from the first on and behind prompts, drafts; tables of 700 and 1100 pages are shared by clusters of 8 and
+    16 CTAs."""
     keep, page = 4, 16
     layer = Layer(cuda, fmt, dtype, 8, 2, d, page, 3, pages, sum(prompts) + 4, keep, 1, 1)
     g = torch.Generator(device=cuda).manual_seed(d + new)
